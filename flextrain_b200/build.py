@@ -20,7 +20,8 @@ LIB = PKG / "_lib"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 CUDA_HOME = Path(NVCC).resolve().parent.parent
 
-CUDA_SOURCES = ["gemm_tcgen05", "elementwise", "attention", "comm", "moe", "noalloc", "gdn", "gdn_chunk", "lora", "seqmix"]
+CUDA_SOURCES = ["gemm_tcgen05", "elementwise", "attention", "comm", "moe", "noalloc", "gdn", "gdn_chunk", "lora", "seqmix", "fp8", "gemm_fp8"]
+EXACT_SOURCES = {"fp8"}          # compiled without fast math
 CPP_SOURCES = ["dp_solver", "copy_engine"]
 PYEXT_SOURCES = ["fastcall"]
 
@@ -52,7 +53,7 @@ def build_all(force: bool = False, verbose: bool = False) -> dict:
             continue
         out = lib_path(name)
         if force or _newer(src, out, headers):
-            cmd = [NVCC, *NVCC_FLAGS, "-I", str(CSRC), "-o", str(out), str(src), "-lcudart"]
+            cmd = [NVCC, *(f for f in NVCC_FLAGS if f != "--use_fast_math" or name not in EXACT_SOURCES), "-I", str(CSRC), "-o", str(out), str(src), "-lcudart"]
             r = subprocess.run(cmd, capture_output=True, text=True)
             (LIB / f"{name}.ptxas.log").write_text(r.stderr)
             if verbose:

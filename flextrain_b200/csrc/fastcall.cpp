@@ -8,11 +8,14 @@
 //   _ftb_fastcall.bind(path_to_libftb_gemm_tcgen05.so)          -> None
 //   _ftb_fastcall.gemm(A, B, D, C, bias, M, N, K, a_mn, b_mn, lda, ldb, ldd, ldc, alpha, beta, d_fp32, bn,
 //                      max_ctas, stream)                        -> int (the kernel library's return code)
+//   _ftb_fastcall.call(address, *args)                          -> int: an entry point int (*)(const int64_t*) on its arguments,
+//                      ints, floats (as the bits of a double) and None (0), in 8 bytes each
 //   _ftb_fastcall.calls()                                       -> number of gemm() calls so far
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <dlfcn.h>
 #include <stdint.h>
+#include <string.h>
 
 namespace {
 
@@ -90,12 +93,42 @@ PyObject* py_gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
+constexpr Py_ssize_t MAX_ARGS = 48;
+
+PyObject* py_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n < 1 || n - 1 > MAX_ARGS) {
+    PyErr_SetString(PyExc_TypeError, "call() takes an address and at most 48 arguments");
+    return nullptr;
+  }
+  void* fn;
+  if (!as_ptr(a[0], &fn)) return nullptr;
+  if (fn == nullptr) {
+    PyErr_SetString(PyExc_ValueError, "call() of a null address");
+    return nullptr;
+  }
+  int64_t v[MAX_ARGS] = {};
+  for (Py_ssize_t i = 1; i < n; ++i) {
+    if (a[i] == Py_None) continue;
+    if (PyFloat_CheckExact(a[i])) {
+      const double d = PyFloat_AS_DOUBLE(a[i]);
+      memcpy(&v[i - 1], &d, sizeof d);
+    } else {
+      const long long x = PyLong_AsLongLong(a[i]);
+      if (x == -1 && PyErr_Occurred()) return nullptr;
+      v[i - 1] = x;
+    }
+  }
+  return PyLong_FromLong(reinterpret_cast<int (*)(const int64_t*)>(fn)(v));
+}
+
 PyObject* py_calls(PyObject*, PyObject*) { return PyLong_FromUnsignedLongLong(g_calls); }
 
 PyMethodDef kMethods[] = {
     {"bind", py_bind, METH_O, "bind(path): open the GEMM kernel library"},
     {"gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_gemm)), METH_FASTCALL,
      "gemm(A, B, D, C, bias, M, N, K, a_mn, b_mn, lda, ldb, ldd, ldc, alpha, beta, d_fp32, bn, max_ctas, stream)"},
+    {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_call)), METH_FASTCALL,
+     "call(address, *args): an entry point that takes its arguments in 8 bytes each"},
     {"calls", py_calls, METH_NOARGS, "number of gemm() calls"},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -759,6 +759,10 @@ def top_p_sample(logits, top_p, temperature, generator=None):
 rope_inv_freq = ref.rope_inv_freq
 
 
+# ------------------------------------------------------------ linear layers in 8 bits
+from .fp8 import (Fp8Matrix, dequant_fp8, gemm_fp8, grouped_gemm_fp8, grouped_wgrad_fp8, linear_fp8_dgrad, linear_fp8_fwd,  # noqa: E402
+                  linear_fp8_wgrad, quant_fp8, rmsnorm_fp8_fwd)
+
 # ------------------------------------------------------------------ per-op device timing
 # ``FTB_OP_TIMING=1`` brackets every leaf op of this module with CUDA events on the current stream and
 # ``timing_report()`` aggregates them by (op, shape): the per-kernel time table of a training step without a
@@ -766,7 +770,7 @@ rope_inv_freq = ref.rope_inv_freq
 _TIMED_OPS = ("gemm", "gemm_glu_fwd", "gemm_glu_bwd", "rmsnorm_fwd", "rmsnorm_bwd", "rope", "rope_qkv_fused", "lora_wgrad_fused", "glu_fwd", "glu_bwd",
               "glu_bwd_weighted", "attention_fwd", "attention_bwd", "softmax_ce_", "softmax_ce_loss", "embedding_fwd", "embedding_bwd", "adamw_multi", "topk_route",
               "topk_route_bwd", "gather_rows", "moe_combine", "grouped_gemm", "grouped_wgrad", "l2norm_fwd",
-              "gated_rmsnorm_fwd", "bias_grad")
+              "gated_rmsnorm_fwd", "bias_grad", "quant_fp8", "rmsnorm_fp8_fwd", "gemm_fp8", "grouped_gemm_fp8", "grouped_wgrad_fp8")
 _timing_events: list = []
 
 
@@ -780,6 +784,8 @@ def _timing_key(name, args, kwargs):
         lay = ("T" if ta else "N") + ("T" if tb else "N")
         od = kwargs.get("out_dtype") or (kwargs["out"].dtype if kwargs.get("out") is not None else a.dtype)
         return f"{M}x{N}x{K} {lay}" + (" +C" if kwargs.get("beta", 0.0) else "") + (" f32" if od == torch.float32 else "")
+    if name in ("gemm_fp8", "grouped_gemm_fp8", "grouped_wgrad_fp8"):
+        return " by ".join("x".join(str(s) for s in m.data.shape) for m in args[:2])
     for v in list(args) + list(kwargs.values()):
         if isinstance(v, torch.Tensor):
             return "x".join(str(s) for s in v.shape)

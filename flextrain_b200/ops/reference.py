@@ -635,3 +635,47 @@ def moe_row_weights(w: torch.Tensor, plan: MoEPlan) -> torch.Tensor:
 def moe_rows_to_slots(v: torch.Tensor, plan: MoEPlan, shape) -> torch.Tensor:
     """Inverse of the row layout for a per-row scalar: returns ``(T,K)``."""
     return v[plan.inv.reshape(-1).long()].view(shape)
+
+
+# ------------------------------------------------------- e4m3 with a scale for each block of 128
+FP8_TOP, FP8_FLOOR = 448.0, 2.0 ** -126
+FP8_GROUPS = {"row": (1, 128), "col": (128, 1), "block": (128, 128)}
+
+
+def fp8_spread(scale: torch.Tensor, group: str, m: int, n: int) -> torch.Tensor:
+    """Scales of a matrix of ``m x n`` brought to its elements' shape."""
+    down, along = FP8_GROUPS[group]
+    if down > 1:
+        scale = scale.repeat_interleave(down, -2)
+    if along > 1:
+        scale = scale.repeat_interleave(along, -1)
+    return scale[..., :m, :n]
+
+
+def quant_fp8(x: torch.Tensor, group: str) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(q, scale)``: ``scale = max(max|x| / 448, 2^-126)`` of each group, ``q = e4m3(x * (1 / scale))``."""
+    *b, m, n = x.shape
+    down, along = FP8_GROUPS[group]
+    M, N = -(-m // down), -(-n // along)
+    xf = x.to(F32)
+    if x.numel():
+        padded = F.pad(xf.abs(), (0, N * along - n, 0, M * down - m))
+        top = padded.reshape(*b, M, down, N, along).amax((-3, -1))
+    else:
+        top = xf.new_zeros(*b, M, N)
+    scale = (top / FP8_TOP).clamp(min=FP8_FLOOR)
+    q = (xf * fp8_spread(1.0 / scale, group, m, n)).clamp(-FP8_TOP, FP8_TOP).to(torch.float8_e4m3fn)
+    return q, scale
+
+
+def dequant_fp8(q: torch.Tensor, scale: torch.Tensor, group: str, dtype=F32) -> torch.Tensor:
+    return (q.to(F32) * fp8_spread(scale, group, q.shape[-2], q.shape[-1])).to(dtype)
+
+
+def rmsnorm_fp8_fwd(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, residual: Optional[torch.Tensor] = None):
+    """``(q, scale, rstd, h)`` of ``h = x + residual`` (rounded to ``x``'s type) and ``y = h * rstd * w`` in row groups."""
+    h = x if residual is None else (x.to(F32) + residual.to(F32)).to(x.dtype)
+    hf = h.to(F32)
+    rstd = torch.rsqrt(hf.pow(2).mean(-1) + eps)
+    y = hf * rstd.unsqueeze(-1)
+    return (*quant_fp8(y if w is None else y * w.to(F32), "row"), rstd, h)
