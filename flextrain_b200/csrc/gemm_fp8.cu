@@ -9,8 +9,8 @@
 // whatever the tensor core's adder does.
 //
 //   warp 0     TMA producer (128-byte swizzle; operands K-major or MN-major, as they lie in memory)
-//   warp 1     tcgen05.mma, one thread
-//   warps 4-11 read out, scale and add; at the end of a tile turn it over in shared memory and store whole pieces of rows
+//   warps 1, 2 tcgen05.mma, one thread each: one half of the tile's columns each
+//   warps 4-11 four for each half: read out, scale and add; at the end of a tile turn it over in shared memory and store whole pieces of rows
 //              (a thread's 128 sums, and 32 values on the way, need more than the 168 registers of 384 threads: the first four
 //              warps give theirs up)
 //
@@ -25,31 +25,8 @@ namespace {
 
 constexpr int BM = 128, BK = 128, MMA_K = 32;
 constexpr int EPI_WARPS = 8, EPI_FIRST = 4, THREADS = 32 * (EPI_FIRST + EPI_WARPS);
-constexpr int WARP_BYTES = 32 * 128;                     // a warp's piece of shared memory: 32 rows x 128 bytes
+constexpr int PIECE_BYTES = 32 * 128;                    // a warp's piece of shared memory: 32 rows x 128 bytes
 constexpr int BOX_BYTES = 128 * 128;
-
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float a, float b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 pack2u(uint32_t a, uint32_t b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ void unpack2(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 
 // e4m3 x e4m3 -> fp32
 template <int CG>
@@ -133,131 +110,139 @@ struct Walk {
   }
 };
 
+constexpr int C_BUFS = 2;                                // pieces of C under way for a warp
+constexpr int SB_SLOTS = 4;                              // blocks of column scales under way for a warp
+
 template <int CG, int BN, bool BVEC>
 struct Ring {
   static constexpr int B_BYTES = BN / CG * BK;
   static constexpr int STAGE = BM * BK + B_BYTES;
-  static constexpr int EXTRA = EPI_WARPS * (WARP_BYTES + (BVEC ? 2 * BN / 2 * 4 : 0));
-  static constexpr int STAGES = (227 * 1024 - 1024 - 256 - EXTRA) / STAGE;
-  static constexpr int TOTAL = STAGES * STAGE + EXTRA + 256 + 1024;
-  static constexpr int NACC = 512 / BN;
-  static_assert(STAGES >= 3 && STAGES <= 8 && NACC <= 4, "barriers in 256 bytes");
+  static constexpr int WARP = C_BUFS * PIECE_BYTES + (BVEC ? SB_SLOTS * BN / 2 * 4 : 0);
+  static constexpr int STAGES = (227 * 1024 - 1024 - 512 - EPI_WARPS * WARP) / STAGE;
+  static constexpr int TOTAL = STAGES * STAGE + EPI_WARPS * WARP + 512 + 1024;
+  static constexpr int NACC = 512 / BN;              // accumulators of each half
+  static_assert(STAGES >= 3 && 2 * STAGES + 4 * NACC + 1 <= 64, "barriers in 512 bytes");
 };
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// four bytes, or zeros in their place
+__device__ __forceinline__ void cp_async4(void* dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all of the thread's copies, committed or not
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // 32 rows x 128 bytes of a warp in 16-byte pieces, free of bank conflicts row-wise and piece-wise
 __device__ __forceinline__ uint4* piece_at(uint8_t* buf, int row, int piece) {
   return reinterpret_cast<uint4*>(buf + row * 128 + ((piece ^ (row & 7)) << 4));
 }
-template <typename T>
-__device__ __forceinline__ T* element_at(uint8_t* buf, int row, int e) {
-  const int byte = e * static_cast<int>(sizeof(T));
-  return reinterpret_cast<T*>(buf + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15));
+__device__ __forceinline__ uint8_t* byte_at(uint8_t* buf, int row, int byte) {
+  return buf + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15);
 }
 
-// `cols` columns of `rows` rows between global memory (row r at g + r * ld) and a warp's piece of shared memory
-template <typename T>
-__device__ __forceinline__ void rows_in(uint8_t* buf, const T* g, long ld, int rows, int cols, int vec, int lane) {
+// Where a warp's part of a tile lies in D and C: 32 rows (so many of them real) from column col0 on.  A step is 128 bytes of a row.
+struct Patch {
+  uint8_t* d;
+  const uint8_t* c;
+  long ldd, ldc;                     // bytes
+  int rows, cols;                    // cols: from col0 to the end of a row of D
+};
+// First column, from col0 on, of a thread's columns c, c + 1, ...: a pair of SMs has 64 of each 128 in a half of its tile.
+template <int CG>
+__device__ __forceinline__ constexpr int column(int c) { return CG == 1 ? c : (c >> 6) * 128 + (c & 63); }
+
+// the step of C from column col on its way into a piece of shared memory (complete after a wait for the thread's copies and a __syncwarp)
+__device__ __forceinline__ void fetch_c(const Patch& w, int es, int vec, int col, uint8_t* buf, int lane) {
+  const int bytes = min(128, (w.cols - col) * es);
+  const uint8_t* c = w.c + col * es;
   if (vec) {
-    const int pieces = min(8, cols * static_cast<int>(sizeof(T)) >> 4), lr = lane >> 3, lp = lane & 7;
+    const int lr = lane >> 3, lp = lane & 7;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i * 4 + lr < rows && lp < pieces)
-        *piece_at(buf, i * 4 + lr, lp) = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(g + (i * 4 + lr) * ld) + lp * 16);
+    for (int k = 0; k < 8; ++k)
+      if (k * 4 + lr < w.rows && lp * 16 < bytes) cp_async16(piece_at(buf, k * 4 + lr, lp), c + (k * 4 + lr) * w.ldc + lp * 16);
+  } else if (es == 4) {
+    for (int r = 0; r < w.rows; ++r)
+      if (lane * 4 < bytes) *reinterpret_cast<float*>(byte_at(buf, r, lane * 4)) = *reinterpret_cast<const float*>(c + r * w.ldc + lane * 4);
   } else {
-    for (int r = 0; r < rows; ++r)
-      for (int e = lane; e < min(cols, static_cast<int>(128 / sizeof(T))); e += 32) *element_at<T>(buf, r, e) = g[r * ld + e];
+    for (int r = 0; r < w.rows; ++r)
+      for (int e = lane; e * 2 < bytes; e += 32)
+        *reinterpret_cast<uint16_t*>(byte_at(buf, r, e * 2)) = *reinterpret_cast<const uint16_t*>(c + r * w.ldc + e * 2);
   }
 }
-template <typename T>
-__device__ __forceinline__ void rows_out(uint8_t* buf, T* g, long ld, int rows, int cols, int vec, int lane) {
+__device__ __forceinline__ void store_d(const Patch& w, int es, int vec, int col, uint8_t* buf, int lane) {
+  const int bytes = min(128, (w.cols - col) * es);
+  uint8_t* d = w.d + col * es;
   if (vec) {
-    const int pieces = min(8, cols * static_cast<int>(sizeof(T)) >> 4), lr = lane >> 3, lp = lane & 7;
+    const int lr = lane >> 3, lp = lane & 7;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i * 4 + lr < rows && lp < pieces)
-        *reinterpret_cast<uint4*>(reinterpret_cast<char*>(g + (i * 4 + lr) * ld) + lp * 16) = *piece_at(buf, i * 4 + lr, lp);
+    for (int k = 0; k < 8; ++k)
+      if (k * 4 + lr < w.rows && lp * 16 < bytes) *reinterpret_cast<uint4*>(d + (k * 4 + lr) * w.ldd + lp * 16) = *piece_at(buf, k * 4 + lr, lp);
+  } else if (es == 4) {
+    for (int r = 0; r < w.rows; ++r)
+      if (lane * 4 < bytes) *reinterpret_cast<float*>(d + r * w.ldd + lane * 4) = *reinterpret_cast<const float*>(byte_at(buf, r, lane * 4));
   } else {
-    for (int r = 0; r < rows; ++r)
-      for (int e = lane; e < min(cols, static_cast<int>(128 / sizeof(T))); e += 32) g[r * ld + e] = *element_at<T>(buf, r, e);
+    for (int r = 0; r < w.rows; ++r)
+      for (int e = lane; e * 2 < bytes; e += 32)
+        *reinterpret_cast<uint16_t*>(d + r * w.ldd + e * 2) = *reinterpret_cast<const uint16_t*>(byte_at(buf, r, e * 2));
   }
 }
 
-// A thread's row of NP pairs of sums, from column col0 of D on: alpha, bias, C, rounding once, and out in 128-byte pieces.
-template <int NP>
-__device__ __forceinline__ void store_tile(const Params& p, const f32x2 (&acc)[NP], uint8_t* buf, long row, long skip, int rows,
-                                           int col0, int lane) {
-  if (rows <= 0) return;                               // (the whole warp)
+// A thread's row of NC sums: alpha, bias, C, rounding once, and out step by step.  The first C_BUFS steps of C are under way
+// already, in the pieces of buf.  FP32: type of D, C.
+template <bool FP32, int CG, int NC>
+__device__ __forceinline__ void store_tile(const Params& p, const float (&sum)[NC], const Patch& w, const float* bias, uint8_t* buf, int lane) {
+  constexpr int ES = FP32 ? 4 : 2, STEP = 128 / ES, STEPS = NC / STEP;
   const bool add = p.beta != 0.f;
-  if (p.d_fp32) {
-    float* D = static_cast<float*>(p.D) + skip + row * p.ldd;
-    const float* C = static_cast<const float*>(p.C) + skip + row * p.ldc;
 #pragma unroll
-    for (int c = 0; c < 2 * NP; c += 32) {
-      const int col = col0 + c, cols = p.N - col;
-      if (cols <= 0) break;
-      if (add) {
-        rows_in(buf, C + col, p.ldc, rows, cols, p.vec, lane);
-        __syncwarp();
-      }
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        float v[4];
-        unpack2(acc[c / 2 + 2 * q], v[0], v[1]);
-        unpack2(acc[c / 2 + 2 * q + 1], v[2], v[3]);
-        uint4* at = piece_at(buf, lane, q);
-        const uint4 cu = *at;
-        const float cc[4] = {__uint_as_float(cu.x), __uint_as_float(cu.y), __uint_as_float(cu.z), __uint_as_float(cu.w)};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[j] *= p.alpha;
-          if (p.bias != nullptr && 4 * q + j < cols) v[j] += p.bias[col + 4 * q + j];
-          if (add) v[j] += p.beta * cc[j];
-        }
-        *at = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-      }
-      __syncwarp();
-      rows_out(buf, D + col, p.ldd, rows, cols, p.vec, lane);
+  for (int i = 0; i < STEPS; ++i) {
+    const int col = column<CG>(i * STEP), cols = w.cols - col;
+    if (cols <= 0) break;
+    uint8_t* at = buf + (i % C_BUFS) * PIECE_BYTES;
+    if (add) {
+      if (i == 0 || i + 1 == STEPS) cp_wait_all();
+      else cp_wait<1>();
       __syncwarp();
     }
-  } else {
-    __nv_bfloat16* D = static_cast<__nv_bfloat16*>(p.D) + skip + row * p.ldd;
-    const __nv_bfloat16* C = static_cast<const __nv_bfloat16*>(p.C) + skip + row * p.ldc;
 #pragma unroll
-    for (int c = 0; c < 2 * NP; c += 64) {
-      const int col = col0 + c, cols = p.N - col;
-      if (cols <= 0) break;
-      if (add) {
-        rows_in(buf, C + col, p.ldc, rows, cols, p.vec, lane);
-        __syncwarp();
+    for (int q = 0; q < 8; ++q) {
+      uint4* pc = piece_at(at, lane, q);
+      const uint4 cu = *pc;
+      const uint32_t cw[4] = {cu.x, cu.y, cu.z, cu.w};
+      uint32_t ow[4];
+      constexpr int E = 16 / ES;                         // elements of a piece
+      float v[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        v[j] = sum[i * STEP + q * E + j] * p.alpha;
+        if (bias != nullptr && q * E + j < cols) v[j] += bias[col + q * E + j];
       }
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        uint4* at = piece_at(buf, lane, q);
-        const uint4 cu = *at;
-        const uint32_t cw[4] = {cu.x, cu.y, cu.z, cu.w};
-        uint32_t ow[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float a, b;
-          unpack2(acc[c / 2 + 4 * q + j], a, b);
-          a *= p.alpha;
-          b *= p.alpha;
-          if (p.bias != nullptr) {
-            if (8 * q + 2 * j < cols) a += p.bias[col + 8 * q + 2 * j];
-            if (8 * q + 2 * j + 1 < cols) b += p.bias[col + 8 * q + 2 * j + 1];
-          }
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (FP32) {
+          if (add) v[j] += p.beta * __uint_as_float(cw[j]);
+          ow[j] = __float_as_uint(v[j]);
+        } else {
           if (add) {
-            a += p.beta * __uint_as_float(cw[j] << 16);
-            b += p.beta * __uint_as_float(cw[j] & 0xFFFF0000u);
+            v[2 * j] += p.beta * __uint_as_float(cw[j] << 16);
+            v[2 * j + 1] += p.beta * __uint_as_float(cw[j] & 0xFFFF0000u);
           }
-          const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
           ow[j] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        *at = make_uint4(ow[0], ow[1], ow[2], ow[3]);
       }
-      __syncwarp();
-      rows_out(buf, D + col, p.ldd, rows, cols, p.vec, lane);
-      __syncwarp();
+      *pc = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+    }
+    __syncwarp();
+    store_d(w, ES, p.vec, col, at, lane);
+    __syncwarp();
+    if (add) {
+      if (i + C_BUFS < STEPS && w.cols > column<CG>((i + C_BUFS) * STEP)) fetch_c(w, ES, p.vec, column<CG>((i + C_BUFS) * STEP), at, lane);
+      cp_commit();
     }
   }
 }
@@ -267,15 +252,15 @@ __global__ void __launch_bounds__(THREADS, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
   using R = Ring<CG, BN, BVEC>;
   using W = Walk<BM * CG, 16 / CG>;
-  constexpr int ST = R::STAGES, NACC = R::NACC;
+  constexpr int ST = R::STAGES, NACC = R::NACC, HALF = BN / 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smem_epi = smem + ST * R::STAGE;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem_epi + R::EXTRA);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem_epi + EPI_WARPS * R::WARP);
   uint64_t* empty_bar = full_bar + ST;
   uint64_t* tfull_bar = empty_bar + ST;
-  uint64_t* tempty_bar = tfull_bar + NACC;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + NACC);
+  uint64_t* tempty_bar = tfull_bar + 2 * NACC;            // (of the first half of the columns, then of the second)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2 * NACC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -284,8 +269,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int s = 0; s < ST; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int a = 0; a < NACC; ++a) { mbar_init(&tfull_bar[a], 1); mbar_init(&tempty_bar[a], CG * EPI_WARPS); }
+    for (int s = 0; s < ST; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 2); }
+    for (int a = 0; a < 2 * NACC; ++a) { mbar_init(&tfull_bar[a], 1); mbar_init(&tempty_bar[a], CG * EPI_WARPS / 2); }
     fence_barrier_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
@@ -341,13 +326,22 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           for (uint32_t it = 0; it < (1u << 16); ++it)
             if (mbar_try_wait(&full_bar[s], 0) || mbar_try_wait(&full_bar[s], 1)) break;
     }
-    if (warp == 1 && lane == 0 && cta == 0) {
+    if ((warp == 1 || warp == 2) && lane == 0 && cta == 0) {
+      // A barrier's word is some 250 cycles away while the tensor core reads shared memory, a block's products take 512.  So a
+      // thread asks for both of its barriers at once, and each half of the columns has a thread and accumulators of its own: a
+      // half is multiplied while the other one's are read out.
+      const int half = warp - 1;
+      uint64_t *tfull = tfull_bar + half * NACC, *tempty = tempty_bar + half * NACC;
+      const uint32_t tmem_half = tmem_base + half * NACC * HALF;
       // e4m3 operands (format 0), fp32 sums
       const uint32_t idesc = (1u << 4) | static_cast<uint32_t>(p.a_mn) << 15 | static_cast<uint32_t>(p.b_mn) << 16 |
-                             static_cast<uint32_t>(BN >> 3) << 17 | static_cast<uint32_t>(BM * CG >> 4) << 24;
+                             static_cast<uint32_t>(HALF >> 3) << 17 | static_cast<uint32_t>(BM * CG >> 4) << 24;
       // K-major: 32 bytes along the swizzled row of 128; MN-major: 32 rows of 128 bytes, blocks of 128 wide behind one another
       const uint32_t a_step = p.a_mn ? MMA_K * 128 : MMA_K, b_step = p.b_mn ? MMA_K * 128 : MMA_K;
       const uint32_t a_lbo = p.a_mn ? BOX_BYTES : 16, b_lbo = p.b_mn ? BOX_BYTES : 16;
+      // the half's columns of this CTA's part of B: rows of it, or bytes of its rows, or its second box
+      constexpr int OWN = HALF / CG;
+      const uint32_t b_off = half * (p.b_mn ? (OWN == 128 ? BOX_BYTES : OWN) : OWN * 128);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
@@ -356,16 +350,17 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       for (int tile = first; tile < p.num_tiles && ok; tile += step) {
         if (!walk.at(p, tile, t)) break;
         for (int kb = 0; kb < t.kbs; ++kb) {
-          if (!(ok = mbar_wait(&tempty_bar[acc], acc_phase ^ 1, abort_flag, 20))) break;
-          if (!(ok = mbar_wait(&full_bar[stage], phase, abort_flag, 21))) break;
+          const bool e = mbar_try_wait(&tempty[acc], acc_phase ^ 1), f = mbar_try_wait(&full_bar[stage], phase);
+          if (!e && !(ok = mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, 20))) break;
+          if (!f && !(ok = mbar_wait(&full_bar[stage], phase, abort_flag, 21))) break;
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * R::STAGE), sb = sa + BM * BK;
+          const uint32_t sa = smem_u32(smem + stage * R::STAGE), sb = sa + BM * BK + b_off;
 #pragma unroll
           for (int kk = 0; kk < BK / MMA_K; ++kk)
-            umma_f8<CG>(tmem_base + acc * BN, make_smem_desc(sa + kk * a_step, a_lbo, 1024), make_smem_desc(sb + kk * b_step, b_lbo, 1024),
+            umma_f8<CG>(tmem_half + acc * HALF, make_smem_desc(sa + kk * a_step, a_lbo, 1024), make_smem_desc(sb + kk * b_step, b_lbo, 1024),
                         idesc, kk != 0);
-          if constexpr (CG == 2) { umma_commit_2cta(&empty_bar[stage], 3); umma_commit_2cta(&tfull_bar[acc], 3); }
-          else { umma_commit(&empty_bar[stage]); umma_commit(&tfull_bar[acc]); }
+          if constexpr (CG == 2) { umma_commit_2cta(&tfull[acc], 3); umma_commit_2cta(&empty_bar[stage], 3); }
+          else { umma_commit(&tfull[acc]); umma_commit(&empty_bar[stage]); }
           if (++stage == ST) { stage = 0; phase ^= 1; }
           if (++acc == NACC) { acc = 0; acc_phase ^= 1; }
         }
@@ -373,70 +368,152 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;\n");
-    constexpr int HALF = BN / 2, NP = HALF / 2;
+    constexpr int AHEAD = 3, SEG = CG, SEG_COLS = HALF / SEG;   // (a half of a pair's tile has columns of two blocks of 128)
+    static_assert(AHEAD < SB_SLOTS, "a slot is written when all lanes have read it");
     const int quad = warp & 3, part = (warp - EPI_FIRST) >> 2;
-    uint8_t* buf = smem_epi + (warp - EPI_FIRST) * (R::EXTRA / EPI_WARPS);
-    [[maybe_unused]] float* sbuf = reinterpret_cast<float*>(buf + WARP_BYTES);
+    uint8_t* buf = smem_epi + (warp - EPI_FIRST) * R::WARP;
+    [[maybe_unused]] float* sbuf = reinterpret_cast<float*>(buf + C_BUFS * PIECE_BYTES);
+    const int in_tile = cta * BM + quad * 32, es = p.d_fp32 ? 4 : 2;
+    const bool add = p.beta != 0.f;
+    uint64_t *tfull = tfull_bar + part * NACC, *tempty = tempty_bar + part * NACC;
+    const uint32_t tmem_part = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + part * NACC * HALF;
     int acc = 0;
     uint32_t acc_phase = 0;
-    bool ok = true;
+    [[maybe_unused]] uint32_t slot = 0;                  // of the next block of column scales to be asked for
     W walk;
-    Tile t;
-    for (int tile = first; tile < p.num_tiles && ok; tile += step) {
-      if (!walk.at(p, tile, t)) break;
-      if (t.kbs == 0 && p.mode == 2) continue;           // a group without rows leaves its result as it is
-      const int in_tile = cta * BM + quad * 32;
-      const int rows = max(0, min(32, t.left - in_tile));
-      const int col0 = t.tn * BN + part * HALF;
-      // (rows and columns outside read a scale that exists; what they compute is not stored)
-      const float* sa = p.sa + (min(t.row0 + in_tile + lane, p.M - 1) >> p.sa_shift) * p.sa_m + t.kb0 * p.sa_k;
-      const float* sb = p.sb + t.kb0 * p.sb_k + (p.mode == 1 ? t.g * p.sb_g : 0);
-      if constexpr (!BVEC) sb += (min(col0, p.N - 1) >> 7) * p.sb_n;
-      f32x2 sum[NP];
-#pragma unroll
-      for (int i = 0; i < NP; ++i) sum[i] = 0;
-      for (int kb = 0; kb < t.kbs; ++kb) {
-        const float a = sa[kb * p.sa_k];
-        [[maybe_unused]] float s = 0.f;
-        if constexpr (BVEC) {
+    Tile t = {};
+    const float *sa = nullptr, *sb = nullptr;
+    [[maybe_unused]] long sb_seg = 0;
+    float a_next[AHEAD];                                 // scales of the next blocks, asked for that much before they are needed
+    [[maybe_unused]] float b_next[SEG][AHEAD];
+    auto ask_columns = [&](int kb) {
+      if constexpr (BVEC) {
+        float* to = sbuf + (slot++ & (SB_SLOTS - 1)) * HALF;
+        if (kb < t.kbs) {
 #pragma unroll
           for (int j = 0; j < HALF / 32; ++j) {
-            const int n = col0 + lane + 32 * j;
-            sbuf[(kb & 1) * HALF + lane + 32 * j] = n < p.N ? sb[n * p.sb_n + kb * p.sb_k] : 0.f;
+            const int n = t.tn * BN + part * SEG_COLS + column<CG>(32 * j) + lane;
+            cp_async4(to + lane + 32 * j, sb + (n < p.N ? n * p.sb_n : 0) + kb * p.sb_k, n < p.N);
           }
-          __syncwarp();
-        } else {
-          s = a * sb[kb * p.sb_k];
         }
-        if (!(ok = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag, 30))) break;
+      }
+    };
+    // the tile's place and the scales of its first blocks; false behind the last tile
+    auto begin = [&](int tile) {
+      do {
+        if (tile >= p.num_tiles || !walk.at(p, tile, t)) return -1;
+        if (t.kbs > 0) break;                            // (a group without rows leaves its result as it is)
+        tile += step;
+      } while (true);
+      // (rows and columns outside read a scale that exists; what they compute is not stored)
+      sa = p.sa + (min(t.row0 + in_tile + lane, p.M - 1) >> p.sa_shift) * p.sa_m + t.kb0 * p.sa_k;
+      sb = p.sb + t.kb0 * p.sb_k + (p.mode == 1 ? t.g * p.sb_g : 0);
+      [[maybe_unused]] const int n0 = t.tn * BN + part * SEG_COLS;
+      if constexpr (!BVEC) {
+        sb += (min(n0, p.N - 1) >> 7) * p.sb_n;
+        sb_seg = SEG == 2 && n0 + 128 < p.N ? p.sb_n : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        a_next[i] = i < t.kbs ? sa[i * p.sa_k] : 0.f;
+        if constexpr (!BVEC) {
+#pragma unroll
+          for (int g = 0; g < SEG; ++g) b_next[g][i] = i < t.kbs ? sb[i * p.sb_k + g * sb_seg] : 0.f;
+        }
+        ask_columns(i);
+        if constexpr (BVEC) cp_commit();
+      }
+      return tile;
+    };
+    bool ok = true;
+    for (int tile = begin(first); tile >= 0;) {
+      Patch w;
+      w.rows = max(0, min(32, t.left - in_tile));
+      const int col0 = t.tn * BN + part * SEG_COLS, kbs = t.kbs;
+      w.cols = w.rows > 0 ? max(0, min(SEG * 128 - (SEG - 1) * 64, p.N - col0)) : 0;
+      {
+        const long skip = p.mode == 2 ? t.g * p.d_g : 0, row = static_cast<long>(t.row0) + in_tile;
+        w.ldd = p.ldd * es;
+        w.ldc = p.ldc * es;
+        w.d = static_cast<uint8_t*>(p.D) + (skip + row * p.ldd + col0) * es;
+        w.c = static_cast<const uint8_t*>(p.C) + (skip + row * p.ldc + col0) * es;
+      }
+      auto ask_c = [&](int i) {
+        const int col = column<CG>(i * (128 / es));
+        if (add && i < C_BUFS && i * (128 / es) < HALF && w.cols > col) fetch_c(w, es, p.vec, col, buf + i * PIECE_BYTES, lane);
+      };
+      for (int i = kbs; i < AHEAD; ++i) ask_c(i - kbs);
+      float sum[HALF];
+#pragma unroll
+      for (int i = 0; i < HALF; ++i) sum[i] = 0.f;
+#pragma unroll 1
+      for (int kb = 0; kb < kbs; ++kb) {
+        [[maybe_unused]] const float* cols = nullptr;
+        if constexpr (BVEC) {
+          cols = sbuf + ((slot - AHEAD) & (SB_SLOTS - 1)) * HALF;
+          cp_wait<AHEAD - 1>();
+          __syncwarp();
+        }
+        ask_columns(kb + AHEAD);
+        if (kb + AHEAD >= kbs) ask_c(kb + AHEAD - kbs);
+        if constexpr (BVEC) cp_commit();
+        float s[SEG];
+#pragma unroll
+        for (int g = 0; g < SEG; ++g) s[g] = BVEC ? a_next[0] : a_next[0] * b_next[g][0];
+#pragma unroll
+        for (int i = 0; i + 1 < AHEAD; ++i) {
+          a_next[i] = a_next[i + 1];
+          if constexpr (!BVEC) {
+#pragma unroll
+            for (int g = 0; g < SEG; ++g) b_next[g][i] = b_next[g][i + 1];
+          }
+        }
+        if (kb + AHEAD < kbs) {
+          a_next[AHEAD - 1] = sa[(kb + AHEAD) * p.sa_k];
+          if constexpr (!BVEC) {
+#pragma unroll
+            for (int g = 0; g < SEG; ++g) b_next[g][AHEAD - 1] = sb[(kb + AHEAD) * p.sb_k + g * sb_seg];
+          }
+        }
+        if (!(ok = mbar_wait(&tfull[acc], acc_phase, abort_flag, 30))) break;
         tc_fence_after();
-        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + part * HALF;
-        const f32x2 s2 = BVEC ? pack2(a, a) : pack2(s, s);
 #pragma unroll
         for (int c = 0; c < HALF; c += 32) {
           uint32_t r[32];
-          tmem_ld_32x32(taddr + c, r);
+          tmem_ld_32x32(tmem_part + acc * HALF + c, r);
           tmem_ld_wait();
           if (c + 32 == HALF) {                          // the last of this block's values are in registers
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-              if constexpr (CG == 2) mbar_arrive_leader(&tempty_bar[acc]);
-              else mbar_arrive(&tempty_bar[acc]);
+              if constexpr (CG == 2) mbar_arrive_leader(&tempty[acc]);
+              else mbar_arrive(&tempty[acc]);
             }
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            f32x2 v = pack2u(r[2 * i], r[2 * i + 1]);
-            if constexpr (BVEC) v = mul2(v, *reinterpret_cast<const f32x2*>(&sbuf[(kb & 1) * HALF + c + 2 * i]));
-            sum[c / 2 + i] = fma2(v, s2, sum[c / 2 + i]);
+          for (int i = 0; i < 32; i += 4) {
+            float f[4] = {1.f, 1.f, 1.f, 1.f};
+            if constexpr (BVEC) {
+              const float4 f4 = *reinterpret_cast<const float4*>(cols + c + i);
+              f[0] = f4.x; f[1] = f4.y; f[2] = f4.z; f[3] = f4.w;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              sum[c + i + j] = fmaf(BVEC ? __uint_as_float(r[i + j]) * f[j] : __uint_as_float(r[i + j]), s[BVEC ? 0 : c / SEG_COLS % SEG], sum[c + i + j]);
           }
         }
         if (++acc == NACC) { acc = 0; acc_phase ^= 1; }
       }
       if (!ok) break;
-      store_tile(p, sum, buf, static_cast<long>(t.row0) + in_tile, p.mode == 2 ? t.g * p.d_g : 0, rows, col0, lane);
+      __syncwarp();                                      // (all lanes have read the last slot)
+      tile = begin(tile + step);
+      if (w.cols > 0) {
+        const float* bias = p.bias == nullptr ? nullptr : p.bias + col0;
+        if (p.d_fp32) store_tile<true, CG>(p, sum, w, bias, buf, lane);
+        else store_tile<false, CG>(p, sum, w, bias, buf, lane);
+      }
     }
+    cp_wait_all();                                       // no copy outlives the block
   }
 
   __syncwarp();
