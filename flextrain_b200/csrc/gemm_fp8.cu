@@ -41,6 +41,43 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_
                  : "memory");
 }
 
+// whether a phase is complete, without waiting for it
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(ok)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  return ok != 0;
+}
+
+#define FTB_R16 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}"
+#define FTB_OUT16(r)                                                                                                           \
+  "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),       \
+      "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+// 16 lanes x 32 columns: r[4 j + 2 e + i] is lane 8 e + (thread >> 2), column 8 j + 2 (thread & 3) + i
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 " FTB_R16 ", [%16];" : FTB_OUT16(r) : "r"(taddr) : "memory");
+}
+// a row of 16 columns for each thread
+__device__ __forceinline__ void tmem_ld_row16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 " FTB_R16 ", [%16];" : FTB_OUT16(r) : "r"(taddr) : "memory");
+}
+
+// Tiled stores of a box of shared memory, and its addition to fp32 values where they lie.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(m)),
+               "r"(x), "r"(y), "r"(z), "r"(smem_u32(src))
+               : "memory");
+}
+__device__ __forceinline__ void tma_add_3d(const CUtensorMap* m, const void* src, int x, int y, int z) {
+  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(m)),
+               "r"(x), "r"(y), "r"(z), "r"(smem_u32(src))
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+
 struct Params {
   int M, N, K;
   void* D;
@@ -49,6 +86,7 @@ struct Params {
   long ldd, ldc;                     // elements
   float alpha, beta;
   int d_fp32, vec;                   // vec: rows of D and C in pieces of 16 bytes
+  int add_in_place;                  // C is D, in fp32 with beta = 1: the sums are added to it where it lies, and C is not read
   const float* sa;                   // scale of row m and block kb at sa[(m >> sa_shift) * sa_m + kb * sa_k]
   long sa_m, sa_k;
   int sa_shift;
@@ -111,13 +149,14 @@ struct Walk {
 };
 
 constexpr int C_BUFS = 2;                                // pieces of C under way for a warp
-constexpr int SB_SLOTS = 4;                              // blocks of column scales under way for a warp
+constexpr int SLOTS = 3;                                 // blocks of scales under way for a warp (BVEC)
 
 template <int CG, int BN, bool BVEC>
 struct Ring {
   static constexpr int B_BYTES = BN / CG * BK;
   static constexpr int STAGE = BM * BK + B_BYTES;
-  static constexpr int WARP = C_BUFS * PIECE_BYTES + (BVEC ? SB_SLOTS * BN / 2 * 4 : 0);
+  static constexpr int SLOT = BN / 2 + 32;                // column scales of a half, then row scales of a warp
+  static constexpr int WARP = C_BUFS * PIECE_BYTES + (BVEC ? SLOTS * SLOT * 4 : 0);
   static constexpr int STAGES = (227 * 1024 - 1024 - 512 - EPI_WARPS * WARP) / STAGE;
   static constexpr int TOTAL = STAGES * STAGE + EPI_WARPS * WARP + 512 + 1024;
   static constexpr int NACC = 512 / BN;              // accumulators of each half
@@ -174,17 +213,22 @@ __device__ __forceinline__ void fetch_c(const Patch& w, int es, int vec, int col
         *reinterpret_cast<uint16_t*>(byte_at(buf, r, e * 2)) = *reinterpret_cast<const uint16_t*>(c + r * w.ldc + e * 2);
   }
 }
-__device__ __forceinline__ void store_d(const Patch& w, int es, int vec, int col, uint8_t* buf, int lane) {
+// (add: to what lies there, in fp32)
+__device__ __forceinline__ void store_d(const Patch& w, int es, int vec, bool add, int col, uint8_t* buf, int lane) {
   const int bytes = min(128, (w.cols - col) * es);
   uint8_t* d = w.d + col * es;
-  if (vec) {
+  if (es == 4 && (add || !vec)) {
+    for (int r = 0; r < w.rows; ++r)
+      if (lane * 4 < bytes) {
+        float* to = reinterpret_cast<float*>(d + r * w.ldd + lane * 4);
+        const float v = *reinterpret_cast<const float*>(byte_at(buf, r, lane * 4));
+        *to = add ? *to + v : v;
+      }
+  } else if (vec) {
     const int lr = lane >> 3, lp = lane & 7;
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (k * 4 + lr < w.rows && lp * 16 < bytes) *reinterpret_cast<uint4*>(d + (k * 4 + lr) * w.ldd + lp * 16) = *piece_at(buf, k * 4 + lr, lp);
-  } else if (es == 4) {
-    for (int r = 0; r < w.rows; ++r)
-      if (lane * 4 < bytes) *reinterpret_cast<float*>(d + r * w.ldd + lane * 4) = *reinterpret_cast<const float*>(byte_at(buf, r, lane * 4));
   } else {
     for (int r = 0; r < w.rows; ++r)
       for (int e = lane; e * 2 < bytes; e += 32)
@@ -192,12 +236,14 @@ __device__ __forceinline__ void store_d(const Patch& w, int es, int vec, int col
   }
 }
 
-// A thread's row of NC sums: alpha, bias, C, rounding once, and out step by step.  The first C_BUFS steps of C are under way
-// already, in the pieces of buf.  FP32: type of D, C.
-template <bool FP32, int CG, int NC>
-__device__ __forceinline__ void store_tile(const Params& p, const float (&sum)[NC], const Patch& w, const float* bias, uint8_t* buf, int lane) {
+// A warp's 32 rows of NC sums: alpha, bias, C, rounding once, and out step by step.  ROWS: a thread has a row of them, else the
+// fragments of tmem_ld_16x32, 32 columns after 32 columns.  The first C_BUFS steps of C are under way already, in the pieces of
+// buf.  Whole patches leave as tiled copies, of which the thread does not see the end; `map` is null for patches whose last rows
+// are another group's, and for rows off the 16-byte grid.
+template <bool FP32, bool ROWS, int CG, int NC>
+__device__ __forceinline__ void store_tile(const Params& p, const float (&sum)[NC], const Patch& w, const float* bias, uint8_t* buf,
+                                           const CUtensorMap* map, int x, int y, int z, bool add, int lane) {
   constexpr int ES = FP32 ? 4 : 2, STEP = 128 / ES, STEPS = NC / STEP;
-  const bool add = p.beta != 0.f;
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
     const int col = column<CG>(i * STEP), cols = w.cols - col;
@@ -207,41 +253,92 @@ __device__ __forceinline__ void store_tile(const Params& p, const float (&sum)[N
       if (i == 0 || i + 1 == STEPS) cp_wait_all();
       else cp_wait<1>();
       __syncwarp();
+    } else if (i >= C_BUFS) {
+      if (lane == 0) bulk_wait_read<C_BUFS - 1>();         // the store of this piece has read it
+      __syncwarp();
     }
+    if constexpr (ROWS) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      uint4* pc = piece_at(at, lane, q);
-      const uint4 cu = *pc;
-      const uint32_t cw[4] = {cu.x, cu.y, cu.z, cu.w};
-      uint32_t ow[4];
-      constexpr int E = 16 / ES;                         // elements of a piece
-      float v[E];
+      for (int q = 0; q < 8; ++q) {
+        uint4* pc = piece_at(at, lane, q);
+        uint4 cu = make_uint4(0, 0, 0, 0);
+        if (add) cu = *pc;
+        const uint32_t cw[4] = {cu.x, cu.y, cu.z, cu.w};
+        uint32_t ow[4];
+        constexpr int E = 16 / ES;                       // elements of a piece
+        float v[E];
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        v[j] = sum[i * STEP + q * E + j] * p.alpha;
-        if (bias != nullptr && q * E + j < cols) v[j] += bias[col + q * E + j];
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (FP32) {
-          if (add) v[j] += p.beta * __uint_as_float(cw[j]);
-          ow[j] = __float_as_uint(v[j]);
-        } else {
-          if (add) {
-            v[2 * j] += p.beta * __uint_as_float(cw[j] << 16);
-            v[2 * j + 1] += p.beta * __uint_as_float(cw[j] & 0xFFFF0000u);
-          }
-          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-          ow[j] = *reinterpret_cast<const uint32_t*>(&h);
+        for (int j = 0; j < E; ++j) {
+          v[j] = sum[i * STEP + q * E + j] * p.alpha;
+          if (bias != nullptr && q * E + j < cols) v[j] += bias[col + q * E + j];
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (FP32) {
+            if (add) v[j] += p.beta * __uint_as_float(cw[j]);
+            ow[j] = __float_as_uint(v[j]);
+          } else {
+            if (add) {
+              v[2 * j] += p.beta * __uint_as_float(cw[j] << 16);
+              v[2 * j + 1] += p.beta * __uint_as_float(cw[j] & 0xFFFF0000u);
+            }
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            ow[j] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+        }
+        *pc = make_uint4(ow[0], ow[1], ow[2], ow[3]);
       }
-      *pc = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < STEP; c += 32)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e0 = c + 8 * j + 2 * (lane & 3);       // in the step
+          float b0 = 0.f, b1 = 0.f;
+          if (bias != nullptr && e0 < cols) b0 = bias[col + e0];
+          if (bias != nullptr && e0 + 1 < cols) b1 = bias[col + e0 + 1];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {                    // rows 8 k + (lane >> 2)
+            const float* f = &sum[((i * STEP + c) / 32 * 2 + (k >> 1)) * 16 + 4 * j + 2 * (k & 1)];
+            float v0 = f[0] * p.alpha + b0, v1 = f[1] * p.alpha + b1;
+            uint8_t* to = byte_at(at, 8 * k + (lane >> 2), e0 * ES);
+            if constexpr (FP32) {
+              if (add) {
+                const float2 cc = *reinterpret_cast<const float2*>(to);
+                v0 += p.beta * cc.x;
+                v1 += p.beta * cc.y;
+              }
+              *reinterpret_cast<float2*>(to) = make_float2(v0, v1);
+            } else {
+              if (add) {
+                const float2 cc = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(to));
+                v0 += p.beta * cc.x;
+                v1 += p.beta * cc.y;
+              }
+              *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(v0, v1);
+            }
+          }
+        }
     }
-    __syncwarp();
-    store_d(w, ES, p.vec, col, at, lane);
-    __syncwarp();
+    if (map != nullptr) {
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        if (FP32 && p.add_in_place) tma_add_3d(map, at, x + col, y, z);
+        else tma_store_3d(map, at, x + col, y, z);
+        bulk_commit();
+      }
+    } else {
+      __syncwarp();
+      store_d(w, ES, p.vec, FP32 && p.add_in_place, col, at, lane);
+      __syncwarp();
+    }
     if (add) {
-      if (i + C_BUFS < STEPS && w.cols > column<CG>((i + C_BUFS) * STEP)) fetch_c(w, ES, p.vec, column<CG>((i + C_BUFS) * STEP), at, lane);
+      if (i + C_BUFS < STEPS && w.cols > column<CG>((i + C_BUFS) * STEP)) {
+        if (lane == 0) bulk_wait_read<0>();
+        __syncwarp();
+        fetch_c(w, ES, p.vec, column<CG>((i + C_BUFS) * STEP), at, lane);
+      }
       cp_commit();
     }
   }
@@ -249,13 +346,15 @@ __device__ __forceinline__ void store_tile(const Params& p, const float (&sum)[N
 
 template <int CG, int BN, bool BVEC>
 __global__ void __launch_bounds__(THREADS, 1)
-gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
+gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmD,
+                const Params p) {
   using R = Ring<CG, BN, BVEC>;
   using W = Walk<BM * CG, 16 / CG>;
   constexpr int ST = R::STAGES, NACC = R::NACC, HALF = BN / 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smem_epi = smem + ST * R::STAGE;
+  uint8_t* smem_slots = smem_epi + EPI_WARPS * C_BUFS * PIECE_BYTES;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem_epi + EPI_WARPS * R::WARP);
   uint64_t* empty_bar = full_bar + ST;
   uint64_t* tfull_bar = empty_bar + ST;
@@ -368,37 +467,50 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;\n");
-    constexpr int AHEAD = 3, SEG = CG, SEG_COLS = HALF / SEG;   // (a half of a pair's tile has columns of two blocks of 128)
-    static_assert(AHEAD < SB_SLOTS, "a slot is written when all lanes have read it");
+    constexpr int SEG = CG, SEG_COLS = HALF / SEG;         // (a half of a pair's tile has columns of two blocks of 128)
+    constexpr int AHEAD = 2;
+    static_assert(AHEAD < SLOTS, "a slot is written when all lanes have read it");
     const int quad = warp & 3, part = (warp - EPI_FIRST) >> 2;
-    uint8_t* buf = smem_epi + (warp - EPI_FIRST) * R::WARP;
-    [[maybe_unused]] float* sbuf = reinterpret_cast<float*>(buf + C_BUFS * PIECE_BYTES);
+    uint8_t* buf = smem_epi + (warp - EPI_FIRST) * (C_BUFS * PIECE_BYTES);
+    [[maybe_unused]] float* slots = reinterpret_cast<float*>(smem_slots) + (warp - EPI_FIRST) * (SLOTS * R::SLOT);
     const int in_tile = cta * BM + quad * 32, es = p.d_fp32 ? 4 : 2;
-    const bool add = p.beta != 0.f;
+    const bool add = p.beta != 0.f && !p.add_in_place;
     uint64_t *tfull = tfull_bar + part * NACC, *tempty = tempty_bar + part * NACC;
     const uint32_t tmem_part = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + part * NACC * HALF;
     int acc = 0;
     uint32_t acc_phase = 0;
-    [[maybe_unused]] uint32_t slot = 0;                  // of the next block of column scales to be asked for
+    [[maybe_unused]] int slot = 0;                  // of the next block of scales to be asked for
     W walk;
     Tile t = {};
-    const float *sa = nullptr, *sb = nullptr;
+    const float *sa = nullptr, *sb = nullptr;            // of the next block to be asked for
     [[maybe_unused]] long sb_seg = 0;
-    float a_next[AHEAD];                                 // scales of the next blocks, asked for that much before they are needed
-    [[maybe_unused]] float b_next[SEG][AHEAD];
-    auto ask_columns = [&](int kb) {
+    int asked = 0;
+    // scales of the next blocks, asked for that much before they are needed: in registers (a row's, and those of its blocks of
+    // columns), or, of columns, in shared memory
+    [[maybe_unused]] float a_next[AHEAD], b_next[SEG][AHEAD];
+    auto ask = [&](int to) {
+      const bool there = asked++ < t.kbs;
       if constexpr (BVEC) {
-        float* to = sbuf + (slot++ & (SB_SLOTS - 1)) * HALF;
-        if (kb < t.kbs) {
+        float* at = slots + slot * R::SLOT + lane;
+        slot = slot + 1 == SLOTS ? 0 : slot + 1;
+        if (there) {
 #pragma unroll
           for (int j = 0; j < HALF / 32; ++j) {
             const int n = t.tn * BN + part * SEG_COLS + column<CG>(32 * j) + lane;
-            cp_async4(to + lane + 32 * j, sb + (n < p.N ? n * p.sb_n : 0) + kb * p.sb_k, n < p.N);
+            cp_async4(at + 32 * j, sb + (n < p.N ? n * p.sb_n : 0), n < p.N);
           }
+          cp_async4(at + HALF, sa, true);
         }
+        cp_commit();
+      } else if (there) {
+        a_next[to] = *sa;
+#pragma unroll
+        for (int g = 0; g < SEG; ++g) b_next[g][to] = sb[g * sb_seg];
       }
+      sa += p.sa_k;
+      sb += p.sb_k;
     };
-    // the tile's place and the scales of its first blocks; false behind the last tile
+    // the tile's place and the scales of its first blocks; -1 behind the last tile
     auto begin = [&](int tile) {
       do {
         if (tile >= p.num_tiles || !walk.at(p, tile, t)) return -1;
@@ -408,112 +520,140 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       // (rows and columns outside read a scale that exists; what they compute is not stored)
       sa = p.sa + (min(t.row0 + in_tile + lane, p.M - 1) >> p.sa_shift) * p.sa_m + t.kb0 * p.sa_k;
       sb = p.sb + t.kb0 * p.sb_k + (p.mode == 1 ? t.g * p.sb_g : 0);
-      [[maybe_unused]] const int n0 = t.tn * BN + part * SEG_COLS;
       if constexpr (!BVEC) {
+        const int n0 = t.tn * BN + part * SEG_COLS;
         sb += (min(n0, p.N - 1) >> 7) * p.sb_n;
         sb_seg = SEG == 2 && n0 + 128 < p.N ? p.sb_n : 0;
       }
+      asked = 0;
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        a_next[i] = i < t.kbs ? sa[i * p.sa_k] : 0.f;
-        if constexpr (!BVEC) {
-#pragma unroll
-          for (int g = 0; g < SEG; ++g) b_next[g][i] = i < t.kbs ? sb[i * p.sb_k + g * sb_seg] : 0.f;
-        }
-        ask_columns(i);
-        if constexpr (BVEC) cp_commit();
-      }
+      for (int i = 0; i < AHEAD; ++i) ask(i);
       return tile;
     };
-    bool ok = true;
+    bool ok = true, ready = false;
     for (int tile = begin(first); tile >= 0;) {
-      Patch w;
-      w.rows = max(0, min(32, t.left - in_tile));
-      const int col0 = t.tn * BN + part * SEG_COLS, kbs = t.kbs;
-      w.cols = w.rows > 0 ? max(0, min(SEG * 128 - (SEG - 1) * 64, p.N - col0)) : 0;
-      {
-        const long skip = p.mode == 2 ? t.g * p.d_g : 0, row = static_cast<long>(t.row0) + in_tile;
+      const int row = t.row0 + in_tile, rows = max(0, min(32, t.left - in_tile)), col0 = t.tn * BN + part * SEG_COLS, kbs = t.kbs, g = t.g;
+      auto patch = [&] {
+        Patch w;
+        w.rows = rows;
+        w.cols = rows > 0 ? max(0, min(SEG * 128 - (SEG - 1) * 64, p.N - col0)) : 0;
+        const long skip = p.mode == 2 ? g * p.d_g : 0;
         w.ldd = p.ldd * es;
         w.ldc = p.ldc * es;
         w.d = static_cast<uint8_t*>(p.D) + (skip + row * p.ldd + col0) * es;
         w.c = static_cast<const uint8_t*>(p.C) + (skip + row * p.ldc + col0) * es;
-      }
-      auto ask_c = [&](int i) {
-        const int col = column<CG>(i * (128 / es));
-        if (add && i < C_BUFS && i * (128 / es) < HALF && w.cols > col) fetch_c(w, es, p.vec, col, buf + i * PIECE_BYTES, lane);
+        return w;
       };
-      for (int i = kbs; i < AHEAD; ++i) ask_c(i - kbs);
+      // the first steps of C, asked for during the last blocks
+      auto ask_c = [&](int i) {
+        if (i >= C_BUFS || i * (128 / es) >= HALF) return;
+        const Patch w = patch();
+        const int col = column<CG>(i * (128 / es));
+        if (w.cols <= col) return;
+        if (lane == 0) bulk_wait_read<0>();                // the last tile's stores have read the pieces
+        __syncwarp();
+        fetch_c(w, es, p.vec, col, buf + i * PIECE_BYTES, lane);
+      };
+      if (add)
+        for (int i = kbs; i < AHEAD; ++i) ask_c(i - kbs);
       float sum[HALF];
 #pragma unroll
       for (int i = 0; i < HALF; ++i) sum[i] = 0.f;
 #pragma unroll 1
       for (int kb = 0; kb < kbs; ++kb) {
-        [[maybe_unused]] const float* cols = nullptr;
+        if (!ready && !(ok = mbar_wait(&tfull[acc], acc_phase, abort_flag, 30))) break;
+        tc_fence_after();
+        const uint32_t taddr = tmem_part + acc * HALF;
+        const bool wrap = acc + 1 == NACC;
+        if (add && kb + AHEAD >= kbs) ask_c(kb + AHEAD - kbs);
+        auto release = [&] {                             // the last of this block's values are in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 2) mbar_arrive_leader(&tempty[acc]);
+            else mbar_arrive(&tempty[acc]);
+          }
+        };
         if constexpr (BVEC) {
-          cols = sbuf + ((slot - AHEAD) & (SB_SLOTS - 1)) * HALF;
+          uint32_t r[2][16];
+          tmem_ld_16x32(taddr, r[0]);
           cp_wait<AHEAD - 1>();
           __syncwarp();
-        }
-        ask_columns(kb + AHEAD);
-        if (kb + AHEAD >= kbs) ask_c(kb + AHEAD - kbs);
-        if constexpr (BVEC) cp_commit();
-        float s[SEG];
+          const float* s = slots + (slot >= AHEAD ? slot - AHEAD : slot + SLOTS - AHEAD) * R::SLOT;
+          ask(0);
+          float a[4];
 #pragma unroll
-        for (int g = 0; g < SEG; ++g) s[g] = BVEC ? a_next[0] : a_next[0] * b_next[g][0];
-#pragma unroll
-        for (int i = 0; i + 1 < AHEAD; ++i) {
-          a_next[i] = a_next[i + 1];
-          if constexpr (!BVEC) {
-#pragma unroll
-            for (int g = 0; g < SEG; ++g) b_next[g][i] = b_next[g][i + 1];
-          }
-        }
-        if (kb + AHEAD < kbs) {
-          a_next[AHEAD - 1] = sa[(kb + AHEAD) * p.sa_k];
-          if constexpr (!BVEC) {
-#pragma unroll
-            for (int g = 0; g < SEG; ++g) b_next[g][AHEAD - 1] = sb[(kb + AHEAD) * p.sb_k + g * sb_seg];
-          }
-        }
-        if (!(ok = mbar_wait(&tfull[acc], acc_phase, abort_flag, 30))) break;
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < HALF; c += 32) {
-          uint32_t r[32];
-          tmem_ld_32x32(tmem_part + acc * HALF + c, r);
+          for (int k = 0; k < 4; ++k) a[k] = s[HALF + 8 * k + (lane >> 2)];
           tmem_ld_wait();
-          if (c + 32 == HALF) {                          // the last of this block's values are in registers
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if constexpr (CG == 2) mbar_arrive_leader(&tempty[acc]);
-              else mbar_arrive(&tempty[acc]);
-            }
-          }
+          constexpr int CHUNKS = HALF / 16;
+          float2 f[4];
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float f[4] = {1.f, 1.f, 1.f, 1.f};
-            if constexpr (BVEC) {
-              const float4 f4 = *reinterpret_cast<const float4*>(cols + c + i);
-              f[0] = f4.x; f[1] = f4.y; f[2] = f4.z; f[3] = f4.w;
+          for (int q = 0; q < CHUNKS; ++q) {             // 32 columns of lanes 0 to 15, of lanes 16 to 31
+            if (q + 1 < CHUNKS) tmem_ld_16x32(taddr + (q + 1) / 2 * 32 + (((q + 1) & 1) << 20), r[(q + 1) & 1]);
+            if (q + 1 == CHUNKS) ready = mbar_test(&tfull[wrap ? 0 : acc + 1], acc_phase ^ wrap);
+            if (q % 2 == 0) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const float2*>(s + q / 2 * 32 + 8 * j + 2 * (lane & 3));
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              sum[c + i + j] = fmaf(BVEC ? __uint_as_float(r[i + j]) * f[j] : __uint_as_float(r[i + j]), s[BVEC ? 0 : c / SEG_COLS % SEG], sum[c + i + j]);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float* to = &sum[q * 16 + 4 * j + 2 * e];
+                const uint32_t* v = &r[q & 1][4 * j + 2 * e];
+                to[0] = fmaf(__uint_as_float(v[0]) * f[j].x, a[2 * (q & 1) + e], to[0]);
+                to[1] = fmaf(__uint_as_float(v[1]) * f[j].y, a[2 * (q & 1) + e], to[1]);
+              }
+            if (q + 1 < CHUNKS) tmem_ld_wait();
+            if (q + 2 == CHUNKS) release();
+          }
+        } else {
+          constexpr int CH = 16;
+          uint32_t r[2][CH];
+          tmem_ld_row16(taddr, r[0]);
+          float s[SEG];
+#pragma unroll
+          for (int g = 0; g < SEG; ++g) s[g] = a_next[0] * b_next[g][0];
+#pragma unroll
+          for (int i = 0; i + 1 < AHEAD; ++i) {
+            a_next[i] = a_next[i + 1];
+#pragma unroll
+            for (int g = 0; g < SEG; ++g) b_next[g][i] = b_next[g][i + 1];
+          }
+          ask(AHEAD - 1);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < HALF; c += CH) {
+            if (c + CH < HALF) tmem_ld_row16(taddr + c + CH, r[(c / CH + 1) & 1]);
+            else ready = mbar_test(&tfull[wrap ? 0 : acc + 1], acc_phase ^ wrap);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) sum[c + i] = fmaf(__uint_as_float(r[c / CH & 1][i]), s[c / SEG_COLS % SEG], sum[c + i]);
+            if (c + CH < HALF) tmem_ld_wait();
+            if (c + 2 * CH == HALF) release();
           }
         }
-        if (++acc == NACC) { acc = 0; acc_phase ^= 1; }
+        if (wrap) { acc = 0; acc_phase ^= 1; }
+        else ++acc;
       }
       if (!ok) break;
       __syncwarp();                                      // (all lanes have read the last slot)
+      const Patch w = patch();
       tile = begin(tile + step);
       if (w.cols > 0) {
         const float* bias = p.bias == nullptr ? nullptr : p.bias + col0;
-        if (p.d_fp32) store_tile<true, CG>(p, sum, w, bias, buf, lane);
-        else store_tile<false, CG>(p, sum, w, bias, buf, lane);
+        // a patch whose last rows are not its own, but another group's, is stored row by row
+        const CUtensorMap* map = p.vec && (rows == 32 || p.mode != 1) ? &tmD : nullptr;
+        const int z = p.mode == 2 ? g : 0;
+        if (!add) {
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+        }
+        if (p.d_fp32) store_tile<true, !BVEC, CG>(p, sum, w, bias, buf, map, col0, row, z, add, lane);
+        else store_tile<false, !BVEC, CG>(p, sum, w, bias, buf, map, col0, row, z, add, lane);
       }
     }
     cp_wait_all();                                       // no copy outlives the block
+    if (lane == 0) bulk_wait_all();
   }
 
   __syncwarp();
@@ -543,16 +683,18 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// Map of `depth` stacked row-major byte matrices (rows x inner), boxes of box_rows x 128 bytes.
-int make_map(CUtensorMap* out, const void* base, int rank, uint64_t inner, uint64_t rows, uint64_t depth, uint64_t ld, uint64_t stack,
+// Map of `depth` stacked row-major matrices (rows x inner elements of es bytes, 1: e4m3), strides in bytes, boxes of box_rows x 128
+// bytes.
+int make_map(CUtensorMap* out, const void* base, int rank, int es, uint64_t inner, uint64_t rows, uint64_t depth, uint64_t ld, uint64_t stack,
              uint32_t box_rows) {
   EncodeTiledFn enc = encode_fn();
   if (enc == nullptr) return -100;
   const cuuint64_t dims[3] = {inner, rows, depth}, strides[2] = {ld, stack};
-  const cuuint32_t box[3] = {128, box_rows, 1}, es[3] = {1, 1, 1};
-  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, es,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint32_t box[3] = {128u / es, box_rows, 1}, steps[3] = {1, 1, 1};
+  const CUtensorMapDataType type = es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                           : es == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  const CUresult r = enc(out, type, rank, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -200 - static_cast<int>(r);
 }
 
@@ -569,7 +711,7 @@ int sm_count(int dev) {
 }
 
 template <int CG, int BN, bool BVEC>
-int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int dev, int most, cudaStream_t stream) {
+int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const Params& p, int dev, int most, cudaStream_t stream) {
   using R = Ring<CG, BN, BVEC>;
   auto kern = gemm_fp8_kernel<CG, BN, BVEC>;
   static bool configured[MAX_DEVICES];
@@ -593,7 +735,7 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int de
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, ta, tb, p) == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -400;
+  return cudaLaunchKernelEx(&cfg, kern, ta, tb, td, p) == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -400;
 }
 
 }  // namespace
@@ -653,19 +795,28 @@ int ftb_gemm_fp8(const Fp8GemmArgs* a) {
   if (tiles >= 1ll << 30) return -3;
   p.num_tiles = static_cast<int>(tiles);
 
-  CUtensorMap ta, tb;
+  p.add_in_place = p.d_fp32 && p.beta == 1.f && p.C == p.D && p.ldc == p.ldd;
+
+  CUtensorMap ta, tb, td;
   const uint64_t z = p.mode == 1 ? p.groups : 1;
-  int rc = p.a_mn ? make_map(&ta, a->A, 2, p.M, p.K, 1, a->lda, 0, 128) : make_map(&ta, a->A, 2, p.K, p.M, 1, a->lda, 0, 128);
+  int rc = p.a_mn ? make_map(&ta, a->A, 2, 1, p.M, p.K, 1, a->lda, 0, 128) : make_map(&ta, a->A, 2, 1, p.K, p.M, 1, a->lda, 0, 128);
   if (rc) return rc;
   // (a stack of one has no stride of its own)
   const uint64_t stack = z > 1 ? a->b_g : (p.b_mn ? p.K : p.N) * static_cast<uint64_t>(a->ldb);
-  rc = p.b_mn ? make_map(&tb, a->B, 3, p.N, p.K, z, a->ldb, stack, 128) : make_map(&tb, a->B, 3, p.K, p.N, z, a->ldb, stack, bn / cg);
+  rc = p.b_mn ? make_map(&tb, a->B, 3, 1, p.N, p.K, z, a->ldb, stack, 128) : make_map(&tb, a->B, 3, 1, p.K, p.N, z, a->ldb, stack, bn / cg);
   if (rc) return rc;
+  if (p.vec) {
+    const uint64_t depth = p.mode == 2 ? p.groups : 1;
+    rc = make_map(&td, p.D, 3, static_cast<int>(es), p.N, p.M, depth, p.ldd * es, depth > 1 ? p.d_g * es : p.M * static_cast<uint64_t>(p.ldd * es), 32);
+    if (rc) return rc;
+  } else {
+    td = ta;                            // (not used)
+  }
   const int sms = sm_count(dev), most = a->max_ctas > 0 && a->max_ctas < sms ? static_cast<int>(a->max_ctas) : sms;
   const bool bvec = a->sb_shift == 0;
-  if (variant == 1) return bvec ? launch<1, 128, true>(ta, tb, p, dev, most, a->stream) : launch<1, 128, false>(ta, tb, p, dev, most, a->stream);
-  if (variant == 2) return bvec ? launch<1, 256, true>(ta, tb, p, dev, most, a->stream) : launch<1, 256, false>(ta, tb, p, dev, most, a->stream);
-  return bvec ? launch<2, 256, true>(ta, tb, p, dev, most, a->stream) : launch<2, 256, false>(ta, tb, p, dev, most, a->stream);
+  if (variant == 1) return bvec ? launch<1, 128, true>(ta, tb, td, p, dev, most, a->stream) : launch<1, 128, false>(ta, tb, td, p, dev, most, a->stream);
+  if (variant == 2) return bvec ? launch<1, 256, true>(ta, tb, td, p, dev, most, a->stream) : launch<1, 256, false>(ta, tb, td, p, dev, most, a->stream);
+  return bvec ? launch<2, 256, true>(ta, tb, td, p, dev, most, a->stream) : launch<2, 256, false>(ta, tb, td, p, dev, most, a->stream);
 }
 
 // (and clears it) code * 1000 + where of a wait that ran out, 0 if none did
