@@ -43,23 +43,7 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
     f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
   }
 }
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  uint4 u;
-  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-  return u;
-}
-
 // Eight elements from column c of a row of n: 16-byte loads where the row allows them, zeros behind its end.
-__device__ __forceinline__ void load8(const bf16* row, int c, int n, bool vec, float (&f)[8]) {
-  if (vec && c + 8 <= n) {
-    unpack8(*reinterpret_cast<const uint4*>(row + c), f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = c + j < n ? __bfloat162float(row[c + j]) : 0.f;
-  }
-}
 __device__ __forceinline__ void load8(const float* row, int c, int n, bool vec, float (&f)[8]) {
   if (vec && c + 8 <= n) {
     const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
@@ -71,18 +55,62 @@ __device__ __forceinline__ void load8(const float* row, int c, int n, bool vec, 
   }
 }
 
-__device__ __forceinline__ uint32_t top8(const float (&f)[8]) {
-  uint32_t t = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) t = max(t, magnitude(f[j]));
-  return t;
+// Eight elements of a row as they came: magnitudes' maxima are taken of the bits, bf16 by pairs.
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
-// over the 16 lanes that hold one group of a row
-__device__ __forceinline__ uint32_t top16(uint32_t t) {
+template <typename T>
+struct Raw;
+template <>
+struct Raw<bf16> {
+  uint4 u;
+  static constexpr int TOPS = 4;                 // words of magnitudes: two columns each
+  __device__ __forceinline__ void load(const bf16* row, int c, int n, bool vec) {
+    if (vec && c + 8 <= n) {
+      u = *reinterpret_cast<const uint4*>(row + c);
+    } else {
+      uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
-  return t;
-}
+      for (int j = 0; j < 8; ++j)
+        if (c + j < n) w[j / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row + c + j)) << (16 * (j & 1));
+      u = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  __device__ __forceinline__ void clear() { u = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ uint32_t top(int i) const { return (i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w) & 0x7FFF7FFFu; }
+  __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max_u16x2(a, b); }
+  __device__ __forceinline__ uint32_t top() const { return max_u16x2(max_u16x2(top(0), top(1)), max_u16x2(top(2), top(3))); }
+  // the larger of a word's two, as the bits of an fp32 number
+  __device__ static __forceinline__ uint32_t single(uint32_t t) { return max(t << 16, t & 0xFFFF0000u); }
+  __device__ static __forceinline__ uint32_t column(uint32_t t, int j) { return j & 1 ? t & 0xFFFF0000u : t << 16; }
+  __device__ __forceinline__ void values(float (&f)[8]) const { unpack8(u, f); }
+};
+template <>
+struct Raw<float> {
+  float f[8];
+  static constexpr int TOPS = 8;
+  __device__ __forceinline__ void load(const float* row, int c, int n, bool vec) { load8(row, c, n, vec, f); }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 0.f;
+  }
+  __device__ __forceinline__ uint32_t top(int i) const { return magnitude(f[i]); }
+  __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t t = top(0);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) t = max(t, top(j));
+    return t;
+  }
+  __device__ static __forceinline__ uint32_t single(uint32_t t) { return t; }
+  __device__ static __forceinline__ uint32_t column(uint32_t t, int) { return t; }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = f[j];
+  }
+};
 
 struct QuantParams {
   const void* x;
@@ -97,65 +125,79 @@ struct QuantParams {
 };
 
 // One block per tile of 128 x 128: a thread holds 8 columns of 8 rows that lie 16 apart, so that a warp reads 256 bytes of two
-// rows at a time and the tile's groups are inside the block.
+// rows at a time and the tile's groups are inside the block.  The elements stay packed as they came until they are converted, so
+// that four blocks fit an SM (two for fp32).
 template <int GROUP, typename T>
-__global__ void __launch_bounds__(256) quant_kernel(const QuantParams p) {
-  __shared__ uint32_t sh[GROUP == 1 ? 16 * G : 8];
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quant_kernel(const QuantParams p) {
+  using R = Raw<T>;
+  __shared__ uint32_t sh[GROUP == 1 ? 8 * 16 * R::TOPS : 8];
+  __shared__ float sh_inv[GROUP == 1 ? G : 1];
   const long tile = blockIdx.x;
   const int tn = static_cast<int>(tile % p.tiles_n);
   const long rest = tile / p.tiles_n;
   const int tm = static_cast<int>(rest % p.tiles_m);
   const long b = rest / p.tiles_m;
-  const int l16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
   const int c = tn * G + l16 * 8;
   const T* x = static_cast<const T*>(p.x) + b * p.batch_x;
   float* scale = p.scale + b * p.batch_s;
-  float f[8][8];
+  R raw[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int row = tm * G + r0 + 16 * i;
-    if (row < p.M) {
-      load8(x + row * p.ldx, c, p.N, p.vec, f[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
-    }
+    if (row < p.M) raw[i].load(x + row * p.ldx, c, p.N, p.vec);
+    else raw[i].clear();
   }
   float inv[8];                      // of the rows (row groups) or of the columns (column groups)
   if constexpr (GROUP == 0) {
+    // The maxima of eight rows over 16 lanes: in each of three steps a lane hands over half of its rows and keeps the larger of
+    // the others, so that it ends with one row's, whose two divisions it makes for all.
+    uint32_t t[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = tm * G + r0 + 16 * i;
-      const float s = scale_of(top16(top8(f[i])));
-      inv[i] = 1.f / s;
-      if (l16 == 0 && row < p.M) scale[row * p.scale_m + tn * p.scale_n] = s;
+    for (int i = 0; i < 8; ++i) t[i] = R::single(raw[i].top());
+#pragma unroll
+    for (int h = 4; h > 0; h >>= 1) {
+      const bool up = lane & h;      // keeps the rows from h on
+#pragma unroll
+      for (int i = 0; i < h; ++i) {
+        const uint32_t mine = up ? t[i + h] : t[i], theirs = up ? t[i] : t[i + h];
+        t[i] = max(mine, __shfl_xor_sync(0xffffffffu, theirs, h));
+      }
     }
+    const uint32_t top = max(t[0], __shfl_xor_sync(0xffffffffu, t[0], 8));
+    const float s = scale_of(top), r = 1.f / s;
+    const int row = tm * G + r0 + 16 * (lane & 7);
+    if ((lane & 8) == 0 && row < p.M) scale[row * p.scale_m + tn * p.scale_n] = s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) inv[i] = __shfl_sync(0xffffffffu, r, i, 16);
   } else if constexpr (GROUP == 1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t t = 0;
+    for (int j = 0; j < R::TOPS; ++j) {
+      uint32_t t = raw[0].top(j);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t = max(t, magnitude(f[i][j]));
-      sh[r0 * G + l16 * 8 + j] = t;
+      for (int i = 1; i < 8; ++i) t = R::larger(t, raw[i].top(j));
+      t = R::larger(t, __shfl_xor_sync(0xffffffffu, t, 16));
+      if (lane < 16) sh[warp * (16 * R::TOPS) + l16 * R::TOPS + j] = t;
     }
     __syncthreads();
     if (threadIdx.x < G) {
-      uint32_t t = 0;
+      const int word = threadIdx.x * R::TOPS / 8;
+      uint32_t t = sh[word];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) t = max(t, sh[i * G + threadIdx.x]);
-      const float s = scale_of(t);
+      for (int i = 1; i < 8; ++i) t = R::larger(t, sh[i * (16 * R::TOPS) + word]);
+      const float s = scale_of(R::column(t, threadIdx.x));
       if (tn * G + threadIdx.x < p.N) scale[tm * p.scale_m + (tn * G + threadIdx.x) * p.scale_n] = s;
-      sh[threadIdx.x] = __float_as_uint(1.f / s);     // (row 0 of the column's maxima: read by this thread only)
+      sh_inv[threadIdx.x] = 1.f / s;
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) inv[j] = __uint_as_float(sh[l16 * 8 + j]);
+    for (int j = 0; j < 8; ++j) inv[j] = sh_inv[l16 * 8 + j];
   } else {
-    uint32_t t = 0;
+    uint32_t t = raw[0].top();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t = max(t, top8(f[i]));
-    t = __reduce_max_sync(0xffffffffu, t);
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = t;
+    for (int i = 1; i < 8; ++i) t = R::larger(t, raw[i].top());
+    t = __reduce_max_sync(0xffffffffu, R::single(t));
+    if (lane == 0) sh[warp] = t;
     __syncthreads();
     t = sh[0];
 #pragma unroll
@@ -170,19 +212,22 @@ __global__ void __launch_bounds__(256) quant_kernel(const QuantParams p) {
   for (int i = 0; i < 8; ++i) {
     const int row = tm * G + r0 + 16 * i;
     if (row >= p.M) break;
+    float f[8];
+    raw[i].values(f);
     uint2 o;
     if constexpr (GROUP == 1)
-      o = make_uint2(e4m3x4(f[i][0] * inv[0], f[i][1] * inv[1], f[i][2] * inv[2], f[i][3] * inv[3]),
-                     e4m3x4(f[i][4] * inv[4], f[i][5] * inv[5], f[i][6] * inv[6], f[i][7] * inv[7]));
+      o = make_uint2(e4m3x4(f[0] * inv[0], f[1] * inv[1], f[2] * inv[2], f[3] * inv[3]),
+                     e4m3x4(f[4] * inv[4], f[5] * inv[5], f[6] * inv[6], f[7] * inv[7]));
     else
-      o = e4m3x8(f[i], inv[GROUP == 0 ? i : 0]);
+      o = e4m3x8(f, inv[GROUP == 0 ? i : 0]);
     *reinterpret_cast<uint2*>(q + row * p.ldq + c) = o;
   }
 }
 
 // ------------------------------------------------------------------------------------------------ RMSNorm
 //   h = bf16(x + residual),   r = 1 / sqrt(mean h^2 + eps),   y = h r w,   y in row groups of 8 bits
-// The norm is of the rounded h, which is what the backward pass reads.
+// The norm is of the rounded h, which is what the backward pass reads.  r is common to a row, so it goes into the factor that a
+// group is converted with: q = e4m3((h w) (r / s)), s = max(r max |h w| / 448, 2^-126).
 struct NormParams {
   const bf16* x;
   long ldx;
@@ -201,40 +246,115 @@ struct NormParams {
   int vec_w;
 };
 
-__device__ __forceinline__ void norm_input(const NormParams& p, long row, int c, float (&f)[8]) {
-  load8(p.x + row * p.ldx, c, p.D, p.vec, f);
-  if (p.res == nullptr) return;
-  float r[8];
-  load8(p.res + row * p.ldr, c, p.D, p.vec, r);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] += r[j];
-  const uint4 u = pack8(f);
-  unpack8(u, f);
-  bf16* h = p.h + row * p.D + c;
-  if (p.vec && c + 8 <= p.D) {
-    *reinterpret_cast<uint4*>(h) = u;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < p.D) h[j] = __float2bfloat16_rn(f[j]);
-  }
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
-// (y of eight elements, its group's scale, and their 8 bits)
-__device__ __forceinline__ void norm_output(const NormParams& p, long row, int c, float (&f)[8], float r) {
-  if (p.w != nullptr) {
-    float w[8];
-    load8(p.w, c, p.D, p.vec_w, w);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = f[j] * r * w[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] *= r;
-  }
-  const float s = scale_of(top16(top8(f)));
-  if ((threadIdx.x & 15) == 0 && c < p.D) p.scale[row + (c >> 7) * p.scale_n] = s;
-  if (c < p.ldq) *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = e4m3x8(f, 1.f / s);
+__device__ __forceinline__ void unpack2(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 widen(uint32_t w) { return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+// the largest magnitude; NaN if one is
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
 }
 
+// Eight elements of x and the residual as they came
+struct NormIn {
+  Raw<bf16> x, r;
+  __device__ __forceinline__ void load(const NormParams& p, long row, int c) {
+    x.load(p.x + row * p.ldx, c, p.D, p.vec);
+    if (p.res != nullptr) r.load(p.res + row * p.ldr, c, p.D, p.vec);
+  }
+};
+// h of them, written where there is a residual; adds the squares
+__device__ __forceinline__ uint4 norm_h(const NormParams& p, const NormIn& in, long row, int c, f32x2& ss) {
+  uint4 h = in.x.u;
+  if (p.res != nullptr) {
+    const uint32_t xs[4] = {h.x, h.y, h.z, h.w}, rs[4] = {in.r.u.x, in.r.u.y, in.r.u.z, in.r.u.w};
+    uint32_t hs[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      unpack2(add2(widen(xs[i]), widen(rs[i])), a, b);
+      const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+      hs[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    h = make_uint4(hs[0], hs[1], hs[2], hs[3]);
+    uint16_t* to = reinterpret_cast<uint16_t*>(p.h) + row * p.D + c;
+    if (p.vec && c + 8 <= p.D) {
+      *reinterpret_cast<uint4*>(to) = h;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < p.D) to[j] = static_cast<uint16_t>(hs[j / 2] >> (16 * (j & 1)));
+    }
+  }
+  const uint32_t hs[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x2 v = widen(hs[i]);
+    ss = fma2(v, v, ss);
+  }
+  return h;
+}
+// 8 bits of eight elements, and their group's scale.  The group's two divisions by numbers that are not exact anyway are a
+// multiplication and an approximate reciprocal (off by 2^-23): q and s fit together to that.
+__device__ __forceinline__ void norm_q(const NormParams& p, const uint4& h, const f32x2 (&w)[4], long row, int c, float r) {
+  const uint32_t hs[4] = {h.x, h.y, h.z, h.w};
+  f32x2 t[4];
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t[i] = mul2(widen(hs[i]), w[i]);
+    float a, b;
+    unpack2(t[i], a, b);
+    top = max_abs(max_abs(top, a), b);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));     // the 16 lanes of a group
+  float s = top * r * (1.f / 448.f);
+  s = s < 1.17549435e-38f ? 1.17549435e-38f : s;
+  float inv;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  if ((threadIdx.x & 15) == 0 && c < p.D) p.scale[row + (c >> 7) * p.scale_n] = s;
+  float factor = r * inv;
+  if (!(factor <= 3.402823466e38f)) {                // (groups of next to nothing, and rows that are not numbers)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = mul2(t[i], pack2(r, r));
+    factor = inv;
+  }
+  const f32x2 k = pack2(factor, factor);
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack2(mul2(t[i], k), f[2 * i], f[2 * i + 1]);
+  if (c < p.ldq) *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = make_uint2(e4m3x4(f[0], f[1], f[2], f[3]), e4m3x4(f[4], f[5], f[6], f[7]));
+}
+__device__ __forceinline__ void norm_gain(const NormParams& p, int c, f32x2 (&w)[4]) {
+  float f[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+  if (p.w != nullptr) load8(p.w, c, p.D, p.vec_w, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack2(f[2 * i], f[2 * i + 1]);
+}
+
+// (sh: a piece that the last call did not use)
 template <int NT>
 __device__ __forceinline__ float block_sum(float v, float* sh) {
 #pragma unroll
@@ -244,46 +364,77 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
   v = 0.f;
 #pragma unroll
   for (int i = 0; i < NT / 32; ++i) v += sh[i];
-  __syncthreads();
   return v;
 }
 
-// V > 0: a block of NT threads holds a row of up to 8 NT V elements in registers.  V = 0: longer rows are read twice (the
-// second time h comes from what the first pass wrote, by the same thread).
+constexpr int NORM_THREADS = 768;    // of an SM: blocks of NT threads
+
+// V > 0: a block of NT threads walks over rows of up to 8 NT V elements, its part of the gain in registers, the next row's
+// elements asked for before the current row's sum is known.  V = 0: longer rows are read twice (the second time h comes from what
+// the first pass wrote, by the same thread).
 template <int NT, int V>
-__global__ void __launch_bounds__(NT) rmsnorm_fp8_kernel(const NormParams p) {
-  __shared__ float sh[NT / 32];
-  const long row = blockIdx.x;
-  float ss = 0.f;
+__global__ void __launch_bounds__(NT, NORM_THREADS / NT) rmsnorm_fp8_kernel(const NormParams p) {
+  __shared__ float sh[2][NT / 32];
   const float rD = 1.f / static_cast<float>(p.D);
+  int turn = 0;
+  auto rstd_of = [&](f32x2 ss, long row) {
+    float a, b;
+    unpack2(ss, a, b);
+    const float r = rsqrtf(block_sum<NT>(a + b, sh[turn]) * rD + p.eps);
+    turn ^= 1;
+    if (threadIdx.x == 0) p.rstd[row] = r;
+    return r;
+  };
   if constexpr (V > 0) {
-    float f[V][8];
+    f32x2 w[V][4];
+    NormIn in[V];
+    long row = blockIdx.x;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      norm_input(p, row, (threadIdx.x + i * NT) * 8, f[i]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss += f[i][j] * f[i][j];
+      in[i].load(p, row, (threadIdx.x + i * NT) * 8);
+      norm_gain(p, (threadIdx.x + i * NT) * 8, w[i]);
     }
-    const float r = rsqrtf(block_sum<NT>(ss, sh) * rD + p.eps);
-    if (threadIdx.x == 0) p.rstd[row] = r;
+    while (true) {
+      uint4 h[V];
+      f32x2 ss = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) norm_output(p, row, (threadIdx.x + i * NT) * 8, f[i], r);
+      for (int i = 0; i < V; ++i) h[i] = norm_h(p, in[i], row, (threadIdx.x + i * NT) * 8, ss);
+      const long next = row + gridDim.x;
+      if (next < p.T) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) in[i].load(p, next, (threadIdx.x + i * NT) * 8);
+      }
+      const float r = rstd_of(ss, row);
+#pragma unroll
+      for (int i = 0; i < V; ++i) norm_q(p, h[i], w[i], row, (threadIdx.x + i * NT) * 8, r);
+      if (next >= p.T) break;
+      row = next;
+    }
   } else {
-    float f[8];
-    for (int c0 = 0; c0 < p.D; c0 += 8 * NT) {
-      norm_input(p, row, c0 + threadIdx.x * 8, f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
-    }
-    const float r = rsqrtf(block_sum<NT>(ss, sh) * rD + p.eps);
-    if (threadIdx.x == 0) p.rstd[row] = r;
-    for (int c0 = 0; c0 < p.D; c0 += 8 * NT) {
-      const int c = c0 + threadIdx.x * 8;
-      if (p.res != nullptr) load8(p.h + row * p.D, c, p.D, p.vec, f);
-      else load8(p.x + row * p.ldx, c, p.D, p.vec, f);
-      norm_output(p, row, c, f, r);
+    NormIn in;
+    for (long row = blockIdx.x; row < p.T; row += gridDim.x) {
+      f32x2 ss = 0, w[4];
+      for (int c0 = 0; c0 < p.D; c0 += 8 * NT) {
+        in.load(p, row, c0 + threadIdx.x * 8);
+        norm_h(p, in, row, c0 + threadIdx.x * 8, ss);
+      }
+      const float r = rstd_of(ss, row);
+      for (int c0 = 0; c0 < p.D; c0 += 8 * NT) {
+        const int c = c0 + threadIdx.x * 8;
+        if (p.res != nullptr) in.x.load(p.h + row * p.D, c, p.D, p.vec);
+        else in.x.load(p.x + row * p.ldx, c, p.D, p.vec);
+        norm_gain(p, c, w);
+        norm_q(p, in.x.u, w, row, c, r);
+      }
     }
   }
+}
+
+template <int NT, int V>
+int launch_norm(const NormParams& p, cudaStream_t stream) {
+  const int most = 148 * (NORM_THREADS / NT);
+  rmsnorm_fp8_kernel<NT, V><<<p.T < most ? p.T : most, NT, 0, stream>>>(p);
+  return cudaGetLastError() == cudaSuccess ? 0 : -400;
 }
 
 template <typename T>
@@ -354,15 +505,11 @@ int ftb_rmsnorm_fp8_fwd(const NormArgs* a) {
   auto rows16 = [&](const void* t, long ld) { return (reinterpret_cast<uintptr_t>(t) & 15) == 0 && (a->T == 1 || (ld & 7) == 0); };
   p.vec = rows16(a->x, a->ldx) && (a->res == nullptr || (rows16(a->res, a->ldr) && rows16(a->h, a->D)));
   p.vec_w = (reinterpret_cast<uintptr_t>(a->w) & 15) == 0;
-  const unsigned grid = static_cast<unsigned>(a->T);
-  const int D = p.D;
-  cudaStream_t stream = a->stream;
-  if (D <= 1024) rmsnorm_fp8_kernel<128, 1><<<grid, 128, 0, stream>>>(p);
-  else if (D <= 2048) rmsnorm_fp8_kernel<128, 2><<<grid, 128, 0, stream>>>(p);
-  else if (D <= 4096) rmsnorm_fp8_kernel<256, 2><<<grid, 256, 0, stream>>>(p);
-  else if (D <= 8192) rmsnorm_fp8_kernel<256, 4><<<grid, 256, 0, stream>>>(p);
-  else rmsnorm_fp8_kernel<256, 0><<<grid, 256, 0, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -400;
+  if (p.D <= 1024) return launch_norm<128, 1>(p, a->stream);
+  if (p.D <= 2048) return launch_norm<256, 1>(p, a->stream);
+  if (p.D <= 4096) return launch_norm<256, 2>(p, a->stream);
+  if (p.D <= 8192) return launch_norm<512, 2>(p, a->stream);
+  return launch_norm<256, 0>(p, a->stream);
 }
 
 }  // extern "C"

@@ -59,6 +59,17 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 " FTB_R16 ", [%16];" : FTB_OUT16(r) : "r"(taddr) : "memory");
 }
+// sum += v * f * a on pairs of fp32 in two instructions
+__device__ __forceinline__ void mul_add2(float* sum, const uint32_t* v, float2 f, float a) {
+  unsigned long long x, y, z, w;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "r"(v[0]), "r"(v[1]));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(f.x), "f"(f.y));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(w) : "f"(a));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(z) : "f"(sum[0]), "f"(sum[1]));
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(y));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(z) : "l"(x), "l"(w));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(sum[0]), "=f"(sum[1]) : "l"(z));
+}
 // a row of 16 columns for each thread
 __device__ __forceinline__ void tmem_ld_row16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 " FTB_R16 ", [%16];" : FTB_OUT16(r) : "r"(taddr) : "memory");
@@ -598,12 +609,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float* to = &sum[q * 16 + 4 * j + 2 * e];
-                const uint32_t* v = &r[q & 1][4 * j + 2 * e];
-                to[0] = fmaf(__uint_as_float(v[0]) * f[j].x, a[2 * (q & 1) + e], to[0]);
-                to[1] = fmaf(__uint_as_float(v[1]) * f[j].y, a[2 * (q & 1) + e], to[1]);
-              }
+              for (int e = 0; e < 2; ++e) mul_add2(&sum[q * 16 + 4 * j + 2 * e], &r[q & 1][4 * j + 2 * e], f[j], a[2 * (q & 1) + e]);
             if (q + 1 < CHUNKS) tmem_ld_wait();
             if (q + 2 == CHUNKS) release();
           }
