@@ -14,6 +14,9 @@
 //              (a thread's 128 sums, and 32 values on the way, need more than the 168 registers of 384 threads: the first four
 //              warps give theirs up)
 //
+// SPLIT: products with few tiles.  A cluster of up to eight CTAs takes one tile, a range of the reduction each; the parts are added
+// through the cluster's shared memory, in the order of the ranges, so that results do not depend on who comes first.
+//
 // CG = 2: a pair of SMs works on 256 x BN (each CTA 128 rows, half of B).  Grouped forms take their row or reduction ranges
 // from device offsets.  Every wait is bounded.
 #include <mutex>
@@ -110,6 +113,7 @@ struct Params {
   long d_g;                          // mode 2: elements between the groups' results
   int total;                         // rows that the offsets run over
   int tiles_m, tiles_n, num_tiles, k_blocks;
+  int split_blocks;                  // SPLIT: blocks of a CTA's range (the last one's may be shorter)
 };
 
 struct Tile {
@@ -355,13 +359,24 @@ __device__ __forceinline__ void store_tile(const Params& p, const float (&sum)[N
   }
 }
 
-template <int CG, int BN, bool BVEC>
+// A CTA's part of a tile of 128 x 128 fp32 sums in its shared memory: 16-byte pieces turned over by the row's number.
+__device__ __forceinline__ uint32_t part_offset(int row, int piece) { return row * 512 + ((piece ^ (row & 31)) << 4); }
+__device__ __forceinline__ float4 ld_cluster(uint32_t local, int rank) {
+  uint32_t at;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+template <int CG, int BN, bool BVEC, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmD,
                 const Params p) {
   using R = Ring<CG, BN, BVEC>;
   using W = Walk<BM * CG, 16 / CG>;
   constexpr int ST = R::STAGES, NACC = R::NACC, HALF = BN / 2;
+  static_assert(!SPLIT || (CG == 1 && BN == 128 && ST * R::STAGE >= 128 * 512), "the parts lie where the stages were");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smem_epi = smem + ST * R::STAGE;
@@ -375,7 +390,18 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = CG == 2 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  uint32_t ranges = 1;
+  if constexpr (SPLIT) asm volatile("mov.u32 %0, %cluster_nctaid.x;" : "=r"(ranges));
+  const int range = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
+  const int first = SPLIT ? blockIdx.x / ranges : blockIdx.x / CG, step = SPLIT ? p.num_tiles : gridDim.x / CG;
+  auto locate = [&](W& walk, int tile, Tile& t) {
+    if (!walk.at(p, tile, t)) return false;
+    if constexpr (SPLIT) {
+      t.kb0 = range * p.split_blocks;
+      t.kbs = min(p.split_blocks, p.k_blocks - t.kb0);
+    }
+    return true;
+  };
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -405,7 +431,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       W walk;
       Tile t;
       for (int tile = first; tile < p.num_tiles && ok; tile += step) {
-        if (!walk.at(p, tile, t)) break;
+        if (!locate(walk, tile, t)) break;
         const int row0 = t.row0 + cta * BM;
         const int col0 = t.tn * BN + cta * (BN / CG);
         const int z = p.mode == 1 ? t.g : 0;
@@ -458,7 +484,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       W walk;
       Tile t;
       for (int tile = first; tile < p.num_tiles && ok; tile += step) {
-        if (!walk.at(p, tile, t)) break;
+        if (!locate(walk, tile, t)) break;
         for (int kb = 0; kb < t.kbs; ++kb) {
           const bool e = mbar_try_wait(&tempty[acc], acc_phase ^ 1), f = mbar_try_wait(&full_bar[stage], phase);
           if (!e && !(ok = mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, 20))) break;
@@ -485,7 +511,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     uint8_t* buf = smem_epi + (warp - EPI_FIRST) * (C_BUFS * PIECE_BYTES);
     [[maybe_unused]] float* slots = reinterpret_cast<float*>(smem_slots) + (warp - EPI_FIRST) * (SLOTS * R::SLOT);
     const int in_tile = cta * BM + quad * 32, es = p.d_fp32 ? 4 : 2;
-    const bool add = p.beta != 0.f && !p.add_in_place;
+    const bool add = !SPLIT && p.beta != 0.f && !p.add_in_place;
     uint64_t *tfull = tfull_bar + part * NACC, *tempty = tempty_bar + part * NACC;
     const uint32_t tmem_part = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + part * NACC * HALF;
     int acc = 0;
@@ -524,7 +550,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     // the tile's place and the scales of its first blocks; -1 behind the last tile
     auto begin = [&](int tile) {
       do {
-        if (tile >= p.num_tiles || !walk.at(p, tile, t)) return -1;
+        if (tile >= p.num_tiles || !locate(walk, tile, t)) return -1;
         if (t.kbs > 0) break;                            // (a group without rows leaves its result as it is)
         tile += step;
       } while (true);
@@ -645,7 +671,18 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       __syncwarp();                                      // (all lanes have read the last slot)
       const Patch w = patch();
       tile = begin(tile + step);
-      if (w.cols > 0) {
+      if constexpr (SPLIT) {
+        // (every load and product of this CTA is done: the stages are free)
+#pragma unroll
+        for (int i = 0; i < HALF; i += BVEC ? 2 : 4) {
+          const int c = BVEC ? i / 32 * 32 + i % 16 / 4 * 8 + 2 * (lane & 3) : i;       // of the half
+          const int r = quad * 32 + (BVEC ? i / 16 % 2 * 16 + i / 2 % 2 * 8 + (lane >> 2) : lane), col = part * HALF + c;
+          if (r - quad * 32 >= w.rows) continue;
+          uint8_t* to = smem + part_offset(r, col / 4) + col % 4 * 4;
+          if constexpr (BVEC) *reinterpret_cast<float2*>(to) = make_float2(sum[i], sum[i + 1]);
+          else *reinterpret_cast<float4*>(to) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+        }
+      } else if (w.cols > 0) {
         const float* bias = p.bias == nullptr ? nullptr : p.bias + col0;
         // a patch whose last rows are not its own, but another group's, is stored row by row
         const CUtensorMap* map = p.vec && (rows == 32 || p.mode != 1) ? &tmD : nullptr;
@@ -664,6 +701,54 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 
   __syncwarp();
   tc_fence_before();
+  if constexpr (SPLIT) {
+    cluster_sync_all();
+    W walk;
+    Tile t;
+    if (warp >= EPI_FIRST && walk.at(p, first, t)) {
+      // this CTA's share of the columns: pieces of four, the ranges' parts added in their order
+      const int share = 32 / ranges, rows = min(BM, t.left);
+      for (int i = threadIdx.x - 32 * EPI_FIRST; i < rows * share; i += 32 * EPI_WARPS) {
+        const int r = i / share, piece = range * share + i % share, col = t.tn * BN + 4 * piece;
+        if (col >= p.N) continue;
+        const uint32_t at = smem_u32(smem) + part_offset(r, piece);
+        float4 v = ld_cluster(at, 0);
+        for (uint32_t k = 1; k < ranges; ++k) {
+          const float4 u = ld_cluster(at, k);
+          v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+        }
+        float f[4] = {v.x * p.alpha, v.y * p.alpha, v.z * p.alpha, v.w * p.alpha};
+        const long row = t.row0 + r;
+        float* d32 = static_cast<float*>(p.D) + row * p.ldd + col;
+        __nv_bfloat16* d16 = static_cast<__nv_bfloat16*>(p.D) + row * p.ldd + col;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (col + j >= p.N) break;
+          if (p.bias != nullptr) f[j] += p.bias[col + j];
+          if (p.beta != 0.f)
+            f[j] += p.beta * (p.d_fp32 ? static_cast<const float*>(p.C)[row * p.ldc + col + j]
+                                       : __bfloat162float(static_cast<const __nv_bfloat16*>(p.C)[row * p.ldc + col + j]));
+        }
+        if (p.vec) {                                     // (N is a multiple of four then)
+          if (p.d_fp32) {
+            *reinterpret_cast<float4*>(d32) = make_float4(f[0], f[1], f[2], f[3]);
+          } else {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(f[0], f[1]), hi = __floats2bfloat162_rn(f[2], f[3]);
+            *reinterpret_cast<uint2*>(d16) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (col + j >= p.N) break;
+            if (p.d_fp32) d32[j] = f[j];
+            else d16[j] = __float2bfloat16_rn(f[j]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();                                  // nobody leaves while its part is read
+  }
   __syncthreads();
   if constexpr (CG == 2) cluster_sync_all();             // the leader's MMAs also write the peer's tensor memory
   if (warp == 1) {
@@ -716,10 +801,10 @@ int sm_count(int dev) {
   return counts[dev];
 }
 
-template <int CG, int BN, bool BVEC>
-int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const Params& p, int dev, int most, cudaStream_t stream) {
+template <int CG, int BN, bool BVEC, bool SPLIT = false>
+int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const Params& p, int dev, int most, cudaStream_t stream, int ranges = 1) {
   using R = Ring<CG, BN, BVEC>;
-  auto kern = gemm_fp8_kernel<CG, BN, BVEC>;
+  auto kern = gemm_fp8_kernel<CG, BN, BVEC, SPLIT>;
   static bool configured[MAX_DEVICES];
   if (!configured[dev]) {
     // the warps that ask for registers get them out of the 168 that the others were launched with
@@ -731,13 +816,13 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, 
   const int sms = most < CG ? CG : most / CG * CG;
   const long want = static_cast<long>(p.num_tiles) * CG;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(want < sms ? want : sms));
+  cfg.gridDim = dim3(static_cast<unsigned>(SPLIT ? want * ranges : want < sms ? want : sms));
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = R::TOTAL;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.x = SPLIT ? ranges : CG;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
@@ -820,6 +905,16 @@ int ftb_gemm_fp8(const Fp8GemmArgs* a) {
   }
   const int sms = sm_count(dev), most = a->max_ctas > 0 && a->max_ctas < sms ? static_cast<int>(a->max_ctas) : sms;
   const bool bvec = a->sb_shift == 0;
+  if (variant == 1 && p.mode == 0) {
+    // As many ranges (a power of two) as there are SMs for, each of two blocks at least, none of them empty.
+    int ranges = 8;
+    while (ranges > 1 && (tiles * ranges > most || p.k_blocks < 2 * ranges || (ranges - 1) * ((p.k_blocks + ranges - 1) / ranges) >= p.k_blocks))
+      ranges /= 2;
+    p.split_blocks = (p.k_blocks + ranges - 1) / ranges;
+    if (ranges > 1)
+      return bvec ? launch<1, 128, true, true>(ta, tb, td, p, dev, most, a->stream, ranges)
+                  : launch<1, 128, false, true>(ta, tb, td, p, dev, most, a->stream, ranges);
+  }
   if (variant == 1) return bvec ? launch<1, 128, true>(ta, tb, td, p, dev, most, a->stream) : launch<1, 128, false>(ta, tb, td, p, dev, most, a->stream);
   if (variant == 2) return bvec ? launch<1, 256, true>(ta, tb, td, p, dev, most, a->stream) : launch<1, 256, false>(ta, tb, td, p, dev, most, a->stream);
   return bvec ? launch<2, 256, true>(ta, tb, td, p, dev, most, a->stream) : launch<2, 256, false>(ta, tb, td, p, dev, most, a->stream);

@@ -18,15 +18,19 @@ path.  The scales of two operands are multiplied in fp32, so the product of a pa
 from __future__ import annotations
 
 import ctypes
+import struct
+import sys
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import reference as ref
 
-FP8 = torch.float8_e4m3fn
+_ops = sys.modules[__package__]
+
+FP8, F32, BF16 = torch.float8_e4m3fn, torch.float32, torch.bfloat16
 _GROUPS = ("row", "col", "block")
-_addresses: dict = {}
+_entries: dict = {}
 
 
 class Fp8Matrix(NamedTuple):
@@ -36,49 +40,36 @@ class Fp8Matrix(NamedTuple):
     group: str
 
 
-def _entry(lib: str, name: str) -> int:
-    """Address of a library's entry point that takes its arguments in 8 bytes each."""
-    at = _addresses.get(name)
-    if at is None:
-        from . import cuda
-        at = _addresses[name] = ctypes.cast(getattr(cuda.load(lib), name), ctypes.c_void_p).value
-    return at
-
-
-def _call(lib: str, name: str, *args) -> None:
+def _entry(lib: str, name: str):
+    """A library's entry point that takes its arguments in 8 bytes each, as a function of them."""
     from . import cuda
+    address = ctypes.cast(getattr(cuda.load(lib), name), ctypes.c_void_p).value
     fast = cuda.fastcall()
     if fast is not None:
-        rc = fast.call(_entry(lib, name), *args)
+        return lambda *args, call=fast.call: call(address, *args)
+    entry, bits = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)(address), struct.Struct("d")
+    word = lambda a: 0 if a is None else int.from_bytes(bits.pack(a), "little", signed=True) if isinstance(a, float) else a
+    return lambda *args: entry(ctypes.addressof((ctypes.c_int64 * len(args))(*map(word, args))))
+
+
+def _launch(family: str, index: int, lib: str, name: str, *args) -> None:
+    """One call of a library's entry point on the device of its tensors, on the stream that is current there."""
+    entry = _entries.get(name)
+    if entry is None:
+        entry = _entries[name] = _entry(lib, name)
+    before = torch._C._cuda_getDevice()
+    if before == index:
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        import struct
-        packed = [0 if a is None else struct.unpack("q", struct.pack("d", a))[0] if isinstance(a, float) else a for a in args]
-        rc = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)(_entry(lib, name))(ctypes.addressof((ctypes.c_int64 * len(args))(*packed)))
+        torch._C._cuda_setDevice(index)
+        try:
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+        finally:
+            torch._C._cuda_setDevice(before)
     if rc != 0:
         raise RuntimeError(f"{name} failed with code {rc}")
-
-
-class _On:
-    """The device of ``t`` as the current one, its stream with it."""
-
-    def __init__(self, t):
-        self.index = t.device.index
-
-    def __enter__(self):
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.index:
-            torch._C._cuda_setDevice(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch._C._cuda_setDevice(self.before)
-
-
-def _ran(family: str, launches: int = 1) -> None:
-    from . import _count, _used
-    _count(launches)
-    _used(family, "ftb")
+    _ops._count()
+    _ops._used(family, "ftb")
 
 
 def _rows(t):
@@ -89,9 +80,9 @@ def _rows(t):
 def _empty_q(shape, device):
     """e4m3 room for ``shape`` with rows on 16 bytes, as the products read them; the pieces behind a row's end hold nothing."""
     n = shape[-1]
-    ld = (n + 15) // 16 * 16
-    buf = torch.empty(*shape[:-1], ld, dtype=FP8, device=device)
-    return buf if ld == n else buf[..., :n]
+    if n % 16 == 0:
+        return torch.empty(shape, dtype=FP8, device=device)
+    return torch.empty(*shape[:-1], (n + 15) // 16 * 16, dtype=FP8, device=device)[..., :n]
 
 
 # --------------------------------------------------------------------------------------- quantisers
@@ -110,17 +101,15 @@ def quant_fp8(x: torch.Tensor, group: str = "row") -> Fp8Matrix:
     q = _empty_q(x.shape, x.device)
     m, n = (M + 127) // 128, (N + 127) // 128
     if group == "row":
-        scale = torch.empty(n, M, dtype=torch.float32, device=x.device).t()       # a group's scales of neighbouring rows together
+        scale = torch.empty_strided((M, n), (1, M), dtype=F32, device=x.device)   # a group's scales of neighbouring rows together
     else:
         scale = torch.empty(*x.shape[:-2], m, N if group == "col" else n, dtype=torch.float32, device=x.device)
     if x.numel() == 0:
         return Fp8Matrix(q, scale.fill_(ref.FP8_FLOOR), group)
     E = x.shape[0] if x.dim() == 3 else 1
     batch = (lambda t: t.stride(0) if x.dim() == 3 else 0)
-    with _On(x) as stream:
-        _call("fp8", "ftb_quant_fp8", x.data_ptr(), q.data_ptr(), scale.data_ptr(), x.dtype == torch.float32, x.stride(-2), batch(x),
-              q.stride(-2), batch(q), scale.stride(-2), scale.stride(-1), batch(scale), E, M, N, _GROUPS.index(group), stream)
-    _ran("quant_fp8")
+    _launch("quant_fp8", x.get_device(), "fp8", "ftb_quant_fp8", x.data_ptr(), q.data_ptr(), scale.data_ptr(), x.dtype == F32, x.stride(-2),
+            batch(x), q.stride(-2), batch(q), scale.stride(-2), scale.stride(-1), batch(scale), E, M, N, _GROUPS.index(group))
     return Fp8Matrix(q, scale, group)
 
 
@@ -145,64 +134,65 @@ def rmsnorm_fp8_fwd(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, *, r
         q, scale, rstd, h = ref.rmsnorm_fp8_fwd(x, w, eps, residual)
         return Fp8Matrix(q, scale, "row"), rstd, h
     T, D = x.shape
-    x, residual = _rows(x), None if residual is None else _rows(residual)
-    w = None if w is None else w.to(torch.float32).contiguous()
-    q = _empty_q((T, D), x.device)
-    scale = torch.empty((D + 127) // 128, T, dtype=torch.float32, device=x.device)
-    rstd = torch.empty(T, dtype=torch.float32, device=x.device)
-    h = x if residual is None else torch.empty(T, D, dtype=x.dtype, device=x.device)
+    device, h = x.device, x
+    x = _rows(x)
+    if w is not None and (w.dtype is not F32 or not w.is_contiguous()):
+        w = w.to(F32).contiguous()
+    q = _empty_q((T, D), device)
+    scale = torch.empty_strided((T, (D + 127) // 128), (1, T), dtype=F32, device=device)
+    rstd = torch.empty(T, dtype=F32, device=device)
+    if residual is not None:
+        residual = _rows(residual)
+        h = torch.empty(T, D, dtype=x.dtype, device=device)
     if D == 0:
-        return Fp8Matrix(q, scale.t(), "row"), rstd.fill_(eps ** -0.5), h
+        return Fp8Matrix(q, scale, "row"), rstd.fill_(eps ** -0.5), h
     if T:
-        with _On(x) as stream:
-            _call("fp8", "ftb_rmsnorm_fp8_fwd", x.data_ptr(), None if residual is None else residual.data_ptr(),
-                  None if w is None else w.data_ptr(), q.data_ptr(), scale.data_ptr(), rstd.data_ptr(),
-                  None if residual is None else h.data_ptr(), x.stride(0), 0 if residual is None else residual.stride(0), q.stride(0),
-                  scale.stride(0), T, D, float(eps), stream)
-        _ran("rmsnorm_fp8_fwd")
-    return Fp8Matrix(q, scale.t(), "row"), rstd, h
+        r = (None, None, 0) if residual is None else (residual.data_ptr(), h.data_ptr(), residual.stride(0))
+        _launch("rmsnorm_fp8_fwd", x.get_device(), "fp8", "ftb_rmsnorm_fp8_fwd", x.data_ptr(), r[0], None if w is None else w.data_ptr(),
+                q.data_ptr(), scale.data_ptr(), rstd.data_ptr(), r[1], x.stride(0), r[2], q.stride(0), T, T, D, float(eps))
+    return Fp8Matrix(q, scale, "row"), rstd, h
 
 
 # ----------------------------------------------------------------------------------------- products
 def _check(m, what: str, stacked: bool = False) -> None:
     """That ``m`` is a matrix in 8 bits whose parts fit together."""
     q, s, group = m
-    down, along = ref.FP8_GROUPS.get(group, (0, 0))
-    if not down or q.dtype != FP8 or s.dtype != torch.float32 or q.device != s.device or q.dim() not in (2, 3) or \
-            s.shape != (*q.shape[:-2], (q.shape[-2] + down - 1) // down, (q.shape[-1] + along - 1) // along):
-        raise ValueError(f"{what}: data {tuple(q.shape)} {q.dtype} on {q.device}, scale {tuple(s.shape)} {s.dtype} on {s.device}, "
-                         f"group {group!r}")
-    if stacked != (q.dim() == 3):
-        raise ValueError(f"{what}: data {tuple(q.shape)}, a {'stack of matrices' if stacked else 'matrix'} is read here")
+    if q.dtype is FP8 and s.dtype is F32 and q.dim() == s.dim() == (3 if stacked else 2) and group in _GROUPS and q.get_device() == s.get_device():
+        *b, M, N = q.shape
+        *c, m, n = s.shape
+        if (m == M if group == "row" else m == (M + 127) >> 7) and (n == N if group == "col" else n == (N + 127) >> 7) and b == c:
+            return
+    raise ValueError(f"{what}: {'a stack of matrices' if stacked else 'a matrix'} in 8 bits is read here; data {tuple(q.shape)} {q.dtype} on "
+                     f"{q.device}, scale {tuple(s.shape)} {s.dtype} on {s.device}, group {group!r}")
 
 
 def _along(m, trans: bool, what: str):
     """``(step of a row or column of the product, step of a block of the reduction, shift)`` of an operand's scale.  ``trans``: the
     reduction runs down the data's columns."""
-    if m.group not in (("col", "block") if trans else ("row", "block")):
+    if m[2] != "block" and m[2] != ("col" if trans else "row"):
         raise ValueError(f"{what}: groups {m.group!r}, and the reduction runs {'down the columns' if trans else 'along the rows'}")
-    shift = 7 if m.group == "block" else 0
-    s = m.scale
-    return (s.stride(-1), s.stride(-2), shift) if trans else (s.stride(-2), s.stride(-1), shift)
+    st = m[1].stride()
+    return (st[-1], st[-2], 7 if m[2] == "block" else 0) if trans else (st[-2], st[-1], 7 if m[2] == "block" else 0)
 
 
 def _on_grid(q):
     """Data as the tensor maps describe it: rows contiguous, everything on 16 bytes; copied where it lies otherwise."""
-    if q.data_ptr() % 16 == 0 and (q.shape[-1] == 1 or q.stride(-1) == 1) and (q.stride(-2) % 16 == 0 and q.stride(-2) >= q.shape[-1]) \
-            and (q.dim() == 2 or (q.stride(0) % 16 == 0 and q.stride(0) > 0)):
+    st = q.stride()
+    if not q.data_ptr() & 15 and not st[-2] & 15 and st[-2] >= q.shape[-1] and (st[-1] == 1 or q.shape[-1] == 1) and \
+            (len(st) == 2 or (st[0] > 0 and not st[0] & 15)):
         return q
     buf = _empty_q(q.shape, q.device)
     buf.view(torch.uint8).copy_(q.view(torch.uint8))
     return buf
 
 
-def _result(out, shape, dtype, like, what: str):
+def _result(out, M: int, N: int, dtype, like, what: str):
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    if out.shape != shape or out.dtype not in (torch.bfloat16, torch.float32) or out.device != like.device or \
-            (out.stride(-1) != 1 and out.shape[-1] > 1):
+        return torch.empty((M, N), dtype=dtype, device=like.device)
+    if out.shape != (M, N) or (out.dtype is not BF16 and out.dtype is not F32) or out.get_device() != like.get_device() or \
+            (out.stride(-1) != 1 and N > 1):
         raise ValueError(f"{what}: out {tuple(out.shape)} {out.dtype} on {out.device}, strides {out.stride()}; "
-                         f"{tuple(shape)} in bf16 or fp32 with contiguous rows on {like.device}")
+                         f"{(M, N)} in bf16 or fp32 with contiguous rows on {like.device}")
     return out
 
 
@@ -217,14 +207,14 @@ def gemm_fp8(a: Fp8Matrix, b: Fp8Matrix, *, trans_a: bool = False, trans_b: bool
     qa, qb = a.data, b.data
     K, M = qa.shape if trans_a else qa.shape[::-1]
     N, kb = qb.shape if trans_b else qb.shape[::-1]
-    if K != kb or qa.device != qb.device:
+    if K != kb or qa.get_device() != qb.get_device():
         raise ValueError(f"gemm_fp8: {tuple(qa.shape)} trans_a={trans_a} on {qa.device} by {tuple(qb.shape)} trans_b={trans_b} on {qb.device}")
     dtype = out_dtype or (out.dtype if out is not None else torch.bfloat16)
-    if dtype not in (torch.bfloat16, torch.float32) or (out is not None and out.dtype != dtype):
+    if (dtype is not BF16 and dtype is not F32) or (out is not None and out.dtype != dtype):
         raise ValueError(f"gemm_fp8: a result in {dtype}, out in {None if out is None else out.dtype}")
     if beta != 0.0 and c is None and out is None:
         raise ValueError("gemm_fp8: beta without c or out")
-    D = _result(out, (M, N), dtype, qa, "gemm_fp8")
+    D = _result(out, M, N, dtype, qa, "gemm_fp8")
     if beta == 0.0:
         c = None
     elif c is None:
@@ -240,13 +230,12 @@ def gemm_fp8(a: Fp8Matrix, b: Fp8Matrix, *, trans_a: bool = False, trans_b: bool
     if not qa.is_cuda or K == 0:
         return ref.gemm(ref.dequant_fp8(*a), ref.dequant_fp8(*b), trans_a=trans_a, trans_b=trans_b, alpha=alpha, beta=beta, c=c, bias=bias, out=D)
     qa, qb = _on_grid(qa), _on_grid(qb)
-    bias = None if bias is None else bias.contiguous()
-    with _On(qa) as stream:
-        _call("gemm_fp8", "ftb_gemm_fp8", qa.data_ptr(), qb.data_ptr(), D.data_ptr(), None if c is None else c.data_ptr(),
-              None if bias is None else bias.data_ptr(), a.scale.data_ptr(), b.scale.data_ptr(), None, M, N, K, trans_a, not trans_b,
-              qa.stride(0), qb.stride(0), D.stride(0), 0 if c is None else c.stride(0), sa_m, sa_k, sa_shift, sb_n, sb_k, sb_shift, 0,
-              float(alpha), float(beta), dtype == torch.float32, 0, 0, 0, 0, 0, 0, stream)
-    _ran("gemm_fp8")
+    if bias is not None:
+        bias = bias.contiguous()
+    _launch("gemm_fp8", qa.get_device(), "gemm_fp8", "ftb_gemm_fp8", qa.data_ptr(), qb.data_ptr(), D.data_ptr(),
+            None if c is None else c.data_ptr(), None if bias is None else bias.data_ptr(), a.scale.data_ptr(), b.scale.data_ptr(), None, M, N, K,
+            trans_a, not trans_b, qa.stride(0), qb.stride(0), D.stride(0), 0 if c is None else c.stride(0), sa_m, sa_k, sa_shift, sb_n, sb_k,
+            sb_shift, 0, float(alpha), float(beta), dtype is F32, 0, 0, 0, 0, 0, 0)
     return D
 
 
@@ -289,7 +278,7 @@ def grouped_gemm_fp8(x: Fp8Matrix, w: Fp8Matrix, offsets, *, trans_w: bool = Tru
     off = _offsets(offsets, E, x.data, "grouped_gemm_fp8")
     if beta != 0.0 and out is None:
         raise ValueError("grouped_gemm_fp8: beta without out")
-    D = _result(out, (R, N), torch.bfloat16, x.data, "grouped_gemm_fp8")
+    D = _result(out, R, N, BF16, x.data, "grouped_gemm_fp8")
     if R == 0 or N == 0 or E == 0:
         return D
     if not x.data.is_cuda or K == 0:
@@ -300,11 +289,9 @@ def grouped_gemm_fp8(x: Fp8Matrix, w: Fp8Matrix, offsets, *, trans_w: bool = Tru
                 ref.gemm(xf[i:j], wf[e], trans_b=trans_w, alpha=alpha, beta=beta, out=D[i:j])
         return D
     qx, qw = _on_grid(x.data), _on_grid(w.data)
-    with _On(qx) as stream:
-        _call("gemm_fp8", "ftb_gemm_fp8", qx.data_ptr(), qw.data_ptr(), D.data_ptr(), None, None, x.scale.data_ptr(), w.scale.data_ptr(),
-              off.data_ptr(), R, N, K, 0, not trans_w, qx.stride(0), qw.stride(1), D.stride(0), 0, sa_m, sa_k, sa_shift, sb_n, sb_k, 7,
-              w.scale.stride(0), float(alpha), float(beta), D.dtype == torch.float32, 1, E, qw.stride(0), 0, 0, 0, stream)
-    _ran("grouped_gemm_fp8")
+    _launch("grouped_gemm_fp8", qx.get_device(), "gemm_fp8", "ftb_gemm_fp8", qx.data_ptr(), qw.data_ptr(), D.data_ptr(), None, None,
+            x.scale.data_ptr(), w.scale.data_ptr(), off.data_ptr(), R, N, K, 0, not trans_w, qx.stride(0), qw.stride(1), D.stride(0), 0, sa_m,
+            sa_k, sa_shift, sb_n, sb_k, 7, w.scale.stride(0), float(alpha), float(beta), D.dtype is F32, 1, E, qw.stride(0), 0, 0, 0)
     return D
 
 
@@ -337,9 +324,7 @@ def grouped_wgrad_fp8(dy: Fp8Matrix, x: Fp8Matrix, offsets, gw, *, alpha: float 
     sa_m, sa_k, _ = _along(dy, True, "grouped_wgrad_fp8 (dy)")
     sb_n, sb_k, _ = _along(x, True, "grouped_wgrad_fp8 (x)")
     qd, qx = _on_grid(dy.data), _on_grid(x.data)
-    with _On(gw) as stream:
-        _call("gemm_fp8", "ftb_gemm_fp8", qd.data_ptr(), qx.data_ptr(), gw.data_ptr(), None, None, dy.scale.data_ptr(), x.scale.data_ptr(),
-              off.data_ptr(), N, K, R, 1, 1, qd.stride(0), qx.stride(0), gw.stride(1), 0, sa_m, sa_k, 0, sb_n, sb_k, 0, 0, float(alpha),
-              1.0, gw.dtype == torch.float32, 2, E, 0, gw.stride(0), 0, 0, stream)
-    _ran("grouped_wgrad_fp8")
+    _launch("grouped_wgrad_fp8", gw.get_device(), "gemm_fp8", "ftb_gemm_fp8", qd.data_ptr(), qx.data_ptr(), gw.data_ptr(), None, None,
+            dy.scale.data_ptr(), x.scale.data_ptr(), off.data_ptr(), N, K, R, 1, 1, qd.stride(0), qx.stride(0), gw.stride(1), 0, sa_m, sa_k, 0,
+            sb_n, sb_k, 0, 0, float(alpha), 1.0, gw.dtype is F32, 2, E, 0, gw.stride(0), 0, 0)
     return gw

@@ -178,7 +178,7 @@ def _operands(form, M, N, K, scale_a=1.0):
 
 
 SIZES = [(1, 128, 128), (16, 256, 512), (128, 128, 128), (130, 257, 100), (3, 40, 1000), (300, 520, 129), (1, 1, 1), (513, 600, 16),
-         (640, 512, 640), (1025, 776, 200), (200, 4096, 384), (777, 1031, 2049)]
+         (640, 512, 640), (1025, 776, 200), (200, 4096, 384), (777, 1031, 2049), (5, 300, 5000), (100, 133, 2100), (128, 1000, 1500)]
 
 
 @pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
