@@ -14,7 +14,7 @@
 //              (a thread's 128 sums, and 32 values on the way, need more than the 168 registers of 384 threads: the first four
 //              warps give theirs up)
 //
-// SPLIT: products with few tiles.  A cluster of up to eight CTAs takes one tile, a range of the reduction each; the parts are added
+// SPLIT: products with few tiles.  A cluster of up to four CTAs takes one tile, a range of the reduction each; the parts are added
 // through the cluster's shared memory, in the order of the ranges, so that results do not depend on who comes first.
 //
 // CG = 2: a pair of SMs works on 256 x BN (each CTA 128 rows, half of B).  Grouped forms take their row or reduction ranges
@@ -502,6 +502,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         }
       }
     }
+    if constexpr (SPLIT) {                               // (the others' two barriers, see there)
+      __syncwarp();
+      cluster_sync_all();
+      cluster_sync_all();
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;\n");
     constexpr int SEG = CG, SEG_COLS = HALF / SEG;         // (a half of a pair's tile has columns of two blocks of 128)
@@ -611,7 +616,15 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             else mbar_arrive(&tempty[acc]);
           }
         };
-        if constexpr (BVEC) {
+        if (rows == 0) {                                 // nothing of this warp's is stored: its values stay where they are
+          if constexpr (BVEC) {
+            cp_wait<AHEAD - 1>();
+            __syncwarp();
+          }
+          ask(AHEAD - 1);
+          release();
+          ready = mbar_test(&tfull[wrap ? 0 : acc + 1], acc_phase ^ wrap);
+        } else if constexpr (BVEC) {
           uint32_t r[2][16];
           tmem_ld_16x32(taddr, r[0]);
           cp_wait<AHEAD - 1>();
@@ -640,39 +653,55 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             if (q + 2 == CHUNKS) release();
           }
         } else {
-          constexpr int CH = 16;
-          uint32_t r[2][CH];
-          tmem_ld_row16(taddr, r[0]);
           float s[SEG];
 #pragma unroll
           for (int g = 0; g < SEG; ++g) s[g] = a_next[0] * b_next[g][0];
+          auto scales = [&] {
 #pragma unroll
-          for (int i = 0; i + 1 < AHEAD; ++i) {
-            a_next[i] = a_next[i + 1];
+            for (int i = 0; i + 1 < AHEAD; ++i) {
+              a_next[i] = a_next[i + 1];
 #pragma unroll
-            for (int g = 0; g < SEG; ++g) b_next[g][i] = b_next[g][i + 1];
-          }
-          ask(AHEAD - 1);
-          tmem_ld_wait();
+              for (int g = 0; g < SEG; ++g) b_next[g][i] = b_next[g][i + 1];
+            }
+            ask(AHEAD - 1);
+          };
+          if constexpr (HALF == 64) {                    // there are registers for all of them at once
+            uint32_t r[2][32];
+            tmem_ld_32x32(taddr, r[0]);
+            tmem_ld_32x32(taddr + 32, r[1]);
+            scales();
+            tmem_ld_wait();
+            release();
+            ready = mbar_test(&tfull[wrap ? 0 : acc + 1], acc_phase ^ wrap);
 #pragma unroll
-          for (int c = 0; c < HALF; c += CH) {
-            if (c + CH < HALF) tmem_ld_row16(taddr + c + CH, r[(c / CH + 1) & 1]);
-            else ready = mbar_test(&tfull[wrap ? 0 : acc + 1], acc_phase ^ wrap);
+            for (int i = 0; i < HALF; ++i) sum[i] = fmaf(__uint_as_float(r[i / 32][i % 32]), s[0], sum[i]);
+          } else {
+            constexpr int CH = 16;
+            uint32_t r[2][CH];
+            tmem_ld_row16(taddr, r[0]);
+            scales();
+            tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < CH; ++i) sum[c + i] = fmaf(__uint_as_float(r[c / CH & 1][i]), s[c / SEG_COLS % SEG], sum[c + i]);
-            if (c + CH < HALF) tmem_ld_wait();
-            if (c + 2 * CH == HALF) release();
+            for (int c = 0; c < HALF; c += CH) {
+              if (c + CH < HALF) tmem_ld_row16(taddr + c + CH, r[(c / CH + 1) & 1]);
+              else ready = mbar_test(&tfull[wrap ? 0 : acc + 1], acc_phase ^ wrap);
+#pragma unroll
+              for (int i = 0; i < CH; ++i) sum[c + i] = fmaf(__uint_as_float(r[c / CH & 1][i]), s[c / SEG_COLS % SEG], sum[c + i]);
+              if (c + CH < HALF) tmem_ld_wait();
+              if (c + 2 * CH == HALF) release();
+            }
           }
         }
         if (wrap) { acc = 0; acc_phase ^= 1; }
         else ++acc;
       }
+      // SPLIT: the parts go where the stages were, once both halves' products have read them (a CTA has one tile)
+      if constexpr (SPLIT) asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory");
       if (!ok) break;
       __syncwarp();                                      // (all lanes have read the last slot)
       const Patch w = patch();
       tile = begin(tile + step);
       if constexpr (SPLIT) {
-        // (every load and product of this CTA is done: the stages are free)
 #pragma unroll
         for (int i = 0; i < HALF; i += BVEC ? 2 : 4) {
           const int c = BVEC ? i / 32 * 32 + i % 16 / 4 * 8 + 2 * (lane & 3) : i;       // of the half
@@ -697,26 +726,25 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
     cp_wait_all();                                       // no copy outlives the block
     if (lane == 0) bulk_wait_all();
-  }
-
-  __syncwarp();
-  tc_fence_before();
-  if constexpr (SPLIT) {
-    cluster_sync_all();
-    W walk;
-    Tile t;
-    if (warp >= EPI_FIRST && walk.at(p, first, t)) {
+    if constexpr (SPLIT) {
+      __syncwarp();
+      cluster_sync_all();                                // the ranges' parts lie there
+      W again;
+      again.at(p, first, t);
       // this CTA's share of the columns: pieces of four, the ranges' parts added in their order
       const int share = 32 / ranges, rows = min(BM, t.left);
       for (int i = threadIdx.x - 32 * EPI_FIRST; i < rows * share; i += 32 * EPI_WARPS) {
         const int r = i / share, piece = range * share + i % share, col = t.tn * BN + 4 * piece;
         if (col >= p.N) continue;
         const uint32_t at = smem_u32(smem) + part_offset(r, piece);
-        float4 v = ld_cluster(at, 0);
-        for (uint32_t k = 1; k < ranges; ++k) {
-          const float4 u = ld_cluster(at, k);
-          v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
-        }
+        float4 u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < static_cast<int>(ranges)) u[k] = ld_cluster(at, k);
+        float4 v = u[0];
+#pragma unroll
+        for (int k = 1; k < 4; ++k)
+          if (k < static_cast<int>(ranges)) { v.x += u[k].x; v.y += u[k].y; v.z += u[k].z; v.w += u[k].w; }
         float f[4] = {v.x * p.alpha, v.y * p.alpha, v.z * p.alpha, v.w * p.alpha};
         const long row = t.row0 + r;
         float* d32 = static_cast<float*>(p.D) + row * p.ldd + col;
@@ -745,10 +773,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           }
         }
       }
+      __syncwarp();
+      cluster_sync_all();                                // nobody leaves while its part is read
     }
-    __syncwarp();
-    cluster_sync_all();                                  // nobody leaves while its part is read
   }
+
+  __syncwarp();
+  tc_fence_before();
   __syncthreads();
   if constexpr (CG == 2) cluster_sync_all();             // the leader's MMAs also write the peer's tensor memory
   if (warp == 1) {
@@ -799,6 +830,28 @@ int sm_count(int dev) {
     counts[dev] = n;
   }
   return counts[dev];
+}
+
+// Ranges of the reduction for tiles of 128 x 128: a power of two up to four, as there are SMs for, each of two blocks at least and
+// none empty.  (Clusters of eight start later: 1 x 2048 x 2048 15.3 to 17.2 us, 14.3 with four.)
+int split_ranges(int64_t tiles, int k_blocks, int sms) {
+  int ranges = 4;
+  while (ranges > 1 && (tiles * ranges > sms || k_blocks < 2 * ranges || (ranges - 1) * ((k_blocks + ranges - 1) / ranges) >= k_blocks)) ranges /= 2;
+  return ranges;
+}
+
+// The tile of a product: 1 128 x 128 (cut along the reduction where that fills the GPU), 2 128 x 256, 3 256 x 256 on two SMs.  By
+// the waves and the blocks of each, a block taking some 0.5, 0.7 and 0.66 us (a pair of SMs loads less for the same work, and is
+// bound by power later).  us with 1 / 2 / 3, x W^T: 16 x 4096 x 4096 16 / 27 / 27; 256 x 4096 x 4096 21 / 29 / 29; 200 x 14336 x
+// 4096 40 / 29 / 29; 768 x 4096 x 4096 40 / 29 / 29; 1024 x 2048 x 2048 16 / 21 / 21; 512 x 4096 x 14336 68 / 74 / 73; 8192 x 14336 x
+// 4096 (power) - / 637 / 620.
+int pick_variant(int64_t M, int64_t N, int k_blocks, int sms) {
+  auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const int64_t t1 = up(M, 128) * up(N, 128), t2 = up(M, 128) * up(N, 256), t3 = up(M, 256) * up(N, 256);
+  const int r = split_ranges(t1, k_blocks, sms);
+  const double c1 = up(t1 * r, sms) * up(k_blocks, r) * 0.5 + (r > 1 ? 2.0 : 0.0), c2 = up(t2, sms) * k_blocks * 0.7,
+               c3 = up(t3, sms / 2 > 0 ? sms / 2 : 1) * k_blocks * 0.66;
+  return c3 <= c1 && c3 <= c2 ? 3 : c2 <= c1 ? 2 : 1;
 }
 
 template <int CG, int BN, bool BVEC, bool SPLIT = false>
@@ -876,7 +929,13 @@ int ftb_gemm_fp8(const Fp8GemmArgs* a) {
   p.total = p.mode == 1 ? p.M : p.K;
   p.k_blocks = (p.K + BK - 1) / BK;
 
-  const int variant = a->variant ? static_cast<int>(a->variant) : (p.M >= 512 && p.N >= 512 ? 3 : p.N > 128 && p.M > 128 ? 2 : 1);
+  const int sms = sm_count(dev), most = a->max_ctas > 0 && a->max_ctas < sms ? static_cast<int>(a->max_ctas) : sms;
+  const int variant = a->variant ? static_cast<int>(a->variant)
+                      : p.mode == 0 ? pick_variant(p.M, p.N, p.k_blocks, most)
+                      : p.N <= 128  ? 1
+                      : p.mode == 1 ? 2
+                      : p.M > 128   ? 3
+                                    : 2;
   const int cg = variant == 3 ? 2 : 1, bn = variant == 1 ? 128 : 256;
   const int tile_m = BM * cg;
   p.tiles_m = (p.M + tile_m - 1) / tile_m;
@@ -903,13 +962,9 @@ int ftb_gemm_fp8(const Fp8GemmArgs* a) {
   } else {
     td = ta;                            // (not used)
   }
-  const int sms = sm_count(dev), most = a->max_ctas > 0 && a->max_ctas < sms ? static_cast<int>(a->max_ctas) : sms;
   const bool bvec = a->sb_shift == 0;
   if (variant == 1 && p.mode == 0) {
-    // As many ranges (a power of two) as there are SMs for, each of two blocks at least, none of them empty.
-    int ranges = 8;
-    while (ranges > 1 && (tiles * ranges > most || p.k_blocks < 2 * ranges || (ranges - 1) * ((p.k_blocks + ranges - 1) / ranges) >= p.k_blocks))
-      ranges /= 2;
+    const int ranges = split_ranges(tiles, p.k_blocks, most);
     p.split_blocks = (p.k_blocks + ranges - 1) / ranges;
     if (ranges > 1)
       return bvec ? launch<1, 128, true, true>(ta, tb, td, p, dev, most, a->stream, ranges)

@@ -31,6 +31,7 @@ _ops = sys.modules[__package__]
 FP8, F32, BF16 = torch.float8_e4m3fn, torch.float32, torch.bfloat16
 _GROUPS = ("row", "col", "block")
 _entries: dict = {}
+TILE = 0       # of the products: 0 by size, 1 128 x 128, 2 128 x 256, 3 256 x 256 on two SMs (tests and timings)
 
 
 class Fp8Matrix(NamedTuple):
@@ -235,7 +236,7 @@ def gemm_fp8(a: Fp8Matrix, b: Fp8Matrix, *, trans_a: bool = False, trans_b: bool
     _launch("gemm_fp8", qa.get_device(), "gemm_fp8", "ftb_gemm_fp8", qa.data_ptr(), qb.data_ptr(), D.data_ptr(),
             None if c is None else c.data_ptr(), None if bias is None else bias.data_ptr(), a.scale.data_ptr(), b.scale.data_ptr(), None, M, N, K,
             trans_a, not trans_b, qa.stride(0), qb.stride(0), D.stride(0), 0 if c is None else c.stride(0), sa_m, sa_k, sa_shift, sb_n, sb_k,
-            sb_shift, 0, float(alpha), float(beta), dtype is F32, 0, 0, 0, 0, 0, 0)
+            sb_shift, 0, float(alpha), float(beta), dtype is F32, 0, 0, 0, 0, TILE, 0)
     return D
 
 
@@ -291,7 +292,7 @@ def grouped_gemm_fp8(x: Fp8Matrix, w: Fp8Matrix, offsets, *, trans_w: bool = Tru
     qx, qw = _on_grid(x.data), _on_grid(w.data)
     _launch("grouped_gemm_fp8", qx.get_device(), "gemm_fp8", "ftb_gemm_fp8", qx.data_ptr(), qw.data_ptr(), D.data_ptr(), None, None,
             x.scale.data_ptr(), w.scale.data_ptr(), off.data_ptr(), R, N, K, 0, not trans_w, qx.stride(0), qw.stride(1), D.stride(0), 0, sa_m,
-            sa_k, sa_shift, sb_n, sb_k, 7, w.scale.stride(0), float(alpha), float(beta), D.dtype is F32, 1, E, qw.stride(0), 0, 0, 0)
+            sa_k, sa_shift, sb_n, sb_k, 7, w.scale.stride(0), float(alpha), float(beta), D.dtype is F32, 1, E, qw.stride(0), 0, TILE, 0)
     return D
 
 
@@ -326,5 +327,5 @@ def grouped_wgrad_fp8(dy: Fp8Matrix, x: Fp8Matrix, offsets, gw, *, alpha: float 
     qd, qx = _on_grid(dy.data), _on_grid(x.data)
     _launch("grouped_wgrad_fp8", gw.get_device(), "gemm_fp8", "ftb_gemm_fp8", qd.data_ptr(), qx.data_ptr(), gw.data_ptr(), None, None,
             dy.scale.data_ptr(), x.scale.data_ptr(), off.data_ptr(), N, K, R, 1, 1, qd.stride(0), qx.stride(0), gw.stride(1), 0, sa_m, sa_k, 0,
-            sb_n, sb_k, 0, 0, float(alpha), 1.0, gw.dtype is F32, 2, E, 0, gw.stride(0), 0, 0)
+            sb_n, sb_k, 0, 0, float(alpha), 1.0, gw.dtype is F32, 2, E, 0, gw.stride(0), TILE, 0)
     return gw

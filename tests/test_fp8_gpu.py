@@ -210,13 +210,71 @@ def test_gemm(out_dtype, form, M, N, K):
     _no_errors()
 
 
-@pytest.mark.parametrize("variant", [1, 2, 3])
+@pytest.fixture(params=[0, 1, 2, 3])
+def tile(request, monkeypatch):
+    """The products' tile: by size, 128 x 128, 128 x 256, 256 x 256 on two SMs."""
+    from flextrain_b200.ops import fp8
+    monkeypatch.setattr(fp8, "TILE", request.param)
+    return request.param
+
+
+@pytest.mark.parametrize("form", ["fwd", "rows", "dgrad", "wgrad", "across"])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (130, 257, 300), (257, 129, 640), (300, 520, 130), (600, 1100, 1000)])
+def test_gemm_tiles(tile, form, M, N, K):
+    """Every tile at sizes that end inside it, into both types, with C in place, elsewhere and not at all."""
+    ops = _ops()
+    torch.manual_seed(M + N + K)
+    A, B, ta, tb, want, mag = _operands(form, M, N, K)
+    for dtype in (torch.bfloat16, torch.float32):
+        got = ops.gemm_fp8(A, B, trans_a=ta, trans_b=tb, out_dtype=dtype)
+        assert torch.all((got.double() - want).abs() <= _room(want, mag, K, dtype))
+        Np = (N + 7) // 8 * 8                                    # rows on 16 bytes, and rows that are not
+        for c in (torch.randn(M, Np, device=DEV).to(dtype)[:, :N], torch.randn(M, N, device=DEV).to(dtype)):
+            w2, m2 = want + c.double(), mag + c.abs().double()
+            got = ops.gemm_fp8(A, B, trans_a=ta, trans_b=tb, beta=1.0, c=c, out_dtype=dtype)
+            assert torch.all((got.double() - w2).abs() <= _room(w2, m2, K, dtype))
+            ops.gemm_fp8(A, B, trans_a=ta, trans_b=tb, beta=1.0, out=c)
+            assert torch.all((c.double() - w2).abs() <= _room(w2, m2, K, dtype))
+    _no_errors()
+
+
+@pytest.mark.parametrize("N,K", [(520, 136), (129, 1030)])
+def test_grouped_tiles(tile, N, K):
+    ops = _ops()
+    torch.manual_seed(0)
+    cnt = [3, 0, 129, 1, 300, 0, 255, 128]
+    off = torch.tensor([0] + torch.tensor(cnt).cumsum(0).tolist(), device=DEV, dtype=torch.int32)
+    used, E = sum(cnt), len(cnt)
+    X, W = ops.quant_fp8(torch.randn(used, K, device=DEV), "row"), ops.quant_fp8(torch.randn(E, N, K, device=DEV), "block")
+    vx, vw, o = _value(X), _value(W), off.tolist()
+    for dtype in (torch.bfloat16, torch.float32):
+        out = torch.full((used + 5, N), 7.0, device=DEV, dtype=dtype)
+        ops.grouped_gemm_fp8(X, W, off, out=out[:used])
+        for e in range(E):
+            want, mag = vx[o[e]:o[e + 1]] @ vw[e].t(), vx[o[e]:o[e + 1]].abs() @ vw[e].abs().t()
+            assert torch.all((out[o[e]:o[e + 1]].double() - want).abs() <= _room(want, mag, K, dtype))
+        assert torch.all(out[used:] == 7)
+    cnt = [128, 0, 384, 256]
+    off = torch.tensor([0] + torch.tensor(cnt).cumsum(0).tolist(), device=DEV, dtype=torch.int32)
+    D, X = ops.quant_fp8(torch.randn(768, N, device=DEV), "col"), ops.quant_fp8(torch.randn(768, K, device=DEV), "col")
+    vd, vx, o = _value(D), _value(X), off.tolist()
+    for dtype in (torch.bfloat16, torch.float32):
+        gw = torch.randn(4, N, K, device=DEV).to(dtype)
+        keep = gw.clone()
+        ops.grouped_wgrad_fp8(D, X, off, gw, pad=128)
+        for e in range(4):
+            want = keep[e].double() + vd[o[e]:o[e + 1]].t() @ vx[o[e]:o[e + 1]]
+            mag = keep[e].abs().double() + vd[o[e]:o[e + 1]].abs().t() @ vx[o[e]:o[e + 1]].abs()
+            assert torch.all((gw[e].double() - want).abs() <= _room(want, mag, 768, dtype))
+    _no_errors()
+
+
 @pytest.mark.parametrize("form", ["fwd", "dgrad", "wgrad"])
-def test_gemm_infinities_stay_in_their_rows(variant, form):
+def test_gemm_infinities_stay_in_their_rows(tile, form):
     """A row or column of NaN reaches the results that it is part of and no others; C is not read without beta."""
     ops = _ops()
     torch.manual_seed(0)
-    M, N, K = {1: (100, 130, 300), 2: (260, 700, 300), 3: (700, 800, 300)}[variant]
+    M, N, K = 260, 700, 300
     a, b = torch.randn(M, K, device=DEV), torch.randn(N, K, device=DEV)
     a[M // 2, K - 1] = float("inf")
     a[0, 0] = float("nan")
