@@ -235,13 +235,26 @@ def _init_lora_params(am: ActiveModel, seed: int, a_std: float) -> None:
             t.zero_()
 
 
+def _linear_dtype(linear_dtype, compute_dtype, world_size, tp, ep) -> Optional[torch.dtype]:
+    """``linear_dtype`` of the builders: the type of the operands of the layers' products, the compute type or e4m3."""
+    if linear_dtype is None or linear_dtype == compute_dtype:
+        return None
+    if linear_dtype != torch.float8_e4m3fn:
+        raise ValueError(f"linear_dtype {linear_dtype}: torch.float8_e4m3fn, or the compute type {compute_dtype}")
+    if compute_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"linear_dtype {linear_dtype} with compute_dtype {compute_dtype}: bfloat16 (or float32, on the CPU)")
+    if world_size > 1 or tp not in (1, "auto") or ep not in (1, "auto"):
+        raise NotImplementedError("products in 8 bits run on one GPU: the fused collectives' products are in 16")
+    return linear_dtype
+
+
 def from_dims(dims: Mapping, *, arch: str = "llama", optimizer, max_seq_len: int, max_global_batch_tokens: int,
               max_gpu_mem_bytes: int, max_host_mem_bytes: int, hyperparams: Optional[Mapping] = None,
               init_seed: int = 0xF1EC7, init_std: float = 0.02, device: str = "cuda:0",
               leeway_gpu_mem_bytes: int = 3 * (1 << 30), leeway_host_mem_bytes: int = 4 * (1 << 30),
               compute_dtype: torch.dtype = torch.bfloat16, master_dtype: Optional[torch.dtype] = torch.bfloat16,
               grad_dtype: Optional[torch.dtype] = torch.bfloat16, norm_grad_dtype: torch.dtype = torch.float32,
-              lora_targets=None, lora_rank: int = 16, lora_alpha: float = 16.0,
+              linear_dtype: Optional[torch.dtype] = None, lora_targets=None, lora_rank: int = 16, lora_alpha: float = 16.0,
               lora_adapter_compute_dtype=torch.bfloat16, lora_adapter_master_dtype=torch.bfloat16,
               lora_adapter_grad_dtype=torch.bfloat16, lora_adapter_opt_state_dtype=torch.bfloat16,
               lora_init_seed: int = 20260424, lora_a_std: float = 0.02, hw_cost: Optional[HardwareCost] = None,
@@ -254,6 +267,9 @@ def from_dims(dims: Mapping, *, arch: str = "llama", optimizer, max_seq_len: int
               init_weights: bool = True, init_on_device: bool = False, plan_only: bool = False) -> ActiveModel:
     """Build an :class:`ActiveModel` from a dims dict with deterministic random weights; bypasses HF entirely.
 
+    ``linear_dtype=torch.float8_e4m3fn`` runs the products of attention, FFN and experts on e4m3 operands with a scale for
+    each block of 128 (weights, gradients and optimizer state keep their types).
+
     ``plan_only=True`` stops after the working-set planner and returns its :class:`WorkingSetConfig` (nothing is
     allocated, no process group is needed): what the engine WOULD do for this model, budget and parallel layout."""
     mod = select_arch_module(arch)
@@ -261,7 +277,8 @@ def from_dims(dims: Mapping, *, arch: str = "llama", optimizer, max_seq_len: int
     hyper.update(hyperparams or {})
     mc = mod.config_from_dims(dims, hyper) if hasattr(mod, "config_from_dims") else config_from_dims(dims, arch, hyper)
     norm_dt = torch.float32 if compute_dtype != torch.float64 else torch.float64
-    dt = DTypePolicy(compute_dtype, master_dtype or compute_dtype, grad_dtype or compute_dtype, norm_dt, norm_grad_dtype)
+    dt = DTypePolicy(compute_dtype, master_dtype or compute_dtype, grad_dtype or compute_dtype, norm_dt, norm_grad_dtype,
+                     _linear_dtype(linear_dtype, compute_dtype, world_size, tp, ep))
     lora = resolve_lora(lora_targets, lora_rank, lora_alpha, lora_adapter_compute_dtype, lora_adapter_master_dtype,
                         lora_adapter_grad_dtype, lora_adapter_opt_state_dtype)
     am = _build_active_model(mc, optimizer=optimizer, max_seq_len=max_seq_len,
@@ -290,7 +307,7 @@ def from_pretrained(model_path: str, *, optimizer, max_seq_len: int, max_global_
                     leeway_gpu_mem_bytes: int = 3 * (1 << 30), leeway_host_mem_bytes: int = 4 * (1 << 30),
                     compute_dtype: torch.dtype = torch.bfloat16, master_dtype: Optional[torch.dtype] = torch.bfloat16,
                     grad_dtype: Optional[torch.dtype] = torch.bfloat16, norm_grad_dtype: torch.dtype = torch.float32,
-                    lora_targets=None, lora_rank: int = 16, lora_alpha: float = 16.0,
+                    linear_dtype: Optional[torch.dtype] = None, lora_targets=None, lora_rank: int = 16, lora_alpha: float = 16.0,
                     lora_adapter_compute_dtype=torch.bfloat16, lora_adapter_master_dtype=torch.bfloat16,
                     lora_adapter_grad_dtype=torch.bfloat16, lora_adapter_opt_state_dtype=torch.bfloat16,
                     lora_init_seed: int = 20260424, lora_a_std: float = 0.02, hw_cost: Optional[HardwareCost] = None,
@@ -311,7 +328,8 @@ def from_pretrained(model_path: str, *, optimizer, max_seq_len: int, max_global_
     mc = mod.config_from_hf(hf)
     mc.hf = hf
     norm_dt = torch.float32
-    dt = DTypePolicy(compute_dtype, master_dtype or compute_dtype, grad_dtype or compute_dtype, norm_dt, norm_grad_dtype)
+    dt = DTypePolicy(compute_dtype, master_dtype or compute_dtype, grad_dtype or compute_dtype, norm_dt, norm_grad_dtype,
+                     _linear_dtype(linear_dtype, compute_dtype, world_size, tp, ep))
     lora = resolve_lora(lora_targets, lora_rank, lora_alpha, lora_adapter_compute_dtype, lora_adapter_master_dtype,
                         lora_adapter_grad_dtype, lora_adapter_opt_state_dtype)
     am = _build_active_model(mc, optimizer=optimizer, max_seq_len=max_seq_len,

@@ -157,7 +157,7 @@ def _workspace_bytes(layers, head, chunk: int, act_bytes: int = 2, head_rows: Op
     """Transient GPU memory while one chunk is in flight: residual stream in/out, the widest projection output
     and its gradient, attention workspace, what Gated DeltaNet keeps of its chunks, and one head micro-chunk of logits."""
     from ..ops.linattn_cuda import chunk_work_most
-    widest = lin = 0
+    widest = lin = fp8 = 0
     d = 0
     for l in layers:
         c = l.cfg
@@ -172,9 +172,35 @@ def _workspace_bytes(layers, head, chunk: int, act_bytes: int = 2, head_rows: Op
         if getattr(c, "gdn", None) is not None:
             lin = max(lin, chunk_work_most(chunk, c.gdn.n_v_heads, c.gdn.head_k_dim, c.gdn.head_v_dim))
         widest = max(widest, w)
+        if getattr(c, "linear_fp8", False):
+            fp8 = max(fp8, _fp8_bytes(c, chunk))
     per_tok = (4 * d + 2 * widest) * act_bytes
     head_ws = min(chunk, head_rows or head.head_chunk_size) * head.vocab_size * act_bytes * 2
-    return chunk * per_tok + head_ws + lin + WORKSPACE_ALLOWANCE
+    return chunk * per_tok + head_ws + lin + fp8 + WORKSPACE_ALLOWANCE
+
+
+def _fp8_bytes(c, chunk: int) -> int:
+    """What a product in 8 bits holds besides its operands, at most: the weight in 8 bits, or input and output gradient of the
+    weight gradient, and their scales, an fp32 one for 128 elements."""
+    groups = []                                                            # (out, in) of the weights
+    if c.attn is not None:
+        groups += [(c.attn.q_dim * (2 if c.attn.gated else 1) + 2 * c.attn.kv_dim, c.d_model), (c.d_model, c.attn.q_dim)]
+    if c.ffn is not None:
+        groups += [(2 * c.ffn.ffn_dim, c.d_model), (c.d_model, c.ffn.ffn_dim)]
+    most = 0
+    pad = lambda n: (n + 15) // 16 * 16
+    size = lambda rows, cols: rows * pad(cols) + 4 * ((rows + 127) // 128 * 128) * ((cols + 127) // 128 * 128) // 128
+    if c.moe is not None:
+        from ..ops.reference import moe_rows_bound
+        E, F = c.moe.num_experts, c.moe.expert_dim
+        rows = moe_rows_bound(chunk, c.moe.top_k, E, 128)
+        for out, inp in ((2 * F, c.d_model), (c.d_model, F)):
+            most = max(most, E * size(out, inp) + size(rows, max(out, inp)), size(rows, out) + size(rows, inp))
+        if c.moe.shared_dim:
+            groups += [(2 * c.moe.shared_dim, c.d_model), (c.d_model, c.moe.shared_dim)]
+    for out, inp in groups:
+        most = max(most, size(out, inp) + size(chunk, max(out, inp)), size(chunk, out) + size(chunk, inp))
+    return most
 
 
 def determine_working_set_config(*, layers, embed, head, optimizer, max_seq_len: int, max_global_batch_tokens: int,

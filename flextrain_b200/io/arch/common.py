@@ -84,6 +84,7 @@ class DTypePolicy:
     grad: Optional[torch.dtype] = torch.bfloat16
     norm: torch.dtype = torch.float32
     norm_grad: torch.dtype = torch.float32
+    linear: Optional[torch.dtype] = None             # operands of the layers' products: float8_e4m3fn, or as `compute`
 
 
 def expand_layer_pattern(pattern: str, n_layers: int) -> List[str]:
@@ -158,7 +159,7 @@ def build_decoder_config(mc: ModelConfig, i: int, dt: DTypePolicy, lora: Optiona
     return DecoderConfig(d_model=mc.d_model, attn=attn, gdn=gdn, ffn=ffn, moe=moe, norm_eps=mc.norm_eps,
                          post_norms=mc.post_norms, dtype=dt.compute, norm_dtype=dt.norm, grad_dtype=dt.grad,
                          norm_grad_dtype=dt.norm_grad, master_dtype=dt.master, lora=lora, family=mc.arch,
-                         layer_scalar=mc.layer_scalar)
+                         layer_scalar=mc.layer_scalar, linear_fp8=dt.linear is not None)
 
 
 def build_model_parts(mc: ModelConfig, dt: DTypePolicy, lora: Optional[LoRAConfig], head_chunk_size: int = 4096,

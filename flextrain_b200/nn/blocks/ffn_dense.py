@@ -45,7 +45,7 @@ class GatedFFN:
 
     def fwd(self, h, x_resid, params, slot):
         F = self.cfg.ffn_dim
-        if self.up.tp is None:
+        if self.up.tp is None and not self.up.fp8:
             x13, act = ops.linear_glu_fwd(h, self.up.weight(params), self.cfg.kind, x13=slot.out("x13", h.device))
         else:
             x13 = self.up.fwd(h, params, out=slot.out("x13", h.device))
@@ -60,7 +60,7 @@ class GatedFFN:
         """Returns ``(dh, dx13)``; the caller runs ``self.up.wgrad(dx13, h, ...)`` once ``h`` is re-emitted."""
         F = self.cfg.ffn_dim
         x13 = slot._t["x13"]
-        if self.down.tp is None:
+        if self.down.tp is None and not self.down.fp8:
             dx13, act = ops.linear_glu_bwd(dx, self.down.weight(params), x13, self.cfg.kind)
         else:
             dact = self.down.dgrad(dx, params)

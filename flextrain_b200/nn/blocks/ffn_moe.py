@@ -57,6 +57,20 @@ class MoEFFN:
             self.shared.up = LinearGroup(["w_shared_1", "w_shared_3"], None)
             self.shared.down = LinearGroup(["w_shared_2"], None)
 
+    fp8 = False                    # the experts' products in 8 bits, set by the layer (router and adapters stay in 16)
+
+    def _product(self, x, w, offsets, *, trans_w: bool = True, out=None):
+        if not self.fp8:
+            return ops.grouped_gemm(x, w, offsets, trans_w=trans_w, out=out)
+        if out is None:
+            out = torch.empty(x.shape[0], w.shape[1 if trans_w else 2], dtype=x.dtype, device=x.device)
+        return ops.grouped_gemm_fp8(ops.quant_fp8(x, "row"), ops.quant_fp8(w, "block"), offsets, trans_w=trans_w, out=out)
+
+    def _wgrad(self, dy, x, offsets, gw):
+        if not self.fp8:
+            return ops.grouped_wgrad(dy, x, offsets, gw, pad=ROW_PAD)
+        return ops.grouped_wgrad_fp8(ops.quant_fp8(dy, "col"), ops.quant_fp8(x, "block"), offsets, gw, pad=ROW_PAD)
+
     # ------------------------------------------------------------------ declarations
     def tensor_specs(self):
         c, dt = self.cfg, self.dtype
@@ -140,7 +154,7 @@ class MoEFFN:
     def _experts_fwd(self, h, params, plan, x_up_out=None):
         F = self.cfg.expert_dim
         xs = ops.gather_rows(h, plan.row_src, idx_div=self.cfg.top_k)
-        up = ops.grouped_gemm(xs, self.weight(params, "w_up"), plan.offsets, out=x_up_out)
+        up = self._product(xs, self.weight(params, "w_up"), plan.offsets, out=x_up_out)
         act = ops.glu_fwd(up[:, F:], up[:, :F], self.cfg.kind)
         return xs, up, act
 
@@ -163,7 +177,7 @@ class MoEFFN:
         else:
             plan = ops.moe_plan(idx, c.num_experts, ROW_PAD)
             _, up, act = self._experts_fwd(h, params, plan, slot.out("x_up", h.device))
-            y = ops.grouped_gemm(act, self.weight(params, "w_down"), plan.offsets)
+            y = self._product(act, self.weight(params, "w_down"), plan.offsets)
             out = ops.moe_combine(y, plan.inv, w, x_resid)
         if self.shared is not None:
             ys, g = self._shared_fwd(h, params, slot)
@@ -193,7 +207,7 @@ class MoEFFN:
             up = slot._t["x_up"]
             xs = ops.gather_rows(h, plan.row_src, idx_div=K)
             dy_u = ops.gather_rows(dx, plan.row_src, idx_div=K)                         # unweighted dL/dy rows
-            dact_u = ops.grouped_gemm(dy_u, self.weight(params, "w_down"), plan.offsets, trans_w=False)
+            dact_u = self._product(dy_u, self.weight(params, "w_down"), plan.offsets, trans_w=False)
             # activation (re-emitted), router-weight gradient and weighted dact in one pass
             wrow = ref.moe_row_weights(w, plan)
             dup = torch.empty_like(up)
@@ -201,12 +215,12 @@ class MoEFFN:
                                                   dup=dup[:, :F])
             dw = ref.moe_rows_to_slots(dw_rows, plan, w.shape)
             if "g_down" in grads:       # g_down += dy^T (w * act): the router weight rides on the activation
-                ops.grouped_wgrad(dy_u, act_w, plan.offsets, grads["g_down"], pad=ROW_PAD)
+                self._wgrad(dy_u, act_w, plan.offsets, grads["g_down"])
             if "g_up" in grads:
-                ops.grouped_wgrad(dup, xs, plan.offsets, grads["g_up"], pad=ROW_PAD)
+                self._wgrad(dup, xs, plan.offsets, grads["g_up"])
             self.lora_wgrad("w_down", dy_u, act_w, plan.offsets, params, grads, ROW_PAD)
             self.lora_wgrad("w_up", dup, xs, plan.offsets, params, grads, ROW_PAD)
-            dxs = ops.grouped_gemm(dup, self.weight(params, "w_up"), plan.offsets, trans_w=False)
+            dxs = self._product(dup, self.weight(params, "w_up"), plan.offsets, trans_w=False)
             dh = ops.moe_combine(dxs, plan.inv, None, None)
         # router
         logits = ops.gemm(h, params["w_router"], trans_b=True)

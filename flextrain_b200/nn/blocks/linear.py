@@ -9,6 +9,11 @@
   and the rank-r gradients come from the captured ``(x, dy)``:
   ``gA += s * (dy @ B).T @ x``,  ``gB += s * dy.T @ (x @ A.T)``
   (flextrain/nn/layers/lora_wrapper.py:106-148, 429, 602, 840).
+* **8 bits** (``fp8``; no counterpart in the reference).  The three products of the group run on e4m3 operands with a scale for
+  each block of 128: the input and ``dy`` in row groups, the effective weight in squares; for the weight gradient ``dy`` in column
+  groups (tokens differ in size, and a token's largest must not decide for others in another column) and the input in squares,
+  whose one scale for 128 columns makes that product half as fast again.  Weights stay in their own types and are quantised where they are used, so nothing has to be kept or dropped
+  when they change.  Adapters' gradients stay in 16 bits.
 * **Tensor parallelism** (no counterpart in the reference).  With a bound ``tp`` handle the activations between
   blocks are token-sharded ``(T/tp, d)``.  A ``"col"`` group holds ``out/tp`` rows of each weight: forward is the
   fused all-gather→GEMM, dgrad the fused GEMM→reduce-scatter, wgrad gathers its input.  A ``"row"`` group holds
@@ -71,6 +76,7 @@ class LinearGroup:
         self.bias_names = list(bias_names)
         self.lora = lora
         self.lora_names = [n for n in self.names if lora is not None and n in lora.targets]
+        self.fp8 = False               # products in 8 bits, set by the layer
         self.tp = None                 # TensorParallel handle, bound by the layer when tensor parallelism is on
         self.tp_mode: Optional[str] = None      # "col" | "row"
         self._dy_full = None           # (data_ptr of the local dy, gathered dy) kept between dgrad and wgrad
@@ -114,11 +120,19 @@ class LinearGroup:
     def fwd(self, x, params, *, residual=None, out=None):
         if self.tp is not None:
             return self._tp_fwd(x, params, residual, out)
+        if self.fp8:                                       # (x may come in 8 bits, as the norm in front wrote it)
+            x8 = x if isinstance(x, ops.Fp8Matrix) else ops.quant_fp8(x, "row")
+            w = self.weight(params)
+            return ops.linear_fp8_fwd(x8, ops.quant_fp8(w, "block"), bias=self.bias(params), residual=residual, out=out,
+                                      out_dtype=w.dtype)
         return ops.linear_fwd(x, self.weight(params), bias=self.bias(params), residual=residual, out=out)
 
     def dgrad(self, dy, params, *, out=None, accumulate=False):
         if self.tp is not None:
             return self._tp_dgrad(dy, params, out, accumulate)
+        if self.fp8:
+            return ops.linear_fp8_dgrad(ops.quant_fp8(dy, "row"), ops.quant_fp8(self.weight(params), "block"), out=out,
+                                        accumulate=accumulate, out_dtype=dy.dtype)
         return ops.linear_dgrad(dy, self.weight(params), out=out, accumulate=accumulate)
 
     # -- tensor-parallel passes -----------------------------------------------------
@@ -168,18 +182,27 @@ class LinearGroup:
         """Accumulate weight (and bias / LoRA) gradients of every member from ``(x, dy)``."""
         if self.tp is not None:
             dy, x = self._tp_wgrad_operands(dy, x)
+        linear_wgrad = ops.linear_wgrad
+        if self.fp8:
+            x8 = []
+
+            def linear_wgrad(dy, x, gw, *, alpha):
+                if not x8:                                 # one input for all members
+                    x8.append(ops.quant_fp8(x, "block"))
+                ops.linear_fp8_wgrad(ops.quant_fp8(dy, "col"), x8[0], gw, alpha=alpha)
+
         gnames = ["g_" + n[2:] for n in self.names]
         trainable = [g in grads for g in gnames]
         if all(trainable) and not self.lora_names:
             gs = [grads[g] for g in gnames]
             fv = gs[0] if len(gs) == 1 else fused_view(gs)
             if fv is not None:
-                ops.linear_wgrad(dy, x, fv, alpha=alpha)
+                linear_wgrad(dy, x, fv, alpha=alpha)
                 gs = None
             if gs is not None:
                 r0 = 0
                 for g in gs:
-                    ops.linear_wgrad(dy[:, r0:r0 + g.shape[0]], x, g, alpha=alpha)
+                    linear_wgrad(dy[:, r0:r0 + g.shape[0]], x, g, alpha=alpha)
                     r0 += g.shape[0]
         else:
             r0, adapters = 0, []
@@ -187,7 +210,7 @@ class LinearGroup:
                 rows = params[n].shape[0]
                 dyn = dy[:, r0:r0 + rows]
                 if gname in grads:
-                    ops.linear_wgrad(dyn, x, grads[gname], alpha=alpha)
+                    linear_wgrad(dyn, x, grads[gname], alpha=alpha)
                 g = "g_" + n[2:] + "_lora_"
                 if n in self.lora_names and grads.get(g + "a") is not None:
                     adapters.append((dyn, params[n + "_lora_a"], params[n + "_lora_b"], grads[g + "a"], grads[g + "b"]))

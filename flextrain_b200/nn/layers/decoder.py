@@ -48,6 +48,7 @@ class DecoderConfig:
     lora: Optional[LoRAConfig] = None
     family: str = "llama"
     layer_scalar: bool = False       # Gemma 4: the layer's output is multiplied by a stored, untrained scalar
+    linear_fp8: bool = False         # products of attention, FFN and experts in 8 bits (Gated DeltaNet, router: as they are)
     seq_parallel: int = 1            # tensor-parallel degree: the residual stream and norm statistics hold T / seq_parallel tokens
 
 
@@ -61,6 +62,14 @@ class DecoderLayer:
         self.ffn = GatedFFN(cfg.ffn, dtype=dt, lora=cfg.lora) if cfg.ffn else None
         self.moe = MoEFFN(cfg.moe, dtype=dt, lora=cfg.lora) if cfg.moe else None
         assert (self.attn is None) != (self.gdn is None) and (self.ffn is None) != (self.moe is None)
+        if cfg.linear_fp8:
+            groups = [self.attn.qkv, self.attn.o] if self.attn else []
+            groups += [self.ffn.up, self.ffn.down] if self.ffn else []
+            if self.moe is not None:
+                self.moe.fp8 = True
+                groups += [self.moe.shared.up, self.moe.shared.down] if self.moe.shared is not None else []
+            for g in groups:
+                g.fp8 = True
         self.param_spec = self._build_param_spec()
         self.activation_schema = self._build_schema()
 
@@ -133,6 +142,12 @@ class DecoderLayer:
         return ActivationSchema(fields, max_tier=3)
 
     # --------------------------------------------------------------------- forward
+    def _norm(self, x, w, dense: bool):
+        """``(normed input, rstd)``; in 8 bits where only products in 8 bits read it."""
+        if self.cfg.linear_fp8 and dense:
+            return ops.rmsnorm_fp8_fwd(x, w, self.cfg.norm_eps)[:2]
+        return ops.rmsnorm_fwd(x, w, self.cfg.norm_eps)
+
     def _mixer_fwd(self, h1, resid, meta, params, slot, ctx):
         if self.attn is not None:
             qkv = None
@@ -156,7 +171,7 @@ class DecoderLayer:
     def _forward(self, x, meta: ChunkMeta, params: Dict[str, torch.Tensor], slot, ctx: LayerContext):
         c = self.cfg
         x = slot.put("x_inp", x)
-        h1, r1 = ops.rmsnorm_fwd(x, params["w_attn_norm"], c.norm_eps)
+        h1, r1 = self._norm(x, params["w_attn_norm"], self.attn is not None)
         slot.put("attn_norm_rstd", r1)
         if c.post_norms:
             a = slot.put("attn_branch", self._mixer_fwd(h1, None, meta, params, slot, ctx))
@@ -166,7 +181,7 @@ class DecoderLayer:
         else:
             xo = self._mixer_fwd(h1, x, meta, params, slot, ctx)
         xo = slot.put("xo", xo)
-        h2, r2 = ops.rmsnorm_fwd(xo, params["w_ffn_norm"], c.norm_eps)
+        h2, r2 = self._norm(xo, params["w_ffn_norm"], self.ffn is not None)
         slot.put("ffn_norm_rstd", r2)
         if c.post_norms:
             f = slot.put("ffn_branch", self._ffn_fwd(h2, None, params, slot, ctx))
@@ -188,7 +203,7 @@ class DecoderLayer:
             if need_out or need_q or need_xo:
                 h1 = None
                 if need_q or (c.attn.gated and not slot.has("xgate")):
-                    h1, _ = ops.rmsnorm_fwd(x, params["w_attn_norm"], c.norm_eps)
+                    h1, _ = self._norm(x, params["w_attn_norm"], True)
                 self.attn.recompute(h1, meta, params, slot, ctx, need_out=need_out)
             if need_xo:
                 attn_in = t["attn_result"]
@@ -215,7 +230,7 @@ class DecoderLayer:
         need_ffn = (not slot.has("x13")) if self.ffn is not None else \
             (not slot.has("x_up") or (self.moe.shared is not None and not slot.has("x13_shared")))
         if need_ffn or (c.post_norms and not slot.has("ffn_branch")):
-            h2, _ = ops.rmsnorm_fwd(t["xo"], params["w_ffn_norm"], c.norm_eps)
+            h2, _ = self._norm(t["xo"], params["w_ffn_norm"], self.ffn is not None)
             ffn.recompute(h2, params, slot)
             if c.post_norms and not slot.has("ffn_branch"):
                 sc = _Passthrough(slot)
@@ -253,7 +268,7 @@ class DecoderLayer:
 
             def h_fn():
                 if "h" not in cache:
-                    cache["h"], _ = ops.rmsnorm_fwd(x, params["w_attn_norm"], c.norm_eps)
+                    cache["h"], _ = self._norm(x, params["w_attn_norm"], True)
                 return cache["h"]
 
             dh1, dqkv = self.attn.bwd(d_branch, h_fn, meta, params, grads, slot, ctx)
@@ -274,6 +289,8 @@ class DecoderLayer:
         """Route the projections through the tensor-parallel handle (fused all-gather→GEMM / GEMM→reduce-scatter)."""
         if tp is None:
             return
+        if self.cfg.linear_fp8:
+            raise NotImplementedError("tensor parallelism runs its projections in 16 bits")
         if self.attn is None or self.ffn is None:
             raise NotImplementedError("tensor parallelism covers dense attention + gated-FFN layers")
         for g in (self.attn.qkv, self.attn.o, self.ffn.up, self.ffn.down):

@@ -40,6 +40,10 @@ class Fp8Matrix(NamedTuple):
     scale: torch.Tensor
     group: str
 
+    @property
+    def device(self):
+        return self.data.device
+
 
 def _entry(lib: str, name: str):
     """A library's entry point that takes its arguments in 8 bytes each, as a function of them."""
@@ -240,18 +244,19 @@ def gemm_fp8(a: Fp8Matrix, b: Fp8Matrix, *, trans_a: bool = False, trans_b: bool
     return D
 
 
-def linear_fp8_fwd(x: Fp8Matrix, w: Fp8Matrix, *, bias=None, residual=None, out=None):
+def linear_fp8_fwd(x: Fp8Matrix, w: Fp8Matrix, *, bias=None, residual=None, out=None, out_dtype=None):
     """``y = x @ w.T (+ bias) (+ residual)``, ``x`` in row groups, ``w (out, in)`` in blocks (or row groups)."""
-    return gemm_fp8(x, w, trans_b=True, beta=0.0 if residual is None else 1.0, c=residual, bias=bias, out=out)
+    return gemm_fp8(x, w, trans_b=True, beta=0.0 if residual is None else 1.0, c=residual, bias=bias, out=out, out_dtype=out_dtype)
 
 
-def linear_fp8_dgrad(dy: Fp8Matrix, w: Fp8Matrix, *, out=None, accumulate=False):
+def linear_fp8_dgrad(dy: Fp8Matrix, w: Fp8Matrix, *, out=None, accumulate=False, out_dtype=None):
     """``dx = dy @ w``, ``dy`` in row groups, the same ``w (out, in)`` in blocks read across; optionally accumulated into ``out``."""
-    return gemm_fp8(dy, w, beta=1.0 if accumulate else 0.0, out=out)
+    return gemm_fp8(dy, w, beta=1.0 if accumulate else 0.0, out=out, out_dtype=out_dtype)
 
 
 def linear_fp8_wgrad(dy: Fp8Matrix, x: Fp8Matrix, gw, *, alpha=1.0, accumulate=True):
-    """``gw (out, in) (+)= alpha * dy.T @ x`` of operands in column groups (the reduction runs over the tokens)."""
+    """``gw (out, in) (+)= alpha * dy.T @ x`` of operands in column groups or blocks (the reduction runs over the tokens); ``x`` in
+    blocks is the fast form: a scale for each column of the result costs as much again as its sums."""
     return gemm_fp8(dy, x, trans_a=True, alpha=alpha, beta=1.0 if accumulate else 0.0, out=gw)
 
 
@@ -297,13 +302,14 @@ def grouped_gemm_fp8(x: Fp8Matrix, w: Fp8Matrix, offsets, *, trans_w: bool = Tru
 
 
 def grouped_wgrad_fp8(dy: Fp8Matrix, x: Fp8Matrix, offsets, gw, *, alpha: float = 1.0, pad: int = 1):
-    """``gw[e] += alpha * dy[rows_e].T @ x[rows_e]`` of operands in column groups, ``gw (E, N, K)`` bf16 or fp32.  Every expert's segment
+    """``gw[e] += alpha * dy[rows_e].T @ x[rows_e]``, ``dy`` in column groups and ``x`` in those or blocks, ``gw (E, N, K)`` bf16 or
+    fp32.  Every expert's segment
     is padded to a multiple of 128 rows with zero rows (``pad``, as the routing plan lays them out), so that no group of 128 tokens
     lies in two segments.  An expert without rows keeps its ``gw``."""
     _check(dy, "grouped_wgrad_fp8 (dy)")
     _check(x, "grouped_wgrad_fp8 (x)")
-    if dy.group != "col" or x.group != "col":
-        raise ValueError(f"grouped_wgrad_fp8: dy in groups {dy.group!r}, x in {x.group!r}; 'col' is read")
+    if dy.group != "col" or x.group not in ("col", "block"):
+        raise ValueError(f"grouped_wgrad_fp8: dy in groups {dy.group!r}, x in {x.group!r}; 'col', and 'col' or 'block', are read")
     if pad < 1 or pad % 128:
         raise ValueError(f"grouped_wgrad_fp8: segments padded to {pad} rows; a multiple of 128 is read")
     (R, N), (Rx, K) = dy.data.shape, x.data.shape
@@ -323,9 +329,9 @@ def grouped_wgrad_fp8(dy: Fp8Matrix, x: Fp8Matrix, offsets, gw, *, alpha: float 
                 ref.gemm(df[i:j], xf[i:j], trans_a=True, alpha=alpha, beta=1.0, out=gw[e])
         return gw
     sa_m, sa_k, _ = _along(dy, True, "grouped_wgrad_fp8 (dy)")
-    sb_n, sb_k, _ = _along(x, True, "grouped_wgrad_fp8 (x)")
+    sb_n, sb_k, sb_shift = _along(x, True, "grouped_wgrad_fp8 (x)")
     qd, qx = _on_grid(dy.data), _on_grid(x.data)
     _launch("grouped_wgrad_fp8", gw.get_device(), "gemm_fp8", "ftb_gemm_fp8", qd.data_ptr(), qx.data_ptr(), gw.data_ptr(), None, None,
             dy.scale.data_ptr(), x.scale.data_ptr(), off.data_ptr(), N, K, R, 1, 1, qd.stride(0), qx.stride(0), gw.stride(1), 0, sa_m, sa_k, 0,
-            sb_n, sb_k, 0, 0, float(alpha), 1.0, gw.dtype is F32, 2, E, 0, gw.stride(0), TILE, 0)
+            sb_n, sb_k, sb_shift, 0, float(alpha), 1.0, gw.dtype is F32, 2, E, 0, gw.stride(0), TILE, 0)
     return gw

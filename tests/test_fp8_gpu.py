@@ -167,11 +167,13 @@ def _operands(form, M, N, K, scale_a=1.0):
         A, B = ops.quant_fp8(a, "block"), ops.quant_fp8(b, "block")
     elif form == "dgrad":
         A, B = ops.quant_fp8(a, "row"), ops.quant_fp8(b.t().contiguous(), "block")
+    elif form == "wgrad_block":
+        A, B = ops.quant_fp8(a.t().contiguous(), "col"), ops.quant_fp8(b.t().contiguous(), "block")
     elif form == "wgrad":
         A, B = ops.quant_fp8(a.t().contiguous(), "col"), ops.quant_fp8(b.t().contiguous(), "col")
     else:                                                        # a read across, b along
         A, B = ops.quant_fp8(a.t().contiguous(), "col"), ops.quant_fp8(b, "row")
-    ta, tb = form in ("wgrad", "across"), form not in ("dgrad", "wgrad")
+    ta, tb = form in ("wgrad", "wgrad_block", "across"), form not in ("dgrad", "wgrad", "wgrad_block")
     va, vb = _value(A), _value(B)
     va, vb = va.t() if ta else va, vb.t() if tb else vb
     return A, B, ta, tb, va @ vb, va.abs() @ vb.abs()
@@ -182,7 +184,7 @@ SIZES = [(1, 128, 128), (16, 256, 512), (128, 128, 128), (130, 257, 100), (3, 40
 
 
 @pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("form", ["fwd", "rows", "blocks", "dgrad", "wgrad", "across"])
+@pytest.mark.parametrize("form", ["fwd", "rows", "blocks", "dgrad", "wgrad", "wgrad_block", "across"])
 @pytest.mark.parametrize("M,N,K", SIZES)
 def test_gemm(out_dtype, form, M, N, K):
     """Plain, with bias and alpha, with a C of other strides, into a strided result whose neighbours stay as they are."""
@@ -356,10 +358,11 @@ def test_grouped_gemm(counts, trans_w, N, K):
     _no_errors()
 
 
+@pytest.mark.parametrize("group", ["col", "block"])
 @pytest.mark.parametrize("counts", [[128, 256, 0, 384], [0, 128, 0], [1280, 128], [128] * 9])
 @pytest.mark.parametrize("N,K", [(128, 128), (520, 136), (300, 1030), (768, 512)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_grouped_wgrad(counts, N, K, dtype):
+def test_grouped_wgrad(counts, N, K, dtype, group):
     ops = _ops()
     torch.manual_seed(N + K)
     E, used = len(counts), sum(counts)
@@ -367,7 +370,7 @@ def test_grouped_wgrad(counts, N, K, dtype):
     dy, x = torch.randn(used + 128, N, device=DEV), torch.randn(used + 128, K, device=DEV)
     dy[used:] = float("nan")
     x[5] = 0
-    DY, X = ops.quant_fp8(dy, "col"), ops.quant_fp8(x, "col")
+    DY, X = ops.quant_fp8(dy, "col"), ops.quant_fp8(x, group)
     vd, vx = _value(DY), _value(X)
     gw = torch.randn(E, N, K, device=DEV).to(dtype)
     keep = gw.clone()

@@ -95,6 +95,9 @@ def build_arg_parser() -> argparse.ArgumentParser:
     p.add_argument("--max-chunk-size", type=int, default=None)
     p.add_argument("--master-dtype", choices=tuple(_DT), default="bfloat16")
     p.add_argument("--grad-dtype", choices=tuple(_DT), default="bfloat16")
+    p.add_argument("--linear-dtype", choices=("float8_e4m3fn",), default=None,
+                   help="operands of the products of attention, FFN and experts (one GPU): e4m3 with a scale for each block of "
+                        "128; weights, gradients and optimizer state keep their types")
     p.add_argument("--opt-state-dtype", choices=tuple(_DT), default=None)
     p.add_argument("--opt-state", choices=("auto", "host", "device"), default="auto",
                    help="where optimizer state lives: the planner decides, pinned host memory (streamed through a "
@@ -198,6 +201,7 @@ def main(argv=None) -> int:
                   compute_dtype=torch.bfloat16 if use_cuda else torch.float32,
                   master_dtype=_DT[args.master_dtype] if use_cuda else torch.float32,
                   grad_dtype=_DT[args.grad_dtype] if use_cuda else torch.float32,
+                  linear_dtype=getattr(torch, args.linear_dtype) if args.linear_dtype else None,
                   lora_targets="all" if lora else None, lora_rank=args.lora_rank, lora_alpha=args.lora_alpha,
                   force_saved_act_level=args.force_save_level, min_chunk_size=args.min_chunk_size,
                   max_chunk_size=args.max_chunk_size, verbose=args.verbose and rank == 0, world_size=world, rank=rank,
