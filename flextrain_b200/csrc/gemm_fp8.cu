@@ -31,17 +31,29 @@ constexpr int EPI_WARPS = 8, EPI_FIRST = 4, THREADS = 32 * (EPI_FIRST + EPI_WARP
 constexpr int PIECE_BYTES = 32 * 128;                    // a warp's piece of shared memory: 32 rows x 128 bytes
 constexpr int BOX_BYTES = 128 * 128;
 
-// e4m3 x e4m3 -> fp32
+// The four products of a stage (e4m3 x e4m3, fp32 sums from zero on), as one piece: a thread that puts descriptors together
+// between them takes longer than the tensor core.  Descriptors come in halves, of which the lower one holds the address in units
+// of 16 bytes; a_step and b_step are those units from one product to the next.
+#define FTB_MMA4(CG_)                                                                                                          \
+  asm volatile(                                                                                                                \
+      "{\n.reg .pred z, a;\n.reg .b32 x, y;\n.reg .b64 da, db;\n"                                                             \
+      "setp.ne.b32 z, 0, 0;\nsetp.eq.b32 a, 0, 0;\n"                                                                           \
+      "mov.b64 da, {%1, %2};\nmov.b64 db, {%3, %4};\n"                                                                         \
+      "tcgen05.mma.cta_group::" CG_ ".kind::f8f6f4 [%0], da, db, %7, z;\n"                                                     \
+      "add.u32 x, %1, %5;\nadd.u32 y, %3, %6;\nmov.b64 da, {x, %2};\nmov.b64 db, {y, %4};\n"                                  \
+      "tcgen05.mma.cta_group::" CG_ ".kind::f8f6f4 [%0], da, db, %7, a;\n"                                                     \
+      "add.u32 x, x, %5;\nadd.u32 y, y, %6;\nmov.b64 da, {x, %2};\nmov.b64 db, {y, %4};\n"                                    \
+      "tcgen05.mma.cta_group::" CG_ ".kind::f8f6f4 [%0], da, db, %7, a;\n"                                                     \
+      "add.u32 x, x, %5;\nadd.u32 y, y, %6;\nmov.b64 da, {x, %2};\nmov.b64 db, {y, %4};\n"                                    \
+      "tcgen05.mma.cta_group::" CG_ ".kind::f8f6f4 [%0], da, db, %7, a;\n}\n" ::"r"(tmem_d),                                   \
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(a_step), "r"(b_step), "r"(idesc)                                         \
+      : "memory")
 template <int CG>
-__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (CG == 1)
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
-                 "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-                 : "memory");
-  else
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
-                 "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-                 : "memory");
+__device__ __forceinline__ void umma4_f8(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t a_step,
+                                         uint32_t b_step, uint32_t idesc) {
+  static_assert(BK / MMA_K == 4, "four products of a stage");
+  if constexpr (CG == 1) FTB_MMA4("1");
+  else FTB_MMA4("2");
 }
 
 // whether a phase is complete, without waiting for it
@@ -473,11 +485,14 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       const uint32_t idesc = (1u << 4) | static_cast<uint32_t>(p.a_mn) << 15 | static_cast<uint32_t>(p.b_mn) << 16 |
                              static_cast<uint32_t>(HALF >> 3) << 17 | static_cast<uint32_t>(BM * CG >> 4) << 24;
       // K-major: 32 bytes along the swizzled row of 128; MN-major: 32 rows of 128 bytes, blocks of 128 wide behind one another
-      const uint32_t a_step = p.a_mn ? MMA_K * 128 : MMA_K, b_step = p.b_mn ? MMA_K * 128 : MMA_K;
-      const uint32_t a_lbo = p.a_mn ? BOX_BYTES : 16, b_lbo = p.b_mn ? BOX_BYTES : 16;
+      const uint32_t a_step = (p.a_mn ? MMA_K * 128 : MMA_K) >> 4, b_step = (p.b_mn ? MMA_K * 128 : MMA_K) >> 4;
       // the half's columns of this CTA's part of B: rows of it, or bytes of its rows, or its second box
       constexpr int OWN = HALF / CG;
       const uint32_t b_off = half * (p.b_mn ? (OWN == 128 ? BOX_BYTES : OWN) : OWN * 128);
+      const uint64_t a_desc = make_smem_desc(smem_u32(smem), p.a_mn ? BOX_BYTES : 16, 1024);
+      const uint64_t b_desc = make_smem_desc(smem_u32(smem) + BM * BK + b_off, p.b_mn ? BOX_BYTES : 16, 1024);
+      const uint32_t a_lo = static_cast<uint32_t>(a_desc), a_hi = static_cast<uint32_t>(a_desc >> 32);
+      const uint32_t b_lo = static_cast<uint32_t>(b_desc), b_hi = static_cast<uint32_t>(b_desc >> 32);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
@@ -490,11 +505,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           if (!e && !(ok = mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, 20))) break;
           if (!f && !(ok = mbar_wait(&full_bar[stage], phase, abort_flag, 21))) break;
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * R::STAGE), sb = sa + BM * BK + b_off;
-#pragma unroll
-          for (int kk = 0; kk < BK / MMA_K; ++kk)
-            umma_f8<CG>(tmem_half + acc * HALF, make_smem_desc(sa + kk * a_step, a_lbo, 1024), make_smem_desc(sb + kk * b_step, b_lbo, 1024),
-                        idesc, kk != 0);
+          const uint32_t at = stage * (R::STAGE >> 4);
+          umma4_f8<CG>(tmem_half + acc * HALF, a_lo + at, a_hi, b_lo + at, b_hi, a_step, b_step, idesc);
           if constexpr (CG == 2) { umma_commit_2cta(&tfull[acc], 3); umma_commit_2cta(&empty_bar[stage], 3); }
           else { umma_commit(&tfull[acc]); umma_commit(&empty_bar[stage]); }
           if (++stage == ST) { stage = 0; phase ^= 1; }
