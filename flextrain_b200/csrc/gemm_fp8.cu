@@ -19,6 +19,18 @@
 //
 // CG = 2: a pair of SMs works on 256 x BN (each CTA 128 rows, half of B).  Grouped forms take their row or reduction ranges
 // from device offsets.  Every wait is bounded.
+//
+// What bounds it.  A block of 256 x 256 x 128 takes a pair of SMs some 1050 cycles of the 512 that the tensor cores would need: an
+// accumulator is multiplied (400 cycles for a half, 400 behind the other half), seen to be complete and read out (500), released
+// across the pair and multiplied into again (550), and tensor memory holds four halves.  Sustained, power does: of 2390 us of
+// 16384 x 28672 x 4096, the additions are 250, reading tensor memory 150 (without both, 1890 us at 1.52 GHz; the library's product
+// with one scale for everything, which accumulates in tensor memory throughout, 1535).  Measured beside it, us of that product:
+// one thread and one product for all 256 columns 2540, which reads A once but lets both halves wait for one another; tiles of 256 x
+// 128 with four accumulators 3070; sixteen warps of 64 columns each 3050; additions on pairs of fp32 2360; chunks of 32 columns
+// 2480 (registers spilled).
+//   16384 x 28672 x 4096      2.37 ms  1625 TFLOP/s      8192 x 4096 x 14336, B across     585 us  1645 TFLOP/s
+//   3001 x 4096 x 14336 + C    237 us  1487 TFLOP/s      4096 x 2048 x 9377, both across   143 us  1100 TFLOP/s (column scales)
+//   14336 x 4096 x 16384      1.21 ms  1590 TFLOP/s (weight gradient, B in blocks)         16 x 4096 x 4096  14 us
 #include <mutex>
 
 #include "ptx.cuh"
@@ -447,6 +459,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         const int row0 = t.row0 + cta * BM;
         const int col0 = t.tn * BN + cta * (BN / CG);
         const int z = p.mode == 1 ? t.g : 0;
+        // a segment of the reduction that starts inside a group of 128 has no scales of its own
+        if (p.mode == 2 && p.offsets[t.g] % BK != 0 && t.kbs > 0) set_error(3, 40);
         for (int kb = 0; kb < t.kbs; ++kb) {
           if (!(ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, 10))) break;
           uint8_t* sa = smem + stage * R::STAGE;
@@ -922,7 +936,8 @@ int ftb_gemm_fp8(const Fp8GemmArgs* a) {
   if (a->M <= 0 || a->N <= 0 || (a->mode != 0 && a->groups <= 0)) return 0;
   if (a->K <= 0) return -1;
   if (((a->lda | a->ldb | a->b_g) & 15) || ((reinterpret_cast<uintptr_t>(a->A) | reinterpret_cast<uintptr_t>(a->B)) & 15)) return -2;
-  if (a->M >= 1ll << 31 || a->N >= 1ll << 31 || a->K >= 1ll << 31) return -3;
+  constexpr int64_t MOST = 0x7FFFFC00ll;          // rows, columns and depth, a tile behind the last one included, in 31 bits
+  if (a->M > MOST || a->N > MOST || a->K > MOST) return -3;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return -4;
   Params p;
@@ -932,6 +947,7 @@ int ftb_gemm_fp8(const Fp8GemmArgs* a) {
   p.alpha = static_cast<float>(a->alpha); p.beta = static_cast<float>(a->beta);
   p.d_fp32 = static_cast<int>(a->d_fp32);
   const int64_t es = p.d_fp32 ? 4 : 2;
+  if (p.M == 1 && a->mode != 2) p.ldd = p.ldc = (p.N * es + 15) / 16 * 16 / es;      // (a single row has no stride of its own)
   p.vec = ((reinterpret_cast<uintptr_t>(p.D) | reinterpret_cast<uintptr_t>(p.C) | static_cast<uintptr_t>(p.N * es) |
             static_cast<uintptr_t>(p.ldd * es) | static_cast<uintptr_t>(p.ldc * es) | static_cast<uintptr_t>(a->mode == 2 ? a->d_g * es : 0)) & 15) == 0;
   p.sa = a->sa; p.sa_m = a->sa_m; p.sa_k = a->sa_k; p.sa_shift = static_cast<int>(a->sa_shift);

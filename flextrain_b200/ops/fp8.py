@@ -246,18 +246,18 @@ def gemm_fp8(a: Fp8Matrix, b: Fp8Matrix, *, trans_a: bool = False, trans_b: bool
 
 def linear_fp8_fwd(x: Fp8Matrix, w: Fp8Matrix, *, bias=None, residual=None, out=None, out_dtype=None):
     """``y = x @ w.T (+ bias) (+ residual)``, ``x`` in row groups, ``w (out, in)`` in blocks (or row groups)."""
-    return gemm_fp8(x, w, trans_b=True, beta=0.0 if residual is None else 1.0, c=residual, bias=bias, out=out, out_dtype=out_dtype)
+    return _ops.gemm_fp8(x, w, trans_b=True, beta=0.0 if residual is None else 1.0, c=residual, bias=bias, out=out, out_dtype=out_dtype)
 
 
 def linear_fp8_dgrad(dy: Fp8Matrix, w: Fp8Matrix, *, out=None, accumulate=False, out_dtype=None):
     """``dx = dy @ w``, ``dy`` in row groups, the same ``w (out, in)`` in blocks read across; optionally accumulated into ``out``."""
-    return gemm_fp8(dy, w, beta=1.0 if accumulate else 0.0, out=out, out_dtype=out_dtype)
+    return _ops.gemm_fp8(dy, w, beta=1.0 if accumulate else 0.0, out=out, out_dtype=out_dtype)
 
 
 def linear_fp8_wgrad(dy: Fp8Matrix, x: Fp8Matrix, gw, *, alpha=1.0, accumulate=True):
     """``gw (out, in) (+)= alpha * dy.T @ x`` of operands in column groups or blocks (the reduction runs over the tokens); ``x`` in
     blocks is the fast form: a scale for each column of the result costs as much again as its sums."""
-    return gemm_fp8(dy, x, trans_a=True, alpha=alpha, beta=1.0 if accumulate else 0.0, out=gw)
+    return _ops.gemm_fp8(dy, x, trans_a=True, alpha=alpha, beta=1.0 if accumulate else 0.0, out=gw)
 
 
 def _offsets(offsets, E: int, like, what: str):
@@ -305,7 +305,8 @@ def grouped_wgrad_fp8(dy: Fp8Matrix, x: Fp8Matrix, offsets, gw, *, alpha: float 
     """``gw[e] += alpha * dy[rows_e].T @ x[rows_e]``, ``dy`` in column groups and ``x`` in those or blocks, ``gw (E, N, K)`` bf16 or
     fp32.  Every expert's segment
     is padded to a multiple of 128 rows with zero rows (``pad``, as the routing plan lays them out), so that no group of 128 tokens
-    lies in two segments.  An expert without rows keeps its ``gw``."""
+    lies in two segments (the library's error word reports offsets that are not, ``device_error_words``).  An expert without rows
+    keeps its ``gw``."""
     _check(dy, "grouped_wgrad_fp8 (dy)")
     _check(x, "grouped_wgrad_fp8 (x)")
     if dy.group != "col" or x.group not in ("col", "block"):

@@ -386,6 +386,50 @@ def test_grouped_wgrad(counts, N, K, dtype, group):
     _no_errors()
 
 
+def test_offsets_that_are_none():
+    """Offsets that descend, that lie outside of the rows or inside a group of 128: nothing outside is read or written, and the last
+    are reported."""
+    ops = _ops()
+    from flextrain_b200.ops import cuda as k
+    torch.manual_seed(0)
+    X, W = ops.quant_fp8(torch.randn(300, 256, device=DEV), "row"), ops.quant_fp8(torch.randn(3, 200, 256, device=DEV), "block")
+    room = torch.full((900, 200), 7.0, device=DEV, dtype=torch.bfloat16)
+    for off in ([-50, 100, 90, 5000], [0, 1 << 30, 0, -1], [300, 300, 300, 300], [400, 500, 600, 700]):
+        ops.grouped_gemm_fp8(X, W, torch.tensor(off, device=DEV, dtype=torch.int32), out=room[300:600])
+        torch.cuda.synchronize()
+        assert torch.all(room[:300] == 7) and torch.all(room[600:] == 7)
+    assert k.device_error_words().get("gemm_fp8", 0) == 0
+    D, X = ops.quant_fp8(torch.randn(300, 200, device=DEV), "col"), ops.quant_fp8(torch.randn(300, 256, device=DEV), "col")
+    gw = torch.zeros(5, 200, 256, device=DEV)
+    ops.grouped_wgrad_fp8(D, X, torch.tensor([-3, 128, 1000], device=DEV, dtype=torch.int32), gw[1:3], pad=128)
+    torch.cuda.synchronize()
+    assert torch.all(gw[0] == 0) and torch.all(gw[3:] == 0)
+    k.device_error_words()
+    ops.grouped_wgrad_fp8(D, X, torch.tensor([0, 100, 300], device=DEV, dtype=torch.int32), gw[1:3], pad=128)
+    torch.cuda.synchronize()
+    assert k.device_error_words()["gemm_fp8"] == 3040 and k.device_error_words()["gemm_fp8"] == 0
+
+
+def test_gemm_in_place_and_expanded():
+    """C that is the result itself or one row for all, results of a single row with any stride, NaN in what is not read."""
+    ops = _ops()
+    torch.manual_seed(0)
+    A, B = ops.quant_fp8(torch.randn(300, 200, device=DEV), "row"), ops.quant_fp8(torch.randn(264, 200, device=DEV), "block")
+    want = ops.linear_fp8_fwd(A, B, out_dtype=torch.float32)
+    row = torch.randn(1, 264, device=DEV)
+    assert torch.equal(ops.gemm_fp8(A, B, trans_b=True, beta=1.0, c=row.expand(300, 264), out_dtype=torch.float32), want + row)
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.randn(300, 264, device=DEV).to(dtype)
+        keep = out.clone()
+        ops.gemm_fp8(A, B, trans_b=True, beta=1.0, c=out, out=out)
+        assert torch.equal(out, (want + keep.float()).to(dtype))
+    one = ops.Fp8Matrix(A.data[:1], A.scale[:1], "row")
+    for out in (torch.empty(264, 1, device=DEV).t(), torch.empty(1, 264, device=DEV).expand(1, 264), torch.empty(1, 270, device=DEV)[:, 3:267]):
+        assert torch.equal(ops.linear_fp8_fwd(one, B, out=out), want[:1])
+    none = torch.full((300, 264), float("nan"), device=DEV)
+    assert torch.equal(ops.gemm_fp8(A, B, trans_b=True, c=none, out=none), want)
+
+
 # --------------------------------------------------------------------------------- together, as used
 def _layer(ops, x, res, gain, w, dy):
     """Norm, projection and their backward pass as a training step runs them: everything that it hands on."""

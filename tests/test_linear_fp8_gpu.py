@@ -25,9 +25,8 @@ def _model(arch, dims, **kw):
 def test_training_step(monkeypatch, arch, dims, kw):
     """The sums of a product of K terms: 2^-24 for each block of 128 and 128 * 2^-23 in a block, of the terms' magnitudes; the result's
     rounding 2^-8 of it, of what is added to it included."""
-    from flextrain_b200.ops import fp8
     seen = {"fwd": 0, "dgrad": 0, "wgrad": 0}
-    real = fp8.gemm_fp8
+    real = ops.gemm_fp8
 
     def checked(a, b, *, trans_a=False, trans_b=False, alpha=1.0, beta=0.0, c=None, bias=None, out=None, out_dtype=None):
         A, B = (ops.dequant_fp8(m, torch.float32).double() for m in (a, b))
@@ -45,7 +44,7 @@ def test_training_step(monkeypatch, arch, dims, kw):
     seqs = ft.SyntheticTokenSource(512, 160, seed=0).get_sequences(640)
     am.fwd_bwd(seqs)
     am.step()
-    monkeypatch.setattr(fp8, "gemm_fp8", checked)
+    monkeypatch.setattr(ops, "gemm_fp8", checked)
     ops.reset_backends_used()
     st = am.fwd_bwd(seqs)
     used = ops.backends_used()
