@@ -31,7 +31,7 @@
 //   16384 x 28672 x 4096      2.37 ms  1625 TFLOP/s      8192 x 4096 x 14336, B across     585 us  1645 TFLOP/s
 //   3001 x 4096 x 14336 + C    237 us  1487 TFLOP/s      4096 x 2048 x 9377, both across   143 us  1100 TFLOP/s (column scales)
 //   14336 x 4096 x 16384      1.21 ms  1590 TFLOP/s (weight gradient, B in blocks)         16 x 4096 x 4096  14 us
-#include <mutex>
+#include <type_traits>
 
 #include "ptx.cuh"
 
@@ -282,103 +282,110 @@ __device__ __forceinline__ void store_d(const Patch& w, int es, int vec, bool ad
 template <bool FP32, bool ROWS, int CG, int NC>
 __device__ __forceinline__ void store_tile(const Params& p, const float (&sum)[NC], const Patch& w, const float* bias, uint8_t* buf,
                                            const CUtensorMap* map, int x, int y, int z, bool add, int lane) {
-  constexpr int ES = FP32 ? 4 : 2, STEP = 128 / ES, STEPS = NC / STEP;
+  constexpr int ES = FP32 ? 4 : 2, STEP = 128 / ES, STEPS = NC / STEP, TURN = STEPS < C_BUFS ? STEPS : C_BUFS;
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int col = column<CG>(i * STEP), cols = w.cols - col;
-    if (cols <= 0) break;
-    uint8_t* at = buf + (i % C_BUFS) * PIECE_BYTES;
+  for (int turn = 0; turn < STEPS; turn += TURN) {         // as many steps at a time as there are pieces
+    if (w.cols <= column<CG>(turn * STEP)) break;
     if (add) {
-      if (i == 0 || i + 1 == STEPS) cp_wait_all();
-      else cp_wait<1>();
+      cp_wait_all();
       __syncwarp();
-    } else if (i >= C_BUFS) {
-      if (lane == 0) bulk_wait_read<C_BUFS - 1>();         // the store of this piece has read it
+    } else if (turn > 0) {
+      if (lane == 0) bulk_wait_read<0>();                  // the stores of the last turn have read the pieces
       __syncwarp();
     }
-    if constexpr (ROWS) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        uint4* pc = piece_at(at, lane, q);
-        uint4 cu = make_uint4(0, 0, 0, 0);
-        if (add) cu = *pc;
-        const uint32_t cw[4] = {cu.x, cu.y, cu.z, cu.w};
-        uint32_t ow[4];
-        constexpr int E = 16 / ES;                       // elements of a piece
-        float v[E];
+    for (int i = turn; i < turn + TURN; ++i) {
+      const int col = column<CG>(i * STEP), cols = w.cols - col;
+      if (cols <= 0) break;
+      uint8_t* at = buf + (i % C_BUFS) * PIECE_BYTES;
+      // (PLAIN: neither C nor bias; the tests for them, element by element, took four times as long as the rest)
+      auto write = [&](auto plain) {
+        constexpr bool PLAIN = decltype(plain)::value;
+        if constexpr (ROWS) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          v[j] = sum[i * STEP + q * E + j] * p.alpha;
-          if (bias != nullptr && q * E + j < cols) v[j] += bias[col + q * E + j];
-        }
+          for (int q = 0; q < 8; ++q) {
+            uint4* pc = piece_at(at, lane, q);
+            constexpr int E = 16 / ES;                     // elements of a piece
+            float v[E];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (FP32) {
-            if (add) v[j] += p.beta * __uint_as_float(cw[j]);
-            ow[j] = __float_as_uint(v[j]);
-          } else {
-            if (add) {
-              v[2 * j] += p.beta * __uint_as_float(cw[j] << 16);
-              v[2 * j + 1] += p.beta * __uint_as_float(cw[j] & 0xFFFF0000u);
-            }
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-            ow[j] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-        }
-        *pc = make_uint4(ow[0], ow[1], ow[2], ow[3]);
-      }
-    } else {
+            for (int j = 0; j < E; ++j) v[j] = sum[i * STEP + q * E + j] * p.alpha;
+            if constexpr (!PLAIN) {
+              if (bias != nullptr) {
 #pragma unroll
-      for (int c = 0; c < STEP; c += 32)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int e0 = c + 8 * j + 2 * (lane & 3);       // in the step
-          float b0 = 0.f, b1 = 0.f;
-          if (bias != nullptr && e0 < cols) b0 = bias[col + e0];
-          if (bias != nullptr && e0 + 1 < cols) b1 = bias[col + e0 + 1];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {                    // rows 8 k + (lane >> 2)
-            const float* f = &sum[((i * STEP + c) / 32 * 2 + (k >> 1)) * 16 + 4 * j + 2 * (k & 1)];
-            float v0 = f[0] * p.alpha + b0, v1 = f[1] * p.alpha + b1;
-            uint8_t* to = byte_at(at, 8 * k + (lane >> 2), e0 * ES);
-            if constexpr (FP32) {
-              if (add) {
-                const float2 cc = *reinterpret_cast<const float2*>(to);
-                v0 += p.beta * cc.x;
-                v1 += p.beta * cc.y;
+                for (int j = 0; j < E; ++j)
+                  if (q * E + j < cols) v[j] += bias[col + q * E + j];
               }
-              *reinterpret_cast<float2*>(to) = make_float2(v0, v1);
-            } else {
               if (add) {
-                const float2 cc = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(to));
-                v0 += p.beta * cc.x;
-                v1 += p.beta * cc.y;
+                const uint4 cu = *pc;
+                const uint32_t cw[4] = {cu.x, cu.y, cu.z, cu.w};
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                  v[j] += p.beta * __uint_as_float(FP32 ? cw[j % 4] : j & 1 ? cw[j / 2] & 0xFFFF0000u : cw[j / 2] << 16);
               }
-              *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(v0, v1);
             }
+            uint32_t ow[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if constexpr (FP32) {
+                ow[j] = __float_as_uint(v[j]);
+              } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+                ow[j] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+            }
+            *pc = make_uint4(ow[0], ow[1], ow[2], ow[3]);
           }
+        } else {
+#pragma unroll
+          for (int c = 0; c < STEP; c += 32)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int e0 = c + 8 * j + 2 * (lane & 3);     // in the step
+              float b0 = 0.f, b1 = 0.f;
+              if constexpr (!PLAIN) {
+                if (bias != nullptr && e0 < cols) b0 = bias[col + e0];
+                if (bias != nullptr && e0 + 1 < cols) b1 = bias[col + e0 + 1];
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {                  // rows 8 k + (lane >> 2)
+                const float* f = &sum[((i * STEP + c) / 32 * 2 + (k >> 1)) * 16 + 4 * j + 2 * (k & 1)];
+                float v0 = f[0] * p.alpha + b0, v1 = f[1] * p.alpha + b1;
+                uint8_t* to = byte_at(at, 8 * k + (lane >> 2), e0 * ES);
+                if constexpr (!PLAIN) {
+                  if (add) {
+                    const float2 cc = FP32 ? *reinterpret_cast<const float2*>(to) : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(to));
+                    v0 += p.beta * cc.x;
+                    v1 += p.beta * cc.y;
+                  }
+                }
+                if constexpr (FP32) *reinterpret_cast<float2*>(to) = make_float2(v0, v1);
+                else *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(v0, v1);
+              }
+            }
         }
+      };
+      if (bias == nullptr && !add) write(std::true_type());
+      else write(std::false_type());
     }
-    if (map != nullptr) {
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) {
-        if (FP32 && p.add_in_place) tma_add_3d(map, at, x + col, y, z);
-        else tma_store_3d(map, at, x + col, y, z);
-        bulk_commit();
-      }
-    } else {
-      __syncwarp();
-      store_d(w, ES, p.vec, FP32 && p.add_in_place, col, at, lane);
-      __syncwarp();
+    if (map != nullptr) fence_proxy_async();
+    __syncwarp();
+#pragma unroll
+    for (int i = turn; i < turn + TURN; ++i) {
+      const int col = column<CG>(i * STEP);
+      if (w.cols <= col) break;
+      uint8_t* at = buf + (i % C_BUFS) * PIECE_BYTES;
+      if (map == nullptr) store_d(w, ES, p.vec, FP32 && p.add_in_place, col, at, lane);
+      else if (lane == 0 && FP32 && p.add_in_place) tma_add_3d(map, at, x + col, y, z);
+      else if (lane == 0) tma_store_3d(map, at, x + col, y, z);
     }
-    if (add) {
-      if (i + C_BUFS < STEPS && w.cols > column<CG>((i + C_BUFS) * STEP)) {
-        if (lane == 0) bulk_wait_read<0>();
-        __syncwarp();
-        fetch_c(w, ES, p.vec, column<CG>((i + C_BUFS) * STEP), at, lane);
-      }
-      cp_commit();
+    if (map == nullptr) __syncwarp();
+    else if (lane == 0) bulk_commit();
+    if (add && turn + TURN < STEPS) {
+      if (lane == 0) bulk_wait_read<0>();
+      __syncwarp();
+#pragma unroll
+      for (int i = turn + TURN; i < turn + 2 * TURN; ++i)
+        if (w.cols > column<CG>(i * STEP)) fetch_c(w, ES, p.vec, column<CG>(i * STEP), buf + (i % C_BUFS) * PIECE_BYTES, lane);
     }
   }
 }
