@@ -124,9 +124,11 @@ struct QuantParams {
   int vec;
 };
 
-// One block per tile of 128 x 128: a thread holds 8 columns of 8 rows that lie 16 apart, so that a warp reads 256 bytes of two
+// Bound by memory: 16384 x 4096 bf16, 203 MB, 37 us (5.5 TB/s; the measured copy 6.5) in rows and columns, 36 in squares; fp32 of half
+// the rows 33 us (5.1 TB/s).  One block per tile of 128 x 128: a thread holds 8 columns of 8 rows that lie 16 apart, so that a warp reads 256 bytes of two
 // rows at a time and the tile's groups are inside the block.  The elements stay packed as they came until they are converted, so
-// that four blocks fit an SM (two for fp32).
+// that four blocks fit an SM (two for fp32): unpacked in registers two fit, with each row's divisions in all of its lanes, and the
+// rows took 123 us.
 template <int GROUP, typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quant_kernel(const QuantParams p) {
   using R = Raw<T>;
@@ -276,19 +278,22 @@ __device__ __forceinline__ float max_abs(float a, float b) {
   return r;
 }
 
-// Eight elements of x and the residual as they came
+// Eight elements of x, and of the residual where there is one, as they came
+template <bool RES>
 struct NormIn {
-  Raw<bf16> x, r;
+  Raw<bf16> x[RES ? 2 : 1];
   __device__ __forceinline__ void load(const NormParams& p, long row, int c) {
-    x.load(p.x + row * p.ldx, c, p.D, p.vec);
-    if (p.res != nullptr) r.load(p.res + row * p.ldr, c, p.D, p.vec);
+    x[0].load(p.x + row * p.ldx, c, p.D, p.vec);
+    if constexpr (RES) x[1].load(p.res + row * p.ldr, c, p.D, p.vec);
   }
 };
 // h of them, written where there is a residual; adds the squares
-__device__ __forceinline__ uint4 norm_h(const NormParams& p, const NormIn& in, long row, int c, f32x2& ss) {
-  uint4 h = in.x.u;
-  if (p.res != nullptr) {
-    const uint32_t xs[4] = {h.x, h.y, h.z, h.w}, rs[4] = {in.r.u.x, in.r.u.y, in.r.u.z, in.r.u.w};
+template <bool RES>
+__device__ __forceinline__ uint4 norm_h(const NormParams& p, const NormIn<RES>& in, long row, int c, f32x2& ss) {
+  uint4 h = in.x[0].u;
+  if constexpr (RES) {
+    const uint4 r = in.x[1].u;
+    const uint32_t xs[4] = {h.x, h.y, h.z, h.w}, rs[4] = {r.x, r.y, r.z, r.w};
     uint32_t hs[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -369,10 +374,14 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
 
 constexpr int NORM_THREADS = 768;    // of an SM: blocks of NT threads
 
+// Bound by memory with a residual: 16384 x 4096, 472 MB, 75 us (6.3 TB/s); without one, 201 MB, 45 us (4.5 TB/s), half by the chain of
+// a row's sum, scale and conversion.  A block for each row, which read the gain again and waited for its loads, took 99 and 67 us;
+// blocks of 128 threads 99 and 70, of 512 82 and 56.
+//
 // V > 0: a block of NT threads walks over rows of up to 8 NT V elements, its part of the gain in registers, the next row's
-// elements asked for before the current row's sum is known.  V = 0: longer rows are read twice (the second time h comes from what
+// elements asked for before the current row's sum is known (two rows ahead gained nothing).  V = 0: longer rows are read twice (the second time h comes from what
 // the first pass wrote, by the same thread).
-template <int NT, int V>
+template <int NT, int V, bool RES>
 __global__ void __launch_bounds__(NT, NORM_THREADS / NT) rmsnorm_fp8_kernel(const NormParams p) {
   __shared__ float sh[2][NT / 32];
   const float rD = 1.f / static_cast<float>(p.D);
@@ -387,7 +396,7 @@ __global__ void __launch_bounds__(NT, NORM_THREADS / NT) rmsnorm_fp8_kernel(cons
   };
   if constexpr (V > 0) {
     f32x2 w[V][4];
-    NormIn in[V];
+    NormIn<RES> in[V];
     long row = blockIdx.x;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -411,7 +420,7 @@ __global__ void __launch_bounds__(NT, NORM_THREADS / NT) rmsnorm_fp8_kernel(cons
       row = next;
     }
   } else {
-    NormIn in;
+    NormIn<RES> in;
     for (long row = blockIdx.x; row < p.T; row += gridDim.x) {
       f32x2 ss = 0, w[4];
       for (int c0 = 0; c0 < p.D; c0 += 8 * NT) {
@@ -421,10 +430,11 @@ __global__ void __launch_bounds__(NT, NORM_THREADS / NT) rmsnorm_fp8_kernel(cons
       const float r = rstd_of(ss, row);
       for (int c0 = 0; c0 < p.D; c0 += 8 * NT) {
         const int c = c0 + threadIdx.x * 8;
-        if (p.res != nullptr) in.x.load(p.h + row * p.D, c, p.D, p.vec);
-        else in.x.load(p.x + row * p.ldx, c, p.D, p.vec);
+        Raw<bf16> h;
+        if constexpr (RES) h.load(p.h + row * p.D, c, p.D, p.vec);
+        else h.load(p.x + row * p.ldx, c, p.D, p.vec);
         norm_gain(p, c, w);
-        norm_q(p, in.x.u, w, row, c, r);
+        norm_q(p, h.u, w, row, c, r);
       }
     }
   }
@@ -433,7 +443,9 @@ __global__ void __launch_bounds__(NT, NORM_THREADS / NT) rmsnorm_fp8_kernel(cons
 template <int NT, int V>
 int launch_norm(const NormParams& p, cudaStream_t stream) {
   const int most = 148 * (NORM_THREADS / NT);
-  rmsnorm_fp8_kernel<NT, V><<<p.T < most ? p.T : most, NT, 0, stream>>>(p);
+  const int grid = p.T < most ? p.T : most;
+  if (p.res != nullptr) rmsnorm_fp8_kernel<NT, V, true><<<grid, NT, 0, stream>>>(p);
+  else rmsnorm_fp8_kernel<NT, V, false><<<grid, NT, 0, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : -400;
 }
 

@@ -560,6 +560,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const float *sa = nullptr, *sb = nullptr;            // of the next block to be asked for
     [[maybe_unused]] long sb_seg = 0;
     int asked = 0;
+    [[maybe_unused]] int sb_left = 0;
     // scales of the next blocks, asked for that much before they are needed: in registers (a row's, and those of its blocks of
     // columns), or, of columns, in shared memory
     [[maybe_unused]] float a_next[AHEAD], b_next[SEG][AHEAD];
@@ -571,8 +572,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         if (there) {
 #pragma unroll
           for (int j = 0; j < HALF / 32; ++j) {
-            const int n = t.tn * BN + part * SEG_COLS + column<CG>(32 * j) + lane;
-            cp_async4(at + 32 * j, sb + (n < p.N ? n * p.sb_n : 0), n < p.N);
+            const bool in = column<CG>(32 * j) < sb_left;
+            cp_async4(at + 32 * j, sb + (in ? column<CG>(32 * j) * p.sb_n : 0), in);
           }
           cp_async4(at + HALF, sa, true);
         }
@@ -595,6 +596,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       // (rows and columns outside read a scale that exists; what they compute is not stored)
       sa = p.sa + (min(t.row0 + in_tile + lane, p.M - 1) >> p.sa_shift) * p.sa_m + t.kb0 * p.sa_k;
       sb = p.sb + t.kb0 * p.sb_k + (p.mode == 1 ? t.g * p.sb_g : 0);
+      if constexpr (BVEC) {
+        const int n = t.tn * BN + part * SEG_COLS + lane;
+        sb_left = p.N - n;
+        if (sb_left > 0) sb += n * p.sb_n;
+      }
       if constexpr (!BVEC) {
         const int n0 = t.tn * BN + part * SEG_COLS;
         sb += (min(n0, p.N - 1) >> 7) * p.sb_n;
@@ -669,19 +675,21 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           for (int k = 0; k < 4; ++k) a[k] = s[HALF + 8 * k + (lane >> 2)];
           tmem_ld_wait();
           constexpr int CHUNKS = HALF / 16;
-          float2 f[4];
+          float2 f[2][4];
+          auto columns = [&](int g) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[g & 1][j] = *reinterpret_cast<const float2*>(s + g * 32 + 8 * j + 2 * (lane & 3));
+          };
+          columns(0);
 #pragma unroll
           for (int q = 0; q < CHUNKS; ++q) {             // 32 columns of lanes 0 to 15, of lanes 16 to 31
             if (q + 1 < CHUNKS) tmem_ld_16x32(taddr + (q + 1) / 2 * 32 + (((q + 1) & 1) << 20), r[(q + 1) & 1]);
             if (q + 1 == CHUNKS) ready = mbar_test(&tfull[wrap ? 0 : acc + 1], acc_phase ^ wrap);
-            if (q % 2 == 0) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const float2*>(s + q / 2 * 32 + 8 * j + 2 * (lane & 3));
-            }
+            if (q % 2 == 1 && q + 1 < CHUNKS) columns(q / 2 + 1);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) mul_add2(&sum[q * 16 + 4 * j + 2 * e], &r[q & 1][4 * j + 2 * e], f[j], a[2 * (q & 1) + e]);
+              for (int e = 0; e < 2; ++e) mul_add2(&sum[q * 16 + 4 * j + 2 * e], &r[q & 1][4 * j + 2 * e], f[q / 2 & 1][j], a[2 * (q & 1) + e]);
             if (q + 1 < CHUNKS) tmem_ld_wait();
             if (q + 2 == CHUNKS) release();
           }
