@@ -2,7 +2,8 @@
 
     python -m flextrain_b200.bench.kernel_cases gemm_fwd|gemm_dgrad|gemm_wgrad|rmsnorm_bwd|softmax_ce|attn_fwd|attn_bwd|
                                                   attn_fwd_one_tile|attn_bwd_unordered|attn_bwd_thread_reds|attn_fwd_32k|attn_bwd_32k|attn_bwd_32k_thread_reds|gdn_fwd|gdn_bwd|
-                                                  gdn_long_fwd|rope|ffn_glu_fwd|ffn_glu_bwd|moe_grouped_gemm|moe_grouped_wgrad|moe_plan|gdn_fla_fwd|attn_fa2_fwd|attn_fa2_bwd|attn_fa2_fwd_32k|attn_fa2_bwd_32k
+                                                  gdn_long_fwd|rope|ffn_glu_fwd|ffn_glu_bwd|moe_grouped_gemm|moe_grouped_wgrad|moe_plan|gdn_fla_fwd|attn_fa2_fwd|attn_fa2_bwd|attn_fa2_fwd_32k|attn_fa2_bwd_32k|
+                                                  fp8_fwd|fp8_dgrad|fp8_wgrad|fp8_quant|fp8_rmsnorm
 
 Each case holds a few hundred MB on the device (inputs larger than the 126 MB L2), runs three warm-up launches and
 ten timed launches with CUDA events, and prints achieved TFLOP/s or GB/s.  They are the commands behind the
@@ -207,6 +208,26 @@ def main(case: str) -> None:
         sep = _time(two)
         print(f"{case}: M={M} K={K} F={F}  fused {fused:.3f} ms ({fl / fused / 1e9:.0f} TFLOP/s)  "
               f"GEMM + activation pass {sep:.3f} ms")
+    elif case in ("fp8_fwd", "fp8_dgrad", "fp8_wgrad"):
+        # a gated FFN's up projection in 8 bits, one 16,384-token chunk: forward, input gradient, weight gradient
+        M, N, K = {"fp8_fwd": (16384, 28672, 4096), "fp8_dgrad": (16384, 4096, 28672), "fp8_wgrad": (28672, 4096, 16384)}[case]
+        a = torch.randn(*((K, M) if case == "fp8_wgrad" else (M, K)), device=dev, dtype=bf)
+        b = torch.randn(*((N, K) if case == "fp8_fwd" else (K, N)), device=dev, dtype=bf)
+        a, b = ops.quant_fp8(a, "col" if case == "fp8_wgrad" else "row"), ops.quant_fp8(b, "block")
+        out = torch.empty(M, N, device=dev, dtype=bf)
+        ms = _time(lambda: ops.gemm_fp8(a, b, trans_a=case == "fp8_wgrad", trans_b=case == "fp8_fwd", out=out))
+        print(f"{case}: M={M} N={N} K={K}  {ms:.3f} ms  {2.0 * M * N * K / ms / 1e9:.0f} TFLOP/s")
+    elif case in ("fp8_quant", "fp8_rmsnorm"):
+        T, D = 16384, 4096
+        x, r = torch.randn(T, D, device=dev, dtype=bf), torch.randn(T, D, device=dev, dtype=bf)
+        w = torch.ones(D, device=dev)
+        if case == "fp8_rmsnorm":
+            ms = _time(lambda: ops.rmsnorm_fp8_fwd(x, w, 1e-5, residual=r))
+            print(f"{case}: T={T} D={D} with a residual  {ms:.3f} ms  {7.0 * T * D / ms / 1e6:.0f} GB/s")
+        else:
+            for group in ("row", "col", "block"):
+                ms = _time(lambda: ops.quant_fp8(x, group))
+                print(f"{case}: T={T} D={D} {group}  {ms:.3f} ms  {3.0 * T * D / ms / 1e6:.0f} GB/s")
     else:
         raise SystemExit(f"unknown case {case}")
     print("device error words:", k.device_error_words())

@@ -25,8 +25,34 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
   return static_cast<uint32_t>(hi) << 16 | lo;
 }
-__device__ __forceinline__ uint2 e4m3x8(const float (&f)[8], float inv) {
-  return make_uint2(e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv), e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 widen(uint32_t w) { return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+__device__ __forceinline__ uint32_t e4m3x4(f32x2 lo, f32x2 hi) {
+  float a, b, c, d;
+  unpack2(lo, a, b);
+  unpack2(hi, c, d);
+  return e4m3x4(a, b, c, d);
 }
 
 // the scale of a group from the bits of its largest magnitude (NaN stays NaN: the comparison is false for it)
@@ -35,14 +61,6 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
   return s < 1.17549435e-38f ? 1.17549435e-38f : s;
 }
 
-__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
-}
 // Eight elements from column c of a row of n: 16-byte loads where the row allows them, zeros behind its end.
 __device__ __forceinline__ void load8(const float* row, int c, int n, bool vec, float (&f)[8]) {
   if (vec && c + 8 <= n) {
@@ -85,7 +103,7 @@ struct Raw<bf16> {
   // the larger of a word's two, as the bits of an fp32 number
   __device__ static __forceinline__ uint32_t single(uint32_t t) { return max(t << 16, t & 0xFFFF0000u); }
   __device__ static __forceinline__ uint32_t column(uint32_t t, int j) { return j & 1 ? t & 0xFFFF0000u : t << 16; }
-  __device__ __forceinline__ void values(float (&f)[8]) const { unpack8(u, f); }
+  __device__ __forceinline__ f32x2 pair(int i) const { return widen(i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w); }
 };
 template <>
 struct Raw<float> {
@@ -106,10 +124,7 @@ struct Raw<float> {
   }
   __device__ static __forceinline__ uint32_t single(uint32_t t) { return t; }
   __device__ static __forceinline__ uint32_t column(uint32_t t, int) { return t; }
-  __device__ __forceinline__ void values(float (&v)[8]) const {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = f[j];
-  }
+  __device__ __forceinline__ f32x2 pair(int i) const { return pack2(f[2 * i], f[2 * i + 1]); }
 };
 
 struct QuantParams {
@@ -214,14 +229,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quant_kernel(cons
   for (int i = 0; i < 8; ++i) {
     const int row = tm * G + r0 + 16 * i;
     if (row >= p.M) break;
-    float f[8];
-    raw[i].values(f);
-    uint2 o;
-    if constexpr (GROUP == 1)
-      o = make_uint2(e4m3x4(f[0] * inv[0], f[1] * inv[1], f[2] * inv[2], f[3] * inv[3]),
-                     e4m3x4(f[4] * inv[4], f[5] * inv[5], f[6] * inv[6], f[7] * inv[7]));
-    else
-      o = e4m3x8(f, inv[GROUP == 0 ? i : 0]);
+    f32x2 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x2 k = GROUP == 1 ? pack2(inv[2 * j], inv[2 * j + 1]) : pack2(inv[GROUP == 0 ? i : 0], inv[GROUP == 0 ? i : 0]);
+      v[j] = mul2(raw[i].pair(j), k);
+    }
+    const uint2 o = make_uint2(e4m3x4(v[0], v[1]), e4m3x4(v[2], v[3]));
     *reinterpret_cast<uint2*>(q + row * p.ldq + c) = o;
   }
 }
@@ -248,29 +262,6 @@ struct NormParams {
   int vec_w;
 };
 
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float a, float b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpack2(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 widen(uint32_t w) { return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
 // the largest magnitude; NaN if one is
 __device__ __forceinline__ float max_abs(float a, float b) {
   float r;
