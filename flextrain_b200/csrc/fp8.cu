@@ -61,12 +61,51 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
   return s < 1.17549435e-38f ? 1.17549435e-38f : s;
 }
 
+// Eight bf16 elements from wherever they start, in the largest pieces that may be read there.
+__device__ __forceinline__ uint4 load8_any(const uint16_t* x) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(x);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(x);
+  if ((at & 7) == 0) {
+    const uint2 a = *reinterpret_cast<const uint2*>(x), b = *reinterpret_cast<const uint2*>(x + 4);
+    return make_uint4(a.x, a.y, b.x, b.y);
+  }
+  if ((at & 3) == 0) return make_uint4(w[0], w[1], w[2], w[3]);
+  const uint32_t first = x[0], last = x[7];
+  w = reinterpret_cast<const uint32_t*>(x + 1);
+  const uint32_t a = w[0], b = w[1], c = w[2];
+  return make_uint4(first | a << 16, a >> 16 | b << 16, b >> 16 | c << 16, c >> 16 | last << 16);
+}
+__device__ __forceinline__ void store8_any(uint16_t* x, const uint4& u) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(x);
+  uint32_t* w = reinterpret_cast<uint32_t*>(x);
+  if ((at & 7) == 0) {
+    *reinterpret_cast<uint2*>(x) = make_uint2(u.x, u.y);
+    *reinterpret_cast<uint2*>(x + 4) = make_uint2(u.z, u.w);
+  } else if ((at & 3) == 0) {
+    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+  } else {
+    x[0] = static_cast<uint16_t>(u.x);
+    w = reinterpret_cast<uint32_t*>(x + 1);
+    w[0] = u.x >> 16 | u.y << 16;
+    w[1] = u.y >> 16 | u.z << 16;
+    w[2] = u.z >> 16 | u.w << 16;
+    x[7] = static_cast<uint16_t>(u.w >> 16);
+  }
+}
+
 // Eight elements from column c of a row of n: 16-byte loads where the row allows them, zeros behind its end.
 __device__ __forceinline__ void load8(const float* row, int c, int n, bool vec, float (&f)[8]) {
   if (vec && c + 8 <= n) {
     const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
     f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  } else if (c + 8 <= n && (reinterpret_cast<uintptr_t>(row) & 7) == 0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 a = *reinterpret_cast<const float2*>(row + c + 2 * j);
+      f[2 * j] = a.x;
+      f[2 * j + 1] = a.y;
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = c + j < n ? row[c + j] : 0.f;
@@ -88,6 +127,8 @@ struct Raw<bf16> {
   __device__ __forceinline__ void load(const bf16* row, int c, int n, bool vec) {
     if (vec && c + 8 <= n) {
       u = *reinterpret_cast<const uint4*>(row + c);
+    } else if (c + 8 <= n) {
+      u = load8_any(reinterpret_cast<const uint16_t*>(row + c));
     } else {
       uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -297,6 +338,8 @@ __device__ __forceinline__ uint4 norm_h(const NormParams& p, const NormIn<RES>& 
     uint16_t* to = reinterpret_cast<uint16_t*>(p.h) + row * p.D + c;
     if (p.vec && c + 8 <= p.D) {
       *reinterpret_cast<uint4*>(to) = h;
+    } else if (c + 8 <= p.D) {
+      store8_any(to, h);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -363,7 +406,10 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
   return v;
 }
 
-constexpr int NORM_THREADS = 768;    // of an SM: blocks of NT threads
+// Threads of an SM, in blocks of NT: what fits with a row's pieces and the gain's in registers.  16384 x 2048 with a residual and
+// without: 43 and 27 us with 1024, 47 and 32 with 768; x 4096 84 / 43 and 75 / 43; x 8192 (half the rows) 77 / 41 with 512 in blocks
+// of 256, 82 / 45 with 1024 in blocks of 512.
+constexpr int norm_threads(int V) { return V > 2 ? 512 : V == 2 ? 768 : 1024; }
 
 // Bound by memory with a residual: 16384 x 4096, 472 MB, 75 us (6.3 TB/s); without one, 201 MB, 45 us (4.5 TB/s), half by the chain of
 // a row's sum, scale and conversion.  A block for each row, which read the gain again and waited for its loads, took 99 and 67 us;
@@ -373,7 +419,7 @@ constexpr int NORM_THREADS = 768;    // of an SM: blocks of NT threads
 // elements asked for before the current row's sum is known (two rows ahead gained nothing).  V = 0: longer rows are read twice (the second time h comes from what
 // the first pass wrote, by the same thread).
 template <int NT, int V, bool RES>
-__global__ void __launch_bounds__(NT, NORM_THREADS / NT) rmsnorm_fp8_kernel(const NormParams p) {
+__global__ void __launch_bounds__(NT, norm_threads(V) / NT) rmsnorm_fp8_kernel(const NormParams p) {
   __shared__ float sh[2][NT / 32];
   const float rD = 1.f / static_cast<float>(p.D);
   int turn = 0;
@@ -433,7 +479,7 @@ __global__ void __launch_bounds__(NT, NORM_THREADS / NT) rmsnorm_fp8_kernel(cons
 
 template <int NT, int V>
 int launch_norm(const NormParams& p, cudaStream_t stream) {
-  const int most = 148 * (NORM_THREADS / NT);
+  const int most = 148 * (norm_threads(V) / NT);
   const int grid = p.T < most ? p.T : most;
   if (p.res != nullptr) rmsnorm_fp8_kernel<NT, V, true><<<grid, NT, 0, stream>>>(p);
   else rmsnorm_fp8_kernel<NT, V, false><<<grid, NT, 0, stream>>>(p);
@@ -511,7 +557,8 @@ int ftb_rmsnorm_fp8_fwd(const NormArgs* a) {
   if (p.D <= 1024) return launch_norm<128, 1>(p, a->stream);
   if (p.D <= 2048) return launch_norm<256, 1>(p, a->stream);
   if (p.D <= 4096) return launch_norm<256, 2>(p, a->stream);
-  if (p.D <= 8192) return launch_norm<512, 2>(p, a->stream);
+  if (p.D <= 6144) return launch_norm<256, 3>(p, a->stream);
+  if (p.D <= 8192) return launch_norm<256, 4>(p, a->stream);
   return launch_norm<256, 0>(p, a->stream);
 }
 

@@ -244,12 +244,28 @@ __device__ __forceinline__ void fetch_c(const Patch& w, int es, int vec, int col
     for (int k = 0; k < 8; ++k)
       if (k * 4 + lr < w.rows && lp * 16 < bytes) cp_async16(piece_at(buf, k * 4 + lr, lp), c + (k * 4 + lr) * w.ldc + lp * 16);
   } else if (es == 4) {
-    for (int r = 0; r < w.rows; ++r)
-      if (lane * 4 < bytes) *reinterpret_cast<float*>(byte_at(buf, r, lane * 4)) = *reinterpret_cast<const float*>(c + r * w.ldc + lane * 4);
+    if (lane * 4 < bytes)
+      for (int r = 0; r < w.rows; ++r) cp_async4(byte_at(buf, r, lane * 4), c + r * w.ldc + lane * 4, true);
   } else {
-    for (int r = 0; r < w.rows; ++r)
-      for (int e = lane; e * 2 < bytes; e += 32)
-        *reinterpret_cast<uint16_t*>(byte_at(buf, r, e * 2)) = *reinterpret_cast<const uint16_t*>(c + r * w.ldc + e * 2);
+    // two elements of a row for each lane: as one copy where the row starts on four bytes, else four rows' loads before their stores
+    const int at = lane * 4, n = min(2, (bytes - at) >> 1);
+    for (int r0 = 0; r0 < w.rows; r0 += 4) {
+      uint32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint16_t* from = reinterpret_cast<const uint16_t*>(c + (r0 + i) * w.ldc + at);
+        v[i] = 0;
+        if (r0 + i >= w.rows || n <= 0) continue;
+        if (n == 2 && (reinterpret_cast<uintptr_t>(from) & 3) == 0) cp_async4(byte_at(buf, r0 + i, at), from, true);
+        else v[i] = n == 2 ? from[0] | static_cast<uint32_t>(from[1]) << 16 : from[0];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint16_t* from = reinterpret_cast<const uint16_t*>(c + (r0 + i) * w.ldc + at);
+        if (r0 + i < w.rows && n > 0 && !(n == 2 && (reinterpret_cast<uintptr_t>(from) & 3) == 0))
+          *reinterpret_cast<uint32_t*>(byte_at(buf, r0 + i, at)) = v[i];
+      }
+    }
   }
 }
 // (add: to what lies there, in fp32)
@@ -257,21 +273,36 @@ __device__ __forceinline__ void store_d(const Patch& w, int es, int vec, bool ad
   const int bytes = min(128, (w.cols - col) * es);
   uint8_t* d = w.d + col * es;
   if (es == 4 && (add || !vec)) {
-    for (int r = 0; r < w.rows; ++r)
-      if (lane * 4 < bytes) {
+    if (lane * 4 < bytes) {
+#pragma unroll 4
+      for (int r = 0; r < w.rows; ++r) {
         float* to = reinterpret_cast<float*>(d + r * w.ldd + lane * 4);
         const float v = *reinterpret_cast<const float*>(byte_at(buf, r, lane * 4));
-        *to = add ? *to + v : v;
+        // (each element is added to once: the order of the additions is that of the launches)
+        if (add) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(to), "f"(v) : "memory");
+        else *to = v;
       }
+    }
   } else if (vec) {
     const int lr = lane >> 3, lp = lane & 7;
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (k * 4 + lr < w.rows && lp * 16 < bytes) *reinterpret_cast<uint4*>(d + (k * 4 + lr) * w.ldd + lp * 16) = *piece_at(buf, k * 4 + lr, lp);
   } else {
-    for (int r = 0; r < w.rows; ++r)
-      for (int e = lane; e * 2 < bytes; e += 32)
-        *reinterpret_cast<uint16_t*>(d + r * w.ldd + e * 2) = *reinterpret_cast<const uint16_t*>(byte_at(buf, r, e * 2));
+    const int at = lane * 4, n = min(2, (bytes - at) >> 1);
+    if (n > 0) {
+#pragma unroll 4
+      for (int r = 0; r < w.rows; ++r) {
+        uint16_t* to = reinterpret_cast<uint16_t*>(d + r * w.ldd + at);
+        const uint32_t v = *reinterpret_cast<const uint32_t*>(byte_at(buf, r, at));
+        if (n == 2 && (reinterpret_cast<uintptr_t>(to) & 3) == 0) {
+          *reinterpret_cast<uint32_t*>(to) = v;
+        } else {
+          to[0] = static_cast<uint16_t>(v);
+          if (n == 2) to[1] = static_cast<uint16_t>(v >> 16);
+        }
+      }
+    }
   }
 }
 
