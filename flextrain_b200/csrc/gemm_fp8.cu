@@ -695,29 +695,34 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       float sum[HALF];
 #pragma unroll
       for (int i = 0; i < HALF; ++i) sum[i] = 0.f;
+      auto release = [&] {                               // the last of a block's values are in registers
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 2) mbar_arrive_leader(&tempty[acc]);
+          else mbar_arrive(&tempty[acc]);
+        }
+      };
+      // Warps of which nothing is stored leave their values where they are.
 #pragma unroll 1
-      for (int kb = 0; kb < kbs; ++kb) {
+      for (int kb = rows == 0 ? 0 : kbs; kb < kbs; ++kb) {
+        if (!ready && !(ok = mbar_wait(&tfull[acc], acc_phase, abort_flag, 30))) break;
+        ready = false;
+        if constexpr (BVEC) {
+          cp_wait<AHEAD - 1>();
+          __syncwarp();
+        }
+        ask(AHEAD - 1);
+        release();
+        if (++acc == NACC) { acc = 0; acc_phase ^= 1; }
+      }
+#pragma unroll 1
+      for (int kb = rows == 0 ? kbs : 0; kb < kbs; ++kb) {
         if (!ready && !(ok = mbar_wait(&tfull[acc], acc_phase, abort_flag, 30))) break;
         tc_fence_after();
         const uint32_t taddr = tmem_part + acc * HALF;
         const bool wrap = acc + 1 == NACC;
-        auto release = [&] {                             // the last of this block's values are in registers
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (CG == 2) mbar_arrive_leader(&tempty[acc]);
-            else mbar_arrive(&tempty[acc]);
-          }
-        };
-        if (rows == 0) {                                 // nothing of this warp's is stored: its values stay where they are
-          if constexpr (BVEC) {
-            cp_wait<AHEAD - 1>();
-            __syncwarp();
-          }
-          ask(AHEAD - 1);
-          release();
-          ready = mbar_test(&tfull[wrap ? 0 : acc + 1], acc_phase ^ wrap);
-        } else if constexpr (BVEC) {
+        if constexpr (BVEC) {
           uint32_t r[2][16];
           tmem_ld_16x32(taddr, r[0]);
           cp_wait<AHEAD - 1>();
