@@ -86,6 +86,8 @@ def _empty_q(shape, device):
     """e4m3 room for ``shape`` with rows on 16 bytes, as the products read them; the pieces behind a row's end hold nothing."""
     n = shape[-1]
     if n % 16 == 0:
+        if len(shape) == 2:
+            return torch.empty_strided(shape, (n, 1), dtype=FP8, device=device)     # (1.5 us on the host for 2.4 of torch.empty)
         return torch.empty(shape, dtype=FP8, device=device)
     return torch.empty(*shape[:-1], (n + 15) // 16 * 16, dtype=FP8, device=device)[..., :n]
 
@@ -193,11 +195,11 @@ def _on_grid(q):
 
 def _result(out, M: int, N: int, dtype, like, what: str):
     if out is None:
-        return torch.empty((M, N), dtype=dtype, device=like.device)
+        return torch.empty_strided((M, N), (N, 1), dtype=dtype, device=like.device)
     if out.shape != (M, N) or (out.dtype is not BF16 and out.dtype is not F32) or out.get_device() != like.get_device() or \
-            (out.stride(-1) != 1 and N > 1):
+            (out.stride(-1) != 1 and N > 1) or (M > 1 and out.stride(0) < N):
         raise ValueError(f"{what}: out {tuple(out.shape)} {out.dtype} on {out.device}, strides {out.stride()}; "
-                         f"{(M, N)} in bf16 or fp32 with contiguous rows on {like.device}")
+                         f"{(M, N)} in bf16 or fp32 with contiguous rows, none over another, on {like.device}")
     return out
 
 
@@ -303,8 +305,7 @@ def grouped_gemm_fp8(x: Fp8Matrix, w: Fp8Matrix, offsets, *, trans_w: bool = Tru
 
 def grouped_wgrad_fp8(dy: Fp8Matrix, x: Fp8Matrix, offsets, gw, *, alpha: float = 1.0, pad: int = 1):
     """``gw[e] += alpha * dy[rows_e].T @ x[rows_e]``, ``dy`` in column groups and ``x`` in those or blocks, ``gw (E, N, K)`` bf16 or
-    fp32.  Every expert's segment
-    is padded to a multiple of 128 rows with zero rows (``pad``, as the routing plan lays them out), so that no group of 128 tokens
+    fp32.  Every expert's segment is padded to a multiple of 128 rows with zero rows (``pad``, as the routing plan lays them out), so that no group of 128 tokens
     lies in two segments (the library's error word reports offsets that are not, ``device_error_words``).  An expert without rows
     keeps its ``gw``."""
     _check(dy, "grouped_wgrad_fp8 (dy)")

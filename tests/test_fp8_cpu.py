@@ -131,6 +131,8 @@ def _m(groups, M, N, **over):
     lambda: ops.gemm_fp8(_m("row", 4, 8), _m("block", 8, 4), out=torch.ones(4, 4), out_dtype=torch.bfloat16),
     lambda: ops.gemm_fp8(_m("row", 4, 8), _m("block", 8, 4), out=torch.ones(4, 5)),
     lambda: ops.gemm_fp8(_m("row", 4, 8), _m("block", 8, 4), out=torch.ones(4, 4).t()),
+    lambda: ops.gemm_fp8(_m("row", 4, 8), _m("block", 8, 4), out=torch.ones(1, 4).expand(4, 4)),     # rows over one another
+    lambda: ops.gemm_fp8(_m("row", 4, 8), _m("block", 8, 4), out=torch.ones(16).as_strided((4, 4), (2, 1))),
     lambda: ops.gemm_fp8(_m("row", 4, 8), _m("block", 8, 4), beta=1.0),
     lambda: ops.gemm_fp8(_m("row", 4, 8), _m("block", 8, 4), beta=1.0, c=torch.ones(4, 4)),          # c in fp32, result in bf16
     lambda: ops.gemm_fp8(_m("row", 4, 8), _m("block", 8, 4), bias=torch.ones(5)),

@@ -405,9 +405,14 @@ def test_offsets_that_are_none():
     torch.cuda.synchronize()
     assert torch.all(gw[0] == 0) and torch.all(gw[3:] == 0)
     k.device_error_words()
-    ops.grouped_wgrad_fp8(D, X, torch.tensor([0, 100, 300], device=DEV, dtype=torch.int32), gw[1:3], pad=128)
-    torch.cuda.synchronize()
-    assert k.device_error_words()["gemm_fp8"] == 3040 and k.device_error_words()["gemm_fp8"] == 0
+    for off in ([0, 100, 300], [0, 128, 200], [0, 200, 200]):
+        ops.grouped_wgrad_fp8(D, X, torch.tensor(off, device=DEV, dtype=torch.int32), gw[1:3], pad=128)
+        torch.cuda.synchronize()
+        assert k.device_error_words()["gemm_fp8"] == 3040 and k.device_error_words()["gemm_fp8"] == 0
+    for off in ([0, 128, 300], [0, 300, 300], [0, 0, 256]):            # (the rows end where the data does, or on a multiple)
+        ops.grouped_wgrad_fp8(D, X, torch.tensor(off, device=DEV, dtype=torch.int32), gw[1:3], pad=128)
+        torch.cuda.synchronize()
+        assert k.device_error_words()["gemm_fp8"] == 0
 
 
 def test_gemm_in_place_and_expanded():
