@@ -941,16 +941,18 @@ int split_ranges(int64_t tiles, int k_blocks, int sms) {
 }
 
 // The tile of a product: 1 128 x 128 (cut along the reduction where that fills the GPU), 2 128 x 256, 3 256 x 256 on two SMs.  By
-// the waves and the blocks of each, a block taking some 0.5, 0.7 and 0.66 us (a pair of SMs loads less for the same work, and is
-// bound by power later).  us with 1 / 2 / 3, x W^T: 16 x 4096 x 4096 16 / 27 / 27; 256 x 4096 x 4096 21 / 29 / 29; 200 x 14336 x
-// 4096 40 / 29 / 29; 768 x 4096 x 4096 40 / 29 / 29; 1024 x 2048 x 2048 16 / 21 / 21; 512 x 4096 x 14336 68 / 74 / 73; 8192 x 14336 x
-// 4096 (power) - / 637 / 620.
-int pick_variant(int64_t M, int64_t N, int k_blocks, int sms) {
+// the waves and the blocks of each: a block takes some 0.5, 0.7 and 0.66 us, with column scales 0.51, 0.86 and 0.84, joined ranges 2 us
+// and a pair's start 1.5 (a pair loads less for the same work, and is bound by power later).  us with 1 / 2 / 3, x W^T:
+//   16 x 4096 x 4096     14 / 23 / 25     256 x 4096 x 4096    18 / 27 / 27     200 x 14336 x 4096   36 / 27 / 29
+//   768 x 4096 x 4096    36 / 27 / 29     1024 x 2048 x 2048   14 / 18 / 18     512 x 4096 x 14336   57 / 70 / 69
+//   column scales: 768 x 4096 x 4096   40 / 34 / 36     1536 x 4096 x 4096   57 / 61 / 64
+int pick_variant(int64_t M, int64_t N, int k_blocks, int sms, bool columns) {
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const int64_t t1 = up(M, 128) * up(N, 128), t2 = up(M, 128) * up(N, 256), t3 = up(M, 256) * up(N, 256);
   const int r = split_ranges(t1, k_blocks, sms);
-  const double c1 = up(t1 * r, sms) * up(k_blocks, r) * 0.5 + (r > 1 ? 2.0 : 0.0), c2 = up(t2, sms) * k_blocks * 0.7,
-               c3 = up(t3, sms / 2 > 0 ? sms / 2 : 1) * k_blocks * 0.66;
+  const double c1 = up(t1 * r, sms) * up(k_blocks, r) * (columns ? 0.51 : 0.5) + (r > 1 ? 2.0 : 0.0),
+               c2 = up(t2, sms) * k_blocks * (columns ? 0.86 : 0.7),
+               c3 = up(t3, sms / 2 > 0 ? sms / 2 : 1) * k_blocks * (columns ? 0.84 : 0.66) + 1.5;
   return c3 <= c1 && c3 <= c2 ? 3 : c2 <= c1 ? 2 : 1;
 }
 
@@ -1033,7 +1035,7 @@ int ftb_gemm_fp8(const Fp8GemmArgs* a) {
 
   const int sms = sm_count(dev), most = a->max_ctas > 0 && a->max_ctas < sms ? static_cast<int>(a->max_ctas) : sms;
   const int variant = a->variant ? static_cast<int>(a->variant)
-                      : p.mode == 0 ? pick_variant(p.M, p.N, p.k_blocks, most)
+                      : p.mode == 0 ? pick_variant(p.M, p.N, p.k_blocks, most, a->sb_shift == 0)
                       : p.N <= 128  ? 1
                       : p.mode == 1 ? 2
                       : p.M > 128   ? 3
