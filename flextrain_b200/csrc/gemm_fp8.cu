@@ -131,6 +131,7 @@ struct Params {
   const float* sb;                   // scale of column n at sb[(n >> 7, or n) * sb_n + kb * sb_k]
   long sb_n, sb_k, sb_g;
   int a_mn, b_mn;
+  int stage_bytes;                   // that a CTA's copies of a stage bring
   // mode 0 one product; 1 row segments, each with a B of its own; 2 segments of the reduction, each with a D of its own
   int mode, groups;
   const int* offsets;
@@ -527,7 +528,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           if (!(ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, 10))) break;
           uint8_t* sa = smem + stage * R::STAGE;
           uint8_t* sb = sa + BM * BK;
-          if (cta == 0) mbar_expect_tx(&full_bar[stage], CG * R::STAGE);
+          if (cta == 0) mbar_expect_tx(&full_bar[stage], CG * p.stage_bytes);
           const int k0 = (t.kb0 + kb) * BK;
           if constexpr (CG == 2) tma_load_2d_2cta(sa, &tmA, &full_bar[stage], p.a_mn ? row0 : k0, p.a_mn ? k0 : row0);
           else tma_load_2d(sa, &tmA, &full_bar[stage], p.a_mn ? row0 : k0, p.a_mn ? k0 : row0);
@@ -1053,7 +1054,11 @@ int ftb_gemm_fp8(const Fp8GemmArgs* a) {
 
   CUtensorMap ta, tb, td;
   const uint64_t z = p.mode == 1 ? p.groups : 1;
-  int rc = p.a_mn ? make_map(&ta, a->A, 2, 1, p.M, p.K, 1, a->lda, 0, 128) : make_map(&ta, a->A, 2, 1, p.K, p.M, 1, a->lda, 0, 128);
+  // Few rows are copied as they are, without zeros behind them: a copy takes its time by rows, and the products of what the stage held
+  // there are rows of their own, which nothing reads (1 x 14336 x 4096 24.5 -> 18.5 us).
+  const int a_rows = !p.a_mn && p.M < BM ? (p.M + 7) / 8 * 8 : BM;
+  p.stage_bytes = a_rows * BK + bn / cg * BK;
+  int rc = p.a_mn ? make_map(&ta, a->A, 2, 1, p.M, p.K, 1, a->lda, 0, 128) : make_map(&ta, a->A, 2, 1, p.K, p.M, 1, a->lda, 0, a_rows);
   if (rc) return rc;
   // (a stack of one has no stride of its own)
   const uint64_t stack = z > 1 ? a->b_g : (p.b_mn ? p.K : p.N) * static_cast<uint64_t>(a->ldb);
