@@ -22,15 +22,18 @@
 //
 // What bounds it.  A block of 256 x 256 x 128 takes a pair of SMs some 1050 cycles of the 512 that the tensor cores would need: an
 // accumulator is multiplied (400 cycles for a half, 400 behind the other half), seen to be complete and read out (500), released
-// across the pair and multiplied into again (550), and tensor memory holds four halves.  Sustained, power does: of 2390 us of
-// 16384 x 28672 x 4096, the additions are 250, reading tensor memory 150 (without both, 1890 us at 1.52 GHz; the library's product
-// with one scale for everything, which accumulates in tensor memory throughout, 1535).  Measured beside it, us of that product:
-// one thread and one product for all 256 columns 2540, which reads A once but lets both halves wait for one another; tiles of 256 x
-// 128 with four accumulators 3070; sixteen warps of 64 columns each 3050; additions on pairs of fp32 2360; chunks of 32 columns
-// 2480 (registers spilled).
-//   16384 x 28672 x 4096      2.37 ms  1625 TFLOP/s      8192 x 4096 x 14336, B across     585 us  1645 TFLOP/s
-//   3001 x 4096 x 14336 + C    237 us  1487 TFLOP/s      4096 x 2048 x 9377, both across   143 us  1100 TFLOP/s (column scales)
-//   14336 x 4096 x 16384      1.21 ms  1590 TFLOP/s (weight gradient, B in blocks)         16 x 4096 x 4096  14 us
+// across the pair and multiplied into again (550), and tensor memory holds four halves.  Sustained, power does: 16384 x 28672 x 4096
+// runs at 1.6 GHz (without additions and without reading tensor memory, 1890 us at 1.52 GHz; the library's product with one scale
+// for everything, which accumulates in tensor memory throughout, 1535).  Measured beside 2390 us of that product: one thread and one
+// product for all 256 columns 2540, which reads A once but lets both halves wait for one another; tiles of 256 x 128 with four
+// accumulators 3070; sixteen warps of 64 columns each 3050; additions on pairs of fp32 2360; chunks of 32 columns 2480 (registers
+// spilled).  What brought it to 2280: four products in one piece of code, C on its way before the loop over the blocks and not
+// within it, and warps without rows in a loop of their own.  Back to back for a second:
+//   16384 x 28672 x 4096      2.28 ms  1690 TFLOP/s      8192 x 4096 x 14336, B across     560 us  1715 TFLOP/s
+//   3001 x 4096 x 14336 + C    229 us  1540 TFLOP/s      4096 x 2048 x 9377, both across   132 us  1190 TFLOP/s (column scales)
+//   14336 x 4096 x 16384      1.18 ms  1624 TFLOP/s (weight gradient, B in blocks)         16 x 4096 x 4096  10 us
+// 16384 x 28672 x 4096 takes 1.97 ms, 1950 TFLOP/s, where the power limit is not reached.  Few rows: 1 x 14336 x 4096 18.5 us, of which
+// some 8 are the launch, the start and the end, 9 the weights at memory rate (twice the stages in flight: the same).
 #include <type_traits>
 
 #include "ptx.cuh"
