@@ -48,8 +48,8 @@ class DecoderConfig:
     lora: Optional[LoRAConfig] = None
     family: str = "llama"
     layer_scalar: bool = False       # Gemma 4: the layer's output is multiplied by a stored, untrained scalar
-    linear_fp8: bool = False         # products of attention, FFN and experts in 8 bits (Gated DeltaNet, router: as they are)
     seq_parallel: int = 1            # tensor-parallel degree: the residual stream and norm statistics hold T / seq_parallel tokens
+    linear_fp8: bool = False         # products of attention, FFN and experts in 8 bits (Gated DeltaNet, router: as they are)
 
 
 class DecoderLayer:
