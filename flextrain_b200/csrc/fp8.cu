@@ -310,6 +310,12 @@ __device__ __forceinline__ float max_abs(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // Eight elements of x, and of the residual where there is one, as they came
 template <bool RES>
 struct NormIn {
@@ -354,8 +360,9 @@ __device__ __forceinline__ uint4 norm_h(const NormParams& p, const NormIn<RES>& 
   }
   return h;
 }
-// 8 bits of eight elements, and their group's scale.  The group's two divisions by numbers that are not exact anyway are a
-// multiplication and an approximate reciprocal (off by 2^-23): q and s fit together to that.
+// 8 bits of eight elements, and their group's scale.  y / s is 448 (h w) / max |h w|: r and the rounding of s have no part in it, and
+// the factor is one reciprocal (approximate, then one step of Newton's, which leaves little more than a rounding).  q and s fit
+// together to a few 2^-24.
 __device__ __forceinline__ void norm_q(const NormParams& p, const uint4& h, const f32x2 (&w)[4], long row, int c, float r) {
   const uint32_t hs[4] = {h.x, h.y, h.z, h.w};
   f32x2 t[4];
@@ -371,14 +378,13 @@ __device__ __forceinline__ void norm_q(const NormParams& p, const uint4& h, cons
   for (int o = 8; o > 0; o >>= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));     // the 16 lanes of a group
   float s = top * r * (1.f / 448.f);
   s = s < 1.17549435e-38f ? 1.17549435e-38f : s;
-  float inv;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s));
   if ((threadIdx.x & 15) == 0 && c < p.D) p.scale[row + (c >> 7) * p.scale_n] = s;
-  float factor = r * inv;
+  const float inv = reciprocal(top);
+  float factor = s == 1.17549435e-38f ? r * 0x1p126f : 448.f * fmaf(inv, fmaf(-top, inv, 1.f), inv);
   if (!(factor <= 3.402823466e38f)) {                // (groups of next to nothing, and rows that are not numbers)
 #pragma unroll
     for (int i = 0; i < 4; ++i) t[i] = mul2(t[i], pack2(r, r));
-    factor = inv;
+    factor = reciprocal(s);
   }
   const f32x2 k = pack2(factor, factor);
   float f[8];
