@@ -1067,20 +1067,20 @@ int ftb_gemm_fp8(const Fp8GemmArgs* a) {
   const uint64_t stack = z > 1 ? a->b_g : (p.b_mn ? p.K : p.N) * static_cast<uint64_t>(a->ldb);
   rc = p.b_mn ? make_map(&tb, a->B, 3, 1, p.N, p.K, z, a->ldb, stack, 128) : make_map(&tb, a->B, 3, 1, p.K, p.N, z, a->ldb, stack, bn / cg);
   if (rc) return rc;
+  const bool bvec = a->sb_shift == 0;
+  if (variant == 1 && p.mode == 0) {
+    const int ranges = split_ranges(tiles, p.k_blocks, most);
+    p.split_blocks = (p.k_blocks + ranges - 1) / ranges;
+    if (ranges > 1)
+      return bvec ? launch<1, 128, true, true>(ta, tb, ta, p, dev, most, a->stream, ranges)
+                  : launch<1, 128, false, true>(ta, tb, ta, p, dev, most, a->stream, ranges);
+  }
   if (p.vec) {
     const uint64_t depth = p.mode == 2 ? p.groups : 1;
     rc = make_map(&td, p.D, 3, static_cast<int>(es), p.N, p.M, depth, p.ldd * es, depth > 1 ? p.d_g * es : p.M * static_cast<uint64_t>(p.ldd * es), 32);
     if (rc) return rc;
   } else {
     td = ta;                            // (not used)
-  }
-  const bool bvec = a->sb_shift == 0;
-  if (variant == 1 && p.mode == 0) {
-    const int ranges = split_ranges(tiles, p.k_blocks, most);
-    p.split_blocks = (p.k_blocks + ranges - 1) / ranges;
-    if (ranges > 1)
-      return bvec ? launch<1, 128, true, true>(ta, tb, td, p, dev, most, a->stream, ranges)
-                  : launch<1, 128, false, true>(ta, tb, td, p, dev, most, a->stream, ranges);
   }
   if (variant == 1) return bvec ? launch<1, 128, true>(ta, tb, td, p, dev, most, a->stream) : launch<1, 128, false>(ta, tb, td, p, dev, most, a->stream);
   if (variant == 2) return bvec ? launch<1, 256, true>(ta, tb, td, p, dev, most, a->stream) : launch<1, 256, false>(ta, tb, td, p, dev, most, a->stream);

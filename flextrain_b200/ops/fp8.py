@@ -164,11 +164,13 @@ def rmsnorm_fp8_fwd(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, *, r
 def _check(m, what: str, stacked: bool = False) -> None:
     """That ``m`` is a matrix in 8 bits whose parts fit together."""
     q, s, group = m
-    if q.dtype is FP8 and s.dtype is F32 and q.dim() == s.dim() == (3 if stacked else 2) and group in _GROUPS and q.get_device() == s.get_device():
-        *b, M, N = q.shape
-        *c, m, n = s.shape
-        if (m == M if group == "row" else m == (M + 127) >> 7) and (n == N if group == "col" else n == (N + 127) >> 7) and b == c:
-            return
+    if q.dtype is FP8 and s.dtype is F32 and group in _GROUPS and q.get_device() == s.get_device():
+        a, b = q.shape, s.shape
+        if len(a) == len(b) == (3 if stacked else 2):
+            rows, cols = a[-2], a[-1]
+            if b[-2] == (rows if group == "row" else (rows + 127) >> 7) and b[-1] == (cols if group == "col" else (cols + 127) >> 7) and \
+                    (not stacked or a[0] == b[0]):
+                return
     raise ValueError(f"{what}: {'a stack of matrices' if stacked else 'a matrix'} in 8 bits is read here; data {tuple(q.shape)} {q.dtype} on "
                      f"{q.device}, scale {tuple(s.shape)} {s.dtype} on {s.device}, group {group!r}")
 
@@ -183,14 +185,14 @@ def _along(m, trans: bool, what: str):
 
 
 def _on_grid(q):
-    """Data as the tensor maps describe it: rows contiguous, everything on 16 bytes; copied where it lies otherwise."""
-    st = q.stride()
-    if not q.data_ptr() & 15 and not st[-2] & 15 and st[-2] >= q.shape[-1] and (st[-1] == 1 or q.shape[-1] == 1) and \
-            (len(st) == 2 or (st[0] > 0 and not st[0] & 15)):
-        return q
-    buf = _empty_q(q.shape, q.device)
-    buf.view(torch.uint8).copy_(q.view(torch.uint8))
-    return buf
+    """Data as the tensor maps describe it (rows contiguous, everything on 16 bytes; copied where it lies otherwise), its address and
+    what is between its rows and matrices."""
+    st, at = q.stride(), q.data_ptr()
+    if at & 15 or st[-2] & 15 or st[-2] < q.shape[-1] or (st[-1] != 1 and q.shape[-1] != 1) or (len(st) == 3 and (st[0] <= 0 or st[0] & 15)):
+        buf = _empty_q(q.shape, q.device)
+        buf.view(torch.uint8).copy_(q.view(torch.uint8))
+        q, st, at = buf, buf.stride(), buf.data_ptr()
+    return q, at, st[-2], st[0]
 
 
 def _result(out, M: int, N: int, dtype, like, what: str):
@@ -236,12 +238,12 @@ def gemm_fp8(a: Fp8Matrix, b: Fp8Matrix, *, trans_a: bool = False, trans_b: bool
         return D
     if not qa.is_cuda or K == 0:
         return ref.gemm(ref.dequant_fp8(*a), ref.dequant_fp8(*b), trans_a=trans_a, trans_b=trans_b, alpha=alpha, beta=beta, c=c, bias=bias, out=D)
-    qa, qb = _on_grid(qa), _on_grid(qb)
+    (qa, at, lda, _), (qb, bt, ldb, _) = _on_grid(qa), _on_grid(qb)
     if bias is not None:
         bias = bias.contiguous()
-    _launch("gemm_fp8", qa.get_device(), "gemm_fp8", "ftb_gemm_fp8", qa.data_ptr(), qb.data_ptr(), D.data_ptr(),
+    _launch("gemm_fp8", qa.get_device(), "gemm_fp8", "ftb_gemm_fp8", at, bt, D.data_ptr(),
             None if c is None else c.data_ptr(), None if bias is None else bias.data_ptr(), a.scale.data_ptr(), b.scale.data_ptr(), None, M, N, K,
-            trans_a, not trans_b, qa.stride(0), qb.stride(0), D.stride(0), 0 if c is None else c.stride(0), sa_m, sa_k, sa_shift, sb_n, sb_k,
+            trans_a, not trans_b, lda, ldb, D.stride(0), 0 if c is None else c.stride(0), sa_m, sa_k, sa_shift, sb_n, sb_k,
             sb_shift, 0, float(alpha), float(beta), dtype is F32, 0, 0, 0, 0, TILE, 0)
     return D
 
@@ -296,10 +298,10 @@ def grouped_gemm_fp8(x: Fp8Matrix, w: Fp8Matrix, offsets, *, trans_w: bool = Tru
             if j > i:
                 ref.gemm(xf[i:j], wf[e], trans_b=trans_w, alpha=alpha, beta=beta, out=D[i:j])
         return D
-    qx, qw = _on_grid(x.data), _on_grid(w.data)
-    _launch("grouped_gemm_fp8", qx.get_device(), "gemm_fp8", "ftb_gemm_fp8", qx.data_ptr(), qw.data_ptr(), D.data_ptr(), None, None,
-            x.scale.data_ptr(), w.scale.data_ptr(), off.data_ptr(), R, N, K, 0, not trans_w, qx.stride(0), qw.stride(1), D.stride(0), 0, sa_m,
-            sa_k, sa_shift, sb_n, sb_k, 7, w.scale.stride(0), float(alpha), float(beta), D.dtype is F32, 1, E, qw.stride(0), 0, TILE, 0)
+    (qx, xt, ldx, _), (qw, wt, ldw, stack) = _on_grid(x.data), _on_grid(w.data)
+    _launch("grouped_gemm_fp8", qx.get_device(), "gemm_fp8", "ftb_gemm_fp8", xt, wt, D.data_ptr(), None, None,
+            x.scale.data_ptr(), w.scale.data_ptr(), off.data_ptr(), R, N, K, 0, not trans_w, ldx, ldw, D.stride(0), 0, sa_m,
+            sa_k, sa_shift, sb_n, sb_k, 7, w.scale.stride(0), float(alpha), float(beta), D.dtype is F32, 1, E, stack, 0, TILE, 0)
     return D
 
 
@@ -332,8 +334,8 @@ def grouped_wgrad_fp8(dy: Fp8Matrix, x: Fp8Matrix, offsets, gw, *, alpha: float 
         return gw
     sa_m, sa_k, _ = _along(dy, True, "grouped_wgrad_fp8 (dy)")
     sb_n, sb_k, sb_shift = _along(x, True, "grouped_wgrad_fp8 (x)")
-    qd, qx = _on_grid(dy.data), _on_grid(x.data)
-    _launch("grouped_wgrad_fp8", gw.get_device(), "gemm_fp8", "ftb_gemm_fp8", qd.data_ptr(), qx.data_ptr(), gw.data_ptr(), None, None,
-            dy.scale.data_ptr(), x.scale.data_ptr(), off.data_ptr(), N, K, R, 1, 1, qd.stride(0), qx.stride(0), gw.stride(1), 0, sa_m, sa_k, 0,
+    (qd, dt, ldd, _), (qx, xt, ldx, _) = _on_grid(dy.data), _on_grid(x.data)
+    _launch("grouped_wgrad_fp8", gw.get_device(), "gemm_fp8", "ftb_gemm_fp8", dt, xt, gw.data_ptr(), None, None,
+            dy.scale.data_ptr(), x.scale.data_ptr(), off.data_ptr(), N, K, R, 1, 1, ldd, ldx, gw.stride(1), 0, sa_m, sa_k, 0,
             sb_n, sb_k, sb_shift, 0, float(alpha), 1.0, gw.dtype is F32, 2, E, 0, gw.stride(0), TILE, 0)
     return gw
