@@ -435,6 +435,34 @@ def test_gemm_in_place_and_expanded():
     assert torch.equal(ops.gemm_fp8(A, B, trans_b=True, c=none, out=none), want)
 
 
+def _far(t, ld):
+    """``t`` with its rows ``ld`` elements apart."""
+    out = torch.empty_strided(t.shape, (ld, 1), dtype=t.dtype, device=DEV)
+    out.copy_(t) if t.dtype != torch.float8_e4m3fn else out.view(torch.uint8).copy_(t.view(torch.uint8))
+    return out
+
+
+@pytest.mark.parametrize("tile", [0, 1, 2, 3])
+@pytest.mark.parametrize("dtype,N", [(torch.bfloat16, 264), (torch.float32, 264), (torch.float32, 261)])
+def test_gemm_rows_far_apart(monkeypatch, tile, dtype, N):
+    """Operands and results whose rows begin beyond 2^31 elements: the same bits as where they lie together."""
+    from flextrain_b200.ops import fp8
+    ops = _ops()
+    monkeypatch.setattr(fp8, "TILE", tile)
+    torch.manual_seed(N)
+    A, B = ops.quant_fp8(torch.randn(300, 200, device=DEV), "row"), ops.quant_fp8(torch.randn(N, 200, device=DEV), "block")
+    at, bt = ops.quant_fp8(torch.randn(200, 300, device=DEV), "col"), ops.quant_fp8(torch.randn(200, N, device=DEV), "block")
+    c = torch.randn(300, N, device=DEV).to(dtype)
+    for a, b, ta, tb in ((A, B, False, True), (at, bt, True, False)):
+        want = ops.gemm_fp8(a, b, trans_a=ta, trans_b=tb, beta=1.0, c=c, out_dtype=dtype)
+        far_a, far_b = (m._replace(data=_far(m.data, 1 << 24)) for m in (a, b))
+        for out in (_far(c, (1 << 23) + 8), c.clone()):
+            got = ops.gemm_fp8(far_a, far_b, trans_a=ta, trans_b=tb, beta=1.0, out=out)
+            assert torch.equal(got, want)
+        assert torch.equal(ops.gemm_fp8(a, b, trans_a=ta, trans_b=tb, beta=1.0, c=_far(c, (1 << 23) + 8), out_dtype=dtype), want)
+    _no_errors()
+
+
 # --------------------------------------------------------------------------------- together, as used
 def _layer(ops, x, res, gain, w, dy):
     """Norm, projection and their backward pass as a training step runs them: everything that it hands on."""
