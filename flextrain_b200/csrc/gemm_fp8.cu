@@ -9,7 +9,7 @@
 // whatever the tensor core's adder does.
 //
 //   warp 0     TMA producer (128-byte swizzle; operands K-major or MN-major, as they lie in memory)
-//   warps 1, 2 tcgen05.mma, one thread each: one half of the tile's columns each
+//   warps 1, 2 tcgen05.mma, one thread each: one half of the tile's 256 columns each (128 columns: warp 1, all of them)
 //   warps 4-11 four for each half: read out, scale and add; at the end of a tile turn it over in shared memory and store whole pieces of rows
 //              (a thread's 128 sums, and 32 values on the way, need more than the 168 registers of 384 threads: the first four
 //              warps give theirs up)
@@ -202,7 +202,10 @@ struct Ring {
   static constexpr int WARP = C_BUFS * PIECE_BYTES + (BVEC ? SLOTS * SLOT * 4 : 0);
   static constexpr int STAGES = (227 * 1024 - 1024 - 512 - EPI_WARPS * WARP) / STAGE;
   static constexpr int TOTAL = STAGES * STAGE + EPI_WARPS * WARP + 512 + 1024;
-  static constexpr int NACC = 512 / BN;              // accumulators of each half
+  static constexpr int NACC = 512 / BN;              // accumulators of each issuer
+  // (128 columns have four accumulators as they are, and A is read once: 1024 x 2048 x 2048 14.3 -> 13.4 us, 4096 x 4096 x 4096 in
+  // such tiles 108 -> 105, where the second level of cache brings 10 TB/s)
+  static constexpr int ISSUERS = BN == 128 ? 1 : 2;
   static_assert(STAGES >= 3 && 2 * STAGES + 4 * NACC + 1 <= 64, "barriers in 512 bytes");
 };
 
@@ -474,7 +477,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem_epi + EPI_WARPS * R::WARP);
   uint64_t* empty_bar = full_bar + ST;
   uint64_t* tfull_bar = empty_bar + ST;
-  uint64_t* tempty_bar = tfull_bar + 2 * NACC;            // (of the first half of the columns, then of the second)
+  uint64_t* tempty_bar = tfull_bar + 2 * NACC;            // (of the first issuer, then of the second)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2 * NACC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -495,8 +498,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int s = 0; s < ST; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 2); }
-    for (int a = 0; a < 2 * NACC; ++a) { mbar_init(&tfull_bar[a], 1); mbar_init(&tempty_bar[a], CG * EPI_WARPS / 2); }
+    for (int s = 0; s < ST; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], R::ISSUERS); }
+    for (int a = 0; a < 2 * NACC; ++a) { mbar_init(&tfull_bar[a], 1); mbar_init(&tempty_bar[a], CG * EPI_WARPS / R::ISSUERS); }
     fence_barrier_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
@@ -554,20 +557,21 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           for (uint32_t it = 0; it < (1u << 16); ++it)
             if (mbar_try_wait(&full_bar[s], 0) || mbar_try_wait(&full_bar[s], 1)) break;
     }
-    if ((warp == 1 || warp == 2) && lane == 0 && cta == 0) {
+    if ((warp == 1 || (warp == 2 && R::ISSUERS == 2)) && lane == 0 && cta == 0) {
       // A barrier's word is some 250 cycles away while the tensor core reads shared memory, a block's products take 512.  So a
       // thread asks for both of its barriers at once, and each half of the columns has a thread and accumulators of its own: a
       // half is multiplied while the other one's are read out.
       const int half = warp - 1;
       uint64_t *tfull = tfull_bar + half * NACC, *tempty = tempty_bar + half * NACC;
       const uint32_t tmem_half = tmem_base + half * NACC * HALF;
+      constexpr int WIDE = BN / R::ISSUERS;
       // e4m3 operands (format 0), fp32 sums
       const uint32_t idesc = (1u << 4) | static_cast<uint32_t>(p.a_mn) << 15 | static_cast<uint32_t>(p.b_mn) << 16 |
-                             static_cast<uint32_t>(HALF >> 3) << 17 | static_cast<uint32_t>(BM * CG >> 4) << 24;
+                             static_cast<uint32_t>(WIDE >> 3) << 17 | static_cast<uint32_t>(BM * CG >> 4) << 24;
       // K-major: 32 bytes along the swizzled row of 128; MN-major: 32 rows of 128 bytes, blocks of 128 wide behind one another
       const uint32_t a_step = (p.a_mn ? MMA_K * 128 : MMA_K) >> 4, b_step = (p.b_mn ? MMA_K * 128 : MMA_K) >> 4;
       // the half's columns of this CTA's part of B: rows of it, or bytes of its rows, or its second box
-      constexpr int OWN = HALF / CG;
+      constexpr int OWN = WIDE / CG;
       const uint32_t b_off = half * (p.b_mn ? (OWN == 128 ? BOX_BYTES : OWN) : OWN * 128);
       const uint64_t a_desc = make_smem_desc(smem_u32(smem), p.a_mn ? BOX_BYTES : 16, 1024);
       const uint64_t b_desc = make_smem_desc(smem_u32(smem) + BM * BK + b_off, p.b_mn ? BOX_BYTES : 16, 1024);
@@ -586,7 +590,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           if (!f && !(ok = mbar_wait(&full_bar[stage], phase, abort_flag, 21))) break;
           tc_fence_after();
           const uint32_t at = stage * (R::STAGE >> 4);
-          umma4_f8<CG>(tmem_half + acc * HALF, a_lo + at, a_hi, b_lo + at, b_hi, a_step, b_step, idesc);
+          umma4_f8<CG>(tmem_half + acc * WIDE, a_lo + at, a_hi, b_lo + at, b_hi, a_step, b_step, idesc);
           if constexpr (CG == 2) { umma_commit_2cta(&tfull[acc], 3); umma_commit_2cta(&empty_bar[stage], 3); }
           else { umma_commit(&tfull[acc]); umma_commit(&empty_bar[stage]); }
           if (++stage == ST) { stage = 0; phase ^= 1; }
@@ -609,8 +613,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     [[maybe_unused]] float* slots = reinterpret_cast<float*>(smem_slots) + (warp - EPI_FIRST) * (SLOTS * R::SLOT);
     const int in_tile = cta * BM + quad * 32, es = p.d_fp32 ? 4 : 2;
     const bool add = !SPLIT && p.beta != 0.f && !p.add_in_place;
-    uint64_t *tfull = tfull_bar + part * NACC, *tempty = tempty_bar + part * NACC;
-    const uint32_t tmem_part = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + part * NACC * HALF;
+    uint64_t *tfull = tfull_bar + (R::ISSUERS == 2 ? part * NACC : 0), *tempty = tempty_bar + (R::ISSUERS == 2 ? part * NACC : 0);
+    const uint32_t tmem_part = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + part * (R::ISSUERS == 2 ? NACC * HALF : HALF);
+    constexpr int ACC_STEP = BN / R::ISSUERS;
     int acc = 0;
     uint32_t acc_phase = 0;
     [[maybe_unused]] int slot = 0;                  // of the next block of scales to be asked for
@@ -724,7 +729,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       for (int kb = rows == 0 ? kbs : 0; kb < kbs; ++kb) {
         if (!ready && !(ok = mbar_wait(&tfull[acc], acc_phase, abort_flag, 30))) break;
         tc_fence_after();
-        const uint32_t taddr = tmem_part + acc * HALF;
+        const uint32_t taddr = tmem_part + acc * ACC_STEP;
         const bool wrap = acc + 1 == NACC;
         if constexpr (BVEC) {
           uint32_t r[2][16];
