@@ -18,6 +18,7 @@ path.  The scales of two operands are multiplied in fp32, so the product of a pa
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 import sys
 from typing import NamedTuple, Optional
@@ -51,7 +52,7 @@ def _entry(lib: str, name: str):
     address = ctypes.cast(getattr(cuda.load(lib), name), ctypes.c_void_p).value
     fast = cuda.fastcall()
     if fast is not None:
-        return lambda *args, call=fast.call: call(address, *args)
+        return functools.partial(fast.call, address)
     entry, bits = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)(address), struct.Struct("d")
     word = lambda a: 0 if a is None else int.from_bytes(bits.pack(a), "little", signed=True) if isinstance(a, float) else a
     return lambda *args: entry(ctypes.addressof((ctypes.c_int64 * len(args))(*map(word, args))))
