@@ -86,11 +86,11 @@ def _rows(t):
 def _empty_q(shape, device):
     """e4m3 room for ``shape`` with rows on 16 bytes, as the products read them; the pieces behind a row's end hold nothing."""
     n = shape[-1]
-    if n % 16 == 0:
-        if len(shape) == 2:
-            return torch.empty_strided(shape, (n, 1), dtype=FP8, device=device)     # (1.5 us on the host for 2.4 of torch.empty)
-        return torch.empty(shape, dtype=FP8, device=device)
-    return torch.empty(*shape[:-1], (n + 15) // 16 * 16, dtype=FP8, device=device)[..., :n]
+    ld = (n + 15) // 16 * 16
+    if len(shape) != 2:
+        return torch.empty(*shape[:-1], ld, dtype=FP8, device=device)[..., :n]
+    q = torch.empty_strided((shape[0], ld), (ld, 1), dtype=FP8, device=device)      # (1.5 us on the host for 2.4 of torch.empty; a view
+    return q if n == ld else q.as_strided((shape[0], n), (ld, 1))                     # of it 0.9 for 2.2 of a slice)
 
 
 # --------------------------------------------------------------------------------------- quantisers
