@@ -308,9 +308,9 @@ def grouped_gemm_fp8(x: Fp8Matrix, w: Fp8Matrix, offsets, *, trans_w: bool = Tru
 
 def grouped_wgrad_fp8(dy: Fp8Matrix, x: Fp8Matrix, offsets, gw, *, alpha: float = 1.0, pad: int = 1):
     """``gw[e] += alpha * dy[rows_e].T @ x[rows_e]``, ``dy`` in column groups and ``x`` in those or blocks, ``gw (E, N, K)`` bf16 or
-    fp32.  Every expert's segment is padded to a multiple of 128 rows with zero rows (``pad``, as the routing plan lays them out), so that no group of 128 tokens
-    lies in two segments (the library's error word reports offsets that are not, ``device_error_words``).  An expert without rows
-    keeps its ``gw``."""
+    fp32.  Every expert's segment is padded to a multiple of 128 rows with zero rows (``pad``, as the routing plan lays them out), so
+    that no group of 128 tokens lies in two segments (the library's error word reports offsets that are not, ``device_error_words``).
+    An expert without rows keeps its ``gw``."""
     _check(dy, "grouped_wgrad_fp8 (dy)")
     _check(x, "grouped_wgrad_fp8 (x)")
     if dy.group != "col" or x.group not in ("col", "block"):
