@@ -180,11 +180,12 @@ struct QuantParams {
   int vec;
 };
 
-// Bound by memory: 16384 x 4096 bf16, 203 MB, 37 us (5.5 TB/s; the measured copy 6.5) in rows and columns, 36 in squares; fp32 of half
-// the rows 33 us (5.1 TB/s).  One block per tile of 128 x 128: a thread holds 8 columns of 8 rows that lie 16 apart, so that a warp reads 256 bytes of two
-// rows at a time and the tile's groups are inside the block.  The elements stay packed as they came until they are converted, so
-// that four blocks fit an SM (two for fp32): unpacked in registers two fit, with each row's divisions in all of its lanes, and the
-// rows took 123 us.
+// Bound by memory: 16384 x 4096 bf16, 203 MB, 37 us (5.5 TB/s; back to back 35; the measured copy 6.5) in rows and columns, 36 in
+// squares; fp32 of half the rows 33 us (5.1 TB/s).  One block per tile of 128 x 128: a thread holds 8 columns of 8 rows that lie 16
+// apart, so that a warp reads 256 bytes of two rows at a time and the tile's groups are inside the block.  The elements stay packed as
+// they came until they are converted, so that four blocks fit an SM (two for fp32): unpacked in registers two fit, with each row's
+// divisions in all of its lanes, and the rows took 123 us.  Five blocks 35 to 37, six, with spills, 40 to 52; two or three that walk
+// over tiles, the next one's elements asked for before the current one's are converted, 34 to 41.
 template <int GROUP, typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quant_kernel(const QuantParams p) {
   using R = Raw<T>;
@@ -422,8 +423,8 @@ constexpr int norm_threads(int V) { return V > 2 ? 512 : V == 2 ? 768 : 1024; }
 // blocks of 128 threads 99 and 70, of 512 82 and 56.
 //
 // V > 0: a block of NT threads walks over rows of up to 8 NT V elements, its part of the gain in registers, the next row's
-// elements asked for before the current row's sum is known (two rows ahead gained nothing).  V = 0: longer rows are read twice (the second time h comes from what
-// the first pass wrote, by the same thread).
+// elements asked for before the current row's sum is known (two rows ahead gained nothing).  V = 0: longer rows are read twice (the
+// second time h comes from what the first pass wrote, by the same thread).
 template <int NT, int V, bool RES>
 __global__ void __launch_bounds__(NT, norm_threads(V) / NT) rmsnorm_fp8_kernel(const NormParams p) {
   __shared__ float sh[2][NT / 32];

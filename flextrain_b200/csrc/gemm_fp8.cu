@@ -529,7 +529,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         const int col0 = t.tn * BN + cta * (BN / CG);
         const int z = p.mode == 1 ? t.g : 0;
         // a segment of the reduction that starts or ends inside a group of 128 has no scales of its own
-        if (p.mode == 2 && t.kbs > 0 && (p.offsets[t.g] % BK != 0 || (p.offsets[t.g + 1] % BK != 0 && p.offsets[t.g + 1] < p.total))) set_error(3, 40);
+        if (p.mode == 2 && t.kbs > 0 && (p.offsets[t.g] % BK != 0 || (p.offsets[t.g + 1] % BK != 0 && p.offsets[t.g + 1] < p.total)))
+          set_error(3, 40);
         for (int kb = 0; kb < t.kbs; ++kb) {
           if (!(ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, 10))) break;
           uint8_t* sa = smem + stage * R::STAGE;

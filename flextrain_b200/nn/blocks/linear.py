@@ -12,8 +12,8 @@
 * **8 bits** (``fp8``; no counterpart in the reference).  The three products of the group run on e4m3 operands with a scale for
   each block of 128: the input and ``dy`` in row groups, the effective weight in squares; for the weight gradient ``dy`` in column
   groups (tokens differ in size, and a token's largest must not decide for others in another column) and the input in squares,
-  whose one scale for 128 columns makes that product half as fast again.  Weights stay in their own types and are quantised where they are used, so nothing has to be kept or dropped
-  when they change.  Adapters' gradients stay in 16 bits.
+  whose one scale for 128 columns makes that product half as fast again.  Weights stay in their own types and are quantised where
+  they are used, so nothing has to be kept or dropped when they change.  Adapters' gradients stay in 16 bits.
 * **Tensor parallelism** (no counterpart in the reference).  With a bound ``tp`` handle the activations between
   blocks are token-sharded ``(T/tp, d)``.  A ``"col"`` group holds ``out/tp`` rows of each weight: forward is the
   fused all-gather→GEMM, dgrad the fused GEMM→reduce-scatter, wgrad gathers its input.  A ``"row"`` group holds
