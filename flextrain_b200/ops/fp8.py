@@ -55,7 +55,11 @@ def _entry(lib: str, name: str):
         return functools.partial(fast.call, address)
     entry, bits = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)(address), struct.Struct("d")
     word = lambda a: 0 if a is None else int.from_bytes(bits.pack(a), "little", signed=True) if isinstance(a, float) else a
-    return lambda *args: entry(ctypes.addressof((ctypes.c_int64 * len(args))(*map(word, args))))
+
+    def call(*args):
+        words = (ctypes.c_int64 * len(args))(*map(word, args))       # (held until the entry point has returned)
+        return entry(ctypes.addressof(words))
+    return call
 
 
 def _launch(family: str, index: int, lib: str, name: str, *args) -> None:

@@ -152,3 +152,33 @@ def _m(groups, M, N, **over):
 def test_refusals(call):
     with pytest.raises(ValueError):
         call()
+
+
+@pytest.mark.parametrize("extension", [True, False])
+def test_an_entry_point_gets_its_arguments(monkeypatch, extension):
+    """All words of a call (integers, addresses, None as 0, floats as the bits of a double) are there while the library reads them,
+    through the extension and through ctypes."""
+    import ctypes
+    import struct
+    from types import SimpleNamespace
+
+    from flextrain_b200.ops import cuda, fp8
+    args = [*range(1000, 1033), (1 << 62) + 5, -7, 0.5, -3e-40, None, True, False]
+    got = []
+
+    @ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)
+    def library(at):
+        [bytearray(8 * len(args)) for _ in range(64)]              # (whatever a callee allocates)
+        got.append(list((ctypes.c_int64 * len(args)).from_address(at)))
+        return 17
+
+    if extension:
+        assert cuda.fastcall() is not None, "fastcall extension was not built"
+    else:
+        monkeypatch.setattr(cuda, "fastcall", lambda: None)
+    monkeypatch.setattr(cuda, "load", lambda name: SimpleNamespace(entry=library))
+    entry = fp8._entry("lib", "entry")
+    want = [struct.unpack("q", struct.pack("d", a))[0] if isinstance(a, float) else int(a or 0) for a in args]
+    for _ in range(3):
+        assert entry(*args) == 17
+    assert got == [want] * 3

@@ -567,3 +567,26 @@ def test_experts_with_the_routing_plan():
         assert torch.all((gw[e].double() - want).abs() <= _room(want, _value(d8)[i:j].abs().t() @ _value(x8)[i:j].abs(), j - i + 1, torch.float32))
     assert used % 128 == 0 and off[-1] == off[-2]
     _no_errors()
+
+
+def test_without_the_fast_call_extension(monkeypatch):
+    """Every operator through ctypes, the path without the extension: the same bits."""
+    from flextrain_b200.ops import cuda, fp8
+    ops = _ops()
+    ins = _layer_inputs(300, 256, 384)
+    W = ops.quant_fp8(torch.randn(3, 200, 256, device=DEV), "block")
+    off = torch.tensor([0, 128, 128, 256], device=DEV, dtype=torch.int32)
+    gw = torch.randn(3, 384, 256, device=DEV)
+
+    def everything():
+        y = ops.grouped_gemm_fp8(ops.quant_fp8(ins[0]), W, off)[:256]
+        g = ops.grouped_wgrad_fp8(ops.quant_fp8(ins[4], "col"), ops.quant_fp8(ins[0], "block"), off, gw.clone(), pad=128)
+        return (*_layer(ops, *ins), y, g)
+
+    want = everything()
+    monkeypatch.setattr(cuda, "fastcall", lambda: None)
+    monkeypatch.setattr(fp8, "_entries", {})
+    got = everything()
+    assert len(fp8._entries) == 3 and not any(hasattr(e, "func") for e in fp8._entries.values())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    _no_errors()
