@@ -713,10 +713,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           else mbar_arrive(&tempty[acc]);
         }
       };
+      // Whether the block's values are there.  Lanes see a barrier's phase end each for itself, early (`ready`) or in the wait; what reads
+      // tensor memory is one instruction of the whole warp, so all lanes meet here and go one way.
+      auto complete = [&](bool early) { return __all_sync(0xffffffffu, early || mbar_wait(&tfull[acc], acc_phase, abort_flag, 30)) != 0; };
       // Warps of which nothing is stored leave their values where they are.
 #pragma unroll 1
       for (int kb = rows == 0 ? 0 : kbs; kb < kbs; ++kb) {
-        if (!ready && !(ok = mbar_wait(&tfull[acc], acc_phase, abort_flag, 30))) break;
+        if (!(ok = complete(ready))) break;
         ready = false;
         if constexpr (BVEC) {
           cp_wait<AHEAD - 1>();
@@ -728,7 +731,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       }
 #pragma unroll 1
       for (int kb = rows == 0 ? kbs : 0; kb < kbs; ++kb) {
-        if (!ready && !(ok = mbar_wait(&tfull[acc], acc_phase, abort_flag, 30))) break;
+        if (!(ok = complete(ready))) break;
         tc_fence_after();
         const uint32_t taddr = tmem_part + acc * ACC_STEP;
         const bool wrap = acc + 1 == NACC;

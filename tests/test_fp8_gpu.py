@@ -590,3 +590,26 @@ def test_without_the_fast_call_extension(monkeypatch):
     assert len(fp8._entries) == 3 and not any(hasattr(e, "func") for e in fp8._entries.values())
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     _no_errors()
+
+
+@pytest.mark.parametrize("form", ["fwd", "wgrad"])
+def test_gemm_long_reductions_beside_another_stream(tile, form):
+    """Hundreds of blocks whose values come early for some and late for others, memory and tensor cores busy with something else:
+    right, and the same bits each time."""
+    ops = _ops()
+    torch.manual_seed(tile)
+    M, N, K = 300, 520, 40001
+    A, B, ta, tb, want, mag = _operands(form, M, N, K)
+    busy = torch.randn(4096, 4096, device=DEV).bfloat16()
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(8):
+        with torch.cuda.stream(other):
+            busy.copy_(busy.flip(0))
+            ops.linear_fp8_fwd(ops.quant_fp8(busy[:512]), ops.quant_fp8(busy, "block"))
+        got.append(ops.gemm_fp8(A, B, trans_a=ta, trans_b=tb, out_dtype=torch.float32))
+    torch.cuda.synchronize()
+    assert torch.all((got[0].double() - want).abs() <= _room(want, mag, K, torch.float32))
+    assert all(torch.equal(g, got[0]) for g in got[1:])
+    _no_errors()
