@@ -145,7 +145,7 @@ struct Params {
 };
 
 struct Tile {
-  int row0, left, tn, g, kb0, kbs;
+  int row0, left, tn, g, kb0, kbs;    // kbs: blocks of the reduction; -1 for a segment that is left out
 };
 
 // Where a tile lies.  Tiles come in ascending order, and the walk over the groups goes on where the last tile left it.
@@ -181,6 +181,9 @@ struct Walk {
       const int a = min(max(p.offsets[t.g], 0), p.total), b = min(max(p.offsets[t.g + 1], a), p.total);
       t.kb0 = a / BK;
       t.kbs = (b - a + BK - 1) / BK;
+      // A segment that starts or ends inside a group of 128 would take its neighbour's rows along, whose scales are the same: it is left
+      // out, and reported.
+      if (t.kbs > 0 && (p.offsets[t.g] % BK != 0 || (p.offsets[t.g + 1] % BK != 0 && p.offsets[t.g + 1] < p.total))) t.kbs = -1;
     }
     const int per_group = GM * p.tiles_n, grp = tile / per_group;
     const int gm = min(GM, p.tiles_m - grp * GM), r = tile - grp * per_group;
@@ -528,9 +531,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         const int row0 = t.row0 + cta * BM;
         const int col0 = t.tn * BN + cta * (BN / CG);
         const int z = p.mode == 1 ? t.g : 0;
-        // a segment of the reduction that starts or ends inside a group of 128 has no scales of its own
-        if (p.mode == 2 && t.kbs > 0 && (p.offsets[t.g] % BK != 0 || (p.offsets[t.g + 1] % BK != 0 && p.offsets[t.g + 1] < p.total)))
-          set_error(3, 40);
+        if (t.kbs < 0) set_error(3, 40);
         for (int kb = 0; kb < t.kbs; ++kb) {
           if (!(ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, 10))) break;
           uint8_t* sa = smem + stage * R::STAGE;
@@ -655,7 +656,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     auto begin = [&](int tile) {
       do {
         if (tile >= p.num_tiles || !locate(walk, tile, t)) return -1;
-        if (t.kbs > 0) break;                            // (a group without rows leaves its result as it is)
+        if (t.kbs > 0) break;                            // (a group without rows, or left out, leaves its result as it is)
         tile += step;
       } while (true);
       // (rows and columns outside read a scale that exists; what they compute is not stored)

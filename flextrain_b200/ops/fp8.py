@@ -313,8 +313,9 @@ def grouped_gemm_fp8(x: Fp8Matrix, w: Fp8Matrix, offsets, *, trans_w: bool = Tru
 def grouped_wgrad_fp8(dy: Fp8Matrix, x: Fp8Matrix, offsets, gw, *, alpha: float = 1.0, pad: int = 1):
     """``gw[e] += alpha * dy[rows_e].T @ x[rows_e]``, ``dy`` in column groups and ``x`` in those or blocks, ``gw (E, N, K)`` bf16 or
     fp32.  Every expert's segment is padded to a multiple of 128 rows with zero rows (``pad``, as the routing plan lays them out), so
-    that no group of 128 tokens lies in two segments (the library's error word reports offsets that are not, ``device_error_words``).
-    An expert without rows keeps its ``gw``."""
+    that no group of 128 tokens lies in two segments.  A segment that starts or ends inside a group is not read, and its expert keeps
+    its ``gw``: on a GPU the library's error word reports it (``device_error_words``), on the CPU it is a ``ValueError``.  An expert
+    without rows keeps its ``gw``."""
     _check(dy, "grouped_wgrad_fp8 (dy)")
     _check(x, "grouped_wgrad_fp8 (x)")
     if dy.group != "col" or x.group not in ("col", "block"):
@@ -332,8 +333,11 @@ def grouped_wgrad_fp8(dy: Fp8Matrix, x: Fp8Matrix, offsets, gw, *, alpha: float 
         return gw
     if not gw.is_cuda:
         df, xf, o = ref.dequant_fp8(*dy), ref.dequant_fp8(*x), off.tolist()
-        for e in range(E):
-            i, j = min(max(o[e], 0), R), min(o[e + 1], R)
+        segments = [(min(max(i, 0), R), min(j, R)) for i, j in zip(o, o[1:])]
+        for e, (i, j) in enumerate(segments):
+            if j > i and (o[e] % 128 or (o[e + 1] % 128 and j < R)):
+                raise ValueError(f"grouped_wgrad_fp8: rows {o[e]}:{o[e + 1]} of {R} start or end inside a group of 128")
+        for e, (i, j) in enumerate(segments):
             if j > i:
                 ref.gemm(df[i:j], xf[i:j], trans_a=True, alpha=alpha, beta=1.0, out=gw[e])
         return gw

@@ -182,3 +182,25 @@ def test_an_entry_point_gets_its_arguments(monkeypatch, extension):
     for _ in range(3):
         assert entry(*args) == 17
     assert got == [want] * 3
+
+
+@pytest.mark.parametrize("off", [[0, 100, 256], [0, 128, 200], [-3, 128, 256], [0, 130, 130], [64, 64, 128]])
+def test_experts_gradients_of_part_of_a_group(off):
+    """A segment that starts or ends inside a group of 128 tokens: refused before anything is written."""
+    D, X = ops.quant_fp8(torch.randn(256, 40), "col"), ops.quant_fp8(torch.randn(256, 70), "block")
+    gw = torch.ones(2, 40, 70)
+    with pytest.raises(ValueError, match="inside a group of 128"):
+        ops.grouped_wgrad_fp8(D, X, torch.tensor(off), gw, pad=128)
+    assert torch.all(gw == 1)
+
+
+def test_experts_gradients_of_the_last_rows():
+    """Rows that end where the data does, an empty segment wherever it lies, offsets behind the rows: taken."""
+    D, X = ops.quant_fp8(torch.randn(200, 40), "col"), ops.quant_fp8(torch.randn(200, 70), "block")
+    vd, vx = ops.dequant_fp8(D, torch.float64), ops.dequant_fp8(X, torch.float64)
+    for off, rows in (([0, 128, 200], [(0, 128), (128, 200)]), ([0, 0, 1000], [(0, 0), (0, 200)]), ([0, 128, 128], [(0, 128), (0, 0)]),
+                      ([130, 130, 130], [(0, 0), (0, 0)])):
+        gw = torch.ones(2, 40, 70)
+        ops.grouped_wgrad_fp8(D, X, torch.tensor(off), gw, pad=128)
+        for g, (i, j) in zip(gw, rows):
+            torch.testing.assert_close(g.double(), 1 + vd[i:j].t() @ vx[i:j], rtol=1e-5, atol=1e-4)

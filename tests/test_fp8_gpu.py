@@ -613,3 +613,31 @@ def test_gemm_long_reductions_beside_another_stream(tile, form):
     assert torch.all((got[0].double() - want).abs() <= _room(want, mag, K, torch.float32))
     assert all(torch.equal(g, got[0]) for g in got[1:])
     _no_errors()
+
+
+@pytest.mark.parametrize("group", ["col", "block"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_experts_gradients_of_part_of_a_group(tile, group, dtype):
+    """A segment that starts or ends inside a group of 128 tokens: reported, its expert's sums as they were, the others' right."""
+    ops = _ops()
+    from flextrain_b200.ops import cuda as k
+    torch.manual_seed(0)
+    R, N, K = 700, 520, 136
+    D, X = ops.quant_fp8(torch.randn(R, N, device=DEV), "col"), ops.quant_fp8(torch.randn(R, K, device=DEV), group)
+    vd, vx = _value(D), _value(X)
+    keep = torch.randn(4, N, K, device=DEV).to(dtype)
+    k.device_error_words()
+    for off, good in (([0, 128, 200, 384, R], [0, 3]), ([0, 256, 256, 300, 300], [0]), ([3, 128, 256, 384, 640], [1, 2, 3]), ([0, 100, 228, 356, R], [])):
+        gw = keep.clone()
+        ops.grouped_wgrad_fp8(D, X, torch.tensor(off, device=DEV, dtype=torch.int32), gw, pad=128)
+        torch.cuda.synchronize()
+        assert k.device_error_words()["gemm_fp8"] == 3040
+        for e in range(4):
+            i, j = off[e], off[e + 1]
+            if e not in good:
+                assert torch.equal(gw[e], keep[e])
+                continue
+            want = keep[e].double() + vd[i:j].t() @ vx[i:j]
+            mag = keep[e].abs().double() + vd[i:j].abs().t() @ vx[i:j].abs()
+            assert torch.all((gw[e].double() - want).abs() <= _room(want, mag, j - i, dtype))
+    _no_errors()
