@@ -235,14 +235,14 @@ def _init_lora_params(am: ActiveModel, seed: int, a_std: float) -> None:
             t.zero_()
 
 
-def _linear_dtype(linear_dtype, compute_dtype, world_size, tp, ep) -> Optional[torch.dtype]:
+def _linear_dtype(linear_dtype, compute_dtype, device, world_size, tp, ep) -> Optional[torch.dtype]:
     """``linear_dtype`` of the builders: the type of the operands of the layers' products, the compute type or e4m3."""
     if linear_dtype is None or linear_dtype == compute_dtype:
         return None
     if linear_dtype != torch.float8_e4m3fn:
         raise ValueError(f"linear_dtype {linear_dtype}: torch.float8_e4m3fn, or the compute type {compute_dtype}")
-    if compute_dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"linear_dtype {linear_dtype} with compute_dtype {compute_dtype}: bfloat16 (or float32, on the CPU)")
+    if compute_dtype not in ((torch.bfloat16, torch.float32) if torch.device(device).type == "cpu" else (torch.bfloat16,)):
+        raise ValueError(f"linear_dtype {linear_dtype} with compute_dtype {compute_dtype} on {device}: bfloat16 (or float32, on the CPU)")
     if world_size > 1 or tp not in (1, "auto") or ep not in (1, "auto"):
         raise NotImplementedError("products in 8 bits run on one GPU: the fused collectives' products are in 16")
     return linear_dtype
@@ -278,7 +278,7 @@ def from_dims(dims: Mapping, *, arch: str = "llama", optimizer, max_seq_len: int
     mc = mod.config_from_dims(dims, hyper) if hasattr(mod, "config_from_dims") else config_from_dims(dims, arch, hyper)
     norm_dt = torch.float32 if compute_dtype != torch.float64 else torch.float64
     dt = DTypePolicy(compute_dtype, master_dtype or compute_dtype, grad_dtype or compute_dtype, norm_dt, norm_grad_dtype,
-                     _linear_dtype(linear_dtype, compute_dtype, world_size, tp, ep))
+                     _linear_dtype(linear_dtype, compute_dtype, device, world_size, tp, ep))
     lora = resolve_lora(lora_targets, lora_rank, lora_alpha, lora_adapter_compute_dtype, lora_adapter_master_dtype,
                         lora_adapter_grad_dtype, lora_adapter_opt_state_dtype)
     am = _build_active_model(mc, optimizer=optimizer, max_seq_len=max_seq_len,
@@ -329,7 +329,7 @@ def from_pretrained(model_path: str, *, optimizer, max_seq_len: int, max_global_
     mc.hf = hf
     norm_dt = torch.float32
     dt = DTypePolicy(compute_dtype, master_dtype or compute_dtype, grad_dtype or compute_dtype, norm_dt, norm_grad_dtype,
-                     _linear_dtype(linear_dtype, compute_dtype, world_size, tp, ep))
+                     _linear_dtype(linear_dtype, compute_dtype, device, world_size, tp, ep))
     lora = resolve_lora(lora_targets, lora_rank, lora_alpha, lora_adapter_compute_dtype, lora_adapter_master_dtype,
                         lora_adapter_grad_dtype, lora_adapter_opt_state_dtype)
     am = _build_active_model(mc, optimizer=optimizer, max_seq_len=max_seq_len,

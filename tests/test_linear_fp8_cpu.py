@@ -191,3 +191,13 @@ def test_refusals(kw, err):
     with pytest.raises(err):
         build_tiny("llama", dims=DIMS, **kw)
     assert build_tiny("llama", dims=DIMS, linear_dtype=torch.float32).layers[0].cfg.linear_fp8 is False
+
+
+@pytest.mark.parametrize("device", ["cuda:0", "cuda", torch.device("cuda", 0)])
+def test_full_precision_on_a_gpu_is_refused_when_the_model_is_built(device):
+    """The norm and the quantisers' products write bf16 there; a model of another type says so before anything is allocated."""
+    for kw in (dict(linear_dtype=FP8, device=device), dict(linear_dtype=FP8, device=device, plan_only=True)):
+        with pytest.raises(ValueError, match="on the CPU"):
+            build_tiny("llama", dims=DIMS, **kw)
+    assert ft.from_dims(DIMS, arch="llama", optimizer=ft.AdamW(lr=1e-3), max_seq_len=128, max_global_batch_tokens=256, device=device,
+                        max_gpu_mem_bytes=64 << 30, max_host_mem_bytes=8 << 30, linear_dtype=FP8, plan_only=True) is not None
