@@ -641,3 +641,94 @@ def test_experts_gradients_of_part_of_a_group(tile, group, dtype):
             mag = keep[e].abs().double() + vd[i:j].abs().t() @ vx[i:j].abs()
             assert torch.all((gw[e].double() - want).abs() <= _room(want, mag, j - i, dtype))
     _no_errors()
+
+
+def _within(got, want, room):
+    return bool(torch.all((got.double().cpu() - want.cpu()).abs() <= room.cpu()))
+
+
+@pytest.mark.parametrize("group", ["block", "col"])
+@pytest.mark.parametrize("T,D,N", [(1, 256, 512), (130, 384, 640), (1000, 1024, 768)])
+def test_layer_terms(T, D, N, group):
+    """The run of a layer, each step against 64 bits of the operands that it reads (``group``: of a weight gradient's input; models have
+    squares).  What a step hands on is 8 bits or bf16, and the next step's oracle starts from that, so that the room is a step's own
+    roundings: a product's as everywhere here; of the norm's backward pass bf16's 2^-8 of each result, and 2^-24 for each of the D
+    terms of a row's sum, the T terms of a gain's, and 16 more operations.  An oracle that misses a term is off by more."""
+    ops = _ops()
+    x, res, gain, w, dy = _layer_inputs(T, D, N)
+    h8, rstd, h = ops.rmsnorm_fp8_fwd(x, gain, 1e-5, residual=res)
+    w8, dy8, dyc = ops.quant_fp8(w, "block"), ops.quant_fp8(dy, "row"), ops.quant_fp8(dy, "col")
+    y = ops.linear_fp8_fwd(h8, w8)
+    dh = ops.linear_fp8_dgrad(dy8, w8)
+    dgain = torch.zeros_like(gain)
+    dx, n = ops.rmsnorm_bwd(dh, h, gain, rstd, dx_add=res, emit_y=True, dw_out=dgain)
+    n8 = ops.quant_fp8(n, group)
+    dw = torch.zeros(w.shape, device=DEV)
+    ops.linear_fp8_wgrad(dyc, n8, dw)
+    if group == "col":                                           # (as the other tests run it)
+        assert all(torch.equal(a, b) for a, b in zip((y, dx, dw, dgain), _layer(ops, x, res, gain, w, dy)))
+
+    # the operands in 8 bits: half a step of e4m3, the norm's scale and root
+    hd, g = h.double(), gain.double()
+    r = rstd.double()[:, None]
+    xh = hd * r
+    assert torch.equal(h, (x.float() + res.float()).bfloat16())
+    assert torch.all((r - 1 / torch.sqrt((hd * hd).mean(-1, keepdim=True) + 1e-5)).abs() <= ((D / 128 + 20) * 2.0 ** -25 + 2.0 ** -22) * r)
+    for m, v in ((h8, xh * g), (w8, w.double()), (dy8, dy.double()), (dyc, dy.double()), (n8, n.double())):
+        step = torch.maximum(2.0 ** -4 * v.abs(), 2.0 ** -10 * _spread(m)) + 2.0 ** -20 * v.abs()
+        assert torch.all((_value(m) - v).abs() <= step)
+
+    vh, vw, vr, vc, vn = (_value(m) for m in (h8, w8, dy8, dyc, n8))
+    for got, a, b, dtype in ((y, vh, vw.t(), torch.bfloat16), (dh, vr, vw, torch.bfloat16), (dw, vc.t(), vn, torch.float32)):
+        want, mag = a @ b, a.abs() @ b.abs()
+        assert _within(got, want, _room(want, mag, a.shape[1], dtype))
+        for some in (a[:, :-1] @ b[:-1], torch.zeros_like(want)):          # a term too few in the reduction, nothing at all
+            assert not _within(got, some, _room(some, mag, a.shape[1], dtype))
+
+    assert _within(n, xh * g, (2.0 ** -8 + 8 * 2.0 ** -24) * (xh * g).abs())
+    dn = dh.double() * g
+    mean = (dn * xh).mean(-1, keepdim=True)
+    mag = r * (dn.abs() + xh.abs() * (dn * xh).abs().mean(-1, keepdim=True)) + res.double().abs()
+    room = lambda v: 2.0 ** -8 * v.abs() + (D + 16) * 2.0 ** -24 * mag
+    want = r * (dn - xh * mean) + res.double()
+    assert _within(dx, want, room(want))
+    for wrong in (want - res.double(), r * dn + res.double(), r * (dh.double() - xh * mean) + res.double()):
+        assert not _within(dx, wrong, room(wrong))
+    terms = dh.double() * xh
+    room = (T + 16) * 2.0 ** -24 * terms.abs().sum(0)
+    assert _within(dgain, terms.sum(0), room)
+    assert not _within(dgain, terms[:-1].sum(0), room) and not _within(dgain, torch.zeros_like(g), room)
+    _no_errors()
+
+
+def test_experts_with_squares():
+    """What the layers run for experts: products by the routing plan, gradients of columns by squares; padded rows add nothing."""
+    ops = _ops()
+    torch.manual_seed(1)
+    T, D, F, E, K = 300, 256, 384, 8, 2
+    x, dy = torch.randn(T, D, device=DEV).bfloat16(), torch.randn(T, F, device=DEV).bfloat16()
+    experts = torch.stack([torch.randperm(E - 1, device=DEV)[:K] for _ in range(T)]).to(torch.int32)
+    plan = ops.moe_plan(experts, E, pad=128)
+    off = plan.offsets.tolist()
+    rows, drows = (ops.gather_rows(t, plan.row_src, idx_div=K) for t in (x, dy))
+    d8, x8 = ops.quant_fp8(drows, "col"), ops.quant_fp8(rows, "block")
+    for dtype in (torch.bfloat16, torch.float32):
+        gw = torch.randn(E, F, D, device=DEV).to(dtype)
+        keep = gw.clone()
+        ops.grouped_wgrad_fp8(d8, x8, plan.offsets, gw, pad=128)
+        vd, vx = _value(d8), _value(x8)
+        for e in range(E):
+            i, j = off[e], off[e + 1]
+            want = keep[e].double() + vd[i:j].t() @ vx[i:j]
+            mag = keep[e].double().abs() + vd[i:j].abs().t() @ vx[i:j].abs()
+            room = _room(want, mag, j - i, dtype)
+            assert _within(gw[e], want, room)
+            tokens = (experts == e).any(1)
+            # the tokens that the plan sends there, in 2-norm: two operands' roundings of 2^-4 / sqrt(6) each, four times that
+            a, b = dy[tokens].double(), x[tokens].double()
+            noise = 4 * 2.0 ** -4 / 3 ** 0.5 * ((a * a).t() @ (b * b)).sum().sqrt() + 2.0 ** -8 * want.norm()
+            assert (gw[e].double() - keep[e].double() - a.t() @ b).norm() <= noise
+            if j > i:
+                assert not _within(keep[e], want, room) and (a.t() @ b).norm() > noise
+    assert off[-1] == off[-2]
+    _no_errors()
