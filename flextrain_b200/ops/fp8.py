@@ -210,10 +210,21 @@ def _result(out, M: int, N: int, dtype, like, what: str):
     return out
 
 
+def _partly_over(c, d) -> bool:
+    """Whether ``c`` shares elements with ``d`` other than as the same matrix in the same place (both with contiguous rows)."""
+    (M, N), (lc, _), (ld, _), es = d.shape, c.stride(), d.stride(), d.element_size()
+    at = c.data_ptr() - d.data_ptr()
+    if at == 0 and (M == 1 or lc == ld):
+        return False
+    if at >= ((M - 1) * ld + N) * es or -at >= ((M - 1) * lc + N) * es:
+        return False
+    return M == 1 or lc != ld or not N * es <= at % (ld * es) <= (ld - N) * es
+
+
 def gemm_fp8(a: Fp8Matrix, b: Fp8Matrix, *, trans_a: bool = False, trans_b: bool = False, alpha: float = 1.0, beta: float = 0.0, c=None,
              bias=None, out=None, out_dtype=None):
     """``alpha * op(a) @ op(b) + beta * c (+ bias)`` as :func:`gemm` has it, of operands in 8 bits; ``c`` is ``out`` where only that is
-    given.  The result is bf16 or fp32, rounded once from fp32 sums."""
+    given, and may be ``out`` itself, but not lie partly over it.  The result is bf16 or fp32, rounded once from fp32 sums."""
     _check(a, "gemm_fp8 (a)")
     _check(b, "gemm_fp8 (b)")
     sa_m, sa_k, sa_shift = _along(a, trans_a, "gemm_fp8 (a)")
@@ -237,6 +248,8 @@ def gemm_fp8(a: Fp8Matrix, b: Fp8Matrix, *, trans_a: bool = False, trans_b: bool
         raise ValueError(f"gemm_fp8: c {tuple(c.shape)} {c.dtype} on {c.device} for a result {tuple(D.shape)} {dtype}")
     else:
         c = _rows(c)
+        if out is not None and M and N and _partly_over(c, D):
+            raise ValueError(f"gemm_fp8: c (strides {c.stride()}) lies partly over the result (strides {D.stride()})")
     if bias is not None and (bias.shape != (N,) or bias.dtype != torch.float32 or bias.device != D.device):
         raise ValueError(f"gemm_fp8: bias {tuple(bias.shape)} {bias.dtype} on {bias.device}, fp32 of {N} is read")
     if M == 0 or N == 0:

@@ -204,3 +204,41 @@ def test_experts_gradients_of_the_last_rows():
         ops.grouped_wgrad_fp8(D, X, torch.tensor(off), gw, pad=128)
         for g, (i, j) in zip(gw, rows):
             torch.testing.assert_close(g.double(), 1 + vd[i:j].t() @ vx[i:j], rtol=1e-5, atol=1e-4)
+
+
+
+@pytest.mark.parametrize("out,c,apart", [
+    (((4, 8), (8, 1), 8), ((4, 8), (8, 1), 0), False),                       # a row further down
+    (((4, 8), (8, 1), 3), ((4, 8), (8, 1), 0), False),                       # three elements further on
+    (((4, 8), (20, 1), 4), ((4, 8), (20, 1), 0), False),                     # columns that meet
+    (((4, 8), (8, 1), 0), ((4, 8), (0, 1), 8), False),                       # one of the result's rows for all
+    (((4, 8), (8, 1), 0), ((4, 8), (16, 1), 0), False),                      # the same place with other strides
+    (((4, 8), (8, 1), 0), ((4, 8), (8, 1), 0), True),                        # the result itself
+    (((4, 8), (20, 1), 0), ((4, 8), (20, 1), 8), True),                      # columns beside it
+    (((4, 8), (20, 1), 12), ((4, 8), (20, 1), 0), True),
+    (((4, 8), (8, 1), 0), ((4, 8), (8, 1), 32), True),                       # rows behind it
+    (((4, 8), (8, 1), 0), ((4, 8), (0, 1), 32), True),
+    (((4, 8), (8, 1), 0), ((4, 8), (1, 4), 0), True),                        # (columns that lie apart are copied first)
+])
+def test_c_over_the_result(out, c, apart):
+    """C is read while the result is written: what lies partly over it is refused, what lies beside it or is the result itself is taken."""
+    torch.manual_seed(0)
+    base = torch.randn(200)
+    a, b = _m("row", 4, 8), _m("block", 8, 8)
+    d, c = base.as_strided(*out), base.as_strided(*c)
+    if not apart:
+        with pytest.raises(ValueError, match="over the result"):
+            ops.gemm_fp8(a, b, beta=1.0, c=c, out=d)
+        return
+    want = 8 + c.clone()
+    assert torch.equal(ops.gemm_fp8(a, b, beta=1.0, c=c, out=d), want) and torch.equal(d, want)
+
+
+def test_a_single_row_of_c_has_no_stride():
+    base = torch.randn(40)
+    a, b = _m("row", 1, 8), _m("block", 8, 8)
+    out, c = base.as_strided((1, 8), (8, 1), 4), base.as_strided((1, 8), (30, 1), 4)
+    want = 8 + c.clone()
+    assert torch.equal(ops.gemm_fp8(a, b, beta=1.0, c=c, out=out), want)
+    with pytest.raises(ValueError, match="over the result"):
+        ops.gemm_fp8(a, b, beta=1.0, c=base.as_strided((1, 8), (30, 1), 5), out=out)
