@@ -285,6 +285,8 @@ def linear_fp8_wgrad(dy: Fp8Matrix, x: Fp8Matrix, gw, *, alpha=1.0, accumulate=T
 def _offsets(offsets, E: int, like, what: str):
     if offsets.shape != (E + 1,) or offsets.dtype not in (torch.int32, torch.int64) or offsets.device != like.device:
         raise ValueError(f"{what}: offsets {tuple(offsets.shape)} {offsets.dtype} on {offsets.device} for {E} experts on {like.device}")
+    if offsets.dtype is torch.int64:                     # (what lies outside of 32 bits stays outside of the rows)
+        offsets = offsets.clamp(-(1 << 31), (1 << 31) - 1)
     return offsets.to(torch.int32).contiguous()
 
 

@@ -242,3 +242,26 @@ def test_a_single_row_of_c_has_no_stride():
     assert torch.equal(ops.gemm_fp8(a, b, beta=1.0, c=c, out=out), want)
     with pytest.raises(ValueError, match="over the result"):
         ops.gemm_fp8(a, b, beta=1.0, c=base.as_strided((1, 8), (30, 1), 5), out=out)
+
+
+def test_offsets_of_64_bits_do_not_wrap():
+    """Offsets beyond 32 bits name rows outside of those that there are, not others inside."""
+    far = 1 << 32
+    X, W = ops.quant_fp8(torch.randn(256, 40), "row"), ops.quant_fp8(torch.randn(2, 24, 40), "block")
+    want = torch.full((256, 24), 7.0)
+    ops.grouped_gemm_fp8(X, W, torch.tensor([0, 100, 256]), out=want)
+    for off, rows in (([0, 100, far + 120], slice(0, 256)), ([0, far + 90, far + 120], None), ([far, far + 10, far + 20], slice(0, 0)),
+                      ([-far - 3, 100, far], slice(0, 256))):
+        out = torch.full((256, 24), 7.0)
+        ops.grouped_gemm_fp8(X, W, torch.tensor(off), out=out)
+        if rows is not None:
+            assert torch.equal(out[rows], want[rows]) and torch.all(out[rows.stop:] == 7), off
+        else:                                                    # the first expert has all rows, the second none
+            ref = torch.full((256, 24), 7.0)
+            ops.grouped_gemm_fp8(X, W, torch.tensor([0, 256, 256]), out=ref)
+            assert torch.equal(out, ref)
+    D, X = ops.quant_fp8(torch.randn(256, 24), "col"), ops.quant_fp8(torch.randn(256, 40), "block")
+    got, want = torch.zeros(2, 24, 40), torch.zeros(2, 24, 40)
+    ops.grouped_wgrad_fp8(D, X, torch.tensor([0, 128, far + 128]), got, pad=128)
+    ops.grouped_wgrad_fp8(D, X, torch.tensor([0, 128, 256]), want, pad=128)
+    assert torch.equal(got, want)
