@@ -732,3 +732,24 @@ def test_experts_with_squares():
                 assert not _within(keep[e], want, room) and (a.t() @ b).norm() > noise
     assert off[-1] == off[-2]
     _no_errors()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 128, 128), (130, 257, 300), (300, 129, 130), (600, 520, 1000)])
+def test_gemm_squares_read_down_their_columns(tile, M, N, K):
+    """A in squares read across (a weight gradient of it), beside each kind of B."""
+    ops = _ops()
+    torch.manual_seed(M + N + K)
+    a, b = torch.randn(K, M, device=DEV) * torch.exp(torch.randn(K, 1, device=DEV)), 0.1 * torch.randn(K, N, device=DEV)
+    A = ops.quant_fp8(a, "block")
+    for B, tb in ((ops.quant_fp8(b, "block"), False), (ops.quant_fp8(b, "col"), False), (ops.quant_fp8(b.t().contiguous(), "row"), True),
+                  (ops.quant_fp8(b.t().contiguous(), "block"), True)):
+        va, vb = _value(A).t(), _value(B).t() if tb else _value(B)
+        want, mag = va @ vb, va.abs() @ vb.abs()
+        for dtype in (torch.bfloat16, torch.float32):
+            got = ops.gemm_fp8(A, B, trans_a=True, trans_b=tb, out_dtype=dtype)
+            assert _within(got, want, _room(want, mag, K, dtype))
+            c = torch.randn(M, N, device=DEV).to(dtype)
+            w2, keep = want + c.double(), mag + c.abs().double()
+            ops.gemm_fp8(A, B, trans_a=True, trans_b=tb, beta=1.0, out=c)
+            assert _within(c, w2, _room(w2, keep, K, dtype))
+    _no_errors()
