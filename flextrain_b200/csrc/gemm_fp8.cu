@@ -20,20 +20,21 @@
 // CG = 2: a pair of SMs works on 256 x BN (each CTA 128 rows, half of B).  Grouped forms take their row or reduction ranges
 // from device offsets.  Every wait is bounded.
 //
-// What bounds it.  A block of 256 x 256 x 128 takes a pair of SMs some 1050 cycles of the 512 that the tensor cores would need: an
-// accumulator is multiplied (400 cycles for a half, 400 behind the other half), seen to be complete and read out (500), released
-// across the pair and multiplied into again (550), and tensor memory holds four halves.  Sustained, power does: 16384 x 28672 x 4096
-// runs at 1.6 GHz (without additions and without reading tensor memory, 1890 us at 1.52 GHz; the library's product with one scale
-// for everything, which accumulates in tensor memory throughout, 1535).  Measured beside 2390 us of that product: one thread and one
-// product for all 256 columns 2540, which reads A once but lets both halves wait for one another; tiles of 256 x 128 with four
-// accumulators 3070; sixteen warps of 64 columns each 3050; additions on pairs of fp32 2360; chunks of 32 columns 2480 (registers
-// spilled).  What brought it to 2280: four products in one piece of code, C on its way before the loop over the blocks and not
-// within it, and warps without rows in a loop of their own.  Back to back for a second:
-//   16384 x 28672 x 4096      2.28 ms  1690 TFLOP/s      8192 x 4096 x 14336, B across     560 us  1715 TFLOP/s
-//   3001 x 4096 x 14336 + C    229 us  1540 TFLOP/s      4096 x 2048 x 9377, both across   132 us  1190 TFLOP/s (column scales)
-//   14336 x 4096 x 16384      1.18 ms  1624 TFLOP/s (weight gradient, B in blocks)         16 x 4096 x 4096  10 us
-// 16384 x 28672 x 4096 takes 1.97 ms, 1950 TFLOP/s, where the power limit is not reached.  Few rows: 1 x 14336 x 4096 18.5 us, of which
-// some 8 are the launch, the start and the end, 9 the weights at memory rate (twice the stages in flight: the same).
+// What bounds it.  A block of 256 x 256 x 128 takes a pair of SMs some 1035 cycles of the 512 that the tensor cores would need: an
+// accumulator is multiplied (400 cycles for a half, 400 behind the other half), seen to be complete (250), read out (490), released
+// across the pair and multiplied into again (530), 2070 in all, and each half has two of them in tensor memory.  Sustained, power
+// does: 16384 x 28672 x 4096 runs at 1.56 GHz (without additions and without reading tensor memory, 1890 us at 1.52 GHz; the library's
+// product with one scale for everything, which accumulates in tensor memory throughout, 1535).  Measured beside 2390 us of that
+// product: one thread and one product for all 256 columns 2540, which reads A once but lets both halves wait for one another; tiles of
+// 256 x 128 with four accumulators 3070; sixteen warps of 64 columns each 3050; additions on pairs of fp32 2360; chunks of 32 columns
+// 2480 (registers spilled).  What brought it to 2290: four products in one piece of code, C on its way before the loop over the blocks
+// and not within it, and warps without rows in a loop of their own.  Back to back for a second:
+//   16384 x 28672 x 4096      2.29 ms  1680 TFLOP/s      8192 x 4096 x 14336, B across     560 us  1718 TFLOP/s
+//   3001 x 4096 x 14336 + C    233 us  1510 TFLOP/s      4096 x 2048 x 9377, both across   134 us  1178 TFLOP/s (column scales)
+//   14336 x 4096 x 16384      1.18 ms  1626 TFLOP/s (weight gradient, B in blocks; in columns 1.51 ms)
+// 16384 x 28672 x 4096 takes 1.95 ms, 1974 TFLOP/s, where the power limit is not reached.  Few rows, in a graph, the weight in the second
+// level of cache: 16 x 4096 x 4096 8.2 us, 1 x 14336 x 4096 15.9, 1 x 4096 x 14336 15.0; from memory 10 and 18.5 for the first two, of which
+// some 8 are the launch, the start and the end (twice the stages in flight: the same).
 #include <type_traits>
 
 #include "ptx.cuh"
@@ -956,10 +957,11 @@ int split_ranges(int64_t tiles, int k_blocks, int sms) {
 
 // The tile of a product: 1 128 x 128 (cut along the reduction where that fills the GPU), 2 128 x 256, 3 256 x 256 on two SMs.  By
 // the waves and the blocks of each: a block takes some 0.5, 0.7 and 0.66 us, with column scales 0.51, 0.86 and 0.84, joined ranges 2 us
-// and a pair's start 1.5 (a pair loads less for the same work, and is bound by power later).  us with 1 / 2 / 3, x W^T:
-//   16 x 4096 x 4096     14 / 23 / 25     256 x 4096 x 4096    18 / 27 / 27     200 x 14336 x 4096   36 / 27 / 29
-//   768 x 4096 x 4096    36 / 27 / 29     1024 x 2048 x 2048   14 / 18 / 18     512 x 4096 x 14336   57 / 70 / 69
-//   column scales: 768 x 4096 x 4096   40 / 34 / 36     1536 x 4096 x 4096   57 / 61 / 64
+// and a pair's start 1.5 (a pair loads less for the same work, and is bound by power later).  us on the device with 1 / 2 / 3, back to back
+// in a graph, x W^T:
+//   16 x 4096 x 4096    8.2 / 20 / 21     256 x 4096 x 4096    15 / 23 / 23     200 x 14336 x 4096   32 / 24 / 24
+//   768 x 4096 x 4096    32 / 23 / 23     1024 x 2048 x 2048   12 / 15 / 15     512 x 4096 x 14336   52 / 66 / 63
+//   column scales: 768 x 4096 x 4096   37 / 31 / 33     1536 x 4096 x 4096   52 / 59 / 60
 int pick_variant(int64_t M, int64_t N, int k_blocks, int sms, bool columns) {
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const int64_t t1 = up(M, 128) * up(N, 128), t2 = up(M, 128) * up(N, 256), t3 = up(M, 256) * up(N, 256);

@@ -13,7 +13,7 @@ group      elements     scale of ``(M, N)`` data                read by
 An element's value is ``data * scale``, ``scale = max(largest magnitude / 448, 2^-126)``.  A group with an infinity or a NaN has a
 scale that is one, and reads as NaN.  On a GPU everything here runs on the package's own kernels or raises; there is no library
 path.  The scales of two operands are multiplied in fp32, so the product of a pair of scales has to be finite and not below
-2^-126 to count.
+2^-126 to count, and sums below that are zero.
 """
 from __future__ import annotations
 
