@@ -20,8 +20,8 @@ LIB = PKG / "_lib"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 CUDA_HOME = Path(NVCC).resolve().parent.parent
 
-CUDA_SOURCES = ["gemm_tcgen05", "elementwise", "attention", "comm", "moe", "noalloc", "gdn", "gdn_chunk", "lora", "seqmix", "fp8", "gemm_fp8"]
-EXACT_SOURCES = {"fp8"}          # compiled without fast math
+CUDA_SOURCES = ["gemm_tcgen05", "elementwise", "attention", "comm", "moe", "noalloc", "gdn", "gdn_chunk", "lora", "seqmix", "fp8", "gemm_fp8", "token_loss"]
+EXACT_SOURCES = {"fp8", "token_loss"}          # compiled without fast math
 CPP_SOURCES = ["dp_solver", "copy_engine"]
 PYEXT_SOURCES = ["fastcall"]
 

@@ -763,6 +763,10 @@ rope_inv_freq = ref.rope_inv_freq
 from .fp8 import (Fp8Matrix, dequant_fp8, gemm_fp8, grouped_gemm_fp8, grouped_wgrad_fp8, linear_fp8_dgrad, linear_fp8_fwd,  # noqa: E402
                   linear_fp8_wgrad, quant_fp8, rmsnorm_fp8_fwd)
 
+# ------------------------------------------------------------ token probabilities
+from .token_loss import (PolicyTerms, TokenLogprobs, distill_loss, distill_loss_, policy_loss, policy_loss_, token_logprobs,  # noqa: E402
+                         token_logprobs_bwd_)
+
 # ------------------------------------------------------------------ per-op device timing
 # ``FTB_OP_TIMING=1`` brackets every leaf op of this module with CUDA events on the current stream and
 # ``timing_report()`` aggregates them by (op, shape): the per-kernel time table of a training step without a
@@ -770,7 +774,8 @@ from .fp8 import (Fp8Matrix, dequant_fp8, gemm_fp8, grouped_gemm_fp8, grouped_wg
 _TIMED_OPS = ("gemm", "gemm_glu_fwd", "gemm_glu_bwd", "rmsnorm_fwd", "rmsnorm_bwd", "rope", "rope_qkv_fused", "lora_wgrad_fused", "glu_fwd", "glu_bwd",
               "glu_bwd_weighted", "attention_fwd", "attention_bwd", "softmax_ce_", "softmax_ce_loss", "embedding_fwd", "embedding_bwd", "adamw_multi", "topk_route",
               "topk_route_bwd", "gather_rows", "moe_combine", "grouped_gemm", "grouped_wgrad", "l2norm_fwd",
-              "gated_rmsnorm_fwd", "bias_grad", "quant_fp8", "rmsnorm_fp8_fwd", "gemm_fp8", "grouped_gemm_fp8", "grouped_wgrad_fp8")
+              "gated_rmsnorm_fwd", "bias_grad", "quant_fp8", "rmsnorm_fp8_fwd", "gemm_fp8", "grouped_gemm_fp8", "grouped_wgrad_fp8", "token_logprobs",
+              "token_logprobs_bwd_", "policy_loss", "policy_loss_", "distill_loss", "distill_loss_")
 _timing_events: list = []
 
 

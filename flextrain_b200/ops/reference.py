@@ -290,6 +290,135 @@ def softmax_ce_fwd_bwd(logits: torch.Tensor, targets: torch.Tensor, *, grad_scal
     return loss, dz.to(logits.dtype)
 
 
+def _scaled(logits: torch.Tensor, temperature: float, softcap: float):
+    """``(u, du / dz)``, fp32, of what :func:`token_logprobs` and its kin call ``u``."""
+    z = logits.to(F32)
+    if not softcap:
+        return z, torch.ones((), dtype=F32, device=z.device)
+    t = torch.tanh(z / softcap)
+    return softcap * t, 1.0 - t * t
+
+
+def _where_on(on, *tensors):
+    return tuple(torch.where(on if t.dim() == 1 else on[:, None], t, torch.zeros((), dtype=t.dtype, device=t.device)) for t in tensors)
+
+
+def _entropy(logp):
+    return -torch.where(logp == float("-inf"), torch.zeros_like(logp), logp.exp() * logp).sum(-1)
+
+
+def _added_at(d, ids, values):
+    """``d[row, ids[row]] += values[row]``; ids outside the row have no part."""
+    inside = (ids >= 0) & (ids < d.shape[1])
+    return d.scatter_add_(1, torch.where(inside, ids, 0), torch.where(inside, values, torch.zeros_like(values)))
+
+
+def token_logprobs(logits, targets, on, temperature, softcap, top_k):
+    """``(logprobs or None, entropy, lse, top_ids or None, top_logprobs or None)`` of the rows that are ``on``."""
+    x = _scaled(logits, temperature, softcap)[0] / temperature
+    logp = torch.log_softmax(x, -1)
+    lse = torch.logsumexp(x, -1)
+    lse = torch.where(lse.isinf(), torch.full_like(lse, float("nan")), lse)
+    ent, lse = _where_on(on, _entropy(logp), lse)
+    lp = ids = top = None
+    if targets is not None:
+        lp, = _where_on(on, logp.gather(1, torch.where(on, targets, 0)[:, None])[:, 0])
+    if top_k:
+        ids = torch.sort(logits.to(F32), dim=-1, descending=True, stable=True).indices[:, :top_k]
+        top = torch.where(on[:, None], logp.gather(1, ids), float("-inf"))
+        ids = torch.where(on[:, None], ids, -1)
+    return lp, ent, lse, ids, top
+
+
+def token_logprobs_bwd(logits, targets, on, lse, entropy, dlogprobs, dentropy, top_ids, dtop, grad_scale, temperature, softcap):
+    u, slope = _scaled(logits, temperature, softcap)
+    logp = u / temperature - lse[:, None]
+    p = logp.exp()
+    total = torch.zeros_like(lse)
+    if dlogprobs is not None:
+        total = total + dlogprobs
+    if dtop is not None:
+        total = total + torch.where((top_ids >= 0) & (top_ids < logits.shape[1]), dtop, 0.0).sum(-1)
+    d = -p * total[:, None]
+    if dentropy is not None:
+        d = d - torch.where(p == 0, 0.0, dentropy[:, None] * p * (logp + entropy[:, None]))
+    if dlogprobs is not None:
+        _added_at(d, torch.where(on, targets, -1)[:, None], dlogprobs[:, None])
+    if dtop is not None:
+        _added_at(d, top_ids, dtop)
+    return _where_on(on, d * slope * (grad_scale / temperature))[0].to(logits.dtype)
+
+
+def policy_loss(logits, targets, on, advantages, old, kept, clip_low, clip_high, kl_beta, entropy_coef, temperature, softcap, grad_scale, grad):
+    """``((loss, logprobs, entropy), dlogits or None)``; see ``token_loss.policy_loss_``."""
+    u, slope = _scaled(logits, temperature, softcap)
+    logp = torch.log_softmax(u / temperature, -1)
+    at = torch.where(on, targets, 0)[:, None]
+    lp, ent = logp.gather(1, at)[:, 0], _entropy(logp)
+    a = advantages if advantages is not None else torch.ones_like(lp)
+    if old is None:
+        loss, g = -a * lp, -a
+    else:
+        r = torch.exp(lp - old)
+        free, held = r * a, r.clamp(1 - clip_low, 1 + clip_high) * a
+        loss, g = -torch.minimum(free, held), torch.where(free <= held, -free, torch.where(free.isnan(), free, 0.0))
+    if kept is not None and kl_beta:
+        e = torch.expm1(kept - lp)
+        loss, g = loss + kl_beta * (e - (kept - lp)), g - kl_beta * e
+    if entropy_coef:
+        loss = loss - entropy_coef * ent
+    dz = None
+    if grad:
+        p = logp.exp()
+        d = -p * g[:, None]
+        if entropy_coef:
+            d = d + torch.where(p == 0, 0.0, entropy_coef * p * (logp + ent[:, None]))
+        d.scatter_add_(1, at, g[:, None])
+        dz = _where_on(on, d * slope * (grad_scale / temperature))[0].to(logits.dtype)
+    return _where_on(on, loss, lp, ent), dz
+
+
+def distill_loss(logits, ids, teacher, targets, on, bucket, ce_weight, temperature, softcap, grad_scale, grad):
+    """``(loss, dlogits or None)``; see ``token_loss.distill_loss_``."""
+    u, slope = _scaled(logits, temperature, softcap)
+    logp = torch.log_softmax(u / temperature, -1)
+    V = logits.shape[1]
+    inside = (ids >= 0) & (ids < V)
+    at = torch.where(inside, ids, 0)
+    t = torch.where(inside, teacher, float("-inf"))
+    if not bucket:
+        norm = torch.logsumexp(t, -1, keepdim=True)
+        t = t - torch.where(norm == float("-inf"), 0.0, norm)
+    q = t.exp()
+    known = torch.zeros(logits.shape[0], V + 1, dtype=torch.bool, device=logits.device)
+    known = known.scatter_(1, torch.where(inside, ids, V), True)[:, :V]
+    kl = torch.where(q > 0, q * (t - logp.gather(1, at)), 0.0).sum(-1)
+    share = q.sum(-1)
+    if bucket:
+        others = logp.masked_fill(known, float("-inf"))
+        lr = torch.logsumexp(others, -1)
+        qr = torch.where(lr.isneginf(), 0.0, (1 - share).clamp(min=0))
+        kl = kl + torch.where(qr > 0, qr * (qr.log() - lr), 0.0)
+        share = share + qr
+    loss = (1 - ce_weight) * temperature * temperature * kl
+    if ce_weight:
+        hard = torch.log_softmax(u, -1)
+        label = torch.where(on, targets, 0)[:, None]
+        loss = loss - ce_weight * hard.gather(1, label)[:, 0]
+    dz = None
+    if grad:
+        d = logp.exp() * share[:, None]
+        if bucket:
+            d = d - torch.where(known | (qr == 0)[:, None], 0.0, qr[:, None] * torch.exp(others - lr[:, None]))
+        _added_at(d, ids, -q)
+        d = d * ((1 - ce_weight) * temperature)
+        if ce_weight:
+            h = hard.exp()
+            d = d + ce_weight * h.scatter_add_(1, label, torch.full_like(h[:, :1], -1.0))
+        dz = _where_on(on, d * slope * grad_scale)[0].to(logits.dtype)
+    return _where_on(on, loss)[0], dz
+
+
 def embedding_fwd(tokens: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     y = table[tokens.long()]
     return (y.to(F32) * scale).to(table.dtype) if scale != 1.0 else y
