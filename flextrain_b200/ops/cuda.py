@@ -100,7 +100,8 @@ def device_error_words() -> dict:
     """Read (and clear) the error word of each loaded kernel library: ``{lib: code*1000 + where}``."""
     out = {}
     for name, fn in (("gemm_tcgen05", "ftb_gemm_error"), ("attention", "ftb_attn_error"), ("comm", "ftb_comm_error"),
-                     ("moe", "ftb_moe_error"), ("gdn", "ftb_gdn_error"), ("gemm_fp8", "ftb_gemm_fp8_error")):
+                     ("moe", "ftb_moe_error"), ("gdn", "ftb_gdn_error"), ("gemm_fp8", "ftb_gemm_fp8_error"),
+                     ("token_loss", "ftb_token_loss_error")):
         lib = _libs.get(name)
         if lib is not None and hasattr(lib, fn):
             f = getattr(lib, fn)

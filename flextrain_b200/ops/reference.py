@@ -296,7 +296,7 @@ def _scaled(logits: torch.Tensor, temperature: float, softcap: float):
     if not softcap:
         return z, torch.ones((), dtype=F32, device=z.device)
     t = torch.tanh(z / softcap)
-    return softcap * t, 1.0 - t * t
+    return torch.where(z == float("-inf"), z, softcap * t), 1.0 - t * t
 
 
 def _where_on(on, *tensors):

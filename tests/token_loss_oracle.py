@@ -13,7 +13,7 @@ F64 = torch.float64
 
 
 def u_of(z, cap):
-    return cap * torch.tanh(z / cap) if cap else z
+    return torch.where(z == float("-inf"), z, cap * torch.tanh(z / cap)) if cap else z
 
 
 def on_rows(T, V, targets, mask, ignore=-100, device="cpu"):
@@ -318,6 +318,16 @@ def check_distill(T, V, dtype, device, K=4, tau=1.0, cap=0.0, rest="drop", ce=0.
 def check_not_finite(device):
     """Logits of -inf and of the type's lowest value; rows of nothing else; NaN and infinities in rows that are left out, and in others."""
     inf = float("inf")
+    # under a soft-cap -inf is no token, the lowest value is one at the cap
+    z = torch.randn(3, 12, generator=torch.Generator().manual_seed(4)).to(device)
+    z[0, 3:], z[1, 5:], z[2] = -inf, torch.finfo(torch.float32).min, -inf
+    t = torch.tensor([1, 2, 0], device=device)
+    s = ops.token_logprobs(z, t, softcap=3.0, top_k=4)
+    want = torch.log_softmax(u_of(z.double(), 3.0), -1)
+    assert bool(((s.logprobs[:2] - want[[0, 1], [1, 2]]).abs() < 64 * 2.0 ** -24).all()) and s.logprobs[2].isnan()
+    assert s.top_ids[0, 3] == 3 and s.top_logprobs[0, 3] == -inf
+    p = ops.policy_loss_(z, t, softcap=3.0, out=(out := torch.empty_like(z)))
+    assert bool((out[0, 3:] == 0).all()) and bool(out[:2].isfinite().all()) and p.loss[2].isnan()
     for dtype in (torch.float32, torch.bfloat16, torch.float16):
         z = torch.randn(8, 12, generator=torch.Generator().manual_seed(3)).to(dtype).to(device)
         z[0, 3:] = -inf
