@@ -32,6 +32,8 @@ from ..core.save_level import (HardwareCost, SaveLevelPlan, TransmissionSchedule
                                plan_from_solution)
 from ..core.working_set import WorkingSetConfig
 from ..io.sequence import Sequence, as_sequence
+from ..nn.loss import TokenScorer
+from ..ops.token_loss import MOST_TOP, TokenLogprobs
 from .buffers import BufferManager
 from .schedule import ChunkPolicy, prepare_training_chunks, split_sequences
 from .streams import EventBook, StreamBundle
@@ -177,14 +179,23 @@ class ActiveModel:
                     raise ValueError(f"sequence {s.seq_id}: {len(t)} targets for {n} tokens")
                 if bool(((t >= vocab) | ((t < 0) & (t != -100))).any()):
                     raise ValueError(f"sequence {s.seq_id} has a target outside [0, {vocab}) that is not -100")
-            for name in ("loss_mask", "advantages", "ref_logprobs"):
+            for name in ("loss_mask", "advantages", "ref_logprobs", "old_logprobs", "teacher_ids", "teacher_logprobs"):
                 extra = getattr(s, name, None)
                 if extra is not None and len(extra) != n:
                     raise ValueError(f"sequence {s.seq_id}: {len(extra)} {name} entries for {n} tokens")
+            ids, lps = s.teacher_ids, s.teacher_logprobs
+            if (ids is None) != (lps is None) or ids is not None and (
+                    ids.dim() != 2 or ids.shape != lps.shape or ids.is_floating_point() or not 1 <= ids.shape[1] <= MOST_TOP):
+                raise ValueError(f"sequence {s.seq_id}: teacher_ids {None if ids is None else (tuple(ids.shape), ids.dtype)} and teacher_logprobs "
+                                 f"{None if lps is None else tuple(lps.shape)}; (tokens, K) of each, K of 1 to {MOST_TOP}")
+        if len({s.old_logprobs is None for s in seqs}) > 1:
+            raise ValueError("some sequences of the step carry old_logprobs and some do not")
 
     def _fwd_bwd(self, seqs, loss_scale_factor, total_tokens_per_step, loss_fn, forward_only, t0) -> StepStats:
         ws = self.ws
         self._check_sequences(seqs)
+        if hasattr(loss_fn, "check_sequences"):
+            loss_fn.check_sequences(seqs)
         if loss_scale_factor is None:
             loss_scale_factor = 1.0 / max(sum(s.active_token_count for s in seqs), 1)
         total_tokens_per_step = total_tokens_per_step or sum(len(s) for s in seqs)
@@ -200,7 +211,7 @@ class ActiveModel:
             self.fwd_bwd_serial += 1
         loss_acc = torch.zeros((), dtype=torch.float32, device=self.device)
         act_acc = torch.zeros((), dtype=torch.int64, device=self.device)
-        pending_losses = []
+        pending_losses, pending_scores = [], []
         in_place = False                                   # a tied head's gradient, see _tied_in_place
         with _nvtx("Fwd+Bwd"):
             for r, rseqs in enumerate(rounds):
@@ -241,6 +252,8 @@ class ActiveModel:
                             loss_acc += ls.total_loss
                             act_acc += ls.active_tokens
                             pending_losses.append((rseqs, meta, ls.per_token_loss))
+                            if isinstance(loss_fn, TokenScorer):
+                                pending_scores.append((rseqs, meta, loss_fn.take()))
                     if forward_only:
                         self.streams.synchronize_all()      # saved activations are dropped: let their copies finish
                     else:
@@ -262,6 +275,7 @@ class ActiveModel:
         stats.loss_sum = float(loss_acc)
         stats.active_tokens = int(act_acc)
         self._write_back_losses(pending_losses)
+        self._write_back_scores(pending_scores)
         if not forward_only:
             self._pending_tokens += stats.tokens
         stats.elapsed_s = time.perf_counter() - t0
@@ -297,6 +311,36 @@ class ActiveModel:
         the step counter are untouched (``stats.loss`` is the mean over active tokens; per-token losses are written
         back to the sequences)."""
         return self.fwd_bwd(seqs, loss_scale_factor=1.0, loss_fn=loss_fn, forward_only=True)
+
+    def score(self, seqs: Seq[Sequence], *, top_k: int = 0, temperature: float = 1.0) -> List[TokenLogprobs]:
+        """Log probabilities of ``seqs``' targets under the current weights, forward only, with each position's entropy, ``lse`` and
+        ``top_k`` most likely tokens: a ``TokenLogprobs`` of CPU tensors for each sequence, also left in its ``scores``.  Its
+        ``logprobs`` are what ``Sequence.old_logprobs`` and ``ref_logprobs`` hold, its ``top_ids`` and ``top_logprobs`` what a student's
+        ``teacher_ids`` and ``teacher_logprobs`` do (at the same temperature).  Positions without a target or masked are zero.  The
+        per-token losses written back are the negative log probabilities."""
+        given = list(seqs)
+        mine = [as_sequence(s) for s in given]
+        if not 0 <= top_k <= min(MOST_TOP, int(self.embed.vocab_size)) or not 0.0 < temperature < float("inf"):
+            raise ValueError(f"score: top_k {top_k} (0 to {min(MOST_TOP, int(self.embed.vocab_size))}), temperature {temperature} (above zero)")
+        self.fwd_bwd(mine, loss_scale_factor=1.0, loss_fn=TokenScorer(top_k, temperature), forward_only=True)
+        return [s.scores for s in mine]
+
+    def _write_back_scores(self, pending) -> None:
+        for s in {id(s): s for rseqs, _, _ in pending for s in rseqs}.values():
+            s.scores = None
+        for rseqs, meta, scores in pending:
+            if self.tp is not None:
+                scores = scores._make(None if t is None else self.tp.all_gather(t) for t in scores)
+            host = scores._make(None if t is None else t.to("cpu") for t in scores)
+            off = 0
+            for i, start, n in meta.extra["pieces"]:
+                s = rseqs[i]
+                if s.scores is None:
+                    s.scores = host._make(None if t is None else torch.zeros(len(s), *t.shape[1:], dtype=t.dtype) for t in host)
+                for whole, part in zip(s.scores, host):
+                    if whole is not None:
+                        whole[start:start + n] = part[off:off + n]
+                off += n
 
     def _fold_tied_head_grad(self) -> None:
         """Tied embeddings are ONE parameter used twice: the head's share of its gradient is added to the embedding's
@@ -472,7 +516,8 @@ class ActiveModel:
                              f"(use sequence lengths / chunk sizes that are multiples of it)")
         a, b = tp.rank * (T // W), (tp.rank + 1) * (T // W)
         cut = lambda t: None if t is None else t[a:b]
-        extra = {k: (v[a:b] if k in ("advantages", "ref_logprobs") and v is not None else v)
+        per_token = ("advantages", "ref_logprobs", "old_logprobs", "teacher_ids", "teacher_logprobs")
+        extra = {k: (v[a:b] if k in per_token and v is not None else v)
                  for k, v in meta.extra.items() if not (isinstance(k, tuple) and k[0] == "_shard")}
         sh = dataclasses.replace(meta, tokens=cut(meta.tokens), targets=cut(meta.targets),
                                  loss_mask=cut(meta.loss_mask), extra=extra)

@@ -149,6 +149,23 @@ def prepare_training_chunks(seqs: Seq[Sequence], max_chunk_size: int, device, *,
                 ref = torch.cat([(seqs[i].ref_logprobs[st:st + n] if seqs[i].ref_logprobs is not None else torch.zeros(n))
                                  for i, st, n in plan.pieces])
                 meta.extra["ref_logprobs"] = tail(ref, 0.0).to(dev, non_blocking=True)
+        for name in ("old_logprobs", "ref_logprobs"):          # (the reference's also where there are no advantages)
+            if name not in meta.extra and any(getattr(seqs[i], name) is not None for i, _, _ in plan.pieces):
+                v = torch.cat([(getattr(seqs[i], name)[st:st + n] if getattr(seqs[i], name) is not None else torch.zeros(n))
+                               for i, st, n in plan.pieces])
+                meta.extra[name] = tail(v, 0.0).to(dev, non_blocking=True)
+        K = max((seqs[i].teacher_ids.shape[1] for i, _, _ in plan.pieces if seqs[i].teacher_ids is not None), default=0)
+        if K:
+            # fewer tokens of a teacher, and sequences and filler without one, are padded with tokens that are none
+            ids, lps = torch.full((T, K), -1, dtype=torch.int64), torch.zeros(T, K, dtype=torch.float32)
+            off = 0
+            for i, st, n in plan.pieces:
+                if seqs[i].teacher_ids is not None:
+                    k = seqs[i].teacher_ids.shape[1]
+                    ids[off:off + n, :k] = seqs[i].teacher_ids[st:st + n]
+                    lps[off:off + n, :k] = seqs[i].teacher_logprobs[st:st + n]
+                off += n
+            meta.extra["teacher_ids"], meta.extra["teacher_logprobs"] = ids.to(dev, non_blocking=True), lps.to(dev, non_blocking=True)
         if mrope:
             pos = [compute_mrope_position_ids(seqs[i], start, n) for i, start, n in plan.pieces]
             if pad:                                            # filler continues after the sequence's last position

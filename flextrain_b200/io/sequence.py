@@ -17,6 +17,10 @@ class Sequence:
     modality_inputs: Optional[Dict[str, Any]] = None
     seq_id: int = 0
     per_token_loss: Optional[torch.Tensor] = None  # filled by the engine after fwd_bwd (fp32, CPU)
+    old_logprobs: Optional[torch.Tensor] = None    # (L,) of the policy that sampled the targets
+    teacher_ids: Optional[torch.Tensor] = None     # (L, K) a teacher's most likely tokens (-1: none) ...
+    teacher_logprobs: Optional[torch.Tensor] = None  # ... and their log probabilities
+    scores: Optional[Any] = None                   # filled by ActiveModel.score (TokenLogprobs on the CPU)
     _active: Optional[int] = field(default=None, repr=False)
 
     def __post_init__(self):
@@ -39,8 +43,8 @@ class Sequence:
 
 def as_sequence(obj) -> "Sequence":
     """A :class:`Sequence` for anything that carries ``tokens`` (duck typing, as the reference's engine allows:
-    ``tokens``, optionally ``targets``, ``loss_mask``, ``advantages``, ``ref_logprobs``, ``modality_inputs``,
-    ``seq_id``).  A :class:`Sequence` is returned as it is."""
+    ``tokens``, optionally ``targets``, ``loss_mask``, ``advantages``, ``ref_logprobs``, ``old_logprobs``,
+    ``teacher_ids``, ``teacher_logprobs``, ``modality_inputs``, ``seq_id``).  A :class:`Sequence` is returned as it is."""
     if isinstance(obj, Sequence):
         return obj
     if not hasattr(obj, "tokens"):
@@ -49,4 +53,5 @@ def as_sequence(obj) -> "Sequence":
     as64 = lambda t: None if t is None else torch.as_tensor(t).to(torch.int64)
     return Sequence(as64(obj.tokens), targets=as64(pick("targets")), loss_mask=pick("loss_mask"),
                     advantages=pick("advantages"), ref_logprobs=pick("ref_logprobs"),
-                    modality_inputs=pick("modality_inputs"), seq_id=int(pick("seq_id") or 0))
+                    old_logprobs=pick("old_logprobs"), teacher_ids=as64(pick("teacher_ids")),
+                    teacher_logprobs=pick("teacher_logprobs"), modality_inputs=pick("modality_inputs"), seq_id=int(pick("seq_id") or 0))

@@ -11,7 +11,7 @@ import torch
 
 from .. import ops
 from ..core.layer import ChunkMeta, LossStats, ParamSpec, TensorSpec
-from .loss import CrossEntropyLoss, TokenSlice, apply_loss
+from .loss import CrossEntropyLoss, TokenSlice, apply_loss, has_loss_only
 
 
 class LMHead:
@@ -39,15 +39,17 @@ class LMHead:
         # held-out data with the stock loss: nothing reads the logits' gradient
         loss_only = (not want_dx and gW is None and isinstance(loss_fn, CrossEntropyLoss) and loss_fn._native
                      and type(loss_fn).__call__ is CrossEntropyLoss.__call__
-                     and type(loss_fn).loss_only is CrossEntropyLoss.loss_only)
+                     and type(loss_fn).loss_only is CrossEntropyLoss.loss_only) or (not want_dx and gW is None and has_loss_only(loss_fn))
         for a in range(0, T, self.head_chunk_size):
             b = min(T, a + self.head_chunk_size)
             xa = x[a:b]
             hn, rstd = ops.rmsnorm_fwd(xa, params["w_final_norm"], self.norm_eps)
             logits = ops.gemm(hn, W, trans_b=True)
-            sl = TokenSlice(meta.targets[a:b], meta.loss_mask[a:b] if meta.loss_mask is not None else None,
-                            meta.extra.get("advantages")[a:b] if meta.extra.get("advantages") is not None else None,
-                            meta.extra.get("ref_logprobs")[a:b] if meta.extra.get("ref_logprobs") is not None else None)
+            cut = lambda name: meta.extra[name][a:b] if meta.extra.get(name) is not None else None
+            extra = {k: cut(k) for k in ("old_logprobs", "ref_logprobs", "teacher_ids", "teacher_logprobs") if meta.extra.get(k) is not None}
+            # (a reference's log probabilities beside advantages; without them the losses that read them find them in ``extra``)
+            sl = TokenSlice(meta.targets[a:b], meta.loss_mask[a:b] if meta.loss_mask is not None else None, cut("advantages"),
+                            cut("ref_logprobs") if cut("advantages") is not None else None, extra=extra)
             per_tok[a:b] = (loss_fn.loss_only(logits, sl, self.final_softcap) if loss_only else
                             apply_loss(loss_fn, logits, sl, loss_scale, self.final_softcap))
             if gW is not None:

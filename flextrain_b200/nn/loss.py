@@ -139,6 +139,10 @@ class GRPOLoss(_NativeLoss):
         self.kl_beta = float(kl_coef if kl_coef is not None else kl_beta)
 
     def __call__(self, logits, sl: TokenSlice, grad_scale: float, softcap: float = 0.0) -> torch.Tensor:
+        if logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float16, torch.float32):
+            # (as below: no mask but -100, and the logits as they are)
+            return ops.policy_loss_(logits, sl.targets, sl.advantages, ref_logprobs=sl.ref_logprobs, kl_beta=max(self.kl_beta, 0.0),
+                                    grad_scale=grad_scale).loss
         z = logits.to(torch.float32)
         valid = (sl.targets != -100).to(torch.float32)
         tgt = sl.targets.clamp(min=0).long()
@@ -156,3 +160,83 @@ class GRPOLoss(_NativeLoss):
         dz = (onehot - p) * (coef * valid * grad_scale).unsqueeze(1)
         logits.copy_(dz.to(logits.dtype))
         return loss * valid
+
+
+class PolicyLoss(_NativeLoss):
+    """Clipped policy gradient (``ops.policy_loss_``): the ratio to ``Sequence.old_logprobs`` (without them ``-A * logp``), per-token
+    ``advantages``, a k3 KL penalty to ``ref_logprobs`` and an entropy bonus, under the head's soft-cap and at a temperature.  Rows
+    whose target is ``-100`` or whose ``loss_mask`` is not above zero contribute nothing."""
+
+    def __init__(self, clip_low: float = 0.2, clip_high: Optional[float] = None, *, kl_coef: float = 0.0, entropy_coef: float = 0.0,
+                 temperature: float = 1.0, ignore_index: int = -100):
+        self.options = dict(clip_low=float(clip_low), clip_high=None if clip_high is None else float(clip_high), kl_beta=float(kl_coef),
+                            entropy_coef=float(entropy_coef), temperature=float(temperature), ignore_index=int(ignore_index))
+
+    def _given(self, sl: TokenSlice, softcap: float):
+        ref = sl.ref_logprobs if sl.ref_logprobs is not None else sl.extra.get("ref_logprobs")
+        return dict(old_logprobs=sl.extra.get("old_logprobs"), ref_logprobs=ref, softcap=softcap, loss_mask=sl.loss_mask, **self.options)
+
+    def __call__(self, logits, sl: TokenSlice, grad_scale: float, softcap: float = 0.0) -> torch.Tensor:
+        return ops.policy_loss_(logits, sl.targets, sl.advantages, grad_scale=grad_scale, **self._given(sl, softcap)).loss
+
+    def loss_only(self, logits, sl: TokenSlice, softcap: float = 0.0) -> torch.Tensor:
+        """The losses without the gradient: the logits are read once and not written."""
+        return ops.policy_loss(logits, sl.targets, sl.advantages, **self._given(sl, softcap)).loss
+
+
+class DistillationLoss(_NativeLoss):
+    """Distillation from a teacher's most likely tokens (``ops.distill_loss_``), ``Sequence.teacher_ids`` and ``teacher_logprobs`` as
+    ``ActiveModel.score(..., top_k=K, temperature=temperature)`` of the teacher gives them, mixed with ``ce_weight`` of the targets'
+    cross entropy.  Rows of a step without a teacher's tokens have the cross entropy's part alone."""
+
+    def __init__(self, *, rest: str = "drop", ce_weight: float = 0.0, temperature: float = 1.0, ignore_index: int = -100):
+        self.options = dict(rest=rest, ce_weight=float(ce_weight), temperature=float(temperature), ignore_index=int(ignore_index))
+
+    def check_sequences(self, seqs) -> None:
+        if not any(s.teacher_ids is not None for s in seqs):
+            raise ValueError("DistillationLoss: no sequence carries teacher_ids and teacher_logprobs")
+
+    def _given(self, logits, sl: TokenSlice, softcap: float):
+        ids, lps = sl.extra.get("teacher_ids"), sl.extra.get("teacher_logprobs")
+        if ids is None:
+            ids = torch.full((logits.shape[0], 1), -1, dtype=torch.int64, device=logits.device)
+            lps = torch.zeros(logits.shape[0], 1, dtype=torch.float32, device=logits.device)
+        return (logits, ids, lps), dict(targets=sl.targets, softcap=softcap, loss_mask=sl.loss_mask, **self.options)
+
+    def __call__(self, logits, sl: TokenSlice, grad_scale: float, softcap: float = 0.0) -> torch.Tensor:
+        args, kw = self._given(logits, sl, softcap)
+        return ops.distill_loss_(*args, grad_scale=grad_scale, **kw)
+
+    def loss_only(self, logits, sl: TokenSlice, softcap: float = 0.0) -> torch.Tensor:
+        """The losses without the gradient: the logits are read once and not written."""
+        args, kw = self._given(logits, sl, softcap)
+        return ops.distill_loss(*args, **kw)
+
+
+class TokenScorer(_NativeLoss):
+    """What ``ActiveModel.score`` runs in a loss's place: keeps the scores of each micro-chunk; the losses are the negative log
+    probabilities."""
+
+    def __init__(self, top_k: int = 0, temperature: float = 1.0):
+        self.top_k, self.temperature = int(top_k), float(temperature)
+        self._pieces: list = []
+
+    def __call__(self, logits, sl: TokenSlice, grad_scale: float, softcap: float = 0.0) -> torch.Tensor:
+        raise RuntimeError("scores have no gradient here; ops.token_logprobs_bwd_ takes theirs")
+
+    def loss_only(self, logits, sl: TokenSlice, softcap: float = 0.0) -> torch.Tensor:
+        s = ops.token_logprobs(logits, sl.targets, temperature=self.temperature, softcap=softcap, top_k=self.top_k, loss_mask=sl.loss_mask)
+        self._pieces.append(s)
+        return -s.logprobs
+
+    def take(self) -> "ops.TokenLogprobs":
+        """The scores since the last call, row after row."""
+        got, self._pieces = self._pieces, []
+        return ops.TokenLogprobs(*(None if p[0] is None else torch.cat(p) for p in zip(*got)))
+
+
+def has_loss_only(loss_fn) -> bool:
+    """Whether held-out data may take the loss's own form without a gradient: the class that defines the one has to define the other."""
+    owner = lambda name: next((c for c in type(loss_fn).__mro__ if name in vars(c)), None)
+    return (getattr(loss_fn, "_native", False) and isinstance(loss_fn, (PolicyLoss, DistillationLoss, TokenScorer))
+            and owner("__call__") is owner("loss_only"))

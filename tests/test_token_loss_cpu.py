@@ -5,7 +5,11 @@ import itertools
 import pytest
 import torch
 
+import flextrain_b200 as ft
+from conftest import build_tiny
 from flextrain_b200 import ops
+from flextrain_b200.bench.naive import clone_params, naive_forward
+from flextrain_b200.nn.loss import DistillationLoss, PolicyLoss, TokenScorer
 from token_loss_oracle import (check_distill, check_not_finite, check_policy, check_scores, check_scores_grad, distill, on_rows, policy, scores, some_teacher,
                                wide)
 
@@ -181,3 +185,184 @@ def test_refusals():
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"refusal {n} was taken")
+
+
+# ------------------------------------------------------------------------------------- losses and the engine
+DIMS = dict(vocab_size=256, n_layers=2, d_model=64, n_heads=4, n_kv_heads=2, head_dim=16, expert_dim=128, ffn_dim=128, num_routed_experts=0,
+            num_shared_experts=0, top_k=0, is_causal=True)
+
+
+def _sequences(lengths=(40, 24, 61)):
+    """Prompts without a target, a mask, one sequence of more than one chunk."""
+    g = torch.Generator().manual_seed(0)
+    out = []
+    for i, n in enumerate(lengths):
+        t = torch.randint(0, 256, (n,), generator=g)
+        tgt = torch.roll(t, -1)
+        tgt[-1] = -100
+        tgt[:3] = -100
+        out.append(ft.Sequence(t, targets=tgt, seq_id=i, advantages=torch.randn(n, generator=g),
+                               loss_mask=(torch.arange(n) % 7 != 5).float() if i == 1 else None))
+    return out
+
+
+def _model(cap=0.0, seed=None):
+    am = build_tiny(dims=DIMS, max_seq_len=64, batch_tokens=96)
+    am.head.final_softcap = cap
+    if seed is not None:
+        g = torch.Generator().manual_seed(seed)
+        w = am.buffers.head_params()["w_head_proj"]
+        w.copy_(torch.randn(w.shape, generator=g) * 0.2)
+    return am
+
+
+def _rows(am, P, s, cap, tau):
+    am.head.final_softcap = 0.0
+    z = naive_forward(am, P, s.tokens)
+    am.head.final_softcap = cap
+    u = cap * torch.tanh(z / cap) if cap else z
+    on = (s.targets != -100) & (s.loss_mask > 0 if s.loss_mask is not None else True)
+    lp = torch.log_softmax(u / tau, -1)
+    return z, lp, lp.gather(1, s.targets.clamp(min=0)[:, None])[:, 0], -(lp.exp() * lp).sum(-1), on
+
+
+def _gradients_agree(am, P, loss):
+    loss.backward()
+    bm, n = am.buffers, 0
+    for (scope, l, name), p in P.items():
+        g = {"embed": bm.embed_grads(), "head": bm.head_grads()}.get(scope) or bm.grads(l)
+        gname = "g_" + name[2:] if name.startswith("w_") else "g_" + name
+        if gname in g and p.grad is not None:
+            # both sides sum fp32 products of two layers in their own orders: some 16 roundings, 2^-24 each, of the tensor's largest
+            # (68 of the embedding: 6.5e-5)
+            torch.testing.assert_close(g[gname].float(), p.grad, rtol=3e-4, atol=3e-6 + 16 * 2.0 ** -24 * float(p.grad.abs().max()),
+                                       msg=lambda m: f"{scope}/{l}/{name}: {m}")
+            n += 1
+    assert n > 5
+
+
+@pytest.mark.parametrize("cap,tau,K", [(0.0, 1.0, 0), (5.0, 0.7, 6)])
+def test_score(cap, tau, K):
+    """Scores of every sequence against the model written out, also where a sequence takes several chunks and a chunk several pieces of
+    the head; nothing of a step changes."""
+    am, seqs = _model(cap, seed=1), _sequences()
+    am.head.head_chunk_size = 17
+    got = am.score(seqs, top_k=K, temperature=tau)
+    P = clone_params(am)
+    for s, g in zip(seqs, got):
+        assert s.scores is g
+        _, lp, given, ent, on = _rows(am, P, s, cap, tau)
+        torch.testing.assert_close(g.logprobs, (given * on).detach(), rtol=1e-4, atol=1e-5)
+        torch.testing.assert_close(g.entropy, (ent * on).detach(), rtol=1e-4, atol=1e-5)
+        torch.testing.assert_close(s.per_token_loss, -g.logprobs)
+        if K:
+            want = lp.detach().topk(K)
+            torch.testing.assert_close(g.top_logprobs[on], want.values[on], rtol=1e-4, atol=1e-5)
+            assert bool((g.top_ids[~on] == -1).all())
+        else:
+            assert g.top_ids is None
+    assert am.step_num == 0 and am.fwd_bwd_serial == 0
+    for bad in (dict(top_k=129), dict(top_k=-1), dict(temperature=0.0)):
+        with pytest.raises(ValueError):
+            am.score(seqs, **bad)
+    with pytest.raises(RuntimeError):
+        am.fwd_bwd(seqs, loss_fn=TokenScorer())
+
+
+@pytest.mark.parametrize("cap,tau,ref", [(0.0, 1.0, True), (5.0, 0.7, False)])
+def test_policy_loss_through_the_engine(cap, tau, ref):
+    """Rollouts scored under the old weights, then a step's loss and gradients under others."""
+    seqs = _sequences()
+    am = _model(cap, seed=1)
+    for s, g in zip(seqs, am.score(seqs, temperature=tau)):
+        # (at the same weights all ratios are one)
+        s.old_logprobs = g.logprobs + 0.3 * torch.sin(torch.arange(len(s)).float())
+        if ref:
+            s.ref_logprobs = g.logprobs + 0.2 * torch.cos(torch.arange(len(s)).float())
+    if not ref:
+        seqs[0].advantages = seqs[1].advantages = seqs[2].advantages = None
+    P = clone_params(am)
+    total = 0.0
+    for s in seqs:
+        _, lp, given, ent, on = _rows(am, P, s, cap, tau)
+        a = s.advantages if s.advantages is not None else torch.ones(len(s))
+        r = torch.exp(given - s.old_logprobs)
+        l = -torch.minimum(r * a, r.clamp(0.8, 1.25) * a) - 0.01 * ent
+        if ref:
+            d = s.ref_logprobs - given
+            l = l + 0.1 * (d.exp() - d - 1)
+        total = total + (l * on).sum()
+    loss = PolicyLoss(0.2, 0.25, kl_coef=0.1, entropy_coef=0.01, temperature=tau)
+    held_out = am.evaluate(seqs, loss_fn=loss)
+    st = am.fwd_bwd(seqs, loss_scale_factor=1.0, loss_fn=loss)
+    assert abs(st.loss_sum - total.item()) < 1e-3 * max(1.0, abs(total.item())) and held_out.loss_sum == st.loss_sum
+    _gradients_agree(am, P, total)
+
+
+def test_a_reference_without_advantages_counts():
+    seqs = _sequences((40,))
+    seqs[0].advantages = None
+    seqs[0].ref_logprobs = torch.full((40,), -3.0)
+    am = _model(seed=1)
+    with_it = am.evaluate(seqs, loss_fn=PolicyLoss(kl_coef=0.5)).loss_sum
+    assert with_it > am.evaluate(seqs, loss_fn=PolicyLoss()).loss_sum
+
+
+@pytest.mark.parametrize("cap,tau,rest,ce", [(0.0, 2.0, "drop", 0.3), (5.0, 1.0, "bucket", 0.0)])
+def test_distillation_through_the_engine(cap, tau, rest, ce):
+    """A teacher's alternatives as score() gives them; one sequence without a teacher, one with fewer of its tokens."""
+    seqs = _sequences()
+    K = 8
+    for s, g in zip(seqs, _model(cap, seed=2).score(seqs, top_k=K, temperature=tau)):
+        s.teacher_ids, s.teacher_logprobs = g.top_ids, g.top_logprobs
+    seqs[0].teacher_ids, seqs[0].teacher_logprobs = seqs[0].teacher_ids[:, :5], seqs[0].teacher_logprobs[:, :5]
+    seqs[1].teacher_ids = seqs[1].teacher_logprobs = None
+    am = _model(cap, seed=1)
+    P = clone_params(am)
+    total = 0.0
+    for s in seqs:
+        z, lp, _, _, on = _rows(am, P, s, cap, tau)
+        l = torch.zeros(len(s))
+        if s.teacher_ids is not None:
+            ids, t = s.teacher_ids[on], s.teacher_logprobs[on]
+            q = torch.softmax(t, -1) if rest == "drop" else t.exp()
+            kl = (q * (q.log() - lp[on].gather(1, ids))).sum(-1)
+            if rest == "bucket":
+                others = torch.logsumexp(lp[on].scatter(1, ids, float("-inf")), -1)
+                kl = kl + (1 - q.sum(-1)) * ((1 - q.sum(-1)).log() - others)
+            l = torch.zeros(len(s)).index_put((on.nonzero()[:, 0],), (1 - ce) * tau * tau * kl)
+        # (without a teacher's token all tokens are the rest, which has probability one for both)
+        hard = torch.nn.functional.cross_entropy(cap * torch.tanh(z / cap) if cap else z, s.targets, reduction="none")
+        total = total + ((l + ce * hard) * on).sum()
+    loss = DistillationLoss(rest=rest, ce_weight=ce, temperature=tau)
+    held_out = am.evaluate(seqs, loss_fn=loss)
+    st = am.fwd_bwd(seqs, loss_scale_factor=1.0, loss_fn=loss)
+    assert abs(st.loss_sum - total.item()) < 1e-3 * max(1.0, abs(total.item())) and held_out.loss_sum == st.loss_sum
+    _gradients_agree(am, P, total)
+
+
+def test_what_sequences_carry_is_checked():
+    am = _model()
+    ids, lps = torch.zeros(40, 3, dtype=torch.int64), torch.zeros(40, 3)
+    for kw in (dict(teacher_ids=ids), dict(teacher_ids=ids, teacher_logprobs=lps[:, :2]), dict(teacher_ids=ids[:30], teacher_logprobs=lps[:30]),
+               dict(teacher_ids=lps, teacher_logprobs=lps), dict(teacher_ids=ids[:, 0], teacher_logprobs=lps[:, 0]), dict(old_logprobs=lps[:3, 0]),
+               dict(teacher_ids=ids.repeat(1, 50), teacher_logprobs=lps.repeat(1, 50))):
+        s = _sequences((40,))
+        for k, v in kw.items():
+            setattr(s[0], k, v)
+        with pytest.raises(ValueError):
+            am.fwd_bwd(s)
+    s = _sequences((40, 24))
+    s[0].old_logprobs = torch.zeros(40)
+    with pytest.raises(ValueError):
+        am.fwd_bwd(s, loss_fn=PolicyLoss())
+    with pytest.raises(ValueError):
+        am.fwd_bwd(_sequences(), loss_fn=DistillationLoss())
+
+    class Bare:                                               # a sequence of one's own class
+        tokens, targets = s[1].tokens, s[1].targets
+        old_logprobs, teacher_ids, teacher_logprobs = torch.zeros(24), ids[:24].tolist(), lps[:24]
+
+    got = am.score([Bare()], top_k=2)[0]
+    assert got.logprobs.shape == (24,) and got.top_ids.shape == (24, 2)
+    assert am.evaluate([Bare()], loss_fn=DistillationLoss()).loss_sum > 0
