@@ -20,6 +20,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "ptx.cuh"
 
@@ -97,6 +98,30 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ float from_float<float>(float v) { return v; }
 
+// tanh y and 1 - tanh^2 y.  Near zero y (1 + s P(s)), s = y^2, P fitted to (tanh(y) / y - 1) / s on |y| <= 3/4 for the smallest largest
+// relative error (2e-9; with the roundings of fp32 it is some 2^-23.5); beyond it 1 - 2 / (1 + e^2y), whose slope is formed without 1 - t^2.
+constexpr float TANH_NEAR = 0.75f;
+__device__ __forceinline__ float tanh_far(float y, float& slope) {
+  const float r = __fdividef(2.f, 1.f + ex2(fminf(fabsf(y) * (2.f * LOG2E), 100.f)));
+  slope = r * (2.f - r);
+  return y != y ? y : copysignf(1.f - r, y);
+}
+__device__ __forceinline__ float tanh_of(float y, float& slope) {
+  const float s = y * y;
+  float p = 0.001736928359605372f;
+  p = fmaf(p, s, -0.007657244335860014f);
+  p = fmaf(p, s, 0.021452028304338455f);
+  p = fmaf(p, s, -0.053892724215984344f);
+  p = fmaf(p, s, 0.1333269476890564f);
+  p = fmaf(p, s, -0.33333316445350647f);
+  const float near = fmaf(y, s * p, y);
+  float far_slope;
+  const float far = tanh_far(y, far_slope);
+  const bool is_near = fabsf(y) <= TANH_NEAR;
+  slope = is_near ? 1.f - near * near : far_slope;
+  return is_near ? near : far;
+}
+
 // the cap and its slope
 template <bool CAP>
 __device__ __forceinline__ float capped(const Row& a, float z, float& slope) {
@@ -104,8 +129,7 @@ __device__ __forceinline__ float capped(const Row& a, float z, float& slope) {
     slope = 1.f;
     return z;
   }
-  const float t = tanhf(z * a.inv_cap);
-  slope = 1.f - t * t;
+  const float t = tanh_of(z * a.inv_cap, slope);
   return z == -INFINITY ? z : a.cap * t;                       // (a token without probability stays one)
 }
 template <bool CAP>
@@ -172,8 +196,8 @@ __device__ __forceinline__ float policy_row(const Row& a, int row, float lp, flo
 // What a part of a row (one block's) adds to them.  ``m``: largest u of the tokens that are not named (the given token of scores and
 // policy rows, the teacher's of distillation are, and are added by themselves), S and A sums of e and of e log2 e relative to it, S1 of
 // e at a temperature of one.
-struct Part {
-  float m, S, A, S1;
+struct __align__(16) Part {
+  float m, S, A, S1;                      // (S1 of scores: the largest logit itself, the given token's among them)
   float B, En, En1, kl, Q;                // distillation: the named tokens of this part relative to their largest u, B
   float ut, has_t;                        // the given token's u, in the part that holds it
   uint32_t tau;                           // scores: at least K tokens of the part are not below it
@@ -184,8 +208,9 @@ struct Totals {
   float base, k0, ka, kb;                 // gradient of a token that is not named: 2^((u - base) c + k0) (ka + kb log p) ...
   float share, h0;                        // ... + ce 2^((u - M) log2 e - h0); distillation: the sum of q
   uint32_t tau;
+  float top;                              // scores: the largest logit
 };
-constexpr int PART_WORDS = sizeof(Part) / 4;
+constexpr int PART_PIECES = sizeof(Part) / 16;
 
 template <typename F>
 __device__ __forceinline__ float over8(float v, F f) {        // over the eight lanes that hold the parts
@@ -200,7 +225,7 @@ __device__ __forceinline__ float max8(float v) { return over8(v, [](float a, flo
 template <Op OP, bool HARD>
 __device__ __forceinline__ void total(const Row& a, int row, int parts, const Part* rec, float qr, bool first, Totals* fin) {
   const int lane = threadIdx.x & 31;
-  Part p = {-INFINITY, 0.f, 0.f, 0.f, -INFINITY, 0.f, 0.f, 0.f, 0.f, -INFINITY, 0.f, 0u};
+  Part p = {-INFINITY, 0.f, 0.f, OP == SCORES ? -INFINITY : 0.f, -INFINITY, 0.f, 0.f, 0.f, 0.f, -INFINITY, 0.f, 0u};
   if ((lane & 7) < parts) p = rec[lane & 7];
   Totals t = {};
   const float rest = max8(p.m);                               // of the tokens that are not named
@@ -227,6 +252,7 @@ __device__ __forceinline__ void total(const Row& a, int row, int parts, const Pa
 #pragma unroll
       for (int o = 4; o; o >>= 1) tau = max(tau, __shfl_xor_sync(~0u, tau, o));
       t.tau = tau;
+      t.top = max8(p.S1);
       if (first && lane == 0) {
         if (a.logprob) a.logprob[row] = t.lp;
         a.entropy[row] = t.H;
@@ -317,54 +343,115 @@ __device__ __forceinline__ void row_off(const Row& a, int row) {                
     }
 }
 
-// The teacher's entry of thread k: its token (-1: none), q and log q; which entries name a token for the first time.
+// The teacher's entries k = lane, lane + 32, ... by one warp: token (-1: none), q and log q; in the part that holds it the token's logit,
+// and of entries of the same token one that stands for all.
+constexpr int ENTRIES = MOST_TOP / 32;
 struct Named {
-  int id;
-  float q, log_q;
-  bool first;
+  int id[ENTRIES];
+  float q[ENTRIES], log_q[ENTRIES], z[ENTRIES];
+  bool here[ENTRIES], first[ENTRIES];
 };
-// By a block; ``id`` and ``q`` are of MOST_TOP.  Returns what the teacher leaves to all others (0 without the bucket).
-template <int NT>
-__device__ __forceinline__ float teacher_of(const Row& a, int row, int* id, float* q, float* sh, Named& n) {
-  const int tid = threadIdx.x;
-  n = {-1, 0.f, -INFINITY, false};
-  if (tid < a.K) {
-    const long k = a.ids[(size_t)row * a.K + tid];
-    if (k >= 0 && k < a.V) {
-      n.id = static_cast<int>(k);
-      n.log_q = a.teacher[(size_t)row * a.K + tid];
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
+  return v;
+}
+// Returns what the teacher leaves to all others (0 without the bucket); ``id`` and ``q`` are of MOST_TOP, ``named_t``: t is among them.
+__device__ __forceinline__ float teacher_of(const Row& a, int row, long t, int* id, float* q, Named& n, bool& named_t) {
+  const int lane = threadIdx.x & 31;
+  float top = -INFINITY, sum = 0.f;
+  bool has_t = false;
+#pragma unroll
+  for (int j = 0; j < ENTRIES; ++j) {
+    const int k = lane + 32 * j;
+    n.id[j] = -1;
+    n.log_q[j] = -INFINITY;
+    n.here[j] = n.first[j] = false;
+    n.z[j] = 0.f;
+    if (k < a.K) {
+      const long i = a.ids[(size_t)row * a.K + k];
+      if (i >= 0 && i < a.V) {
+        n.id[j] = static_cast<int>(i);
+        n.log_q[j] = a.teacher[(size_t)row * a.K + k];
+        has_t |= i == t;
+      }
+      id[k] = n.id[j];
     }
-    id[tid] = n.id;
+    top = fmaxf(top, n.log_q[j]);
   }
-  if (!a.bucket) {
-    const float top = block_max<NT>(n.log_q, sh);
-    if (top != -INFINITY) n.log_q -= top;
-    const float s = block_sum<NT>(n.id >= 0 ? expf(n.log_q) : 0.f, sh);
-    if (top != -INFINITY) n.log_q -= logf(s);
+  named_t = __any_sync(~0u, has_t);
+  top = warp_max(top);
+  if (a.bucket || top == -INFINITY) top = 0.f;
+#pragma unroll
+  for (int j = 0; j < ENTRIES; ++j) {
+    n.log_q[j] -= top;
+    n.q[j] = n.id[j] >= 0 ? expf(n.log_q[j]) : 0.f;
+    sum += n.q[j];
   }
-  n.q = n.id >= 0 ? expf(n.log_q) : 0.f;
-  const float sum = block_sum<NT>(n.q, sh);
-  if (tid < a.K) q[tid] = n.q;
-  n.first = n.id >= 0;
-  for (int k = 0; n.first && k < tid; ++k) n.first = id[k] != n.id;
-  __syncthreads();
+  sum = warp_sum(sum);
+  if (!a.bucket && sum != 0.f) {
+    const float l = logf(sum);
+#pragma unroll
+    for (int j = 0; j < ENTRIES; ++j) {
+      n.log_q[j] -= l;
+      n.q[j] = n.id[j] >= 0 ? expf(n.log_q[j]) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < ENTRIES; ++j)
+    if (lane + 32 * j < a.K) q[lane + 32 * j] = n.q[j];
   return a.bucket && sum < 1.f ? 1.f - sum : 0.f;
 }
-// its share of the part: B, En, En1, kl, Q in thread 0 (``u`` -inf and ``here`` false where another part holds it)
-template <bool HARD, int NT>
-__device__ __forceinline__ void named_part(const Row& a, const Named& n, bool here, float u, float* sh, Part& p) {
-  p.B = block_max<NT>(here ? u : -INFINITY, sh);
-  const float d = u - (p.B == -INFINITY ? 0.f : p.B);
-  p.En = block_sum<NT>(here && n.first ? ex2(d * a.c) : 0.f, sh);
-  if (HARD) p.En1 = block_sum<NT>(here && n.first ? ex2(d * LOG2E) : 0.f, sh);
-  p.kl = block_sum<NT>(here && n.q != 0.f ? n.q * (n.log_q - d * a.inv_tau) : 0.f, sh);
-  p.Q = block_sum<NT>(here ? n.q : 0.f, sh);
+// B, En, En1, kl and Q of a part
+template <bool CAP, bool HARD>
+__device__ __forceinline__ void named_part(const Row& a, const Named& n, Part& p) {
+  float u[ENTRIES], B = -INFINITY, En = 0.f, En1 = 0.f, kl = 0.f, Q = 0.f;
+#pragma unroll
+  for (int j = 0; j < ENTRIES; ++j) {
+    u[j] = n.here[j] ? capped<CAP>(a, n.z[j]) : -INFINITY;
+    B = fmaxf(B, u[j]);
+  }
+  B = warp_max(B);
+#pragma unroll
+  for (int j = 0; j < ENTRIES; ++j) {
+    const float d = u[j] - (B == -INFINITY ? 0.f : B);
+    if (n.first[j]) En += ex2(d * a.c);
+    if (HARD && n.first[j]) En1 += ex2(d * LOG2E);
+    if (n.here[j] && n.q[j] != 0.f) kl += n.q[j] * (n.log_q[j] - d * a.inv_tau);
+    if (n.here[j]) Q += n.q[j];
+  }
+  p.B = B;
+  p.En = warp_sum(En);
+  if (HARD) p.En1 = warp_sum(En1);
+  p.kl = warp_sum(kl);
+  p.Q = warp_sum(Q);
 }
 __device__ __forceinline__ float q_of(const int* id, const float* q, int K, int mine) {
   float s = 0.f;
   for (int k = 0; k < K; ++k) s += id[k] == mine ? q[k] : 0.f;
   return s;
 }
+// the gradients of the named tokens, by the same warp
+template <typename E, bool CAP, bool HARD>
+__device__ __forceinline__ void write_named(const Row& a, const Totals& t, const Named& n, const int* id, const float* q, long target, float scale, E* out) {
+  bool more = false;
+#pragma unroll
+  for (int j = 0; j < ENTRIES; ++j) more |= n.here[j] && !n.first[j];
+  more = __any_sync(~0u, more);
+#pragma unroll
+  for (int j = 0; j < ENTRIES; ++j)
+    if (n.first[j]) {
+      float slope;
+      const float u = capped<CAP>(a, n.z[j], slope), qs = more ? q_of(id, q, a.K, n.id[j]) : n.q[j];
+      out[n.id[j]] = from_float<E>(grad_named<HARD>(a, t, u, qs, n.id[j] == target) * slope * scale);
+    }
+}
+
 
 // ------------------------------------------------------------------------------------------- rows in shared memory
 // A cluster of up to eight blocks takes a row and keeps it in their shared memory, so that memory is read once and the gradient is the
@@ -386,56 +473,194 @@ __device__ __forceinline__ uint32_t in_cluster(const void* p, int rank) {       
 }
 __device__ __forceinline__ void put32(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
 __device__ __forceinline__ void put64(uint32_t at, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
+// 16 bytes to another block, counted on a barrier there
+__device__ __forceinline__ void send16(uint32_t at, const uint4& v, uint32_t barrier) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w), "r"(barrier)
+               : "memory");
+}
 __device__ __forceinline__ void cluster_arrive() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// what other blocks sent; bounded as ftb::mbar_wait
+__device__ __forceinline__ bool sent_wait(uint64_t* bar, int where) {
+  for (uint32_t it = 0; it < FTB_WAIT_LIMIT; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n"
+        "selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(ftb::smem_u32(bar))
+        : "memory");
+    if (ok) return true;
+  }
+  ftb::set_error(1, where);
+  return false;
+}
 
+// two floats to an instruction
+typedef u64 f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 exp2_2(f32x2 x) {
+  float a, b;
+  split(x, a, b);
+  return pair(ex2(a), ex2(b));
+}
+
+// 16 bytes of a row as pairs of floats, their largest, and back
 template <typename E>
-struct Vec {
-  static constexpr int N = 16 / sizeof(E);
+struct Vec;
+template <>
+struct Vec<bf16> {
+  static constexpr int N = 8;
+  static constexpr float LOW = -0x1p100f;                     // a finite number below all logits that are not a mask's
+  __device__ static uint32_t max2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  __device__ static f32x2 one(uint32_t w) { return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+  __device__ static float top(uint32_t m) { return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u)); }
+  __device__ static uint32_t word(f32x2 v) {
+    float a, b;
+    split(v, a, b);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static constexpr uint32_t NONE = 0xFF80FF80u, FLOOR = 0xF180F180u;      // -inf, LOW
 };
-__device__ __forceinline__ void unpack(const uint4& v, float (&f)[8], bf16) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+template <>
+struct Vec<__half> {
+  static constexpr int N = 8;
+  static constexpr float LOW = -65504.f;
+  __device__ static uint32_t max2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  __device__ static f32x2 one(uint32_t w) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return pair(f.x, f.y);
+  }
+  __device__ static float top(uint32_t m) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
+    return fmaxf(f.x, f.y);
+  }
+  __device__ static uint32_t word(f32x2 v) {
+    float a, b;
+    split(v, a, b);
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static constexpr uint32_t NONE = 0xFC00FC00u, FLOOR = 0xFBFFFBFFu;
+};
+template <>
+struct Vec<float> {
+  static constexpr int N = 4;
+  static constexpr float LOW = -0x1p100f;
+  __device__ static uint32_t max2(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+  __device__ static float top(uint32_t m) { return __uint_as_float(m); }
+  static constexpr uint32_t NONE = 0xFF800000u, FLOOR = 0xF1800000u;
+};
+template <typename E>
+__device__ __forceinline__ uint32_t vec_max(const uint4& v) {
+  return Vec<E>::max2(Vec<E>::max2(v.x, v.y), Vec<E>::max2(v.z, v.w));
+}
+template <typename E>
+__device__ __forceinline__ uint4 vec_floor(const uint4& v) {  // -inf and all below LOW to LOW
+  constexpr uint32_t f = Vec<E>::FLOOR;
+  return make_uint4(Vec<E>::max2(v.x, f), Vec<E>::max2(v.y, f), Vec<E>::max2(v.z, f), Vec<E>::max2(v.w, f));
+}
+template <typename E>
+__device__ __forceinline__ void pairs_of(const uint4& v, f32x2 (&x)[Vec<E>::N / 2]) {
+  if constexpr (sizeof(E) == 4) {
+    x[0] = pair(__uint_as_float(v.x), __uint_as_float(v.y));
+    x[1] = pair(__uint_as_float(v.z), __uint_as_float(v.w));
+  } else {
+    x[0] = Vec<E>::one(v.x); x[1] = Vec<E>::one(v.y); x[2] = Vec<E>::one(v.z); x[3] = Vec<E>::one(v.w);
   }
 }
-__device__ __forceinline__ void unpack(const uint4& v, float (&f)[8], __half) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    f[2 * i] = g.x;
-    f[2 * i + 1] = g.y;
+template <typename E>
+__device__ __forceinline__ uint4 vec_of(const f32x2 (&x)[Vec<E>::N / 2]) {
+  if constexpr (sizeof(E) == 4) {
+    float a, b, c, d;
+    split(x[0], a, b);
+    split(x[1], c, d);
+    return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
+  } else {
+    return make_uint4(Vec<E>::word(x[0]), Vec<E>::word(x[1]), Vec<E>::word(x[2]), Vec<E>::word(x[3]));
   }
 }
-__device__ __forceinline__ void unpack(const uint4& v, float (&f)[4], float) {
-  f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
-}
-__device__ __forceinline__ uint4 pack(const float (&f)[8], bf16) {
-  uint32_t w[4];
+template <typename E>
+__device__ __forceinline__ void floats_of(const uint4& v, float (&f)[Vec<E>::N]) {
+  f32x2 x[Vec<E>::N / 2];
+  pairs_of<E>(v, x);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&h);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  for (int i = 0; i < Vec<E>::N / 2; ++i) split(x[i], f[2 * i], f[2 * i + 1]);
 }
-__device__ __forceinline__ uint4 pack(const float (&f)[8], __half) {
-  uint32_t w[4];
+// z to u in place, and the slopes; the tanh of all pairs near zero by its polynomial, of any beyond it one by one
+template <typename E, bool SLOPE>
+__device__ __forceinline__ void cap_pairs(const Row& a, f32x2 (&x)[Vec<E>::N / 2], f32x2 (&slope)[Vec<E>::N / 2]) {
+  constexpr int P = Vec<E>::N / 2;
+  f32x2 y[P];
+  float most = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  for (int i = 0; i < P; ++i) {
+    y[i] = mul2(x[i], pair(a.inv_cap, a.inv_cap));
+    float c, d;
+    split(y[i], c, d);
+    most = fmaxf(most, fmaxf(fabsf(c), fabsf(d)));
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ uint4 pack(const float (&f)[4], float) {
-  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  if (most <= TANH_NEAR) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const f32x2 s = mul2(y[i], y[i]);
+      f32x2 p = pair(0.001736928359605372f, 0.001736928359605372f);
+      p = fma2(p, s, pair(-0.007657244335860014f, -0.007657244335860014f));
+      p = fma2(p, s, pair(0.021452028304338455f, 0.021452028304338455f));
+      p = fma2(p, s, pair(-0.053892724215984344f, -0.053892724215984344f));
+      p = fma2(p, s, pair(0.1333269476890564f, 0.1333269476890564f));
+      p = fma2(p, s, pair(-0.33333316445350647f, -0.33333316445350647f));
+      const f32x2 t = fma2(y[i], mul2(s, p), y[i]);
+      if (SLOPE) slope[i] = fma2(mul2(t, pair(-1.f, -1.f)), t, pair(1.f, 1.f));
+      x[i] = mul2(t, pair(a.cap, a.cap));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      float c, d, sc, sd;
+      split(x[i], c, d);
+      c = capped<true>(a, c, sc);
+      d = capped<true>(a, d, sd);
+      x[i] = pair(c, d);
+      if (SLOPE) slope[i] = pair(sc, sd);
+    }
+  }
 }
 
 __device__ __forceinline__ u64 key_of(float z, int token) { return static_cast<u64>(order_of(z)) << 32 | static_cast<uint32_t>(~token); }
@@ -445,12 +670,12 @@ __device__ __forceinline__ float logit_of(uint32_t order) {
 
 template <typename E, Op OP, bool TOP, bool CAP, bool HARD, int NT>
 __global__ void __launch_bounds__(NT, NT == 256 ? 5 : 2) slice_kernel(Row a, int slice, int room) {
-  constexpr int VE = Vec<E>::N;
+  constexpr int VE = Vec<E>::N, P = VE / 2, W = NT / 32;
   extern __shared__ __align__(128) unsigned char buf[];
-  __shared__ __align__(8) uint64_t bar;
+  __shared__ __align__(8) uint64_t bar, sent;
   __shared__ int gave_up, found;
-  __shared__ float sh[32];
-  __shared__ Part rec[MOST_PARTS];
+  __shared__ float sh[32], most[W], least[W], sums[3][W];
+  __shared__ Part rec[MOST_PARTS], own;
   __shared__ Totals fin;
   __shared__ int count[2][MOST_PARTS];
   __shared__ int id[OP == DISTILL ? MOST_TOP : 1];
@@ -461,139 +686,226 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 5 : 2) slice_kernel(Row a, int
   int rank, parts;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
-  const int row = blockIdx.x / parts, tid = threadIdx.x, V = a.V;
+  const int row = blockIdx.x / parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V, K = a.K;
   const E* z = static_cast<const E*>(a.z) + row * a.ldz;
   E* out = static_cast<E*>(a.out) + row * a.ldo;
   // the row from the 16-byte piece that it begins in: ``lead`` elements before it, this block's from ``lo`` on, n of them in pieces
   const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(E));
   const int lo = rank * slice, n = max(0, min(lead + V - lo, slice)), nv = (n + VE - 1) / VE, first_token = lo - lead;
+  const bool whole = OP != SCORES && (reinterpret_cast<uintptr_t>(out) & 15) / sizeof(E) == lead;       // the gradient's pieces lie as the logits' do
   const long t = a.targets ? a.targets[row] : -1;
   if (!row_on(a, row, t)) {
-    if (OP != SCORES && a.out) {
-      const int from = max(first_token, 0), to = min(first_token + n, V);
-      for (int j = from + tid; j < to; j += NT) out[j] = from_float<E>(0.f);
-    }
+    if (OP != SCORES && a.out)
+      for (int v = tid; v < nv; v += NT) {
+        const int token = first_token + v * VE;
+        if (whole && token >= 0 && token + VE <= V) {
+          *reinterpret_cast<uint4*>(out + token) = make_uint4(0, 0, 0, 0);
+        } else {
+          for (int e = 0; e < VE; ++e)
+            if (token + e >= 0 && token + e < V) out[token + e] = from_float<E>(0.f);
+        }
+      }
     if (rank == 0) row_off<OP>(a, row);
     return;
   }
   if (tid == 0) {
-    gave_up = 0;
+    gave_up = found = 0;
     ftb::mbar_init(&bar, 1);
+    ftb::mbar_init(&sent, 1);
     ftb::fence_barrier_init();
+    ftb::mbar_expect_tx(&sent, parts * sizeof(Part));
     if (nv > 0) {
       ftb::mbar_expect_tx(&bar, nv * 16);
       ftb::bulk_load_g2s(buf, z - lead + lo, nv * 16, &bar);
     }
   }
-  cluster_arrive();                                           // (the others' shared memory may be written once all have begun)
+  cluster_arrive_relaxed();                                   // (the others may be sent to once all have begun)
   float qr = 0.f;
-  Named mine = {-1, 0.f, -INFINITY, false};
-  if (OP == DISTILL) qr = teacher_of<NT>(a, row, id, q, sh, mine);
-  else __syncthreads();
+  bool named_t = false;
+  Named mine;
+  if (OP == DISTILL && warp == 0) qr = teacher_of(a, row, t, id, q, mine, named_t);
+  __syncthreads();
+  cluster_wait();
   if (nv > 0 && !ftb::mbar_wait(&bar, 0, &gave_up, 1)) {      // (reported; the copy gets as long again before the block goes on)
     int again = 0;
     ftb::mbar_wait(&bar, 0, &again, 2);
   }
 
   // what lies around the row is no token; named tokens by themselves
-  if (tid < VE) {
-    if (lo + tid < lead && tid < nv * VE) zs[tid] = from_float<E>(-INFINITY);
-    if (n + tid < nv * VE) zs[n + tid] = from_float<E>(-INFINITY);
-  }
   const int at_t = static_cast<int>(t) - first_token;         // where the given token lies
   const bool mine_t = a.targets && at_t >= 0 && at_t < n;
-  const bool here = OP == DISTILL && mine.id >= first_token && mine.id < first_token + n && mine.id >= 0;
-  float zt = 0.f, zk = 0.f;
-  if (mine_t && tid == 0) zt = to_float(zs[at_t]);
-  if (here) zk = to_float(zs[mine.id - first_token]);
-  if (OP == DISTILL) __syncthreads();                         // (an entry twice: both have read)
-  if (here) zs[mine.id - first_token] = from_float<E>(-INFINITY);
-  if (OP != DISTILL && mine_t && tid == 0) zs[at_t] = from_float<E>(-INFINITY);
+  float zt = 0.f;
+  if (warp == 0) {
+    if (lane < VE) {
+      if (lo + lane < lead && lane < nv * VE) zs[lane] = from_float<E>(-INFINITY);
+      if (n + lane < nv * VE) zs[n + lane] = from_float<E>(-INFINITY);
+    }
+    if (mine_t) zt = to_float(zs[at_t]);
+    __syncwarp();
+    if (OP != DISTILL && mine_t && lane == 0) zs[at_t] = from_float<E>(-INFINITY);
+    if (OP == DISTILL) {
+      typedef typename std::conditional<sizeof(E) == 2, uint16_t, uint32_t>::type Bits;
+      Bits* tag = reinterpret_cast<Bits*>(buf);
+#pragma unroll
+      for (int j = 0; j < ENTRIES; ++j) {
+        mine.here[j] = mine.id[j] >= first_token && mine.id[j] < first_token + n && mine.id[j] >= 0;
+        if (mine.here[j]) mine.z[j] = to_float(zs[mine.id[j] - first_token]);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < ENTRIES; ++j)                       // of entries of one token, the one whose number stays in its place
+        if (mine.here[j]) tag[mine.id[j] - first_token] = static_cast<Bits>(lane + 32 * j);
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < ENTRIES; ++j) mine.first[j] = mine.here[j] && tag[mine.id[j] - first_token] == static_cast<Bits>(lane + 32 * j);
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < ENTRIES; ++j)
+        if (mine.here[j]) zs[mine.id[j] - first_token] = from_float<E>(-INFINITY);
+    }
+  }
   __syncthreads();
 
   // largest of each thread, of the block
-  float mt = -INFINITY;
-  for (int v = tid; v < nv; v += NT) {
-    float f[VE];
-    unpack(zv[v], f, E());
+  uint32_t m2 = Vec<E>::NONE;
+#pragma unroll 4
+  for (int v = tid; v < nv; v += NT) m2 = Vec<E>::max2(m2, vec_max<E>(zv[v]));
+  const float mt = Vec<E>::top(m2);
+  {
+    const float w = warp_max(mt);
+    if (lane == 0) most[warp] = w;
+    if (TOP) {
+      float l = tid < nv ? mt : INFINITY;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) mt = fmaxf(mt, f[e]);
-  }
-  const float mz = block_max<NT>(mt, sh);
-  Part p = {};
-  p.m = mz == -INFINITY ? mz : capped<CAP>(a, mz);
-  const float base = mz == -INFINITY ? 0.f : p.m;
-  float S = 0.f, A = 0.f, S1 = 0.f;
-  for (int v = tid; v < nv; v += NT) {
-    float f[VE];
-    unpack(zv[v], f, E());
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      const float d = capped<CAP>(a, f[e]) - base, x = d * a.c, w = ex2(x);
-      S += w;
-      if (OP != DISTILL) A += w * max_nan(x, -256.f);
-      if (HARD) S1 += ex2(d * LOG2E);
+      for (int o = 16; o; o >>= 1) l = fminf(l, __shfl_xor_sync(~0u, l, o));
+      if (lane == 0) least[warp] = l;
     }
   }
-  p.S = block_sum<NT>(S, sh);
-  if (OP != DISTILL) p.A = block_sum<NT>(A, sh);
-  if (HARD) p.S1 = block_sum<NT>(S1, sh);
-  p.B = -INFINITY;
-  if (OP == DISTILL) named_part<HARD, NT>(a, mine, here, here ? capped<CAP>(a, zk) : -INFINITY, sh, p);
-  const int K = a.K;
+  __syncthreads();
+  float mz = most[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) mz = fmaxf(mz, most[w]);
+  const float um = mz == -INFINITY ? mz : capped<CAP>(a, mz), base = mz == -INFINITY ? 0.f : um;
+
+  // sums relative to it
+  {
+    f32x2 S = 0, S1 = 0;
+    float A = 0.f;
+    const f32x2 minus = pair(-base, -base), cc = pair(a.c, a.c), l2 = pair(LOG2E, LOG2E);
+#pragma unroll 2
+    for (int v = tid; v < nv; v += NT) {
+      const uint4 w = zv[v];
+      f32x2 x[P], slope[P], part = 0;
+      pairs_of<E>(w, x);
+      if (CAP) cap_pairs<E, false>(a, x, slope);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const f32x2 d = add2(x[i], minus), y = mul2(d, cc), e = exp2_2(y);
+        S = add2(S, e);
+        if (OP != DISTILL) part = fma2(e, y, part);
+        if (HARD) S1 = add2(S1, exp2_2(mul2(d, l2)));
+      }
+      if (OP != DISTILL) {
+        float b, c;
+        split(part, b, c);
+        b += c;
+        if (b != b) {                                         // (a logit of -inf: nothing times minus infinity)
+          float f[VE];
+          floats_of<E>(w, f);
+          b = 0.f;
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const float y = (capped<CAP>(a, f[e]) - base) * a.c;
+            b += ex2(y) * max_nan(y, -256.f);
+          }
+        }
+        A += b;
+      }
+    }
+    float b, c;
+    split(S, b, c);
+    b = warp_sum(b + c);
+    if (lane == 0) sums[0][warp] = b;
+    if (OP != DISTILL) {
+      A = warp_sum(A);
+      if (lane == 0) sums[1][warp] = A;
+    }
+    if (HARD) {
+      split(S1, b, c);
+      b = warp_sum(b + c);
+      if (lane == 0) sums[2][warp] = b;
+    }
+  }
+  uint32_t tau = 0;
   if (TOP) {
     // the largest of some K to K + K / 8 + 8 threads are not below tau (all tokens where fewer threads have any)
-    uint32_t low = 0, high = order_of(mz) + 1;
-    const uint32_t key = tid < nv ? order_of(mt) : 0;
     if (min(nv, NT) >= K) {
+      float l = least[0];
+#pragma unroll
+      for (int w = 1; w < W; ++w) l = fminf(l, least[w]);
+      uint32_t low = order_of(l), high = order_of(mz) + 1;
+      const uint32_t key = tid < nv ? order_of(mt) : 0;
       for (int it = 0; it < 32 && high - low > 1; ++it) {
         const uint32_t mid = low + (high - low) / 2;
-        const int c = __syncthreads_count(tid < nv && key >= mid);
+        const int c = __syncthreads_count(key >= mid);
         if (c >= K) low = mid;
         else high = mid;
         if (c >= K && c <= K + K / 8 + 8) break;
       }
+      tau = low;
     }
-    p.tau = low;
-  }
-  float slope_t = 1.f;
-  if (tid == 0) {
-    p.has_t = mine_t ? 1.f : 0.f;
-    p.ut = mine_t ? capped<CAP>(a, zt, slope_t) : 0.f;
-    rec[rank] = p;
-    found = 0;
   }
   __syncthreads();
-  cluster_wait();
-  // word w of this block's part to every other block
-  for (int i = tid; i < parts * PART_WORDS; i += NT) {
-    const int to = i / PART_WORDS, w = i - to * PART_WORDS;
-    if (to != rank) put32(in_cluster(reinterpret_cast<uint32_t*>(&rec[rank]) + w, to), reinterpret_cast<const uint32_t*>(&rec[rank])[w]);
+  float slope_t = 1.f;
+  if (warp == 0) {
+    Part p = {};
+    p.m = um;
+    float v = lane < W ? sums[0][lane] : 0.f;
+    p.S = warp_sum(v);
+    if (OP != DISTILL) p.A = warp_sum(lane < W ? sums[1][lane] : 0.f);
+    if (HARD) p.S1 = warp_sum(lane < W ? sums[2][lane] : 0.f);
+    p.B = -INFINITY;
+    if (OP == DISTILL) named_part<CAP, HARD>(a, mine, p);
+    p.has_t = mine_t ? 1.f : 0.f;
+    p.ut = mine_t ? capped<CAP>(a, zt, slope_t) : 0.f;
+    if (TOP) p.S1 = mine_t ? fmaxf(mz, zt) : mz;
+    p.tau = tau;
+    if (lane == 0) own = p;
+    __syncwarp();
+    // to every block of the cluster, this one among them
+    if (lane < parts * PART_PIECES) {
+      const int to = lane / PART_PIECES, piece = lane - to * PART_PIECES;
+      send16(in_cluster(reinterpret_cast<const uint4*>(&rec[rank]) + piece, to), reinterpret_cast<const uint4*>(&own)[piece], in_cluster(&sent, to));
+    }
+    if (!sent_wait(&sent, 3)) sent_wait(&sent, 4);
+    total<OP, HARD>(a, row, parts, rec, qr, rank == 0, &fin);
   }
-  cluster_arrive();
-  cluster_wait();
-  if (tid < 32) total<OP, HARD>(a, row, parts, rec, qr, rank == 0, &fin);
+  if (OP == SCORES && !TOP) return;
   __syncthreads();
   const Totals T = fin;
 
   if (OP == SCORES) {
-    if (!TOP) return;
     // tokens from the bound on to one block
     u64* taken = reinterpret_cast<u64*>(buf + max(slice * static_cast<int>(sizeof(E)), room * parts * 8));
     const int keeper = row & (parts - 1);
     const uint32_t theirs = in_cluster(taken + rank * room, keeper);
     auto collect = [&](u64 bound, bool all) {
+      const uint32_t order = static_cast<uint32_t>(bound >> 32);
+      const float from = logit_of(order);
       auto give = [&](u64 key) {
         const int i = atomicAdd(&found, 1);
         if (i < room) put64(theirs + i * 8, key);
       };
       if (tid == 0 && mine_t && key_of(zt, static_cast<int>(t)) >= bound) give(key_of(zt, static_cast<int>(t)));
-      if (all || (tid < nv && order_of(mt) >= static_cast<uint32_t>(bound >> 32)))
+      if (all || (tid < nv && order_of(mt) >= order))
         for (int v = tid; v < nv; v += NT) {
+          const uint4 w = zv[v];
+          if (!all && Vec<E>::top(vec_max<E>(w)) < from) continue;
           float f[VE];
-          unpack(zv[v], f, E());
+          floats_of<E>(w, f);
 #pragma unroll
           for (int e = 0; e < VE; ++e) {
+            if (f[e] < from) continue;
             const int token = first_token + v * VE + e;
             if (token >= 0 && token < V && token != t && key_of(f[e], token) >= bound) give(key_of(f[e], token));
           }
@@ -603,7 +915,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 5 : 2) slice_kernel(Row a, int
       cluster_arrive();
       cluster_wait();
     };
-    collect(static_cast<u64>(T.tau) << 32, T.lS != T.lS);     // (a thread's largest leaves NaN out)
+    collect(static_cast<u64>(T.tau) << 32, T.tau == 0 || T.lS != T.lS);     // (a thread's largest leaves NaN out)
     bool over = false;
     for (int r = 0; r < parts; ++r) over |= count[0][r] > room;
     if (over) {
@@ -613,7 +925,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 5 : 2) slice_kernel(Row a, int
         int c = tid == 0 && mine_t && key_of(zt, static_cast<int>(t)) >= mid;
         for (int v = tid; v < nv; v += NT) {
           float f[VE];
-          unpack(zv[v], f, E());
+          floats_of<E>(zv[v], f);
 #pragma unroll
           for (int e = 0; e < VE; ++e) {
             const int token = first_token + v * VE + e;
@@ -638,10 +950,10 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 5 : 2) slice_kernel(Row a, int
     if (rank != keeper) return;
     // ranks among what was collected, fewer of them first where they are many
     u64* list = reinterpret_cast<u64*>(buf);
-    int total_found = 0;
-    for (int r = 0; r < parts; ++r) total_found += count[0][r];
-    uint32_t low = 0, high = 0xFFFFFFFFu;
-    int kept = total_found;
+    int kept = 0;
+    for (int r = 0; r < parts; ++r) kept += count[0][r];
+    uint32_t low = T.tau, high = order_of(T.top) + 1;
+    if (over || T.lS != T.lS) low = 0, high = 0xFFFFFFFFu;
     for (int it = 0; it < 32 && kept > K + K / 2 + 16 && high - low > 1; ++it) {
       const uint32_t mid = low + (high - low) / 2;
       int c = 0;
@@ -676,20 +988,39 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 5 : 2) slice_kernel(Row a, int
 
   if (!a.out) return;
   const float scale = OP == DISTILL ? a.scale : a.scale * a.inv_tau;
-  const bool whole = (reinterpret_cast<uintptr_t>(out) & 15) / sizeof(E) == lead;       // pieces of the gradient lie as the logits' do
+  // (entropy's gradient has p log p: a mask's logits are brought to a number where it is nothing, unless all of the row are such)
+  const bool careful = OP == POLICY && T.kb != 0.f && (CAP || !(T.M > Vec<E>::LOW * 0.9f) || a.inv_tau < 0.05f);
+  const f32x2 minus = pair(-T.base, -T.base), cc = pair(a.c, a.c), k0 = pair(T.k0, T.k0);
+  const float fa = OP == POLICY ? T.ka * scale : (1.f - a.ce) * a.tau * T.ka * scale, fb = T.kb * LN2 * scale;
+  const f32x2 ka = pair(fa, fa), kb = pair(fb, fb);
+  const f32x2 minus_m = pair(-T.M, -T.M), l2 = pair(LOG2E, LOG2E), h0 = pair(-T.h0, -T.h0), ce = pair(a.ce * scale, a.ce * scale);
+  const bool bonus = OP == POLICY && T.kb != 0.f;
+#pragma unroll 2
   for (int v = tid; v < nv; v += NT) {
-    float f[VE];
-    unpack(zv[v], f, E());
+    f32x2 x[P], slope[P];
+    pairs_of<E>(bonus && !careful ? vec_floor<E>(zv[v]) : zv[v], x);
+    if (CAP) cap_pairs<E, true>(a, x, slope);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      float slope;
-      const float u = capped<CAP>(a, f[e], slope);
-      f[e] = grad_rest<OP, HARD>(a, T, u) * slope * scale;
+    for (int i = 0; i < P; ++i) {
+      f32x2 r;
+      if (OP == POLICY && careful) {
+        float b, c;
+        split(x[i], b, c);
+        r = pair(grad_rest<OP, HARD>(a, T, b) * scale, grad_rest<OP, HARD>(a, T, c) * scale);
+      } else {
+        const f32x2 y = fma2(add2(x[i], minus), cc, k0), p = exp2_2(y);
+        r = mul2(p, bonus ? fma2(kb, y, ka) : ka);
+      }
+      if (HARD) r = fma2(exp2_2(fma2(add2(x[i], minus_m), l2, h0)), ce, r);
+      x[i] = CAP ? mul2(r, slope[i]) : r;
     }
+    const uint4 w = vec_of<E>(x);
     const int token = first_token + v * VE;
     if (whole && token >= 0 && token + VE <= V) {
-      *reinterpret_cast<uint4*>(out + token) = pack(f, E());
+      *reinterpret_cast<uint4*>(out + token) = w;
     } else {
+      float f[VE];
+      floats_of<E>(w, f);
 #pragma unroll
       for (int e = 0; e < VE; ++e)
         if (token + e >= 0 && token + e < V) out[token + e] = from_float<E>(f[e]);
@@ -697,17 +1028,11 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 5 : 2) slice_kernel(Row a, int
   }
   __syncthreads();
   if (OP == POLICY && mine_t && tid == 0) out[t] = from_float<E>(grad_taken(T, a.bonus) * slope_t * scale);
-  if (OP == DISTILL) {
-    if (here && mine.first) {
-      float slope;
-      const float u = capped<CAP>(a, zk, slope);
-      out[mine.id] = from_float<E>(grad_named<HARD>(a, T, u, q_of(id, q, K, mine.id), mine.id == t) * slope * scale);
-    }
-    if (HARD && mine_t && tid == 0) {
-      bool named = false;
-      for (int k = 0; k < K; ++k) named |= id[k] == t;
+  if (OP == DISTILL && warp == 0) {
+    write_named<E, CAP, HARD>(a, T, mine, id, q, t, scale, out);
+    if (HARD && mine_t && lane == 0 && !named_t) {
       const float u = capped<CAP>(a, zt, slope_t);
-      if (!named) out[t] = from_float<E>((grad_rest<OP, HARD>(a, T, u) - a.ce) * slope_t * scale);
+      out[t] = from_float<E>((grad_rest<OP, HARD>(a, T, u) - a.ce) * slope_t * scale);
     }
   }
 }
@@ -735,14 +1060,23 @@ __global__ void __launch_bounds__(LONG_NT) long_kernel(Row a) {
     row_off<OP>(a, row);
     return;
   }
-  float qr = 0.f, zk = 0.f;
-  Named mine = {-1, 0.f, -INFINITY, false};
+  float qr = 0.f;
+  bool named_t = false;
+  Named mine;
   if (OP == DISTILL) {
     for (int i = tid; i < (V + 31) / 32; i += NT) bits[i] = 0;
-    qr = teacher_of<NT>(a, row, id, q, sh, mine);
-    if (mine.id >= 0) {
-      zk = to_float(z[mine.id]);
-      atomicOr(&bits[mine.id >> 5], 1u << (mine.id & 31));
+    __syncthreads();
+    if (tid < 32) {
+      qr = teacher_of(a, row, t, id, q, mine, named_t);
+#pragma unroll
+      for (int j = 0; j < ENTRIES; ++j) {
+        const int i = mine.id[j];
+        if (i < 0) continue;
+        mine.here[j] = true;
+        mine.z[j] = to_float(z[i]);
+        const uint32_t bit = 1u << (i & 31);
+        mine.first[j] = !(atomicOr(&bits[i >> 5], bit) & bit);
+      }
     }
     __syncthreads();
   }
@@ -766,7 +1100,7 @@ __global__ void __launch_bounds__(LONG_NT) long_kernel(Row a) {
   if (OP != DISTILL) p.A = block_sum<NT>(A, sh);
   if (HARD) p.S1 = block_sum<NT>(S1, sh);
   p.B = -INFINITY;
-  if (OP == DISTILL) named_part<HARD, NT>(a, mine, mine.id >= 0, mine.id >= 0 ? capped<CAP>(a, zk) : -INFINITY, sh, p);
+  if (OP == DISTILL && tid < 32) named_part<CAP, HARD>(a, mine, p);
   float slope_t = 1.f, ut = 0.f;
   if (a.targets) ut = capped<CAP>(a, to_float(z[t]), slope_t);
   p.has_t = a.targets ? 1.f : 0.f;
@@ -812,11 +1146,7 @@ __global__ void __launch_bounds__(LONG_NT) long_kernel(Row a) {
     out[i] = from_float<E>(v * slope * scale);
   }
   if (OP == POLICY && tid == 0) out[t] = from_float<E>(grad_taken(T, a.bonus) * slope_t * scale);
-  if (OP == DISTILL && mine.first) {
-    float slope;
-    const float u = capped<CAP>(a, zk, slope);
-    out[mine.id] = from_float<E>(grad_named<HARD>(a, T, u, q_of(id, q, K, mine.id), mine.id == t) * slope * scale);
-  }
+  if (OP == DISTILL && tid < 32) write_named<E, CAP, HARD>(a, T, mine, id, q, t, scale, out);
 }
 
 // -------------------------------------------------------------------------------------------------------- launching
@@ -911,24 +1241,55 @@ int run_rows(Op op, const RowArgs* r) {
 
 // ---------------------------------------------------------------------------------------- gradient of the scores
 //   dz_j = (scale / tau) u'(z_j) [ -p_j (sum of the gradients of log p_t and of the alternatives + dH (log p_j + H)) + the gradients of j's own ]
-constexpr int NT = 512;
+//
+// One pass, nothing between the tokens of a row: blocks of 256 threads take 1,024 pieces of 16 bytes, four a thread that are all asked for
+// before the first is used.  The tokens with gradients of their own are written again behind the others of their block.
+constexpr int GRAD_NT = 256, GRAD_EACH = 4;
 template <typename E, bool CAP>
-__global__ void __launch_bounds__(NT) grad_kernel(Row a, const float* lse, const float* dlogprob, const float* dentropy, const float* dtop) {
-  __shared__ float sh[32];
+__global__ void __launch_bounds__(GRAD_NT) grad_kernel(Row a, const float* lse, const float* dlogprob, const float* dentropy, const float* dtop, int blocks) {
+  constexpr int VE = Vec<E>::N, P = VE / 2;
+  __shared__ float part[GRAD_NT / 32];
   __shared__ int id[MOST_TOP];
   __shared__ float gk[MOST_TOP];
-  const int row = blockIdx.x, tid = threadIdx.x, V = a.V, K = a.K;
+  const int row = blockIdx.x / blocks, tid = threadIdx.x, V = a.V, K = a.K;
   const E* z = static_cast<const E*>(a.z) + row * a.ldz;
   E* out = static_cast<E*>(a.out) + row * a.ldo;
-  const long t = a.targets ? a.targets[row] : 0;
-  const bool on = (!a.targets || (t != a.ignore && t >= 0 && t < V)) && (!a.mask || a.mask[row] > 0.f);
+  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(E)), nv = (lead + V + VE - 1) / VE;
+  const bool whole = (reinterpret_cast<uintptr_t>(out) & 15) / sizeof(E) == lead;
+  const int v0 = (blockIdx.x - row * blocks) * (GRAD_NT * GRAD_EACH), from = v0 * VE - lead, to = from + GRAD_NT * GRAD_EACH * VE;
+  const long t = a.targets ? a.targets[row] : -1;
+  const bool on = row_on(a, row, t);
+  uint4 w[GRAD_EACH];
+  if (on) {
+    const uint4* zv = reinterpret_cast<const uint4*>(z - lead);
+#pragma unroll
+    for (int i = 0; i < GRAD_EACH; ++i) {
+      const int v = v0 + i * GRAD_NT + tid;
+      if (v < nv) w[i] = zv[v];
+    }
+  }
+  auto store = [&](int i, const uint4& u) {
+    const int v = v0 + i * GRAD_NT + tid, token = v * VE - lead;
+    if (v >= nv) return;
+    if (whole && token >= 0 && token + VE <= V) {
+      *reinterpret_cast<uint4*>(out + token) = u;
+    } else {
+      float f[VE];
+      floats_of<E>(u, f);
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (token + e >= 0 && token + e < V) out[token + e] = from_float<E>(f[e]);
+    }
+  };
   if (!on) {
-    for (int i = tid; i < V; i += NT) out[i] = from_float<E>(0.f);
+#pragma unroll
+    for (int i = 0; i < GRAD_EACH; ++i) store(i, make_uint4(0, 0, 0, 0));
     return;
   }
-  // entry 0..K-1: the alternatives; entry K: the given token
+  // thread k < K: the alternatives; thread K: the given token
   int mine = -1;
   float g = 0.f;
+  const float gt = dlogprob ? dlogprob[row] : 0.f;
   if (tid < K) {
     const long k = a.top_ids[(size_t)row * K + tid];
     if (k >= 0 && k < V) {
@@ -938,40 +1299,71 @@ __global__ void __launch_bounds__(NT) grad_kernel(Row a, const float* lse, const
     id[tid] = mine;
     gk[tid] = g;
   }
-  const float gt = dlogprob ? dlogprob[row] : 0.f;
   if (tid == K && dlogprob) {
     mine = static_cast<int>(t);
     g = gt;
   }
-  const float sum = block_sum<NT>(g, sh);
-  float zm = 0.f;
-  bool first = mine >= 0;
-  if (first) {
-    zm = to_float(z[mine]);
-    for (int k = 0; k < (tid < K ? tid : K); ++k) first = first && id[k] != mine;
+  const bool here = mine >= from && mine < to && mine >= 0;
+  const float zm = here ? to_float(z[mine]) : 0.f;
+  if (K > 0) {
+    const float s = warp_sum(g);
+    if ((tid & 31) == 0) part[tid >> 5] = s;
   }
-  const float dh = dentropy ? dentropy[row] : 0.f, ka = -sum - (dentropy ? dh * a.entropy[row] : 0.f), l = lse[row];
-  const float scale = a.scale * a.inv_tau;
-  __syncthreads();
-  auto at = [&](float zi, float own) {
-    float slope;
-    const float y = fmaf(capped<CAP>(a, zi, slope), a.inv_tau, -l) * LOG2E, p = ex2(y);      // (one rounding of the difference)
-    return from_float<E>(((dentropy ? p * (ka - dh * LN2 * max_nan(y, -256.f)) : p * ka) + own) * slope * scale);
+  const bool some = __syncthreads_or(here);                   // (and what is read by index has been read)
+  float sum = gt;
+  if (K > 0) {
+    sum = part[0];
+#pragma unroll
+    for (int i = 1; i < GRAD_NT / 32; ++i) sum += part[i];
+  }
+  const float dh = dentropy ? dentropy[row] : 0.f, l = lse[row], scale = a.scale * a.inv_tau;
+  const float ka = -sum - (dentropy ? dh * a.entropy[row] : 0.f);
+  auto at = [&](float u, float slope, float own) {
+    const float y = fmaf(u, a.inv_tau, -l) * LOG2E, p = ex2(y);               // (one rounding of the difference)
+    return ((dentropy ? p * (ka - dh * LN2 * max_nan(y, -256.f)) : p * ka) + own) * slope * scale;
   };
-  for (int i = tid; i < V; i += NT) out[i] = at(to_float(z[i]), 0.f);
+  const bool careful = dentropy && (CAP || !(l > Vec<E>::LOW * 0.9f * a.inv_tau) || a.inv_tau < 0.05f);
+  const f32x2 it = pair(a.inv_tau, a.inv_tau), ml = pair(-l, -l), l2 = pair(LOG2E, LOG2E), fa = pair(ka * scale, ka * scale);
+  const f32x2 fb = pair(-dh * LN2 * scale, -dh * LN2 * scale);
+#pragma unroll
+  for (int i = 0; i < GRAD_EACH; ++i) {
+    if (v0 + i * GRAD_NT + tid >= nv) break;
+    f32x2 x[P], slope[P];
+    pairs_of<E>(dentropy && !careful ? vec_floor<E>(w[i]) : w[i], x);
+    if (CAP) cap_pairs<E, true>(a, x, slope);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      f32x2 r;
+      if (careful) {
+        float b, c;
+        split(x[j], b, c);
+        r = pair(at(b, 1.f, 0.f), at(c, 1.f, 0.f));
+      } else {
+        const f32x2 y = mul2(fma2(x[j], it, ml), l2);
+        r = mul2(exp2_2(y), dentropy ? fma2(fb, y, fa) : fa);
+      }
+      x[j] = CAP ? mul2(r, slope[j]) : r;
+    }
+    store(i, vec_of<E>(x));
+  }
+  if (!some) return;
   __syncthreads();
-  if (first) {
-    float own = 0.f;
+  if (here) {                                                 // (of a token twice both write the same)
+    float own = 0.f, slope;
     for (int k = 0; k < K; ++k) own += id[k] == mine ? gk[k] : 0.f;
     if (dlogprob && mine == t) own += gt;
-    out[mine] = at(zm, own);
+    const float u = capped<CAP>(a, zm, slope);
+    out[mine] = from_float<E>(at(u, slope, own));
   }
 }
 
 template <typename E>
 int launch_grad(const Row& a, const GradArgs* r) {
+  constexpr int each = GRAD_NT * GRAD_EACH * Vec<E>::N;
+  const int blocks = (a.V + Vec<E>::N - 1 + each - 1) / each;
+  if (static_cast<long>(a.T) * blocks > 0x7FFFFFFFl) return -3;
   auto kernel = a.cap > 0.f ? grad_kernel<E, true> : grad_kernel<E, false>;
-  kernel<<<a.T, NT, 0, r->stream>>>(a, r->lse, r->dlogprob, r->dentropy, r->dtop);
+  kernel<<<a.T * blocks, GRAD_NT, 0, r->stream>>>(a, r->lse, r->dlogprob, r->dentropy, r->dtop, blocks);
   return cudaGetLastError() == cudaSuccess ? 0 : -400;
 }
 

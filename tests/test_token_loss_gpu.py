@@ -6,7 +6,7 @@ import torch
 
 from flextrain_b200 import ops
 from test_token_loss_cpu import CHANGES, refusals, teacher_changes
-from token_loss_oracle import check_distill, check_not_finite, check_policy, check_scores, check_scores_grad, some_targets, wide
+from token_loss_oracle import check_distill, check_not_finite, check_policy, check_scores, check_scores_grad, some_targets, value_error, wide
 
 pytestmark = pytest.mark.gpu
 
@@ -134,16 +134,20 @@ def test_rows_beyond_31_bits():
     near = wide(2, 4099, BF16, "cuda")[1]
     t = torch.tensor([5, 4098], device="cuda")
     a, b = ops.token_logprobs(z, t, top_k=7), ops.token_logprobs(near, t, top_k=7)
-    assert all(torch.equal(x, y) for x, y in zip(a, b))
-    assert torch.equal(ops.policy_loss(z, t).loss, ops.policy_loss(near, t).loss)
+    # the second rows begin at different places in a piece of 16 bytes, so their tokens are summed in other groups: sums of the same
+    # positive terms, each within value_error of the exact one, differ by twice that; gradients by that and by a rounding on either side
+    tol = 2 * value_error(4099)
+    same = lambda x, y, half=0.0: bool(((x.double() - y.double()).abs() <= (tol + 2.02 * half) * (y.double().abs() + (half == 0))).all())
+    assert all(same(a[i], b[i]) for i in (0, 1, 2, 4)) and torch.equal(a.top_ids, b.top_ids)
+    assert same(ops.policy_loss(z, t).loss, ops.policy_loss(near, t).loss)
     out = torch.empty_like(near)
     ops.token_logprobs_bwd_(near, t, b, dlogprobs=torch.ones(2, device="cuda"), out=out)
     ops.token_logprobs_bwd_(z, t, b, dlogprobs=torch.ones(2, device="cuda"))
-    assert torch.equal(z, out)
+    assert torch.equal(z, out)                                # (nothing is summed)
     z.copy_(near)
     ops.policy_loss_(near, t, out=out)
     ops.policy_loss_(z, t)
-    assert torch.equal(z, out)
+    assert same(z, out, 2.0 ** -8)
 
 
 def test_many_rows_and_a_stream_of_ones_own():
