@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -171,23 +172,29 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
   return v;
 }
 
+// What a policy row is given besides its logits, asked for long before it is used.
+struct Given {
+  float adv, old, ref;
+};
+__device__ __forceinline__ Given given_of(const Row& a, int row) {
+  return {a.adv ? a.adv[row] : 1.f, a.old ? a.old[row] : 0.f, a.ref ? a.ref[row] : 0.f};
+}
 // Loss of a policy-gradient row and its derivative by log p of the taken token.  The unclipped side counts where both are equal, so
 // a ratio inside the borders, and on them, has a gradient.
-__device__ __forceinline__ float policy_row(const Row& a, int row, float lp, float H, float& g) {
-  const float adv = a.adv ? a.adv[row] : 1.f;
-  float L = -adv * lp;
-  g = -adv;
+__device__ __forceinline__ float policy_row(const Row& a, const Given& v, float lp, float H, float& g) {
+  float L = -v.adv * lp;
+  g = -v.adv;
   if (a.old) {
-    const float r = expf(lp - a.old[row]);
-    const float free = r * adv, held = fminf(fmaxf(r, 1.f - a.clip_low), 1.f + a.clip_high) * adv;
+    const float r = expf(lp - v.old);
+    const float free = r * v.adv, held = fminf(fmaxf(r, 1.f - a.clip_low), 1.f + a.clip_high) * v.adv;
     L = -fminf(free, held);
     g = free <= held ? -free : 0.f;
-    if (r != r || adv != adv) L = g = r * adv;             // (minima and maxima leave NaN out)
+    if (r != r || v.adv != v.adv) L = g = r * v.adv;         // (minima and maxima leave NaN out)
   }
   if (a.ref && a.kl != 0.f) {
-    const float d = a.ref[row] - lp;
-    L += a.kl * (expm1f(d) - d);
-    g -= a.kl * expm1f(d);
+    const float d = v.ref - lp, e = expm1f(d);
+    L += a.kl * (e - d);
+    g -= a.kl * e;
   }
   return a.bonus != 0.f ? L - a.bonus * H : L;
 }
@@ -197,87 +204,96 @@ __device__ __forceinline__ float policy_row(const Row& a, int row, float lp, flo
 // policy rows, the teacher's of distillation are, and are added by themselves), S and A sums of e and of e log2 e relative to it, S1 of
 // e at a temperature of one.
 struct __align__(16) Part {
-  float m, S, A, S1;                      // (S1 of scores: the largest logit itself, the given token's among them)
+  float m, S, A, S1;
   float B, En, En1, kl, Q;                // distillation: the named tokens of this part relative to their largest u, B
   float ut, has_t;                        // the given token's u, in the part that holds it
-  uint32_t tau;                           // scores: at least K tokens of the part are not below it
+  uint32_t low;                           // scores: as many tokens of the part as is its share of K are not below it
 };
 // what follows from all parts
 struct Totals {
   float M, lS, lp, H, miss, g;            // largest u, log2 of the sum, log p_t, entropy, 1 - p_t, dL/dlog p_t
   float base, k0, ka, kb;                 // gradient of a token that is not named: 2^((u - base) c + k0) (ka + kb log p) ...
   float share, h0;                        // ... + ce 2^((u - M) log2 e - h0); distillation: the sum of q
-  uint32_t tau;
-  float top;                              // scores: the largest logit
+  uint32_t low;                           // scores: at least K tokens are not below it
 };
+constexpr int MOST_PARTS = 8;               // blocks of a cluster
+typedef unsigned long long u64;
 constexpr int PART_PIECES = sizeof(Part) / 16;
 
-template <typename F>
-__device__ __forceinline__ float over8(float v, F f) {        // over the eight lanes that hold the parts
-#pragma unroll
-  for (int o = 4; o; o >>= 1) v = f(v, __shfl_xor_sync(~0u, v, o));
-  return v;
-}
-__device__ __forceinline__ float sum8(float v) { return over8(v, [](float a, float b) { return a + b; }); }
-__device__ __forceinline__ float max8(float v) { return over8(v, [](float a, float b) { return fmaxf(a, b); }); }
-
-// By one warp: lane r of each eight holds part r (those from ``parts`` on hold none), so that all four eights go the same ways.  ``first``: of the row's blocks this one writes its results.
+__device__ __forceinline__ Part no_part() { return {-INFINITY, 0.f, 0.f, 0.f, -INFINITY, 0.f, 0.f, 0.f, 0.f, -INFINITY, 0.f, 0xFFFFFFFFu}; }
+// By one warp, every lane the same over all parts (those that there are not: no_part).  ``first``: of the row's blocks this one writes
+// its results.
 template <Op OP, bool HARD>
-__device__ __forceinline__ void total(const Row& a, int row, int parts, const Part* rec, float qr, bool first, Totals* fin) {
-  const int lane = threadIdx.x & 31;
-  Part p = {-INFINITY, 0.f, 0.f, OP == SCORES ? -INFINITY : 0.f, -INFINITY, 0.f, 0.f, 0.f, 0.f, -INFINITY, 0.f, 0u};
-  if ((lane & 7) < parts) p = rec[lane & 7];
+__device__ __forceinline__ void total(const Row& a, int row, const Part* rec, float qr, const Given& given, bool first, Totals* fin) {
+  const bool writes = first && (threadIdx.x & 31) == 0;
   Totals t = {};
-  const float rest = max8(p.m);                               // of the tokens that are not named
-  const bool none = p.m == -INFINITY;
+  float rest = -INFINITY, ut = -INFINITY, B = -INFINITY;      // largest of the tokens that are not named, the given token's, of the named
+  bool has = false;
+#pragma unroll
+  for (int r = 0; r < MOST_PARTS; ++r) {
+    rest = fmaxf(rest, rec[r].m);
+    if (rec[r].has_t > 0.f) has = true, ut = rec[r].ut;
+    if (OP == DISTILL) B = fmaxf(B, rec[r].B);
+  }
   if (OP != DISTILL) {
-    const float has = max8(p.has_t);
-    const float given = sum8(p.has_t > 0.f ? p.ut : 0.f), ut = has > 0.f ? given : -INFINITY;
     t.M = fmaxf(rest, ut);
-    const float down = none ? 0.f : ex2((p.m - t.M) * a.c);
-    const float O = sum8(down * p.S);
-    float A = sum8(none ? 0.f : down * (p.A + p.S * ((p.m - t.M) * a.c)));
-    const float yt = (ut - t.M) * a.c, et = has > 0.f ? ex2(yt) : 0.f, S = O + et;
-    if (has > 0.f) A += et * max_nan(yt, -256.f);
+    float O = 0.f, A = 0.f;
+#pragma unroll
+    for (int r = 0; r < MOST_PARTS; ++r) {
+        const float d = (rec[r].m - t.M) * a.c;
+      const bool none = rec[r].m == -INFINITY;
+      const float down = none ? 0.f : ex2(d);
+      O += down * rec[r].S;
+      A += none ? 0.f : down * (rec[r].A + rec[r].S * d);
+      if (OP == SCORES) t.low = r == 0 ? rec[r].low : min(t.low, rec[r].low);
+    }
+    const float yt = (ut - t.M) * a.c, et = has ? ex2(yt) : 0.f, S = O + et;
+    if (has) A += et * max_nan(yt, -256.f);
     t.lS = S > 0.f ? log2f(S) : NAN;                          // no finite logit (or a NaN): all that follows is NaN
     // a token that has most of the row: the others' sum by itself, so that a small log p keeps its digits
-    const bool most = has > 0.f && ut >= rest && S > 0.f;
-    t.lp = most ? -log1pf(O) : (yt - t.lS) * LN2;
-    t.H = (most ? log1pf(O) : t.lS * LN2) - A / S * LN2;
+    const bool most = has && ut >= rest && S > 0.f;
+    const float ln_S = most ? log1pf(O) : t.lS * LN2;
+    t.lp = most ? -ln_S : (yt - t.lS) * LN2;
+    t.H = ln_S - A / S * LN2;
     t.miss = O / S;
     t.base = t.M;
     t.k0 = -t.lS;
     if (OP == SCORES) {
-      uint32_t tau = p.tau;
-#pragma unroll
-      for (int o = 4; o; o >>= 1) tau = max(tau, __shfl_xor_sync(~0u, tau, o));
-      t.tau = tau;
-      t.top = max8(p.S1);
-      if (first && lane == 0) {
+      if (writes) {
         if (a.logprob) a.logprob[row] = t.lp;
         a.entropy[row] = t.H;
-        a.lse[row] = t.M * a.inv_tau + (most ? log1pf(O) : t.lS * LN2);
+        a.lse[row] = t.M * a.inv_tau + ln_S;
       }
     } else {
-      const float L = policy_row(a, row, t.lp, t.H, t.g);
+      const float L = policy_row(a, given, t.lp, t.H, t.g);
       t.ka = a.bonus * t.H - t.g;
       t.kb = a.bonus;
-      if (first && lane == 0) {
+      if (writes) {
         a.loss[row] = L;
         a.logprob[row] = t.lp;
         a.entropy[row] = t.H;
       }
     }
   } else {
-    t.M = fmaxf(rest, max8(p.B));
+    t.M = fmaxf(rest, B);
     const float base = rest == -INFINITY ? 0.f : rest;
-    const bool no_names = p.B == -INFINITY;
-    const float others = sum8(none ? 0.f : p.S * ex2((p.m - base) * a.c));
-    const float S = others * (rest == -INFINITY ? 0.f : ex2((base - t.M) * a.c)) + sum8(no_names ? 0.f : p.En * ex2((p.B - t.M) * a.c));
+    float others = 0.f, named = 0.f, S1 = 0.f, Q = 0.f, kl = 0.f;
+#pragma unroll
+    for (int r = 0; r < MOST_PARTS; ++r) {
+        const Part& p = rec[r];
+      const bool none = p.m == -INFINITY, no_names = p.B == -INFINITY;
+      others += none ? 0.f : p.S * ex2((p.m - base) * a.c);
+      if (HARD) S1 += none ? 0.f : p.S1 * ex2((p.m - t.M) * LOG2E);
+      named += no_names ? 0.f : p.En * ex2((p.B - t.M) * a.c);
+      if (HARD) S1 += no_names ? 0.f : p.En1 * ex2((p.B - t.M) * LOG2E);
+      kl += no_names || p.Q == 0.f ? 0.f : p.Q * (t.M - p.B) * a.inv_tau;
+      kl += p.kl;
+      Q += p.Q;
+    }
+    const float S = others * (rest == -INFINITY ? 0.f : ex2((base - t.M) * a.c)) + named;
     t.lS = S > 0.f ? log2f(S) : NAN;
-    const float Q = sum8(p.Q);
     // q (log q - log p), where log p = (u - M) / tau - ln S and a part has (u - B) / tau
-    float kl = sum8(p.kl + (p.Q != 0.f && !no_names ? p.Q * (t.M - p.B) * a.inv_tau : 0.f)) + (Q != 0.f ? Q * t.lS * LN2 : 0.f);
+    if (Q != 0.f) kl += Q * t.lS * LN2;
     t.base = base;
     t.k0 = (base - t.M) * a.c - t.lS;
     t.share = a.bucket ? Q + qr : (Q != 0.f ? 1.f : 0.f);
@@ -298,14 +314,12 @@ __device__ __forceinline__ void total(const Row& a, int row, int parts, const Pa
     }
     float L = (1.f - a.ce) * a.tau * a.tau * kl;
     if (HARD) {
-      const float S1 = sum8(none ? 0.f : p.S1 * ex2((p.m - t.M) * LOG2E)) + sum8(no_names ? 0.f : p.En1 * ex2((p.B - t.M) * LOG2E));
-      const float ut = sum8(p.has_t > 0.f ? p.ut : 0.f);
       t.h0 = S1 > 0.f ? log2f(S1) : NAN;
       L -= a.ce * ((ut - t.M) * LOG2E - t.h0) * LN2;
     }
-    if (first && lane == 0) a.loss[row] = L;
+    if (writes) a.loss[row] = L;
   }
-  if (lane == 0) *fin = t;
+  if ((threadIdx.x & 31) == 0) *fin = t;
 }
 
 // gradients, before the slope of the cap and the scale
@@ -364,8 +378,15 @@ __device__ __forceinline__ float warp_max(float v) {
 // Returns what the teacher leaves to all others (0 without the bucket); ``id`` and ``q`` are of MOST_TOP, ``named_t``: t is among them.
 __device__ __forceinline__ float teacher_of(const Row& a, int row, long t, int* id, float* q, Named& n, bool& named_t) {
   const int lane = threadIdx.x & 31;
-  float top = -INFINITY, sum = 0.f;
+  float top = -INFINITY, sum = 0.f, said[ENTRIES];
   bool has_t = false;
+  long named[ENTRIES];
+#pragma unroll
+  for (int j = 0; j < ENTRIES; ++j) {                         // (all asked for before the first is looked at)
+    const bool in = lane + 32 * j < a.K;
+    named[j] = in ? a.ids[(size_t)row * a.K + lane + 32 * j] : -1;
+    said[j] = in ? a.teacher[(size_t)row * a.K + lane + 32 * j] : 0.f;
+  }
 #pragma unroll
   for (int j = 0; j < ENTRIES; ++j) {
     const int k = lane + 32 * j;
@@ -373,15 +394,13 @@ __device__ __forceinline__ float teacher_of(const Row& a, int row, long t, int* 
     n.log_q[j] = -INFINITY;
     n.here[j] = n.first[j] = false;
     n.z[j] = 0.f;
-    if (k < a.K) {
-      const long i = a.ids[(size_t)row * a.K + k];
-      if (i >= 0 && i < a.V) {
-        n.id[j] = static_cast<int>(i);
-        n.log_q[j] = a.teacher[(size_t)row * a.K + k];
-        has_t |= i == t;
-      }
-      id[k] = n.id[j];
+    const long i = named[j];
+    if (i >= 0 && i < a.V) {
+      n.id[j] = static_cast<int>(i);
+      n.log_q[j] = said[j];
+      has_t |= i == t;
     }
+    if (k < a.K) id[k] = n.id[j];
     top = fmaxf(top, n.log_q[j]);
   }
   named_t = __any_sync(~0u, has_t);
@@ -463,8 +482,6 @@ __device__ __forceinline__ void write_named(const Row& a, const Totals& t, const
 // whole numbers that are in the order of the floats); tokens from the highest of the blocks' bounds on go to one block, which ranks
 // them.  Where they are too many (thousands of equal logits) the cluster halves the interval of (logit, index) of all tokens until
 // exactly K are left.
-constexpr int MOST_PARTS = 8;
-typedef unsigned long long u64;
 
 __device__ __forceinline__ uint32_t in_cluster(const void* p, int rank) {          // the same place in another block's shared memory
   uint32_t r;
@@ -488,21 +505,46 @@ __device__ __forceinline__ void cluster_arrive_relaxed() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// what other blocks sent; bounded as ftb::mbar_wait
-__device__ __forceinline__ bool sent_wait(uint64_t* bar, int where) {
-  for (uint32_t it = 0; it < FTB_WAIT_LIMIT; ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{\n.reg .pred p;\n"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n"
-        "selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(ftb::smem_u32(bar))
-        : "memory");
-    if (ok) return true;
+// what other blocks sent; bounded as ftb::mbar_wait, and once more as long after it was reported
+__device__ __forceinline__ bool sent_wait(uint64_t* bar, uint32_t parity, int where) {
+  for (int again = 0; again < 2; ++again) {
+    for (uint32_t it = 0; it < FTB_WAIT_LIMIT; ++it) {
+      uint32_t ok;
+      asm volatile(
+          "{\n.reg .pred p;\n"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+          "selp.u32 %0, 1, 0, p;\n}\n"
+          : "=r"(ok)
+          : "r"(ftb::smem_u32(bar)), "r"(parity)
+          : "memory");
+      if (ok) return true;
+    }
+    ftb::set_error(1, where);
   }
-  ftb::set_error(1, where);
   return false;
+}
+// A cluster that has not begun is taken over by this one, or none is: the answer's 16 bytes are counted on a barrier.  first: the index
+// of its first block, -1 where there was none (after which there is none any more).
+__device__ __forceinline__ void take_over(void* answer, uint64_t* bar) {
+  ftb::fence_proxy_async();
+  ftb::mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(ftb::smem_u32(answer)),
+               "r"(ftb::smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ int taken_over(const void* answer) {
+  uint32_t got, first;
+  asm volatile(
+      "{\n.reg .b128 h;\n.reg .pred p;\n"
+      "ld.shared.b128 h, [%2];\n"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "mov.u32 %1, 0;\n"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n}\n"
+      : "=r"(got), "=r"(first)
+      : "r"(ftb::smem_u32(answer))
+      : "memory");
+  return got ? static_cast<int>(first) : -1;
 }
 
 // two floats to an instruction
@@ -668,16 +710,26 @@ __device__ __forceinline__ float logit_of(uint32_t order) {
   return order == NAN_ORDER ? NAN : __uint_as_float(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);
 }
 
-template <typename E, Op OP, bool TOP, bool CAP, bool HARD, int NT>
-__global__ void __launch_bounds__(NT, NT == 256 ? 5 : 2) slice_kernel(Row a, int slice, int room) {
-  constexpr int VE = Vec<E>::N, P = VE / 2, W = NT / 32;
+// NW threads work on the tokens; one warp more begins copies, takes the named tokens out and exchanges the parts, so that what it does
+// for a row lies beside the others' passes.  A cluster that is done with a row takes over the row of one that has not begun (``more``:
+// there are some), since beginning blocks costs as long as their work on a row: its first block asks for it while the others are at
+// work and tells them; a copy begins as soon as the last row's tokens are no longer read.
+template <int NW>
+__host__ __device__ constexpr int slice_blocks() { return NW == 128 ? 6 : NW == 256 ? 3 : 1; }      // of an SM
+template <typename E, Op OP, bool TOP, bool CAP, bool HARD, int NW>
+__global__ void __launch_bounds__(NW + 32, slice_blocks<NW>()) slice_kernel(Row a, int slice, int room, int more) {
+  constexpr int VE = Vec<E>::N, P = VE / 2, W = NW / 32, NT = NW + 32;
   extern __shared__ __align__(128) unsigned char buf[];
-  __shared__ __align__(8) uint64_t bar, sent;
+  const bool early = OP == SCORES ? !TOP : a.out == nullptr;  // nothing reads a row's tokens after its sums
+  __shared__ __align__(8) uint64_t bar, sent[2], told[2], answered;
+  __shared__ __align__(16) int4 next[2];                      // a row to come (-1: none), whether it counts, its given token
+  __shared__ __align__(16) int4 answer;
   __shared__ int gave_up, found;
   __shared__ float sh[32], most[W], least[W], sums[3][W];
-  __shared__ Part rec[MOST_PARTS], own;
+  __shared__ Part rec[2][MOST_PARTS], own;
   __shared__ Totals fin;
   __shared__ int count[2][MOST_PARTS];
+  __shared__ uint32_t bounds[MOST_PARTS];
   __shared__ int id[OP == DISTILL ? MOST_TOP : 1];
   __shared__ float q[OP == DISTILL ? MOST_TOP : 1];
   E* zs = reinterpret_cast<E*>(buf);
@@ -686,355 +738,508 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 5 : 2) slice_kernel(Row a, int
   int rank, parts;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
-  const int row = blockIdx.x / parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V, K = a.K;
-  const E* z = static_cast<const E*>(a.z) + row * a.ldz;
-  E* out = static_cast<E*>(a.out) + row * a.ldo;
-  // the row from the 16-byte piece that it begins in: ``lead`` elements before it, this block's from ``lo`` on, n of them in pieces
-  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(E));
-  const int lo = rank * slice, n = max(0, min(lead + V - lo, slice)), nv = (n + VE - 1) / VE, first_token = lo - lead;
-  const bool whole = OP != SCORES && (reinterpret_cast<uintptr_t>(out) & 15) / sizeof(E) == lead;       // the gradient's pieces lie as the logits' do
-  const long t = a.targets ? a.targets[row] : -1;
-  if (!row_on(a, row, t)) {
-    if (OP != SCORES && a.out)
-      for (int v = tid; v < nv; v += NT) {
-        const int token = first_token + v * VE;
-        if (whole && token >= 0 && token + VE <= V) {
-          *reinterpret_cast<uint4*>(out + token) = make_uint4(0, 0, 0, 0);
-        } else {
-          for (int e = 0; e < VE; ++e)
-            if (token + e >= 0 && token + e < V) out[token + e] = from_float<E>(0.f);
-        }
-      }
-    if (rank == 0) row_off<OP>(a, row);
-    return;
-  }
-  if (tid == 0) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V, K = a.K;
+  const bool works = warp < W, takes = more && rank == 0;
+  if (tid == NW) {
     gave_up = found = 0;
     ftb::mbar_init(&bar, 1);
-    ftb::mbar_init(&sent, 1);
-    ftb::fence_barrier_init();
-    ftb::mbar_expect_tx(&sent, parts * sizeof(Part));
-    if (nv > 0) {
-      ftb::mbar_expect_tx(&bar, nv * 16);
-      ftb::bulk_load_g2s(buf, z - lead + lo, nv * 16, &bar);
+    ftb::mbar_init(&answered, 1);
+    for (int i = 0; i < 2; ++i) {
+      ftb::mbar_init(&sent[i], 1);
+      ftb::mbar_init(&told[i], 1);
     }
+    ftb::fence_barrier_init();
   }
   cluster_arrive_relaxed();                                   // (the others may be sent to once all have begun)
-  float qr = 0.f;
-  bool named_t = false;
-  Named mine;
-  if (OP == DISTILL && warp == 0) qr = teacher_of(a, row, t, id, q, mine, named_t);
+  if (tid < 2 * MOST_PARTS && tid % MOST_PARTS >= parts) rec[tid / MOST_PARTS][tid % MOST_PARTS] = no_part();
+  int row = blockIdx.x / parts, answers = 0, loads = 0;
+  long t = a.targets ? a.targets[row] : -1;
+  bool on = row_on(a, row, t);
+  // the row from the 16-byte piece that it begins in: ``lead`` elements before it, this block's from ``lo`` on, in pieces
+  auto lead_of = [&](int r) { return static_cast<int>((reinterpret_cast<uintptr_t>(static_cast<const E*>(a.z) + r * a.ldz) & 15) / sizeof(E)); };
+  auto count_of = [&](int lead) { return max(0, min(lead + V - rank * slice, slice)); };
+  auto load = [&](int r) {                                    // by one thread
+    const int lead = lead_of(r), nv = (count_of(lead) + VE - 1) / VE;
+    if (nv > 0) {
+      ftb::fence_proxy_async();
+      ftb::mbar_expect_tx(&bar, nv * 16);
+      ftb::bulk_load_g2s(buf, static_cast<const E*>(a.z) + r * a.ldz - lead + rank * slice, nv * 16, &bar);
+    }
+  };
+  if (tid == NW && on) load(row);
   __syncthreads();
   cluster_wait();
-  if (nv > 0 && !ftb::mbar_wait(&bar, 0, &gave_up, 1)) {      // (reported; the copy gets as long again before the block goes on)
-    int again = 0;
-    ftb::mbar_wait(&bar, 0, &again, 2);
-  }
+  // Where nothing waits for a row's totals its last part is left for the next row's passes (by the warp that exchanges).
+  int last = -1, last_it = 0;
+  float last_qr = 0.f;
+  Given last_given = {};
+  auto finish = [&] {
+    if (last < 0) return;
+    sent_wait(&sent[last_it & 1], (last_it >> 1) & 1, 3);
+    total<OP, HARD>(a, last, rec[last_it & 1], last_qr, last_given, rank == 0, &fin);
+    last = -1;
+  };
 
-  // what lies around the row is no token; named tokens by themselves
-  const int at_t = static_cast<int>(t) - first_token;         // where the given token lies
-  const bool mine_t = a.targets && at_t >= 0 && at_t < n;
-  float zt = 0.f;
-  if (warp == 0) {
-    if (lane < VE) {
-      if (lo + lane < lead && lane < nv * VE) zs[lane] = from_float<E>(-INFINITY);
-      if (n + lane < nv * VE) zs[n + lane] = from_float<E>(-INFINITY);
+  for (int it = 0; row >= 0; ++it) {
+    const E* z = static_cast<const E*>(a.z) + row * a.ldz;
+    E* out = static_cast<E*>(a.out) + row * a.ldo;
+    const int lo = rank * slice, lead = lead_of(row), n = count_of(lead), nv = (n + VE - 1) / VE, first_token = lo - lead;
+    const bool whole = OP != SCORES && (reinterpret_cast<uintptr_t>(out) & 15) / sizeof(E) == lead;       // the gradient's pieces lie as the logits' do
+    const int now = it & 1, then = now ^ 1;
+    const uint32_t told_parity = (it >> 1) & 1;
+    if (tid == NW) {
+      ftb::mbar_expect_tx(&sent[now], parts * sizeof(Part));
+      if (more) ftb::mbar_expect_tx(&told[then], 16);
     }
-    if (mine_t) zt = to_float(zs[at_t]);
-    __syncwarp();
-    if (OP != DISTILL && mine_t && lane == 0) zs[at_t] = from_float<E>(-INFINITY);
-    if (OP == DISTILL) {
-      typedef typename std::conditional<sizeof(E) == 2, uint16_t, uint32_t>::type Bits;
-      Bits* tag = reinterpret_cast<Bits*>(buf);
-#pragma unroll
-      for (int j = 0; j < ENTRIES; ++j) {
-        mine.here[j] = mine.id[j] >= first_token && mine.id[j] < first_token + n && mine.id[j] >= 0;
-        if (mine.here[j]) mine.z[j] = to_float(zs[mine.id[j] - first_token]);
+    // The next row: asked for when this row's tokens are here (by then all blocks that find room have begun), told to the cluster.
+    auto ask = [&] {
+      if (takes && tid == NW) take_over(&answer, &answered);
+    };
+    auto tell = [&] {
+      if (!takes || works) return;
+      int4 v = make_int4(-1, 0, 0, 0);
+      if (lane == 0) {
+        const int first = sent_wait(&answered, answers & 1, 5) ? taken_over(&answer) : -1;
+        if (first >= 0) {
+          v.x = first / parts;
+          const long given = a.targets ? a.targets[v.x] : -1;
+          v.y = row_on(a, v.x, given);
+          v.z = static_cast<int>(given);                      // (a token where the row counts)
+        }
       }
+      ++answers;
+      v = make_int4(__shfl_sync(~0u, v.x, 0), __shfl_sync(~0u, v.y, 0), __shfl_sync(~0u, v.z, 0), 0);
+      if (lane < parts)
+        send16(in_cluster(&next[then], lane), make_uint4(v.x, v.y, v.z, 0), in_cluster(&told[then], lane));
+    };
+    auto load_next = [&] {                                    // by the warp
+      if (!more) return;
+      if (sent_wait(&told[then], told_parity, 6) && lane == 0 && next[then].x >= 0 && next[then].y) load(next[then].x);
+    };
+    auto send_part = [&](const Part& p) {                     // to every block of the cluster, this one among them
+      if (lane == 0) own = p;
       __syncwarp();
-#pragma unroll
-      for (int j = 0; j < ENTRIES; ++j)                       // of entries of one token, the one whose number stays in its place
-        if (mine.here[j]) tag[mine.id[j] - first_token] = static_cast<Bits>(lane + 32 * j);
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < ENTRIES; ++j) mine.first[j] = mine.here[j] && tag[mine.id[j] - first_token] == static_cast<Bits>(lane + 32 * j);
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < ENTRIES; ++j)
-        if (mine.here[j]) zs[mine.id[j] - first_token] = from_float<E>(-INFINITY);
-    }
-  }
-  __syncthreads();
-
-  // largest of each thread, of the block
-  uint32_t m2 = Vec<E>::NONE;
-#pragma unroll 4
-  for (int v = tid; v < nv; v += NT) m2 = Vec<E>::max2(m2, vec_max<E>(zv[v]));
-  const float mt = Vec<E>::top(m2);
-  {
-    const float w = warp_max(mt);
-    if (lane == 0) most[warp] = w;
-    if (TOP) {
-      float l = tid < nv ? mt : INFINITY;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) l = fminf(l, __shfl_xor_sync(~0u, l, o));
-      if (lane == 0) least[warp] = l;
-    }
-  }
-  __syncthreads();
-  float mz = most[0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) mz = fmaxf(mz, most[w]);
-  const float um = mz == -INFINITY ? mz : capped<CAP>(a, mz), base = mz == -INFINITY ? 0.f : um;
-
-  // sums relative to it
-  {
-    f32x2 S = 0, S1 = 0;
-    float A = 0.f;
-    const f32x2 minus = pair(-base, -base), cc = pair(a.c, a.c), l2 = pair(LOG2E, LOG2E);
-#pragma unroll 2
-    for (int v = tid; v < nv; v += NT) {
-      const uint4 w = zv[v];
-      f32x2 x[P], slope[P], part = 0;
-      pairs_of<E>(w, x);
-      if (CAP) cap_pairs<E, false>(a, x, slope);
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const f32x2 d = add2(x[i], minus), y = mul2(d, cc), e = exp2_2(y);
-        S = add2(S, e);
-        if (OP != DISTILL) part = fma2(e, y, part);
-        if (HARD) S1 = add2(S1, exp2_2(mul2(d, l2)));
+      if (lane < parts * PART_PIECES) {
+        const int to = lane / PART_PIECES, piece = lane - to * PART_PIECES;
+        send16(in_cluster(reinterpret_cast<const uint4*>(&rec[now][rank]) + piece, to), reinterpret_cast<const uint4*>(&own)[piece],
+               in_cluster(&sent[now], to));
       }
-      if (OP != DISTILL) {
-        float b, c;
-        split(part, b, c);
-        b += c;
-        if (b != b) {                                         // (a logit of -inf: nothing times minus infinity)
-          float f[VE];
-          floats_of<E>(w, f);
-          b = 0.f;
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const float y = (capped<CAP>(a, f[e]) - base) * a.c;
-            b += ex2(y) * max_nan(y, -256.f);
+    };
+    auto step = [&] {                                         // by all
+      const bool known = more && sent_wait(&told[then], told_parity, 6);
+      row = known ? next[then].x : -1;
+      on = known && next[then].y;
+      t = on && a.targets ? next[then].z : -1;
+    };
+    if (!on) {
+      // (nothing is exchanged, but no block may be two rows ahead of another, nor of a thread of its own that has not read where to go)
+      __syncthreads();
+      ask();
+      if (works && OP != SCORES && a.out)
+        for (int v = tid; v < nv; v += NW) {
+          const int token = first_token + v * VE;
+          if (whole && token >= 0 && token + VE <= V) {
+            *reinterpret_cast<uint4*>(out + token) = make_uint4(0, 0, 0, 0);
+          } else {
+            for (int e = 0; e < VE; ++e)
+              if (token + e >= 0 && token + e < V) out[token + e] = from_float<E>(0.f);
           }
         }
-        A += b;
+      if (rank == 0) row_off<OP>(a, row);
+      if (!works) {
+        finish();
+        tell();
+        send_part(Part{});
+        load_next();
+        sent_wait(&sent[now], (it >> 1) & 1, 3);
+      }
+      step();
+      continue;
+    }
+    const long given = t;
+    float qr = 0.f;
+    bool named_t = false;
+    Named mine;
+    Given policy = {};
+    if (OP == POLICY && !works) policy = given_of(a, row);
+    if (OP == DISTILL && !works) qr = teacher_of(a, row, t, id, q, mine, named_t);
+    if (nv > 0) {
+      if (!ftb::mbar_wait(&bar, loads & 1, &gave_up, 1)) {    // (reported; the copy gets as long again before the block goes on)
+        int again = 0;
+        ftb::mbar_wait(&bar, loads & 1, &again, 2);
+      }
+      ++loads;
+    }
+
+    // what lies around the row is no token; named tokens by themselves
+    const int at_t = static_cast<int>(t) - first_token;         // where the given token lies
+    const bool mine_t = a.targets && at_t >= 0 && at_t < n;
+    float zt = 0.f;
+    if (!works) {
+      if (lane < VE) {
+        if (lo + lane < lead && lane < nv * VE) zs[lane] = from_float<E>(-INFINITY);
+        if (n + lane < nv * VE) zs[n + lane] = from_float<E>(-INFINITY);
+      }
+      if (mine_t) zt = to_float(zs[at_t]);
+      __syncwarp();
+      if (OP != DISTILL && mine_t && lane == 0) zs[at_t] = from_float<E>(-INFINITY);
+      if (OP == DISTILL) {
+        typedef typename std::conditional<sizeof(E) == 2, uint16_t, uint32_t>::type Bits;
+        Bits* tag = reinterpret_cast<Bits*>(buf);
+#pragma unroll
+        for (int j = 0; j < ENTRIES; ++j) {
+          mine.here[j] = mine.id[j] >= first_token && mine.id[j] < first_token + n && mine.id[j] >= 0;
+          if (mine.here[j]) mine.z[j] = to_float(zs[mine.id[j] - first_token]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < ENTRIES; ++j)                       // of entries of one token, the one whose number stays in its place
+          if (mine.here[j]) tag[mine.id[j] - first_token] = static_cast<Bits>(lane + 32 * j);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < ENTRIES; ++j) mine.first[j] = mine.here[j] && tag[mine.id[j] - first_token] == static_cast<Bits>(lane + 32 * j);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < ENTRIES; ++j)
+          if (mine.here[j]) zs[mine.id[j] - first_token] = from_float<E>(-INFINITY);
+      }
+      ftb::fence_proxy_async();                                 // (the next copy comes after these)
+      ask();
+    }
+    __syncthreads();
+
+    // largest of each thread, of the block
+    float mt = -INFINITY;
+    Part p = {};
+    p.B = -INFINITY;
+    if (works) {
+      uint32_t m2 = Vec<E>::NONE;
+#pragma unroll 4
+      for (int v = tid; v < nv; v += NW) m2 = Vec<E>::max2(m2, vec_max<E>(zv[v]));
+      mt = Vec<E>::top(m2);
+      const float w = warp_max(mt);
+      if (lane == 0) most[warp] = w;
+      if (TOP) {
+        float l = tid < nv ? mt : INFINITY;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l = fminf(l, __shfl_xor_sync(~0u, l, o));
+        if (lane == 0) least[warp] = l;
+      }
+    } else if (OP == DISTILL) {
+      named_part<CAP, HARD>(a, mine, p);
+    }
+    __syncthreads();
+    if (!works) finish();                                     // (before the cluster is told: all have read what they were told last)
+    tell();
+    float mz = most[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) mz = fmaxf(mz, most[w]);
+    const float um = mz == -INFINITY ? mz : capped<CAP>(a, mz), base = mz == -INFINITY ? 0.f : um;
+
+    // sums relative to it.  16-bit logits: the exponent's argument by one fused operation, relative to the rounded product of base and c; what
+    // the rounding is goes into the sums at the end.  (Bases whose product leaves no digits: as fp32 logits.)
+    float off = 0.f, off1 = 0.f;                                // base c and base log2 e less what the sums are relative to
+    if (works) {
+      f32x2 S = 0, S1 = 0;
+      float A = 0.f;
+      const float kb = base * a.c, kb1 = base * LOG2E;
+      const bool fused = sizeof(E) == 2 && fabsf(kb) < 0x1p24f && fabsf(kb1) < 0x1p24f;
+      const f32x2 minus = pair(-base, -base), cc = pair(a.c, a.c), l2 = pair(LOG2E, LOG2E), mk = pair(-kb, -kb), mk1 = pair(-kb1, -kb1);
+      auto pass = [&](auto f) {
+        constexpr bool FUSED = decltype(f)::value;
+#pragma unroll 2
+        for (int v = tid; v < nv; v += NW) {
+          const uint4 w = zv[v];
+          f32x2 x[P], slope[P], part = 0;
+          pairs_of<E>(w, x);
+          if (CAP) cap_pairs<E, false>(a, x, slope);
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            f32x2 y, y1;
+            if (FUSED) {
+              y = fma2(x[i], cc, mk);
+              if (HARD) y1 = fma2(x[i], l2, mk1);
+            } else {
+              const f32x2 d = add2(x[i], minus);
+              y = mul2(d, cc);
+              if (HARD) y1 = mul2(d, l2);
+            }
+            const f32x2 e = exp2_2(y);
+            S = add2(S, e);
+            if (OP != DISTILL) part = fma2(e, y, part);
+            if (HARD) S1 = add2(S1, exp2_2(y1));
+          }
+          if (OP != DISTILL) {
+            float b, c;
+            split(part, b, c);
+            b += c;
+            if (b != b) {                                       // (a logit of -inf: nothing times minus infinity)
+              float g[VE];
+              floats_of<E>(w, g);
+              b = 0.f;
+#pragma unroll
+              for (int e = 0; e < VE; ++e) {
+                const float u = capped<CAP>(a, g[e]), y = FUSED ? fmaf(u, a.c, -kb) : (u - base) * a.c;
+                b += ex2(y) * max_nan(y, -256.f);
+              }
+            }
+            A += b;
+          }
+        }
+      };
+      if (fused) {
+        pass(std::true_type());
+        off = fmaf(base, a.c, -kb);
+        off1 = fmaf(base, LOG2E, -kb1);
+      } else {
+        pass(std::false_type());
+      }
+      auto back = [](float o) { return fabsf(o) < 1e-4f ? fmaf(-o, LN2, 1.f) : ex2(-o); };      // 2^-off
+      float b, c;
+      split(S, b, c);
+      b += c;
+      const float down = back(off);
+      const float s = warp_sum(b * down);
+      if (lane == 0) sums[0][warp] = s;
+      if (OP != DISTILL) {
+        A = warp_sum(down * (A - off * b));
+        if (lane == 0) sums[1][warp] = A;
+      }
+      if (HARD) {
+        split(S1, b, c);
+        b = warp_sum((b + c) * back(off1));
+        if (lane == 0) sums[2][warp] = b;
       }
     }
-    float b, c;
-    split(S, b, c);
-    b = warp_sum(b + c);
-    if (lane == 0) sums[0][warp] = b;
-    if (OP != DISTILL) {
-      A = warp_sum(A);
-      if (lane == 0) sums[1][warp] = A;
-    }
-    if (HARD) {
-      split(S1, b, c);
-      b = warp_sum(b + c);
-      if (lane == 0) sums[2][warp] = b;
-    }
-  }
-  uint32_t tau = 0;
-  if (TOP) {
-    // the largest of some K to K + K / 8 + 8 threads are not below tau (all tokens where fewer threads have any)
-    if (min(nv, NT) >= K) {
+    // the largest of at least ``want`` threads are not below it, and of not many more
+    auto bound_of = [&](int want) {
       float l = least[0];
 #pragma unroll
       for (int w = 1; w < W; ++w) l = fminf(l, least[w]);
       uint32_t low = order_of(l), high = order_of(mz) + 1;
-      const uint32_t key = tid < nv ? order_of(mt) : 0;
+      const uint32_t key = works && tid < nv ? order_of(mt) : 0;
       for (int it = 0; it < 32 && high - low > 1; ++it) {
         const uint32_t mid = low + (high - low) / 2;
         const int c = __syncthreads_count(key >= mid);
-        if (c >= K) low = mid;
+        if (c >= want) low = mid;
         else high = mid;
-        if (c >= K && c <= K + K / 8 + 8) break;
+        if (c >= want && c <= want + want / 4 + 4) break;
       }
-      tau = low;
-    }
-  }
-  __syncthreads();
-  float slope_t = 1.f;
-  if (warp == 0) {
-    Part p = {};
-    p.m = um;
-    float v = lane < W ? sums[0][lane] : 0.f;
-    p.S = warp_sum(v);
-    if (OP != DISTILL) p.A = warp_sum(lane < W ? sums[1][lane] : 0.f);
-    if (HARD) p.S1 = warp_sum(lane < W ? sums[2][lane] : 0.f);
-    p.B = -INFINITY;
-    if (OP == DISTILL) named_part<CAP, HARD>(a, mine, p);
-    p.has_t = mine_t ? 1.f : 0.f;
-    p.ut = mine_t ? capped<CAP>(a, zt, slope_t) : 0.f;
-    if (TOP) p.S1 = mine_t ? fmaxf(mz, zt) : mz;
-    p.tau = tau;
-    if (lane == 0) own = p;
-    __syncwarp();
-    // to every block of the cluster, this one among them
-    if (lane < parts * PART_PIECES) {
-      const int to = lane / PART_PIECES, piece = lane - to * PART_PIECES;
-      send16(in_cluster(reinterpret_cast<const uint4*>(&rec[rank]) + piece, to), reinterpret_cast<const uint4*>(&own)[piece], in_cluster(&sent, to));
-    }
-    if (!sent_wait(&sent, 3)) sent_wait(&sent, 4);
-    total<OP, HARD>(a, row, parts, rec, qr, rank == 0, &fin);
-  }
-  if (OP == SCORES && !TOP) return;
-  __syncthreads();
-  const Totals T = fin;
-
-  if (OP == SCORES) {
-    // tokens from the bound on to one block
-    u64* taken = reinterpret_cast<u64*>(buf + max(slice * static_cast<int>(sizeof(E)), room * parts * 8));
-    const int keeper = row & (parts - 1);
-    const uint32_t theirs = in_cluster(taken + rank * room, keeper);
-    auto collect = [&](u64 bound, bool all) {
-      const uint32_t order = static_cast<uint32_t>(bound >> 32);
-      const float from = logit_of(order);
-      auto give = [&](u64 key) {
-        const int i = atomicAdd(&found, 1);
-        if (i < room) put64(theirs + i * 8, key);
-      };
-      if (tid == 0 && mine_t && key_of(zt, static_cast<int>(t)) >= bound) give(key_of(zt, static_cast<int>(t)));
-      if (all || (tid < nv && order_of(mt) >= order))
-        for (int v = tid; v < nv; v += NT) {
-          const uint4 w = zv[v];
-          if (!all && Vec<E>::top(vec_max<E>(w)) < from) continue;
-          float f[VE];
-          floats_of<E>(w, f);
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            if (f[e] < from) continue;
-            const int token = first_token + v * VE + e;
-            if (token >= 0 && token < V && token != t && key_of(f[e], token) >= bound) give(key_of(f[e], token));
-          }
-        }
-      __syncthreads();
-      if (tid < parts) put32(in_cluster(&count[0][rank], tid), found);
-      cluster_arrive();
-      cluster_wait();
+      return low;
     };
-    collect(static_cast<u64>(T.tau) << 32, T.tau == 0 || T.lS != T.lS);     // (a thread's largest leaves NaN out)
-    bool over = false;
-    for (int r = 0; r < parts; ++r) over |= count[0][r] > room;
-    if (over) {
-      u64 low = 0, high = ~0ull;                              // at least K keys are not below low, fewer not below high
-      for (int it = 0; high - low > 1; ++it) {
-        const u64 mid = low + (high - low) / 2;
-        int c = tid == 0 && mine_t && key_of(zt, static_cast<int>(t)) >= mid;
-        for (int v = tid; v < nv; v += NT) {
-          float f[VE];
-          floats_of<E>(zv[v], f);
+    uint32_t low = 0;
+    if (TOP) {
+      const int filled = (lead + V + slice - 1) / slice, share = (K + filled - 1) / filled;      // (blocks without tokens have no share)
+      if (nv == 0) low = 0xFFFFFFFFu;
+      else if (min(nv, NW) >= share) low = bound_of(share);
+    }
+    __syncthreads();
+    float slope_t = 1.f;
+    if (!works) {
+      p.m = um;
 #pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const int token = first_token + v * VE + e;
-            c += token >= 0 && token < V && token != t && key_of(f[e], token) >= mid;
+      for (int w = 0; w < W; ++w) {
+        p.S += sums[0][w];
+        if (OP != DISTILL) p.A += sums[1][w];
+        if (HARD) p.S1 += sums[2][w];
+      }
+      p.has_t = mine_t ? 1.f : 0.f;
+      p.ut = mine_t ? capped<CAP>(a, zt, slope_t) : 0.f;
+      p.low = low;
+      send_part(p);
+      last = row, last_it = it, last_qr = qr, last_given = policy;
+      if (early) load_next();
+      else finish();
+    }
+    if (early) {
+      step();
+      continue;
+    }
+    __syncthreads();
+    const Totals T = fin;
+
+    if (OP == SCORES) {
+      // tokens from the bound on to every block, which then ranks its own among them
+      u64* taken = reinterpret_cast<u64*>(buf + slice * static_cast<int>(sizeof(E)));
+      const bool broken = T.lS != T.lS;                         // (a thread's largest leaves NaN out)
+      u64* ours = taken + rank * room;
+      // A warp takes the threads with such tokens one by one, half a piece a lane.
+      auto collect = [&](u64 bound, bool all) {
+        typedef typename std::conditional<sizeof(E) == 2, uint2, float2>::type Half;
+        const uint32_t order = static_cast<uint32_t>(bound >> 32);
+        auto give = [&](float f, int token) {
+          const u64 key = key_of(f, token);
+          if (key < bound) return;
+          const int i = atomicAdd(&found, 1);
+          if (i < room) ours[i] = key;
+        };
+        if (tid == NW && mine_t) give(zt, static_cast<int>(t));
+        uint32_t those = __ballot_sync(~0u, works && tid < nv && (all || order_of(mt) >= order));
+        while (those) {
+          const int first = (warp << 5) + __ffs(those) - 1;
+          those &= those - 1;
+          for (int h = lane; h < 2 * ((nv - first + NW - 1) / NW); h += 32) {
+            const int at = (first + (h >> 1) * NW) * VE + (h & 1) * (VE / 2);
+            const Half w = *reinterpret_cast<const Half*>(zs + at);
+            float f[VE / 2];
+            if constexpr (sizeof(E) == 4) {
+              f[0] = w.x, f[1] = w.y;
+            } else {
+              split(Vec<E>::one(w.x), f[0], f[1]);
+              split(Vec<E>::one(w.y), f[2], f[3]);
+            }
+#pragma unroll
+            for (int e = 0; e < VE / 2; ++e) {
+              const int token = first_token + at + e;
+              if (order_of(f[e]) >= order && token >= 0 && token < V && token != t) give(f[e], token);
+            }
           }
         }
-        c = static_cast<int>(block_sum<NT>(static_cast<float>(c), sh));           // (whole numbers below 2^24)
-        if (tid < parts) put32(in_cluster(&count[1 - (it & 1)][rank], tid), c);
+        __syncthreads();
+        const int have = min(found, room);
+        for (int i = tid; i < have * parts; i += NT) {
+          const int to = i % parts, c = i / parts;
+          if (to != rank) put64(in_cluster(ours + c, to), ours[c]);
+        }
+        if (tid < parts) put32(in_cluster(&count[0][rank], tid), found);
         cluster_arrive();
         cluster_wait();
-        int sum = 0;
-        for (int r = 0; r < parts; ++r) sum += count[1 - (it & 1)][r];
-        if (sum >= K) low = mid;
-        else high = mid;
-        if (sum == K) break;
+        bool over = false;
+        for (int r = 0; r < parts; ++r) over |= count[0][r] > room;
+        return over;
+      };
+      u64 bound = static_cast<u64>(T.low) << 32;
+      bool over = collect(bound, T.low == 0 || broken);
+      if (over) {
+        // the blocks' tokens differ: the highest of bounds that K threads of a block each are not below
+        const uint32_t mine_low = min(nv, NW) >= K ? bound_of(K) : 0;
+        if (tid < parts) put32(in_cluster(&bounds[rank], tid), mine_low);
+        if (tid == 0) found = 0;
+        cluster_arrive();                                       // (all have read the last counts)
+        cluster_wait();
+        uint32_t highest = T.low;
+        for (int r = 0; r < parts; ++r) highest = max(highest, bounds[r]);
+        bound = static_cast<u64>(highest) << 32;
+        over = collect(bound, highest == 0 || broken);
+      }
+      if (over) {
+        u64 below = 0, above = ~0ull;                           // at least K keys are not below the one, fewer not below the other
+        for (int it = 0; above - below > 1; ++it) {
+          const u64 mid = below + (above - below) / 2;
+          int c = tid == NW && mine_t && key_of(zt, static_cast<int>(t)) >= mid;
+          if (works)
+            for (int v = tid; v < nv; v += NW) {
+              float f[VE];
+              floats_of<E>(zv[v], f);
+#pragma unroll
+              for (int e = 0; e < VE; ++e) {
+                const int token = first_token + v * VE + e;
+                c += token >= 0 && token < V && token != t && key_of(f[e], token) >= mid;
+              }
+            }
+          c = static_cast<int>(block_sum<NT>(static_cast<float>(c), sh));           // (whole numbers below 2^24)
+          if (tid < parts) put32(in_cluster(&count[1 - (it & 1)][rank], tid), c);
+          cluster_arrive();
+          cluster_wait();
+          int sum = 0;
+          for (int r = 0; r < parts; ++r) sum += count[1 - (it & 1)][r];
+          if (sum >= K) below = mid;
+          else above = mid;
+          if (sum == K) break;
+        }
+        if (tid == 0) found = 0;
+        cluster_arrive();                                       // (all have read the last counts)
+        cluster_wait();
+        bound = below;
+        collect(bound, true);
+      }
+      if (!works) load_next();                                // (the row was read when the counts were exchanged)
+      // eight threads to a token, one for each block's
+      for (int i = tid / MOST_PARTS; i < (count[0][rank] + NT / MOST_PARTS - 1) / (NT / MOST_PARTS) * (NT / MOST_PARTS); i += NT / MOST_PARTS) {
+        const int r = tid % MOST_PARTS, others = r < parts ? count[0][r] : 0;
+        const bool valid = i < count[0][rank];
+        const u64 key = valid ? taken[rank * room + i] : ~0ull;
+        int above = 0;
+#pragma unroll 4
+        for (int j = 0; j < others; ++j) above += taken[r * room + j] > key;
+#pragma unroll
+        for (int o = MOST_PARTS / 2; o; o >>= 1) above += __shfl_xor_sync(~0u, above, o);
+        if (valid && r == 0 && above < K) {
+          const int token = static_cast<int>(~static_cast<uint32_t>(key));
+          a.top_ids[(size_t)row * K + above] = token;
+          a.top_logprob[(size_t)row * K + above] =
+              token == t ? T.lp : ((capped<CAP>(a, logit_of(static_cast<uint32_t>(key >> 32))) - T.M) * a.c - T.lS) * LN2;
+        }
       }
       if (tid == 0) found = 0;
-      cluster_arrive();                                       // (all have read the last counts)
-      cluster_wait();
-      collect(low, true);
+      step();
+      continue;
     }
-    if (rank != keeper) return;
-    // ranks among what was collected, fewer of them first where they are many
-    u64* list = reinterpret_cast<u64*>(buf);
-    int kept = 0;
-    for (int r = 0; r < parts; ++r) kept += count[0][r];
-    uint32_t low = T.tau, high = order_of(T.top) + 1;
-    if (over || T.lS != T.lS) low = 0, high = 0xFFFFFFFFu;
-    for (int it = 0; it < 32 && kept > K + K / 2 + 16 && high - low > 1; ++it) {
-      const uint32_t mid = low + (high - low) / 2;
-      int c = 0;
-      for (int r = 0; r < parts; ++r)
-        for (int i = tid; i < count[0][r]; i += NT) c += static_cast<uint32_t>(taken[r * room + i] >> 32) >= mid;
-      c = static_cast<int>(block_sum<NT>(static_cast<float>(c), sh));
-      if (c >= K) low = mid, kept = c;
-      else high = mid;
-    }
-    __syncthreads();
-    if (tid == 0) found = 0;
-    __syncthreads();
-    for (int r = 0; r < parts; ++r)
-      for (int i = tid; i < count[0][r]; i += NT) {
-        const u64 key = taken[r * room + i];
-        if (static_cast<uint32_t>(key >> 32) >= low) list[atomicAdd(&found, 1)] = key;
-      }
-    __syncthreads();
-    for (int i = tid; i < kept; i += NT) {
-      const u64 key = list[i];
-      int above = 0;
-      for (int j = 0; j < kept; ++j) above += list[j] > key;
-      if (above < K) {
-        const int token = static_cast<int>(~static_cast<uint32_t>(key));
-        a.top_ids[(size_t)row * K + above] = token;
-        a.top_logprob[(size_t)row * K + above] =
-            token == t ? T.lp : ((capped<CAP>(a, logit_of(static_cast<uint32_t>(key >> 32))) - T.M) * a.c - T.lS) * LN2;
-      }
-    }
-    return;
-  }
 
-  if (!a.out) return;
-  const float scale = OP == DISTILL ? a.scale : a.scale * a.inv_tau;
-  // (entropy's gradient has p log p: a mask's logits are brought to a number where it is nothing, unless all of the row are such)
-  const bool careful = OP == POLICY && T.kb != 0.f && (CAP || !(T.M > Vec<E>::LOW * 0.9f) || a.inv_tau < 0.05f);
-  const f32x2 minus = pair(-T.base, -T.base), cc = pair(a.c, a.c), k0 = pair(T.k0, T.k0);
-  const float fa = OP == POLICY ? T.ka * scale : (1.f - a.ce) * a.tau * T.ka * scale, fb = T.kb * LN2 * scale;
-  const f32x2 ka = pair(fa, fa), kb = pair(fb, fb);
-  const f32x2 minus_m = pair(-T.M, -T.M), l2 = pair(LOG2E, LOG2E), h0 = pair(-T.h0, -T.h0), ce = pair(a.ce * scale, a.ce * scale);
-  const bool bonus = OP == POLICY && T.kb != 0.f;
+    const float scale = OP == DISTILL ? a.scale : a.scale * a.inv_tau;
+    if (works) {
+      const bool bonus = OP == POLICY && T.kb != 0.f;
+      // One by one: entropy's gradient where a cap leaves -inf (elsewhere it is brought to a number that has no p log p, unless all of the row
+      // are such), and logits so large that their differences have to be formed first.
+      const bool careful = (bonus && (CAP || !(T.M > Vec<E>::LOW * 0.9f) || a.inv_tau < 0.05f)) ||
+                           (sizeof(E) == 2 && !(fabsf(T.base) * fmaxf(a.c, LOG2E) < 4096.f && fabsf(T.M) * LOG2E < 4096.f));
+      const f32x2 minus = pair(-T.base, -T.base), cc = pair(a.c, a.c), k0 = pair(T.k0, T.k0);
+      const float fa = OP == POLICY ? T.ka * scale : (1.f - a.ce) * a.tau * T.ka * scale, fb = T.kb * LN2 * scale;
+      const float f0 = fmaf(-T.base, a.c, T.k0), f1 = fmaf(-T.M, LOG2E, -T.h0);
+      const f32x2 ka = pair(fa, fa), kb = pair(fb, fb), kc = pair(f0, f0), kh = pair(f1, f1);
+      const f32x2 minus_m = pair(-T.M, -T.M), l2 = pair(LOG2E, LOG2E), h0 = pair(-T.h0, -T.h0), ce = pair(a.ce * scale, a.ce * scale);
+      auto pass = [&](auto with_bonus, auto with_care) {
+        constexpr bool BONUS = decltype(with_bonus)::value, CARE = decltype(with_care)::value;
 #pragma unroll 2
-  for (int v = tid; v < nv; v += NT) {
-    f32x2 x[P], slope[P];
-    pairs_of<E>(bonus && !careful ? vec_floor<E>(zv[v]) : zv[v], x);
-    if (CAP) cap_pairs<E, true>(a, x, slope);
+        for (int v = tid; v < nv; v += NW) {
+          f32x2 x[P], slope[P];
+          pairs_of<E>(BONUS && !CARE ? vec_floor<E>(zv[v]) : zv[v], x);
+          if (CAP) cap_pairs<E, true>(a, x, slope);
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      f32x2 r;
-      if (OP == POLICY && careful) {
-        float b, c;
-        split(x[i], b, c);
-        r = pair(grad_rest<OP, HARD>(a, T, b) * scale, grad_rest<OP, HARD>(a, T, c) * scale);
-      } else {
-        const f32x2 y = fma2(add2(x[i], minus), cc, k0), p = exp2_2(y);
-        r = mul2(p, bonus ? fma2(kb, y, ka) : ka);
+          for (int i = 0; i < P; ++i) {
+            f32x2 r;
+            if (CARE) {
+              float b, c;
+              split(x[i], b, c);
+              r = pair(grad_rest<OP, HARD>(a, T, b) * scale, grad_rest<OP, HARD>(a, T, c) * scale);
+            } else {
+              const f32x2 y = sizeof(E) == 2 ? fma2(x[i], cc, kc) : fma2(add2(x[i], minus), cc, k0);
+              r = mul2(exp2_2(y), BONUS ? fma2(kb, y, ka) : ka);
+              if (HARD) r = fma2(exp2_2(sizeof(E) == 2 ? fma2(x[i], l2, kh) : fma2(add2(x[i], minus_m), l2, h0)), ce, r);
+            }
+            x[i] = CAP ? mul2(r, slope[i]) : r;
+          }
+          const uint4 w = vec_of<E>(x);
+          const int token = first_token + v * VE;
+          if (whole && token >= 0 && token + VE <= V) {
+            *reinterpret_cast<uint4*>(out + token) = w;
+          } else {
+            float f[VE];
+            floats_of<E>(w, f);
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+              if (token + e >= 0 && token + e < V) out[token + e] = from_float<E>(f[e]);
+          }
+        }
+      };
+      if (careful) pass(std::false_type(), std::true_type());
+      else if (OP == POLICY && !CAP && bonus) pass(std::true_type(), std::false_type());
+      else pass(std::false_type(), std::false_type());
+    }
+    __syncthreads();
+    step();
+    if (works) continue;
+    load_next();
+    if (OP == POLICY && mine_t && lane == 0) out[given] = from_float<E>(grad_taken(T, a.bonus) * slope_t * scale);
+    if (OP == DISTILL) {
+      write_named<E, CAP, HARD>(a, T, mine, id, q, given, scale, out);
+      if (HARD && mine_t && lane == 0 && !named_t) {
+        const float u = capped<CAP>(a, zt, slope_t);
+        out[given] = from_float<E>((grad_rest<OP, HARD>(a, T, u) - a.ce) * slope_t * scale);
       }
-      if (HARD) r = fma2(exp2_2(fma2(add2(x[i], minus_m), l2, h0)), ce, r);
-      x[i] = CAP ? mul2(r, slope[i]) : r;
-    }
-    const uint4 w = vec_of<E>(x);
-    const int token = first_token + v * VE;
-    if (whole && token >= 0 && token + VE <= V) {
-      *reinterpret_cast<uint4*>(out + token) = w;
-    } else {
-      float f[VE];
-      floats_of<E>(w, f);
-#pragma unroll
-      for (int e = 0; e < VE; ++e)
-        if (token + e >= 0 && token + e < V) out[token + e] = from_float<E>(f[e]);
     }
   }
-  __syncthreads();
-  if (OP == POLICY && mine_t && tid == 0) out[t] = from_float<E>(grad_taken(T, a.bonus) * slope_t * scale);
-  if (OP == DISTILL && warp == 0) {
-    write_named<E, CAP, HARD>(a, T, mine, id, q, t, scale, out);
-    if (HARD && mine_t && lane == 0 && !named_t) {
-      const float u = capped<CAP>(a, zt, slope_t);
-      out[t] = from_float<E>((grad_rest<OP, HARD>(a, T, u) - a.ce) * slope_t * scale);
-    }
-  }
+  if (!works) finish();
 }
 
 // ---------------------------------------------------------------------------------- rows that shared memory does not hold
@@ -1047,7 +1252,7 @@ __global__ void __launch_bounds__(LONG_NT) long_kernel(Row a) {
   __shared__ u64 best[32];
   __shared__ int id[MOST_TOP];
   __shared__ float q[MOST_TOP];
-  __shared__ Part rec;
+  __shared__ Part rec[MOST_PARTS];
   __shared__ Totals fin;
   extern __shared__ uint32_t bits[];                          // DISTILL: which tokens the teacher names
   const int row = blockIdx.x, tid = threadIdx.x, V = a.V, K = a.K;
@@ -1105,9 +1310,10 @@ __global__ void __launch_bounds__(LONG_NT) long_kernel(Row a) {
   if (a.targets) ut = capped<CAP>(a, to_float(z[t]), slope_t);
   p.has_t = a.targets ? 1.f : 0.f;
   p.ut = ut;
-  if (tid == 0) rec = p;
+  p.low = 0;
+  if (tid < MOST_PARTS) rec[tid] = tid == 0 ? p : no_part();
   __syncthreads();                                            // the logits that are read by index have been read
-  if (tid < 32) total<OP, HARD>(a, row, 1, &rec, qr, true, &fin);
+  if (tid < 32) total<OP, HARD>(a, row, rec, qr, given_of(a, row), true, &fin);
   __syncthreads();
   const Totals T = fin;
   if (OP == SCORES) {
@@ -1165,14 +1371,14 @@ bool allow(K kernel, std::atomic<unsigned long long>& done) {
   return true;
 }
 
-template <typename E, Op OP, bool TOP, bool CAP, bool HARD, int NT>
+template <typename E, Op OP, bool TOP, bool CAP, bool HARD, int NW>
 int launch_slices(const Row& a, int parts, int slice, int room, int smem, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
-  auto kernel = slice_kernel<E, OP, TOP, CAP, HARD, NT>;
+  auto kernel = slice_kernel<E, OP, TOP, CAP, HARD, NW>;
   if (!allow(kernel, done)) return -400;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(a.T) * parts);
-  config.blockDim = dim3(NT);
+  config.blockDim = dim3(NW + 32);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute cluster;
@@ -1181,7 +1387,10 @@ int launch_slices(const Row& a, int parts, int slice, int room, int smem, cudaSt
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.attrs = &cluster;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, a, slice, room) == cudaSuccess ? 0 : -400;
+  // (blocks that an SM holds by their shared memory; where all begin at once there is nothing to take over)
+  const int most = 148 * std::max(1, std::min(slice_blocks<NW>(), (227 * 1024) / (smem + 4096)));
+  const int more = static_cast<long>(a.T) * parts > most;
+  return cudaLaunchKernelEx(&config, kernel, a, slice, room, more) == cudaSuccess ? 0 : -400;
 }
 
 template <typename E, Op OP, bool TOP, bool CAP, bool HARD>
@@ -1190,14 +1399,15 @@ int launch_rows(const Row& a, cudaStream_t stream) {
   const long bytes = static_cast<long>(a.V + VE - 1) * sizeof(E);
   int parts = 1;
   while (parts < MOST_PARTS && (bytes > static_cast<long>(SLICE) * parts || (static_cast<long>(a.T) * parts < 2 * 148 && bytes > 4096l * parts))) parts *= 2;
-  const long slice = ((a.V + VE - 1 + parts - 1) / parts + VE - 1) / VE * VE;
+  const long slice = ((a.V + VE - 1 + parts - 1) / parts + VE - 1) / VE * VE, size = slice * static_cast<long>(sizeof(E));
   // (where fewer threads than K have tokens, there are fewer than 1,024 of them and there is room for all)
-  const int room = TOP ? (a.V < 1024 ? a.V : 64 + 5 * a.K / 2) : 0;
-  const long listed = static_cast<long>(room) * parts * 8, smem = (slice * static_cast<long>(sizeof(E)) > listed ? slice * static_cast<long>(sizeof(E)) : listed) + listed;
+  const int room = TOP ? (a.V < 1024 ? a.V : 32 + 3 * a.K / 2) : 0;
+  const long listed = static_cast<long>(room) * parts * 8, smem = size + listed;
   if (smem <= MOST_SMEM && static_cast<long>(a.T) * parts <= 0x7FFFFFFFl) {
-    const int s = static_cast<int>(slice);
-    return smem > 2 * SLICE ? launch_slices<E, OP, TOP, CAP, HARD, 512>(a, parts, s, room, static_cast<int>(smem), stream)
-                            : launch_slices<E, OP, TOP, CAP, HARD, 256>(a, parts, s, room, static_cast<int>(smem), stream);
+    const int s = static_cast<int>(slice), m = static_cast<int>(smem);
+    if (size <= 48 * 1024) return launch_slices<E, OP, TOP, CAP, HARD, 128>(a, parts, s, room, m, stream);
+    if (size <= 96 * 1024) return launch_slices<E, OP, TOP, CAP, HARD, 256>(a, parts, s, room, m, stream);
+    return launch_slices<E, OP, TOP, CAP, HARD, 512>(a, parts, s, room, m, stream);
   }
   static std::atomic<unsigned long long> done{0};
   auto kernel = long_kernel<E, OP, CAP, HARD>;

@@ -211,3 +211,31 @@ def test_teacher_to_student():
     ops.distill_loss_(student, s.top_ids, s.top_logprobs, targets=t, temperature=tau, out=grad)
     after = ops.distill_loss(student - grad, s.top_ids, s.top_logprobs, targets=t, temperature=tau)
     assert float((after - before).sum()) < 0
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("T,V", [(2100, 300), (700, 20011), (500, 40008)])
+def test_more_rows_than_begin_at_once(T, V, dtype):
+    """Rows are taken over from blocks that have not begun; a third of them and more are left out, some side by side."""
+    check_scores(T, V, dtype, "cuda", masked=True)
+    check_scores(T, V, dtype, "cuda", K=12, masked=True, gap=1)
+    check_policy(T, V, dtype, "cuda", masked=True, gap=3, apart=False)
+    check_policy(T, V, dtype, "cuda", cap=20.0)
+    check_distill(T, V, dtype, "cuda", 9, tau=2.0, rest="bucket", ce=0.3, masked=True, shift=1)
+
+
+@pytest.mark.parametrize("live", [0, 1, 500])
+def test_few_rows_count(live):
+    """Long runs of rows that are left out."""
+    T, V = 1500, 20000
+    z = wide(T, V, BF16, "cuda")[1]
+    t = torch.full((T,), -100, device="cuda")
+    t[T - live:] = 5
+    s = ops.token_logprobs(z, t, top_k=3)
+    assert int((s.logprobs != 0).sum()) == live and int((s.top_ids[:, 0] >= 0).sum()) == live
+    out = torch.full_like(z, 3.0)
+    p = ops.policy_loss_(z, t, out=out)
+    assert bool((out[: T - live] == 0).all()) and bool((out[T - live:].abs().sum(-1) > 0).all()) and int((p.loss != 0).sum()) == live
+    out.fill_(3.0)
+    ops.distill_loss_(z, t.clamp(min=0)[:, None], torch.zeros(T, 1, device="cuda"), targets=t, out=out)
+    assert bool((out[: T - live] == 0).all()) and bool((out[T - live:].abs().sum(-1) > 0).all())
