@@ -19,7 +19,6 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -159,18 +158,6 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
   for (int i = 0; i < NT / 32; ++i) v += sh[i];
   return v;
 }
-template <int NT>
-__device__ __forceinline__ float block_max(float v, float* sh) {
-  __syncthreads();
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sh[0];
-#pragma unroll
-  for (int i = 1; i < NT / 32; ++i) v = fmaxf(v, sh[i]);
-  return v;
-}
 
 // What a policy row is given besides its logits, asked for long before it is used.
 struct Given {
@@ -244,7 +231,7 @@ __device__ __forceinline__ void total(const Row& a, int row, const Part* rec, fl
       const bool none = rec[r].m == -INFINITY;
       const float down = none ? 0.f : ex2(d);
       O += down * rec[r].S;
-      A += none ? 0.f : down * (rec[r].A + rec[r].S * d);
+      A += down == 0.f ? 0.f : down * (rec[r].A + rec[r].S * d);
       if (OP == SCORES) t.low = r == 0 ? rec[r].low : min(t.low, rec[r].low);
     }
     const float yt = (ut - t.M) * a.c, et = has ? ex2(yt) : 0.f, S = O + et;
@@ -472,17 +459,10 @@ __device__ __forceinline__ void write_named(const Row& a, const Totals& t, const
 }
 
 
-// ------------------------------------------------------------------------------------------- rows in shared memory
-// A cluster of up to eight blocks takes a row and keeps it in their shared memory, so that memory is read once and the gradient is the
-// only other traffic: a piece of 16 bytes on for each block, by one bulk copy, rows off the 16-byte grid with the pieces that they
-// begin and end in.  The blocks exchange their parts of the totals through one another's shared memory, at one meeting of the cluster
-// (one more for alternatives).  Several blocks an SM: while one waits for its piece others compute.
-//
-// Alternatives: a bound that at least K tokens are not below, from each block's largest ones by thread (found by halving an interval of
-// whole numbers that are in the order of the floats); tokens from the highest of the blocks' bounds on go to one block, which ranks
-// them.  Where they are too many (thousands of equal logits) the cluster halves the interval of (logit, index) of all tokens until
-// exactly K are left.
-
+// ---------------------------------------------------------------------------------------------- clusters and pieces
+constexpr int BATCH = 8;                   // pieces of 16 bytes that a thread asks for at once
+constexpr int LONG_ROW = 114688;           // bytes of a row from which a block has 512 threads, not 256
+constexpr int FEW_BLOCKS = 2 * 148;        // rows are cut where there are fewer
 __device__ __forceinline__ uint32_t in_cluster(const void* p, int rank) {          // the same place in another block's shared memory
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(ftb::smem_u32(p)), "r"(rank));
@@ -506,45 +486,21 @@ __device__ __forceinline__ void cluster_arrive_relaxed() {
 }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // what other blocks sent; bounded as ftb::mbar_wait, and once more as long after it was reported
-__device__ __forceinline__ bool sent_wait(uint64_t* bar, uint32_t parity, int where) {
+__device__ __forceinline__ void sent_wait(uint64_t* bar, int where) {
   for (int again = 0; again < 2; ++again) {
     for (uint32_t it = 0; it < FTB_WAIT_LIMIT; ++it) {
       uint32_t ok;
       asm volatile(
           "{\n.reg .pred p;\n"
-          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n"
           "selp.u32 %0, 1, 0, p;\n}\n"
           : "=r"(ok)
-          : "r"(ftb::smem_u32(bar)), "r"(parity)
+          : "r"(ftb::smem_u32(bar))
           : "memory");
-      if (ok) return true;
+      if (ok) return;
     }
     ftb::set_error(1, where);
   }
-  return false;
-}
-// A cluster that has not begun is taken over by this one, or none is: the answer's 16 bytes are counted on a barrier.  first: the index
-// of its first block, -1 where there was none (after which there is none any more).
-__device__ __forceinline__ void take_over(void* answer, uint64_t* bar) {
-  ftb::fence_proxy_async();
-  ftb::mbar_expect_tx(bar, 16);
-  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(ftb::smem_u32(answer)),
-               "r"(ftb::smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ int taken_over(const void* answer) {
-  uint32_t got, first;
-  asm volatile(
-      "{\n.reg .b128 h;\n.reg .pred p;\n"
-      "ld.shared.b128 h, [%2];\n"
-      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
-      "selp.u32 %0, 1, 0, p;\n"
-      "mov.u32 %1, 0;\n"
-      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n}\n"
-      : "=r"(got), "=r"(first)
-      : "r"(ftb::smem_u32(answer))
-      : "memory");
-  return got ? static_cast<int>(first) : -1;
 }
 
 // two floats to an instruction
@@ -710,654 +666,485 @@ __device__ __forceinline__ float logit_of(uint32_t order) {
   return order == NAN_ORDER ? NAN : __uint_as_float(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);
 }
 
-// NW threads work on the tokens; one warp more begins copies, takes the named tokens out and exchanges the parts, so that what it does
-// for a row lies beside the others' passes.  A cluster that is done with a row takes over the row of one that has not begun (``more``:
-// there are some), since beginning blocks costs as long as their work on a row: its first block asks for it while the others are at
-// work and tells them; a copy begins as soon as the last row's tokens are no longer read.
-template <int NW>
-__host__ __device__ constexpr int slice_blocks() { return NW == 128 ? 6 : NW == 256 ? 3 : 1; }      // of an SM
-template <typename E, Op OP, bool TOP, bool CAP, bool HARD, int NW>
-__global__ void __launch_bounds__(NW + 32, slice_blocks<NW>()) slice_kernel(Row a, int slice, int room, int more) {
-  constexpr int VE = Vec<E>::N, P = VE / 2, W = NW / 32, NT = NW + 32;
-  extern __shared__ __align__(128) unsigned char buf[];
-  const bool early = OP == SCORES ? !TOP : a.out == nullptr;  // nothing reads a row's tokens after its sums
-  __shared__ __align__(8) uint64_t bar, sent[2], told[2], answered;
-  __shared__ __align__(16) int4 next[2];                      // a row to come (-1: none), whether it counts, its given token
-  __shared__ __align__(16) int4 answer;
-  __shared__ int gave_up, found;
+// --------------------------------------------------------------------------------------------------- a row's passes
+// A block takes a row, or a cluster of up to eight blocks where there are few rows, a piece of it each (pieces of 16 bytes; the ones that
+// a row begins and ends in by single threads).  Memory is read once for the totals: each thread keeps the largest logit that it has seen
+// and its sums relative to it.  The blocks of a cluster send one another their parts of the totals.  The gradient reads the row a second
+// time, from the second level of cache, and is the only other traffic; alternatives read a few threads' pieces again.
+//
+// Alternatives: a bound that at least K tokens are not below, from the largest ones by thread (found by halving an interval of whole
+// numbers that are in the order of the floats); every block gives the tokens from the lowest of the blocks' bounds on to all, and ranks
+// its own among them.  Where these are too many because the blocks' tokens differ, the bound is the highest of bounds by K threads of a
+// block; where thousands of logits are equal, the cluster halves the interval of (logit, index) of all tokens until exactly K are left.
+template <typename E, Op OP, bool TOP, bool CAP, bool HARD, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, int room) {
+  constexpr int VE = Vec<E>::N, P = VE / 2, W = NT / 32, U = BATCH;
+  extern __shared__ __align__(16) unsigned char buf[];        // DISTILL: for each piece which of its tokens are named; TOP: tokens given
+  __shared__ __align__(8) uint64_t sent;
+  __shared__ int found;
   __shared__ float sh[32], most[W], least[W], sums[3][W];
-  __shared__ Part rec[2][MOST_PARTS], own;
+  __shared__ Part rec[MOST_PARTS], own;
   __shared__ Totals fin;
   __shared__ int count[2][MOST_PARTS];
   __shared__ uint32_t bounds[MOST_PARTS];
   __shared__ int id[OP == DISTILL ? MOST_TOP : 1];
   __shared__ float q[OP == DISTILL ? MOST_TOP : 1];
-  E* zs = reinterpret_cast<E*>(buf);
-  const uint4* zv = reinterpret_cast<const uint4*>(buf);
 
   int rank, parts;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V, K = a.K;
-  const bool works = warp < W, takes = more && rank == 0;
-  if (tid == NW) {
-    gave_up = found = 0;
-    ftb::mbar_init(&bar, 1);
-    ftb::mbar_init(&answered, 1);
-    for (int i = 0; i < 2; ++i) {
-      ftb::mbar_init(&sent[i], 1);
-      ftb::mbar_init(&told[i], 1);
-    }
-    ftb::fence_barrier_init();
-  }
-  cluster_arrive_relaxed();                                   // (the others may be sent to once all have begun)
-  if (tid < 2 * MOST_PARTS && tid % MOST_PARTS >= parts) rec[tid / MOST_PARTS][tid % MOST_PARTS] = no_part();
-  int row = blockIdx.x / parts, answers = 0, loads = 0;
-  long t = a.targets ? a.targets[row] : -1;
-  bool on = row_on(a, row, t);
-  // the row from the 16-byte piece that it begins in: ``lead`` elements before it, this block's from ``lo`` on, in pieces
-  auto lead_of = [&](int r) { return static_cast<int>((reinterpret_cast<uintptr_t>(static_cast<const E*>(a.z) + r * a.ldz) & 15) / sizeof(E)); };
-  auto count_of = [&](int lead) { return max(0, min(lead + V - rank * slice, slice)); };
-  auto load = [&](int r) {                                    // by one thread
-    const int lead = lead_of(r), nv = (count_of(lead) + VE - 1) / VE;
-    if (nv > 0) {
-      ftb::fence_proxy_async();
-      ftb::mbar_expect_tx(&bar, nv * 16);
-      ftb::bulk_load_g2s(buf, static_cast<const E*>(a.z) + r * a.ldz - lead + rank * slice, nv * 16, &bar);
-    }
-  };
-  if (tid == NW && on) load(row);
-  __syncthreads();
-  cluster_wait();
-  // Where nothing waits for a row's totals its last part is left for the next row's passes (by the warp that exchanges).
-  int last = -1, last_it = 0;
-  float last_qr = 0.f;
-  Given last_given = {};
-  auto finish = [&] {
-    if (last < 0) return;
-    sent_wait(&sent[last_it & 1], (last_it >> 1) & 1, 3);
-    total<OP, HARD>(a, last, rec[last_it & 1], last_qr, last_given, rank == 0, &fin);
-    last = -1;
-  };
-
-  for (int it = 0; row >= 0; ++it) {
-    const E* z = static_cast<const E*>(a.z) + row * a.ldz;
-    E* out = static_cast<E*>(a.out) + row * a.ldo;
-    const int lo = rank * slice, lead = lead_of(row), n = count_of(lead), nv = (n + VE - 1) / VE, first_token = lo - lead;
-    const bool whole = OP != SCORES && (reinterpret_cast<uintptr_t>(out) & 15) / sizeof(E) == lead;       // the gradient's pieces lie as the logits' do
-    const int now = it & 1, then = now ^ 1;
-    const uint32_t told_parity = (it >> 1) & 1;
-    if (tid == NW) {
-      ftb::mbar_expect_tx(&sent[now], parts * sizeof(Part));
-      if (more) ftb::mbar_expect_tx(&told[then], 16);
-    }
-    // The next row: asked for when this row's tokens are here (by then all blocks that find room have begun), told to the cluster.
-    auto ask = [&] {
-      if (takes && tid == NW) take_over(&answer, &answered);
-    };
-    auto tell = [&] {
-      if (!takes || works) return;
-      int4 v = make_int4(-1, 0, 0, 0);
-      if (lane == 0) {
-        const int first = sent_wait(&answered, answers & 1, 5) ? taken_over(&answer) : -1;
-        if (first >= 0) {
-          v.x = first / parts;
-          const long given = a.targets ? a.targets[v.x] : -1;
-          v.y = row_on(a, v.x, given);
-          v.z = static_cast<int>(given);                      // (a token where the row counts)
-        }
-      }
-      ++answers;
-      v = make_int4(__shfl_sync(~0u, v.x, 0), __shfl_sync(~0u, v.y, 0), __shfl_sync(~0u, v.z, 0), 0);
-      if (lane < parts)
-        send16(in_cluster(&next[then], lane), make_uint4(v.x, v.y, v.z, 0), in_cluster(&told[then], lane));
-    };
-    auto load_next = [&] {                                    // by the warp
-      if (!more) return;
-      if (sent_wait(&told[then], told_parity, 6) && lane == 0 && next[then].x >= 0 && next[then].y) load(next[then].x);
-    };
-    auto send_part = [&](const Part& p) {                     // to every block of the cluster, this one among them
-      if (lane == 0) own = p;
-      __syncwarp();
-      if (lane < parts * PART_PIECES) {
-        const int to = lane / PART_PIECES, piece = lane - to * PART_PIECES;
-        send16(in_cluster(reinterpret_cast<const uint4*>(&rec[now][rank]) + piece, to), reinterpret_cast<const uint4*>(&own)[piece],
-               in_cluster(&sent[now], to));
-      }
-    };
-    auto step = [&] {                                         // by all
-      const bool known = more && sent_wait(&told[then], told_parity, 6);
-      row = known ? next[then].x : -1;
-      on = known && next[then].y;
-      t = on && a.targets ? next[then].z : -1;
-    };
-    if (!on) {
-      // (nothing is exchanged, but no block may be two rows ahead of another, nor of a thread of its own that has not read where to go)
-      __syncthreads();
-      ask();
-      if (works && OP != SCORES && a.out)
-        for (int v = tid; v < nv; v += NW) {
-          const int token = first_token + v * VE;
-          if (whole && token >= 0 && token + VE <= V) {
-            *reinterpret_cast<uint4*>(out + token) = make_uint4(0, 0, 0, 0);
-          } else {
-            for (int e = 0; e < VE; ++e)
-              if (token + e >= 0 && token + e < V) out[token + e] = from_float<E>(0.f);
-          }
-        }
-      if (rank == 0) row_off<OP>(a, row);
-      if (!works) {
-        finish();
-        tell();
-        send_part(Part{});
-        load_next();
-        sent_wait(&sent[now], (it >> 1) & 1, 3);
-      }
-      step();
-      continue;
-    }
-    const long given = t;
-    float qr = 0.f;
-    bool named_t = false;
-    Named mine;
-    Given policy = {};
-    if (OP == POLICY && !works) policy = given_of(a, row);
-    if (OP == DISTILL && !works) qr = teacher_of(a, row, t, id, q, mine, named_t);
-    if (nv > 0) {
-      if (!ftb::mbar_wait(&bar, loads & 1, &gave_up, 1)) {    // (reported; the copy gets as long again before the block goes on)
-        int again = 0;
-        ftb::mbar_wait(&bar, loads & 1, &again, 2);
-      }
-      ++loads;
-    }
-
-    // what lies around the row is no token; named tokens by themselves
-    const int at_t = static_cast<int>(t) - first_token;         // where the given token lies
-    const bool mine_t = a.targets && at_t >= 0 && at_t < n;
-    float zt = 0.f;
-    if (!works) {
-      if (lane < VE) {
-        if (lo + lane < lead && lane < nv * VE) zs[lane] = from_float<E>(-INFINITY);
-        if (n + lane < nv * VE) zs[n + lane] = from_float<E>(-INFINITY);
-      }
-      if (mine_t) zt = to_float(zs[at_t]);
-      __syncwarp();
-      if (OP != DISTILL && mine_t && lane == 0) zs[at_t] = from_float<E>(-INFINITY);
-      if (OP == DISTILL) {
-        typedef typename std::conditional<sizeof(E) == 2, uint16_t, uint32_t>::type Bits;
-        Bits* tag = reinterpret_cast<Bits*>(buf);
-#pragma unroll
-        for (int j = 0; j < ENTRIES; ++j) {
-          mine.here[j] = mine.id[j] >= first_token && mine.id[j] < first_token + n && mine.id[j] >= 0;
-          if (mine.here[j]) mine.z[j] = to_float(zs[mine.id[j] - first_token]);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < ENTRIES; ++j)                       // of entries of one token, the one whose number stays in its place
-          if (mine.here[j]) tag[mine.id[j] - first_token] = static_cast<Bits>(lane + 32 * j);
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < ENTRIES; ++j) mine.first[j] = mine.here[j] && tag[mine.id[j] - first_token] == static_cast<Bits>(lane + 32 * j);
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < ENTRIES; ++j)
-          if (mine.here[j]) zs[mine.id[j] - first_token] = from_float<E>(-INFINITY);
-      }
-      ftb::fence_proxy_async();                                 // (the next copy comes after these)
-      ask();
-    }
-    __syncthreads();
-
-    // largest of each thread, of the block
-    float mt = -INFINITY;
-    Part p = {};
-    p.B = -INFINITY;
-    if (works) {
-      uint32_t m2 = Vec<E>::NONE;
-#pragma unroll 4
-      for (int v = tid; v < nv; v += NW) m2 = Vec<E>::max2(m2, vec_max<E>(zv[v]));
-      mt = Vec<E>::top(m2);
-      const float w = warp_max(mt);
-      if (lane == 0) most[warp] = w;
-      if (TOP) {
-        float l = tid < nv ? mt : INFINITY;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) l = fminf(l, __shfl_xor_sync(~0u, l, o));
-        if (lane == 0) least[warp] = l;
-      }
-    } else if (OP == DISTILL) {
-      named_part<CAP, HARD>(a, mine, p);
-    }
-    __syncthreads();
-    if (!works) finish();                                     // (before the cluster is told: all have read what they were told last)
-    tell();
-    float mz = most[0];
-#pragma unroll
-    for (int w = 1; w < W; ++w) mz = fmaxf(mz, most[w]);
-    const float um = mz == -INFINITY ? mz : capped<CAP>(a, mz), base = mz == -INFINITY ? 0.f : um;
-
-    // sums relative to it.  16-bit logits: the exponent's argument by one fused operation, relative to the rounded product of base and c; what
-    // the rounding is goes into the sums at the end.  (Bases whose product leaves no digits: as fp32 logits.)
-    float off = 0.f, off1 = 0.f;                                // base c and base log2 e less what the sums are relative to
-    if (works) {
-      f32x2 S = 0, S1 = 0;
-      float A = 0.f;
-      const float kb = base * a.c, kb1 = base * LOG2E;
-      const bool fused = sizeof(E) == 2 && fabsf(kb) < 0x1p24f && fabsf(kb1) < 0x1p24f;
-      const f32x2 minus = pair(-base, -base), cc = pair(a.c, a.c), l2 = pair(LOG2E, LOG2E), mk = pair(-kb, -kb), mk1 = pair(-kb1, -kb1);
-      auto pass = [&](auto f) {
-        constexpr bool FUSED = decltype(f)::value;
-#pragma unroll 2
-        for (int v = tid; v < nv; v += NW) {
-          const uint4 w = zv[v];
-          f32x2 x[P], slope[P], part = 0;
-          pairs_of<E>(w, x);
-          if (CAP) cap_pairs<E, false>(a, x, slope);
-#pragma unroll
-          for (int i = 0; i < P; ++i) {
-            f32x2 y, y1;
-            if (FUSED) {
-              y = fma2(x[i], cc, mk);
-              if (HARD) y1 = fma2(x[i], l2, mk1);
-            } else {
-              const f32x2 d = add2(x[i], minus);
-              y = mul2(d, cc);
-              if (HARD) y1 = mul2(d, l2);
-            }
-            const f32x2 e = exp2_2(y);
-            S = add2(S, e);
-            if (OP != DISTILL) part = fma2(e, y, part);
-            if (HARD) S1 = add2(S1, exp2_2(y1));
-          }
-          if (OP != DISTILL) {
-            float b, c;
-            split(part, b, c);
-            b += c;
-            if (b != b) {                                       // (a logit of -inf: nothing times minus infinity)
-              float g[VE];
-              floats_of<E>(w, g);
-              b = 0.f;
-#pragma unroll
-              for (int e = 0; e < VE; ++e) {
-                const float u = capped<CAP>(a, g[e]), y = FUSED ? fmaf(u, a.c, -kb) : (u - base) * a.c;
-                b += ex2(y) * max_nan(y, -256.f);
-              }
-            }
-            A += b;
-          }
-        }
-      };
-      if (fused) {
-        pass(std::true_type());
-        off = fmaf(base, a.c, -kb);
-        off1 = fmaf(base, LOG2E, -kb1);
-      } else {
-        pass(std::false_type());
-      }
-      auto back = [](float o) { return fabsf(o) < 1e-4f ? fmaf(-o, LN2, 1.f) : ex2(-o); };      // 2^-off
-      float b, c;
-      split(S, b, c);
-      b += c;
-      const float down = back(off);
-      const float s = warp_sum(b * down);
-      if (lane == 0) sums[0][warp] = s;
-      if (OP != DISTILL) {
-        A = warp_sum(down * (A - off * b));
-        if (lane == 0) sums[1][warp] = A;
-      }
-      if (HARD) {
-        split(S1, b, c);
-        b = warp_sum((b + c) * back(off1));
-        if (lane == 0) sums[2][warp] = b;
-      }
-    }
-    // the largest of at least ``want`` threads are not below it, and of not many more
-    auto bound_of = [&](int want) {
-      float l = least[0];
-#pragma unroll
-      for (int w = 1; w < W; ++w) l = fminf(l, least[w]);
-      uint32_t low = order_of(l), high = order_of(mz) + 1;
-      const uint32_t key = works && tid < nv ? order_of(mt) : 0;
-      for (int it = 0; it < 32 && high - low > 1; ++it) {
-        const uint32_t mid = low + (high - low) / 2;
-        const int c = __syncthreads_count(key >= mid);
-        if (c >= want) low = mid;
-        else high = mid;
-        if (c >= want && c <= want + want / 4 + 4) break;
-      }
-      return low;
-    };
-    uint32_t low = 0;
-    if (TOP) {
-      const int filled = (lead + V + slice - 1) / slice, share = (K + filled - 1) / filled;      // (blocks without tokens have no share)
-      if (nv == 0) low = 0xFFFFFFFFu;
-      else if (min(nv, NW) >= share) low = bound_of(share);
-    }
-    __syncthreads();
-    float slope_t = 1.f;
-    if (!works) {
-      p.m = um;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        p.S += sums[0][w];
-        if (OP != DISTILL) p.A += sums[1][w];
-        if (HARD) p.S1 += sums[2][w];
-      }
-      p.has_t = mine_t ? 1.f : 0.f;
-      p.ut = mine_t ? capped<CAP>(a, zt, slope_t) : 0.f;
-      p.low = low;
-      send_part(p);
-      last = row, last_it = it, last_qr = qr, last_given = policy;
-      if (early) load_next();
-      else finish();
-    }
-    if (early) {
-      step();
-      continue;
-    }
-    __syncthreads();
-    const Totals T = fin;
-
-    if (OP == SCORES) {
-      // tokens from the bound on to every block, which then ranks its own among them
-      u64* taken = reinterpret_cast<u64*>(buf + slice * static_cast<int>(sizeof(E)));
-      const bool broken = T.lS != T.lS;                         // (a thread's largest leaves NaN out)
-      u64* ours = taken + rank * room;
-      // A warp takes the threads with such tokens one by one, half a piece a lane.
-      auto collect = [&](u64 bound, bool all) {
-        typedef typename std::conditional<sizeof(E) == 2, uint2, float2>::type Half;
-        const uint32_t order = static_cast<uint32_t>(bound >> 32);
-        auto give = [&](float f, int token) {
-          const u64 key = key_of(f, token);
-          if (key < bound) return;
-          const int i = atomicAdd(&found, 1);
-          if (i < room) ours[i] = key;
-        };
-        if (tid == NW && mine_t) give(zt, static_cast<int>(t));
-        uint32_t those = __ballot_sync(~0u, works && tid < nv && (all || order_of(mt) >= order));
-        while (those) {
-          const int first = (warp << 5) + __ffs(those) - 1;
-          those &= those - 1;
-          for (int h = lane; h < 2 * ((nv - first + NW - 1) / NW); h += 32) {
-            const int at = (first + (h >> 1) * NW) * VE + (h & 1) * (VE / 2);
-            const Half w = *reinterpret_cast<const Half*>(zs + at);
-            float f[VE / 2];
-            if constexpr (sizeof(E) == 4) {
-              f[0] = w.x, f[1] = w.y;
-            } else {
-              split(Vec<E>::one(w.x), f[0], f[1]);
-              split(Vec<E>::one(w.y), f[2], f[3]);
-            }
-#pragma unroll
-            for (int e = 0; e < VE / 2; ++e) {
-              const int token = first_token + at + e;
-              if (order_of(f[e]) >= order && token >= 0 && token < V && token != t) give(f[e], token);
-            }
-          }
-        }
-        __syncthreads();
-        const int have = min(found, room);
-        for (int i = tid; i < have * parts; i += NT) {
-          const int to = i % parts, c = i / parts;
-          if (to != rank) put64(in_cluster(ours + c, to), ours[c]);
-        }
-        if (tid < parts) put32(in_cluster(&count[0][rank], tid), found);
-        cluster_arrive();
-        cluster_wait();
-        bool over = false;
-        for (int r = 0; r < parts; ++r) over |= count[0][r] > room;
-        return over;
-      };
-      u64 bound = static_cast<u64>(T.low) << 32;
-      bool over = collect(bound, T.low == 0 || broken);
-      if (over) {
-        // the blocks' tokens differ: the highest of bounds that K threads of a block each are not below
-        const uint32_t mine_low = min(nv, NW) >= K ? bound_of(K) : 0;
-        if (tid < parts) put32(in_cluster(&bounds[rank], tid), mine_low);
-        if (tid == 0) found = 0;
-        cluster_arrive();                                       // (all have read the last counts)
-        cluster_wait();
-        uint32_t highest = T.low;
-        for (int r = 0; r < parts; ++r) highest = max(highest, bounds[r]);
-        bound = static_cast<u64>(highest) << 32;
-        over = collect(bound, highest == 0 || broken);
-      }
-      if (over) {
-        u64 below = 0, above = ~0ull;                           // at least K keys are not below the one, fewer not below the other
-        for (int it = 0; above - below > 1; ++it) {
-          const u64 mid = below + (above - below) / 2;
-          int c = tid == NW && mine_t && key_of(zt, static_cast<int>(t)) >= mid;
-          if (works)
-            for (int v = tid; v < nv; v += NW) {
-              float f[VE];
-              floats_of<E>(zv[v], f);
-#pragma unroll
-              for (int e = 0; e < VE; ++e) {
-                const int token = first_token + v * VE + e;
-                c += token >= 0 && token < V && token != t && key_of(f[e], token) >= mid;
-              }
-            }
-          c = static_cast<int>(block_sum<NT>(static_cast<float>(c), sh));           // (whole numbers below 2^24)
-          if (tid < parts) put32(in_cluster(&count[1 - (it & 1)][rank], tid), c);
-          cluster_arrive();
-          cluster_wait();
-          int sum = 0;
-          for (int r = 0; r < parts; ++r) sum += count[1 - (it & 1)][r];
-          if (sum >= K) below = mid;
-          else above = mid;
-          if (sum == K) break;
-        }
-        if (tid == 0) found = 0;
-        cluster_arrive();                                       // (all have read the last counts)
-        cluster_wait();
-        bound = below;
-        collect(bound, true);
-      }
-      if (!works) load_next();                                // (the row was read when the counts were exchanged)
-      // eight threads to a token, one for each block's
-      for (int i = tid / MOST_PARTS; i < (count[0][rank] + NT / MOST_PARTS - 1) / (NT / MOST_PARTS) * (NT / MOST_PARTS); i += NT / MOST_PARTS) {
-        const int r = tid % MOST_PARTS, others = r < parts ? count[0][r] : 0;
-        const bool valid = i < count[0][rank];
-        const u64 key = valid ? taken[rank * room + i] : ~0ull;
-        int above = 0;
-#pragma unroll 4
-        for (int j = 0; j < others; ++j) above += taken[r * room + j] > key;
-#pragma unroll
-        for (int o = MOST_PARTS / 2; o; o >>= 1) above += __shfl_xor_sync(~0u, above, o);
-        if (valid && r == 0 && above < K) {
-          const int token = static_cast<int>(~static_cast<uint32_t>(key));
-          a.top_ids[(size_t)row * K + above] = token;
-          a.top_logprob[(size_t)row * K + above] =
-              token == t ? T.lp : ((capped<CAP>(a, logit_of(static_cast<uint32_t>(key >> 32))) - T.M) * a.c - T.lS) * LN2;
-        }
-      }
-      if (tid == 0) found = 0;
-      step();
-      continue;
-    }
-
-    const float scale = OP == DISTILL ? a.scale : a.scale * a.inv_tau;
-    if (works) {
-      const bool bonus = OP == POLICY && T.kb != 0.f;
-      // One by one: entropy's gradient where a cap leaves -inf (elsewhere it is brought to a number that has no p log p, unless all of the row
-      // are such), and logits so large that their differences have to be formed first.
-      const bool careful = (bonus && (CAP || !(T.M > Vec<E>::LOW * 0.9f) || a.inv_tau < 0.05f)) ||
-                           (sizeof(E) == 2 && !(fabsf(T.base) * fmaxf(a.c, LOG2E) < 4096.f && fabsf(T.M) * LOG2E < 4096.f));
-      const f32x2 minus = pair(-T.base, -T.base), cc = pair(a.c, a.c), k0 = pair(T.k0, T.k0);
-      const float fa = OP == POLICY ? T.ka * scale : (1.f - a.ce) * a.tau * T.ka * scale, fb = T.kb * LN2 * scale;
-      const float f0 = fmaf(-T.base, a.c, T.k0), f1 = fmaf(-T.M, LOG2E, -T.h0);
-      const f32x2 ka = pair(fa, fa), kb = pair(fb, fb), kc = pair(f0, f0), kh = pair(f1, f1);
-      const f32x2 minus_m = pair(-T.M, -T.M), l2 = pair(LOG2E, LOG2E), h0 = pair(-T.h0, -T.h0), ce = pair(a.ce * scale, a.ce * scale);
-      auto pass = [&](auto with_bonus, auto with_care) {
-        constexpr bool BONUS = decltype(with_bonus)::value, CARE = decltype(with_care)::value;
-#pragma unroll 2
-        for (int v = tid; v < nv; v += NW) {
-          f32x2 x[P], slope[P];
-          pairs_of<E>(BONUS && !CARE ? vec_floor<E>(zv[v]) : zv[v], x);
-          if (CAP) cap_pairs<E, true>(a, x, slope);
-#pragma unroll
-          for (int i = 0; i < P; ++i) {
-            f32x2 r;
-            if (CARE) {
-              float b, c;
-              split(x[i], b, c);
-              r = pair(grad_rest<OP, HARD>(a, T, b) * scale, grad_rest<OP, HARD>(a, T, c) * scale);
-            } else {
-              const f32x2 y = sizeof(E) == 2 ? fma2(x[i], cc, kc) : fma2(add2(x[i], minus), cc, k0);
-              r = mul2(exp2_2(y), BONUS ? fma2(kb, y, ka) : ka);
-              if (HARD) r = fma2(exp2_2(sizeof(E) == 2 ? fma2(x[i], l2, kh) : fma2(add2(x[i], minus_m), l2, h0)), ce, r);
-            }
-            x[i] = CAP ? mul2(r, slope[i]) : r;
-          }
-          const uint4 w = vec_of<E>(x);
-          const int token = first_token + v * VE;
-          if (whole && token >= 0 && token + VE <= V) {
-            *reinterpret_cast<uint4*>(out + token) = w;
-          } else {
-            float f[VE];
-            floats_of<E>(w, f);
-#pragma unroll
-            for (int e = 0; e < VE; ++e)
-              if (token + e >= 0 && token + e < V) out[token + e] = from_float<E>(f[e]);
-          }
-        }
-      };
-      if (careful) pass(std::false_type(), std::true_type());
-      else if (OP == POLICY && !CAP && bonus) pass(std::true_type(), std::false_type());
-      else pass(std::false_type(), std::false_type());
-    }
-    __syncthreads();
-    step();
-    if (works) continue;
-    load_next();
-    if (OP == POLICY && mine_t && lane == 0) out[given] = from_float<E>(grad_taken(T, a.bonus) * slope_t * scale);
-    if (OP == DISTILL) {
-      write_named<E, CAP, HARD>(a, T, mine, id, q, given, scale, out);
-      if (HARD && mine_t && lane == 0 && !named_t) {
-        const float u = capped<CAP>(a, zt, slope_t);
-        out[given] = from_float<E>((grad_rest<OP, HARD>(a, T, u) - a.ce) * slope_t * scale);
-      }
-    }
-  }
-  if (!works) finish();
-}
-
-// ---------------------------------------------------------------------------------- rows that shared memory does not hold
-// A block for a row, which is read from memory in every pass (the alternatives: one pass for each).
-constexpr int LONG_NT = 512;
-template <typename E, Op OP, bool CAP, bool HARD>
-__global__ void __launch_bounds__(LONG_NT) long_kernel(Row a) {
-  constexpr int NT = LONG_NT;
-  __shared__ float sh[32];
-  __shared__ u64 best[32];
-  __shared__ int id[MOST_TOP];
-  __shared__ float q[MOST_TOP];
-  __shared__ Part rec[MOST_PARTS];
-  __shared__ Totals fin;
-  extern __shared__ uint32_t bits[];                          // DISTILL: which tokens the teacher names
-  const int row = blockIdx.x, tid = threadIdx.x, V = a.V, K = a.K;
+  const int row = blockIdx.x / parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V, K = a.K;
   const E* z = static_cast<const E*>(a.z) + row * a.ldz;
   E* out = static_cast<E*>(a.out) + row * a.ldo;
+  // the row from the 16-byte piece that it begins in: ``lead`` elements before it, this block's from ``lo`` on, n of them in nv pieces,
+  // those from full to end_full with no others in them
+  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(E));
+  const int lo = rank * slice, n = max(0, min(lead + V - lo, slice)), nv = (n + VE - 1) / VE, first_token = lo - lead;
+  const int full = first_token < 0 ? 1 : 0, end_full = n / VE;
+  const uint4* zv = reinterpret_cast<const uint4*>(z - lead + lo);
+  const bool whole = OP != SCORES && (reinterpret_cast<uintptr_t>(out) & 15) / sizeof(E) == lead;       // the gradient's pieces lie as the logits' do
   const long t = a.targets ? a.targets[row] : -1;
   if (!row_on(a, row, t)) {
     if (OP != SCORES && a.out)
-      for (int i = tid; i < V; i += NT) out[i] = from_float<E>(0.f);
-    row_off<OP>(a, row);
+      for (int v = tid; v < nv; v += NT) {
+        const int token = first_token + v * VE;
+        if (whole && token >= 0 && token + VE <= V) {
+          *reinterpret_cast<uint4*>(out + token) = make_uint4(0, 0, 0, 0);
+        } else {
+          for (int e = 0; e < VE; ++e)
+            if (token + e >= 0 && token + e < V) out[token + e] = from_float<E>(0.f);
+        }
+      }
+    if (rank == 0) row_off<OP>(a, row);
     return;
+  }
+  if (tid == 0) {
+    found = 0;
+    ftb::mbar_init(&sent, 1);
+    ftb::fence_barrier_init();
+    ftb::mbar_expect_tx(&sent, parts * sizeof(Part));
+  }
+  if (parts > 1) cluster_arrive_relaxed();                    // (the others may be sent to once all have begun)
+  if (tid < MOST_PARTS && tid >= parts) rec[tid] = no_part();
+  const int at_t = static_cast<int>(t) - first_token;         // where the given token lies
+  const bool mine_t = a.targets && at_t >= 0 && at_t < n;
+  const int piece_t = OP != DISTILL && mine_t ? at_t / VE : -1;
+  float zt = 0.f;
+  Given policy = {};
+  if (warp == 0) {
+    if (mine_t) zt = to_float(z[t]);
+    if (OP == POLICY) policy = given_of(a, row);
   }
   float qr = 0.f;
   bool named_t = false;
   Named mine;
   if (OP == DISTILL) {
-    for (int i = tid; i < (V + 31) / 32; i += NT) bits[i] = 0;
+    for (int i = tid; i < (nv + 15) / 16; i += NT) reinterpret_cast<uint4*>(buf)[i] = make_uint4(0, 0, 0, 0);
+    if (warp == 0) qr = teacher_of(a, row, t, id, q, mine, named_t);
     __syncthreads();
-    if (tid < 32) {
-      qr = teacher_of(a, row, t, id, q, mine, named_t);
+    if (warp == 0) {
 #pragma unroll
       for (int j = 0; j < ENTRIES; ++j) {
-        const int i = mine.id[j];
-        if (i < 0) continue;
-        mine.here[j] = true;
-        mine.z[j] = to_float(z[i]);
-        const uint32_t bit = 1u << (i & 31);
-        mine.first[j] = !(atomicOr(&bits[i >> 5], bit) & bit);
+        const int at = mine.id[j] - first_token;
+        mine.here[j] = mine.id[j] >= 0 && at >= 0 && at < n;
+        if (!mine.here[j]) continue;
+        mine.z[j] = to_float(z[mine.id[j]]);
+        const int v = at / VE;
+        const uint32_t bit = 1u << ((v & 3) * 8 + at % VE);
+        mine.first[j] = !(atomicOr(reinterpret_cast<uint32_t*>(buf) + (v >> 2), bit) & bit);      // (of entries of one token, one stands for all)
       }
     }
     __syncthreads();
   }
-  auto named = [&](int i) { return OP == DISTILL ? (bits[i >> 5] >> (i & 31) & 1) != 0 : i == t; };
-  float m = -INFINITY;
-  for (int i = tid; i < V; i += NT)
-    if (!named(i)) m = fmaxf(m, to_float(z[i]));
-  m = block_max<NT>(m, sh);
-  Part p = {};
-  p.m = m == -INFINITY ? m : capped<CAP>(a, m);
-  const float base = m == -INFINITY ? 0.f : p.m;
-  float S = 0.f, A = 0.f, S1 = 0.f;
-  for (int i = tid; i < V; i += NT) {
-    if (named(i)) continue;
-    const float d = capped<CAP>(a, to_float(z[i])) - base, x = d * a.c, e = ex2(x);
-    S += e;
-    if (OP != DISTILL) A += e * max_nan(x, -256.f);
-    if (HARD) S1 += ex2(d * LOG2E);
+
+  // The totals' parts.  struck: tokens of a piece that are not summed here, a bit each.
+  float top = -INFINITY, base = 0.f, A = 0.f;                 // largest logit, u that the sums are relative to
+  f32x2 S = 0, S1 = 0;
+  const f32x2 cc = pair(a.c, a.c), l2 = pair(LOG2E, LOG2E);
+  auto strike = [&](uint4& w, uint32_t struck) {
+    uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (sizeof(E) == 4) {
+        if (struck >> i & 1) x[i] = Vec<E>::NONE;
+      } else {
+        if (struck >> (2 * i) & 1) x[i] = (x[i] & 0xFFFF0000u) | (Vec<E>::NONE & 0xFFFFu);
+        if (struck >> (2 * i + 1) & 1) x[i] = (x[i] & 0xFFFFu) | (Vec<E>::NONE & 0xFFFF0000u);
+      }
+    }
+    w = make_uint4(x[0], x[1], x[2], x[3]);
+  };
+  auto struck_in = [&](int v) -> uint32_t {
+    if (OP == DISTILL) return buf[v];
+    return v == piece_t ? 1u << (at_t % VE) : 0u;
+  };
+  auto raise = [&](float m) {                                 // to logits of up to m
+    if (!(m > top)) return;
+    top = m;
+    const float b = capped<CAP>(a, m), d = base - b, down = ex2(d * a.c);
+    float s0, s1;
+    split(S, s0, s1);
+    if (s0 + s1 != 0.f) {
+      A = down != 0.f ? down * (A + d * a.c * (s0 + s1)) : 0.f;               // (the difference may be minus infinity)
+      S = mul2(S, pair(down, down));
+      if (HARD) {
+        const float down1 = ex2(d * LOG2E);
+        S1 = mul2(S1, pair(down1, down1));
+      }
+    }
+    base = b;
+  };
+  auto add = [&](const uint4& w) {
+    const f32x2 minus = pair(-base, -base);
+    f32x2 x[P], slope[P], part = 0;
+    pairs_of<E>(w, x);
+    if (CAP) cap_pairs<E, false>(a, x, slope);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const f32x2 d = add2(x[i], minus), y = mul2(d, cc), e = exp2_2(y);
+      S = add2(S, e);
+      if (OP != DISTILL) part = fma2(e, y, part);
+      if (HARD) S1 = add2(S1, exp2_2(mul2(d, l2)));
+    }
+    if (OP != DISTILL) {
+      float b, c;
+      split(part, b, c);
+      b += c;
+      if (b != b) {                                           // (a logit of -inf: nothing times minus infinity)
+        float f[VE];
+        floats_of<E>(w, f);
+        b = 0.f;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float y = (capped<CAP>(a, f[e]) - base) * a.c;
+          b += ex2(y) * max_nan(y, -256.f);
+        }
+      }
+      A += b;
+    }
+  };
+  for (int v0 = full + tid; v0 < end_full; v0 += U * NT) {
+    uint4 w[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (v0 + i * NT < end_full) w[i] = zv[v0 + i * NT];
+    uint32_t m2 = Vec<E>::NONE;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (v0 + i * NT < end_full) {
+        const uint32_t struck = struck_in(v0 + i * NT);
+        if (struck) strike(w[i], struck);
+        m2 = Vec<E>::max2(m2, vec_max<E>(w[i]));
+      }
+    raise(Vec<E>::top(m2));
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (v0 + i * NT < end_full) add(w[i]);
   }
-  p.S = block_sum<NT>(S, sh);
-  if (OP != DISTILL) p.A = block_sum<NT>(A, sh);
-  if (HARD) p.S1 = block_sum<NT>(S1, sh);
-  p.B = -INFINITY;
-  if (OP == DISTILL && tid < 32) named_part<CAP, HARD>(a, mine, p);
-  float slope_t = 1.f, ut = 0.f;
-  if (a.targets) ut = capped<CAP>(a, to_float(z[t]), slope_t);
-  p.has_t = a.targets ? 1.f : 0.f;
-  p.ut = ut;
-  p.low = 0;
-  if (tid < MOST_PARTS) rec[tid] = tid == 0 ? p : no_part();
-  __syncthreads();                                            // the logits that are read by index have been read
-  if (tid < 32) total<OP, HARD>(a, row, rec, qr, given_of(a, row), true, &fin);
+  // the pieces with others in them: the first by thread 0, the last by the last thread
+  auto edge = [&](int v) {
+    uint4 w = zv[v];
+    uint32_t struck = struck_in(v);
+    for (int e = 0; e < VE; ++e) {
+      const int token = first_token + v * VE + e;
+      if (token < 0 || token >= V) struck |= 1u << e;
+    }
+    strike(w, struck);
+    raise(Vec<E>::top(vec_max<E>(w)));
+    add(w);
+  };
+  if (tid == 0 && full == 1 && nv > 0) edge(0);
+  if (tid == NT - 1 && end_full < nv && end_full >= full) edge(end_full);
+
+  // of the block
+  {
+    const float w = warp_max(top);
+    if (lane == 0) most[warp] = w;
+    if (TOP) {
+      float l = full + tid < end_full ? top : INFINITY;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) l = fminf(l, __shfl_xor_sync(~0u, l, o));
+      if (lane == 0) least[warp] = l;
+    }
+  }
+  __syncthreads();
+  float mz = most[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) mz = fmaxf(mz, most[w]);
+  const float um = mz == -INFINITY ? mz : capped<CAP>(a, mz);
+  {
+    float b, c;
+    split(S, b, c);
+    b += c;
+    const float d = base - (mz == -INFINITY ? 0.f : um), down = b != 0.f ? ex2(d * a.c) : 0.f;      // (nothing where there is nothing)
+    const float s = warp_sum(b * down);
+    if (lane == 0) sums[0][warp] = s;
+    if (OP != DISTILL) {
+      A = warp_sum(down != 0.f ? down * (A + d * a.c * b) : 0.f);
+      if (lane == 0) sums[1][warp] = A;
+    }
+    if (HARD) {
+      split(S1, b, c);
+      b = warp_sum(b + c != 0.f ? (b + c) * ex2(d * LOG2E) : 0.f);
+      if (lane == 0) sums[2][warp] = b;
+    }
+  }
+  // the largest of at least ``want`` threads are not below it, and of not many more
+  const int busy = min(end_full - full, NT);                  // threads with pieces of their own
+  auto bound_of = [&](int want) {
+    float l = least[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) l = fminf(l, least[w]);
+    uint32_t low = order_of(l), high = order_of(mz) + 1;
+    const uint32_t key = tid < busy ? order_of(top) : 0;
+    for (int it = 0; it < 32 && high - low > 1; ++it) {
+      const uint32_t mid = low + (high - low) / 2;
+      const int c = __syncthreads_count(key >= mid);
+      if (c >= want) low = mid;
+      else high = mid;
+      if (c >= want && c <= want + want / 4 + 4) break;
+    }
+    return low;
+  };
+  uint32_t low = 0;
+  if (TOP) {
+    const int filled = (lead + V + slice - 1) / slice, share = (K + filled - 1) / filled;      // (blocks without tokens have no share)
+    if (nv == 0) low = 0xFFFFFFFFu;
+    else if (busy >= share) low = bound_of(share);
+  }
+  __syncthreads();
+  float slope_t = 1.f;
+  if (parts > 1) cluster_wait();
+  if (warp == 0) {
+    Part p = {};
+    p.B = -INFINITY;
+    if (OP == DISTILL) named_part<CAP, HARD>(a, mine, p);
+    p.m = um;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      p.S += sums[0][w];
+      if (OP != DISTILL) p.A += sums[1][w];
+      if (HARD) p.S1 += sums[2][w];
+    }
+    p.has_t = mine_t ? 1.f : 0.f;
+    p.ut = mine_t ? capped<CAP>(a, zt, slope_t) : 0.f;
+    p.low = low;
+    if (parts > 1) {                                          // to every block of the cluster, this one among them
+      if (lane == 0) own = p;
+      __syncwarp();
+      if (lane < parts * PART_PIECES) {
+        const int to = lane / PART_PIECES, piece = lane - to * PART_PIECES;
+        send16(in_cluster(reinterpret_cast<const uint4*>(&rec[rank]) + piece, to), reinterpret_cast<const uint4*>(&own)[piece], in_cluster(&sent, to));
+      }
+      sent_wait(&sent, 3);
+    } else {
+      if (lane == 0) rec[0] = p;
+      __syncwarp();
+    }
+    total<OP, HARD>(a, row, rec, qr, policy, rank == 0, &fin);
+  }
+  if (OP == SCORES ? !TOP : a.out == nullptr) return;
   __syncthreads();
   const Totals T = fin;
+
   if (OP == SCORES) {
-    u64 below = ~0ull;
-    for (int k = 0; k < K; ++k) {
-      u64 key = 0;
-      for (int i = tid; i < V; i += NT) {
-        const u64 v = key_of(to_float(z[i]), i);
-        if (v < below && v > key) key = v;
+    u64* taken = reinterpret_cast<u64*>(buf);
+    const bool broken = T.lS != T.lS;                         // (a thread's largest leaves NaN out)
+    u64* ours = taken + rank * room;
+    auto give = [&](float f, int token, u64 bound) {
+      const u64 key = key_of(f, token);
+      if (key < bound || token < 0 || token >= V) return;
+      const int i = atomicAdd(&found, 1);
+      if (i < room) ours[i] = key;
+    };
+    auto met = [&] {                                          // of the cluster; what was written to others' shared memory is there
+      if (parts > 1) {
+        cluster_arrive();
+        cluster_wait();
+      } else {
+        __syncthreads();
       }
-      for (int o = 16; o; o >>= 1) {
-        const u64 other = __shfl_xor_sync(~0u, key, o);
-        key = other > key ? other : key;
+    };
+    // A warp takes the threads with such tokens one by one, half a piece a lane; the pieces at the row's ends by themselves.
+    auto collect = [&](u64 bound, bool all) {
+      typedef typename std::conditional<sizeof(E) == 2, uint2, float2>::type Half;
+      const uint32_t order = static_cast<uint32_t>(bound >> 32);
+      if (warp == 0) {
+        const int edge = full == 1 && nv > 0 && lane < VE ? first_token + lane : end_full < nv && end_full >= full && lane >= 8 && lane < 8 + VE ? first_token + end_full * VE + lane - 8 : -1;
+        if (edge >= 0 && edge < V) give(to_float(z[edge]), edge, bound);
       }
+      uint32_t those = __ballot_sync(~0u, tid < busy && (all || order_of(top) >= order));
+      while (those) {
+        const int first = full + (warp << 5) + __ffs(those) - 1;
+        those &= those - 1;
+        for (int h = lane; h < 2 * ((end_full - first + NT - 1) / NT); h += 32) {
+          const int at = (first + (h >> 1) * NT) * VE + (h & 1) * (VE / 2);
+          const Half w = *reinterpret_cast<const Half*>(reinterpret_cast<const E*>(zv) + at);
+          float f[VE / 2];
+          if constexpr (sizeof(E) == 4) {
+            f[0] = w.x, f[1] = w.y;
+          } else {
+            split(Vec<E>::one(w.x), f[0], f[1]);
+            split(Vec<E>::one(w.y), f[2], f[3]);
+          }
+#pragma unroll
+          for (int e = 0; e < VE / 2; ++e) {
+            const int token = first_token + at + e;
+            if (order_of(f[e]) >= order && token != t) give(f[e], token, bound);
+          }
+        }
+      }
+      // (the given token is not among the threads' largest)
+      if (tid == 0 && mine_t && piece_t >= full && piece_t < end_full) give(zt, static_cast<int>(t), bound);
       __syncthreads();
-      if ((tid & 31) == 0) best[tid >> 5] = key;
-      __syncthreads();
-      for (int w = 0; w < NT / 32; ++w) key = best[w] > key ? best[w] : key;
-      below = key;
-      if (tid == 0) {
-        const int i = static_cast<int>(~static_cast<uint32_t>(key));
-        a.top_ids[(size_t)row * K + k] = i;
-        a.top_logprob[(size_t)row * K + k] = i == t ? T.lp : ((capped<CAP>(a, to_float(z[i])) - T.M) * a.c - T.lS) * LN2;
+      if (parts > 1) {
+        const int have = min(found, room);
+        for (int i = tid; i < have * parts; i += NT) {
+          const int to = i % parts, c = i / parts;
+          if (to != rank) put64(in_cluster(ours + c, to), ours[c]);
+        }
+      }
+      if (tid < parts) put32(in_cluster(&count[0][rank], tid), found);
+      met();
+      bool over = false;
+      for (int r = 0; r < parts; ++r) over |= count[0][r] > room;
+      return over;
+    };
+    u64 bound = static_cast<u64>(T.low) << 32;
+    bool over = collect(bound, T.low == 0 || broken);
+    if (over && parts > 1) {
+      // the blocks' tokens differ: the highest of bounds that K threads of a block each are not below
+      const uint32_t mine_low = busy >= K ? bound_of(K) : 0;
+      if (tid < parts) put32(in_cluster(&bounds[rank], tid), mine_low);
+      if (tid == 0) found = 0;
+      met();                                                  // (all have read the last counts)
+      uint32_t highest = T.low;
+      for (int r = 0; r < parts; ++r) highest = max(highest, bounds[r]);
+      bound = static_cast<u64>(highest) << 32;
+      over = collect(bound, highest == 0 || broken);
+    }
+    if (over) {
+      u64 below = 0, above = ~0ull;                           // at least K keys are not below the one, fewer not below the other
+      for (int it = 0; above - below > 1; ++it) {
+        const u64 mid = below + (above - below) / 2;
+        int c = 0;
+        for (int i = tid; i < n; i += NT) {
+          const int token = first_token + i;
+          c += token >= 0 && key_of(to_float(reinterpret_cast<const E*>(zv)[i]), token) >= mid;
+        }
+        c = static_cast<int>(block_sum<NT>(static_cast<float>(c), sh));           // (whole numbers below 2^24)
+        if (tid < parts) put32(in_cluster(&count[1 - (it & 1)][rank], tid), c);
+        met();
+        int sum = 0;
+        for (int r = 0; r < parts; ++r) sum += count[1 - (it & 1)][r];
+        if (sum >= K) below = mid;
+        else above = mid;
+        if (sum == K) break;
+      }
+      if (tid == 0) found = 0;
+      met();                                                  // (all have read the last counts)
+      bound = below;
+      collect(bound, true);
+    }
+    // eight threads to a token, one for each block's (an eighth of them where there is one block)
+    const int mine_found = count[0][rank];
+    for (int i = tid / MOST_PARTS; i < (mine_found + NT / MOST_PARTS - 1) / (NT / MOST_PARTS) * (NT / MOST_PARTS); i += NT / MOST_PARTS) {
+      const int r = tid % MOST_PARTS;
+      const bool valid = i < mine_found;
+      const u64 key = valid ? ours[i] : ~0ull;
+      int above = 0;
+      if (parts > 1) {
+        const int others = r < parts ? count[0][r] : 0;
+#pragma unroll 4
+        for (int j = 0; j < others; ++j) above += taken[r * room + j] > key;
+      } else {
+#pragma unroll 4
+        for (int j = r; j < mine_found; j += MOST_PARTS) above += ours[j] > key;
+      }
+#pragma unroll
+      for (int o = MOST_PARTS / 2; o; o >>= 1) above += __shfl_xor_sync(~0u, above, o);
+      if (valid && r == 0 && above < K) {
+        const int token = static_cast<int>(~static_cast<uint32_t>(key));
+        a.top_ids[(size_t)row * K + above] = token;
+        a.top_logprob[(size_t)row * K + above] =
+            token == t ? T.lp : ((capped<CAP>(a, logit_of(static_cast<uint32_t>(key >> 32))) - T.M) * a.c - T.lS) * LN2;
       }
     }
     return;
   }
-  if (!a.out) return;
+
   const float scale = OP == DISTILL ? a.scale : a.scale * a.inv_tau;
-  for (int i = tid; i < V; i += NT) {
-    if (named(i)) continue;
-    float slope;
-    const float u = capped<CAP>(a, to_float(z[i]), slope);
-    float v = grad_rest<OP, HARD>(a, T, u);
-    if (HARD && i == t) v -= a.ce;
-    out[i] = from_float<E>(v * slope * scale);
+  const bool bonus = OP == POLICY && T.kb != 0.f;
+  // One by one: entropy's gradient where a cap leaves -inf (elsewhere it is brought to a number that has no p log p, unless all of the row
+  // are such), and logits so large that their differences have to be formed first.
+  const bool careful = (bonus && (CAP || !(T.M > Vec<E>::LOW * 0.9f) || a.inv_tau < 0.05f)) ||
+                       (sizeof(E) == 2 && !(fabsf(T.base) * fmaxf(a.c, LOG2E) < 4096.f && fabsf(T.M) * LOG2E < 4096.f));
+  const f32x2 minus = pair(-T.base, -T.base), k0 = pair(T.k0, T.k0);
+  const float fa = OP == POLICY ? T.ka * scale : (1.f - a.ce) * a.tau * T.ka * scale, fb = T.kb * LN2 * scale;
+  const float f0 = fmaf(-T.base, a.c, T.k0), f1 = fmaf(-T.M, LOG2E, -T.h0);
+  const f32x2 ka = pair(fa, fa), kb = pair(fb, fb), kc = pair(f0, f0), kh = pair(f1, f1);
+  const f32x2 minus_m = pair(-T.M, -T.M), h0 = pair(-T.h0, -T.h0), ce = pair(a.ce * scale, a.ce * scale);
+  auto pass = [&](auto with_bonus, auto with_care) {
+    constexpr bool BONUS = decltype(with_bonus)::value, CARE = decltype(with_care)::value;
+    auto grad = [&](uint4 w) {
+      f32x2 x[P], slope[P];
+      pairs_of<E>(BONUS && !CARE ? vec_floor<E>(w) : w, x);
+      if (CAP) cap_pairs<E, true>(a, x, slope);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        f32x2 r;
+        if (CARE) {
+          float b, c;
+          split(x[i], b, c);
+          r = pair(grad_rest<OP, HARD>(a, T, b) * scale, grad_rest<OP, HARD>(a, T, c) * scale);
+        } else {
+          const f32x2 y = sizeof(E) == 2 ? fma2(x[i], cc, kc) : fma2(add2(x[i], minus), cc, k0);
+          r = mul2(exp2_2(y), BONUS ? fma2(kb, y, ka) : ka);
+          if (HARD) r = fma2(exp2_2(sizeof(E) == 2 ? fma2(x[i], l2, kh) : fma2(add2(x[i], minus_m), l2, h0)), ce, r);
+        }
+        x[i] = CAP ? mul2(r, slope[i]) : r;
+      }
+      return vec_of<E>(x);
+    };
+    auto store = [&](int v, const uint4& w) {
+      const int token = first_token + v * VE;
+      if (whole && token >= 0 && token + VE <= V) {
+        *reinterpret_cast<uint4*>(out + token) = w;
+      } else {
+        float f[VE];
+        floats_of<E>(w, f);
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          if (token + e >= 0 && token + e < V) out[token + e] = from_float<E>(f[e]);
+      }
+    };
+    for (int v0 = tid; v0 < nv; v0 += U * NT) {
+      uint4 w[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (v0 + i * NT < nv) w[i] = zv[v0 + i * NT];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (v0 + i * NT < nv) store(v0 + i * NT, grad(w[i]));
+    }
+  };
+  // (the row's named tokens have been read)
+  if (careful) pass(std::false_type(), std::true_type());
+  else if (OP == POLICY && !CAP && bonus) pass(std::true_type(), std::false_type());
+  else pass(std::false_type(), std::false_type());
+  __syncthreads();
+  if (OP == POLICY && mine_t && tid == 0) out[t] = from_float<E>(grad_taken(T, a.bonus) * slope_t * scale);
+  if (OP == DISTILL && warp == 0) {
+    write_named<E, CAP, HARD>(a, T, mine, id, q, t, scale, out);
+    if (HARD && mine_t && lane == 0 && !named_t) {
+      const float u = capped<CAP>(a, zt, slope_t);
+      out[t] = from_float<E>((grad_rest<OP, HARD>(a, T, u) - a.ce) * slope_t * scale);
+    }
   }
-  if (OP == POLICY && tid == 0) out[t] = from_float<E>(grad_taken(T, a.bonus) * slope_t * scale);
-  if (OP == DISTILL && tid < 32) write_named<E, CAP, HARD>(a, T, mine, id, q, t, scale, out);
 }
 
 // -------------------------------------------------------------------------------------------------------- launching
-constexpr int MOST_SMEM = 220 * 1024;      // a block's dynamic shared memory
-constexpr int SLICE = 33 * 1024;           // bytes of a row a block, where eight blocks are enough for that
+constexpr int MOST_SMEM = 200 * 1024;      // a block's dynamic shared memory
 
 // the kernel may ask for as much shared memory as there is; once for each device
 template <typename K>
@@ -1371,14 +1158,14 @@ bool allow(K kernel, std::atomic<unsigned long long>& done) {
   return true;
 }
 
-template <typename E, Op OP, bool TOP, bool CAP, bool HARD, int NW>
-int launch_slices(const Row& a, int parts, int slice, int room, int smem, cudaStream_t stream) {
+template <typename E, Op OP, bool TOP, bool CAP, bool HARD, int NT>
+int launch_block(const Row& a, int parts, int slice, int room, int smem, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
-  auto kernel = slice_kernel<E, OP, TOP, CAP, HARD, NW>;
-  if (!allow(kernel, done)) return -400;
+  auto kernel = row_kernel<E, OP, TOP, CAP, HARD, NT>;
+  if (smem > 40 * 1024 && !allow(kernel, done)) return -400;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(a.T) * parts);
-  config.blockDim = dim3(NW + 32);
+  config.blockDim = dim3(NT);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute cluster;
@@ -1386,36 +1173,29 @@ int launch_slices(const Row& a, int parts, int slice, int room, int smem, cudaSt
   cluster.val.clusterDim.x = parts;
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.attrs = &cluster;
-  config.numAttrs = 1;
-  // (blocks that an SM holds by their shared memory; where all begin at once there is nothing to take over)
-  const int most = 148 * std::max(1, std::min(slice_blocks<NW>(), (227 * 1024) / (smem + 4096)));
-  const int more = static_cast<long>(a.T) * parts > most;
-  return cudaLaunchKernelEx(&config, kernel, a, slice, room, more) == cudaSuccess ? 0 : -400;
+  config.numAttrs = parts > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, a, slice, room) == cudaSuccess ? 0 : -400;
 }
 
 template <typename E, Op OP, bool TOP, bool CAP, bool HARD>
 int launch_rows(const Row& a, cudaStream_t stream) {
   constexpr int VE = 16 / sizeof(E);
   const long bytes = static_cast<long>(a.V + VE - 1) * sizeof(E);
+  // few rows: more blocks to each, down to 4 KB a block
   int parts = 1;
-  while (parts < MOST_PARTS && (bytes > static_cast<long>(SLICE) * parts || (static_cast<long>(a.T) * parts < 2 * 148 && bytes > 4096l * parts))) parts *= 2;
-  const long slice = ((a.V + VE - 1 + parts - 1) / parts + VE - 1) / VE * VE, size = slice * static_cast<long>(sizeof(E));
-  // (where fewer threads than K have tokens, there are fewer than 1,024 of them and there is room for all)
-  const int room = TOP ? (a.V < 1024 ? a.V : 32 + 3 * a.K / 2) : 0;
-  const long listed = static_cast<long>(room) * parts * 8, smem = size + listed;
-  if (smem <= MOST_SMEM && static_cast<long>(a.T) * parts <= 0x7FFFFFFFl) {
-    const int s = static_cast<int>(slice), m = static_cast<int>(smem);
-    if (size <= 48 * 1024) return launch_slices<E, OP, TOP, CAP, HARD, 128>(a, parts, s, room, m, stream);
-    if (size <= 96 * 1024) return launch_slices<E, OP, TOP, CAP, HARD, 256>(a, parts, s, room, m, stream);
-    return launch_slices<E, OP, TOP, CAP, HARD, 512>(a, parts, s, room, m, stream);
-  }
-  static std::atomic<unsigned long long> done{0};
-  auto kernel = long_kernel<E, OP, CAP, HARD>;
-  const int bits = OP == DISTILL ? (a.V + 31) / 32 * 4 : 0;
-  if (bits > MOST_SMEM) return -5;
-  if (!allow(kernel, done)) return -400;
-  kernel<<<a.T, LONG_NT, bits, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? 0 : -400;
+  while (parts < MOST_PARTS && ((static_cast<long>(a.T) * parts < FEW_BLOCKS && bytes > 4096l * parts) ||
+                                (OP == DISTILL && bytes / 16 > static_cast<long>(MOST_SMEM - 64) * parts)))
+    parts *= 2;
+  if (static_cast<long>(a.T) * parts > 0x7FFFFFFFl) return -3;
+  const long slice = ((a.V + VE - 1 + parts - 1) / parts + VE - 1) / VE * VE;
+  // (where fewer threads than K have tokens, there are fewer than 2,048 of them and there is room for all)
+  const int room = TOP ? (a.V < 2048 ? a.V : 32 + 3 * a.K / 2) : 0;
+  const long smem = TOP ? static_cast<long>(room) * parts * 8 : OP == DISTILL ? (slice / VE + 15) / 16 * 16 : 0;
+  if (smem > MOST_SMEM) return -5;
+  const int s = static_cast<int>(slice), m = static_cast<int>(smem);
+  if (slice * static_cast<long>(sizeof(E)) > LONG_ROW || static_cast<long>(a.T) * parts < FEW_BLOCKS)
+    return launch_block<E, OP, TOP, CAP, HARD, 512>(a, parts, s, room, m, stream);
+  return launch_block<E, OP, TOP, CAP, HARD, 256>(a, parts, s, room, m, stream);
 }
 
 template <typename E, bool CAP>
