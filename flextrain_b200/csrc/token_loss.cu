@@ -460,9 +460,17 @@ __device__ __forceinline__ void write_named(const Row& a, const Totals& t, const
 
 
 // ---------------------------------------------------------------------------------------------- clusters and pieces
-constexpr int BATCH = 8;                   // pieces of 16 bytes that a thread asks for at once
-constexpr int LONG_ROW = 114688;           // bytes of a row from which a block has 512 threads, not 256
-constexpr int FEW_BLOCKS = 2 * 148;        // rows are cut where there are fewer
+// Pieces of 16 bytes that a thread asks for at once: 8 for the totals (4096 x 151936 scores 151 us, 172 with 4), 4 under a soft-cap, whose
+// code is long (1001 x 256000: 345 us, 366 with 8), and for the gradient (4096 x 151936: 479 us, 490 with 8, 517 with 2).
+constexpr int BATCH = 8, GRAD_BATCH = 4;
+// Bytes of a row from which a block has 512 threads and not 256, for some operators.  Alternatives: more threads give a closer bound (2048 x
+// 128256, 64 of them: 186 us, 244 with 256 threads).  Policy gradients, and soft-caps: half as many rows at a time, which the second level
+// of cache then still has when the gradient reads them again (4096 x 151936: 430 us, 480 with 256 threads; 1001 x 256000 343 and 348).
+// Scores and distillation: 256 threads, four blocks whose steps lie beside one another (scores 151 us, 187 with 512; held-out distillation
+// 2048 x 151936 113 and 158; with gradient 4096 x 128256 471 and 487).
+constexpr int LONG_ROW = 114688;
+// Rows are cut over a cluster where there are fewer blocks than two for each SM (1 x 151936 with 20 alternatives: 18 us with the host's part).
+constexpr int FEW_BLOCKS = 2 * 148;
 __device__ __forceinline__ uint32_t in_cluster(const void* p, int rank) {          // the same place in another block's shared memory
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(ftb::smem_u32(p)), "r"(rank));
@@ -621,6 +629,20 @@ __device__ __forceinline__ void floats_of(const uint4& v, float (&f)[Vec<E>::N])
 #pragma unroll
   for (int i = 0; i < Vec<E>::N / 2; ++i) split(x[i], f[2 * i], f[2 * i + 1]);
 }
+// What few pieces need lies outside the loops, whose instructions are read from a cache as well.
+__device__ __noinline__ f32x2 cap_far(float inv_cap, float cap, f32x2 z, f32x2& slope) {
+  float c, d, sc, sd;
+  split(z, c, d);
+  const float tc = tanh_of(c * inv_cap, sc), td = tanh_of(d * inv_cap, sd);
+  slope = pair(sc, sd);
+  return pair(c == -INFINITY ? c : cap * tc, d == -INFINITY ? d : cap * td);        // (as capped)
+}
+// sum of e log2 e of a pair, nothing where e is nothing
+__device__ __noinline__ float careful_part(f32x2 y) {
+  float b, c;
+  split(y, b, c);
+  return ex2(b) * max_nan(b, -256.f) + ex2(c) * max_nan(c, -256.f);
+}
 // z to u in place, and the slopes; the tanh of all pairs near zero by its polynomial, of any beyond it one by one
 template <typename E, bool SLOPE>
 __device__ __forceinline__ void cap_pairs(const Row& a, f32x2 (&x)[Vec<E>::N / 2], f32x2 (&slope)[Vec<E>::N / 2]) {
@@ -651,12 +673,9 @@ __device__ __forceinline__ void cap_pairs(const Row& a, f32x2 (&x)[Vec<E>::N / 2
   } else {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      float c, d, sc, sd;
-      split(x[i], c, d);
-      c = capped<true>(a, c, sc);
-      d = capped<true>(a, d, sd);
-      x[i] = pair(c, d);
-      if (SLOPE) slope[i] = pair(sc, sd);
+      f32x2 far;
+      x[i] = cap_far(a.inv_cap, a.cap, x[i], far);
+      if (SLOPE) slope[i] = far;
     }
   }
 }
@@ -676,9 +695,17 @@ __device__ __forceinline__ float logit_of(uint32_t order) {
 // numbers that are in the order of the floats); every block gives the tokens from the lowest of the blocks' bounds on to all, and ranks
 // its own among them.  Where these are too many because the blocks' tokens differ, the bound is the highest of bounds by K threads of a
 // block; where thousands of logits are equal, the cluster halves the interval of (logit, index) of all tokens until exactly K are left.
+//
+// What bounds it (B200, 16-bit logits, device-timed, calls one behind the other): scores by memory, 151 us for 142 at 4096 x 151936 with a
+// quarter of the rows left out (6.2 of 6.55 TB/s); with the gradient by the second reading, whose rows the cache has lost in part (policy
+// gradients 430 us for 332: 6 TB/s with what is read twice), and with cross entropy at another temperature beside it by the exponentials,
+// four an element (distillation 471 us for 281).  Tried: rows in the shared memory of clusters of eight, each block a piece that stays for
+// the gradient, with clusters that take over rows of others (policy gradients 427 us, but scores 206 and distillation 631: the blocks of
+// a row wait for the slowest of them at every row); pieces kept in shared memory up to 208 KB an SM (430 -> 507: what the first level of
+// cache loses was in use for loads on their way), up to 96 KB (425); three and five blocks an SM (173, 159 us of scores).
 template <typename E, Op OP, bool TOP, bool CAP, bool HARD, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, int room) {
-  constexpr int VE = Vec<E>::N, P = VE / 2, W = NT / 32, U = BATCH;
+  constexpr int VE = Vec<E>::N, P = VE / 2, W = NT / 32, U = CAP ? BATCH / 2 : BATCH, GU = GRAD_BATCH;
   extern __shared__ __align__(16) unsigned char buf[];        // DISTILL: for each piece which of its tokens are named; TOP: tokens given
   __shared__ __align__(8) uint64_t sent;
   __shared__ int found;
@@ -689,6 +716,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, in
   __shared__ uint32_t bounds[MOST_PARTS];
   __shared__ int id[OP == DISTILL ? MOST_TOP : 1];
   __shared__ float q[OP == DISTILL ? MOST_TOP : 1];
+  __shared__ Named names[OP == DISTILL ? 32 : 1];
 
   int rank, parts;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -737,8 +765,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, in
   }
   float qr = 0.f;
   bool named_t = false;
-  Named mine;
   if (OP == DISTILL) {
+    Named mine;
     for (int i = tid; i < (nv + 15) / 16; i += NT) reinterpret_cast<uint4*>(buf)[i] = make_uint4(0, 0, 0, 0);
     if (warp == 0) qr = teacher_of(a, row, t, id, q, mine, named_t);
     __syncthreads();
@@ -753,6 +781,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, in
         const uint32_t bit = 1u << ((v & 3) * 8 + at % VE);
         mine.first[j] = !(atomicOr(reinterpret_cast<uint32_t*>(buf) + (v >> 2), bit) & bit);      // (of entries of one token, one stands for all)
       }
+      names[lane] = mine;
     }
     __syncthreads();
   }
@@ -811,35 +840,44 @@ __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, in
       split(part, b, c);
       b += c;
       if (b != b) {                                           // (a logit of -inf: nothing times minus infinity)
-        float f[VE];
-        floats_of<E>(w, f);
         b = 0.f;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          const float y = (capped<CAP>(a, f[e]) - base) * a.c;
-          b += ex2(y) * max_nan(y, -256.f);
-        }
+        for (int i = 0; i < P; ++i) b += careful_part(mul2(add2(x[i], minus), cc));
       }
       A += b;
     }
   };
-  for (int v0 = full + tid; v0 < end_full; v0 += U * NT) {
+  // (piece_t is looked for once in U pieces, by the thread that has it)
+  const int piece_mine = piece_t >= full && (piece_t - full) % NT == tid ? piece_t : -1;
+  auto batch = [&](int v0, int most_v) {                      // pieces v0, v0 + NT, ... up to U of them, below most_v
+    const uint4* at = zv + v0;
     uint4 w[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (v0 + i * NT < end_full) w[i] = zv[v0 + i * NT];
-    uint32_t m2 = Vec<E>::NONE;
+    for (int i = 0; i < U; ++i) w[i] = i == 0 || v0 + i * NT < most_v ? at[i * NT] : make_uint4(Vec<E>::NONE, Vec<E>::NONE, Vec<E>::NONE, Vec<E>::NONE);
+    if (OP == DISTILL) {
 #pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (v0 + i * NT < end_full) {
-        const uint32_t struck = struck_in(v0 + i * NT);
-        if (struck) strike(w[i], struck);
-        m2 = Vec<E>::max2(m2, vec_max<E>(w[i]));
-      }
+      for (int i = 0; i < U; ++i)
+        if (i == 0 || v0 + i * NT < most_v) {
+          const uint32_t struck = buf[v0 + i * NT];
+          if (struck) strike(w[i], struck);
+        }
+    } else if (static_cast<unsigned>(piece_mine - v0) < static_cast<unsigned>(U * NT)) {
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (v0 + i * NT == piece_mine) strike(w[i], 1u << (at_t % VE));
+    }
+    uint32_t m2 = vec_max<E>(w[0]);
+#pragma unroll
+    for (int i = 1; i < U; ++i) m2 = Vec<E>::max2(m2, vec_max<E>(w[i]));
     raise(Vec<E>::top(m2));
 #pragma unroll
     for (int i = 0; i < U; ++i)
-      if (v0 + i * NT < end_full) add(w[i]);
+      if (i == 0 || v0 + i * NT < most_v) add(w[i]);
+  };
+  {
+    int v0 = full + tid;
+    for (; v0 + (U - 1) * NT < end_full; v0 += U * NT) batch(v0, 0x7FFFFFFF);
+    if (v0 < end_full) batch(v0, end_full);
   }
   // the pieces with others in them: the first by thread 0, the last by the last thread
   auto edge = [&](int v) {
@@ -918,7 +956,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, in
   if (warp == 0) {
     Part p = {};
     p.B = -INFINITY;
-    if (OP == DISTILL) named_part<CAP, HARD>(a, mine, p);
+    if (OP == DISTILL) named_part<CAP, HARD>(a, names[lane], p);
     p.m = um;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
@@ -1108,8 +1146,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, in
     };
     auto store = [&](int v, const uint4& w) {
       const int token = first_token + v * VE;
-      if (whole && token >= 0 && token + VE <= V) {
-        *reinterpret_cast<uint4*>(out + token) = w;
+      if (whole && v >= full && v < end_full) {
+        __stcs(reinterpret_cast<uint4*>(out + token), w);
       } else {
         float f[VE];
         floats_of<E>(w, f);
@@ -1118,15 +1156,21 @@ __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, in
           if (token + e >= 0 && token + e < V) out[token + e] = from_float<E>(f[e]);
       }
     };
-    for (int v0 = tid; v0 < nv; v0 += U * NT) {
-      uint4 w[U];
+    auto batch = [&](int v0, int most_v) {
+      const uint4* at = zv + v0;
+      uint4 w[GU];
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (v0 + i * NT < nv) w[i] = zv[v0 + i * NT];
+      for (int i = 0; i < GU; ++i)
+        if (i == 0 || v0 + i * NT < most_v) w[i] = __ldcs(at + i * NT);
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (v0 + i * NT < nv) store(v0 + i * NT, grad(w[i]));
-    }
+      for (int i = 0; i < GU; ++i)
+        if (i == 0 || v0 + i * NT < most_v) store(v0 + i * NT, grad(w[i]));
+    };
+    int v0 = full + tid;
+    for (; v0 + (GU - 1) * NT < end_full; v0 += GU * NT) batch(v0, 0x7FFFFFFF);
+    if (v0 < end_full) batch(v0, end_full);
+    if (tid == 0 && full == 1 && nv > 0) store(0, grad(zv[0]));
+    if (tid == NT - 1 && end_full < nv && end_full >= full) store(end_full, grad(zv[end_full]));
   };
   // (the row's named tokens have been read)
   if (careful) pass(std::false_type(), std::true_type());
@@ -1135,7 +1179,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, in
   __syncthreads();
   if (OP == POLICY && mine_t && tid == 0) out[t] = from_float<E>(grad_taken(T, a.bonus) * slope_t * scale);
   if (OP == DISTILL && warp == 0) {
-    write_named<E, CAP, HARD>(a, T, mine, id, q, t, scale, out);
+    write_named<E, CAP, HARD>(a, T, names[lane], id, q, t, scale, out);
     if (HARD && mine_t && lane == 0 && !named_t) {
       const float u = capped<CAP>(a, zt, slope_t);
       out[t] = from_float<E>((grad_rest<OP, HARD>(a, T, u) - a.ce) * slope_t * scale);
@@ -1193,7 +1237,7 @@ int launch_rows(const Row& a, cudaStream_t stream) {
   const long smem = TOP ? static_cast<long>(room) * parts * 8 : OP == DISTILL ? (slice / VE + 15) / 16 * 16 : 0;
   if (smem > MOST_SMEM) return -5;
   const int s = static_cast<int>(slice), m = static_cast<int>(smem);
-  if (slice * static_cast<long>(sizeof(E)) > LONG_ROW || static_cast<long>(a.T) * parts < FEW_BLOCKS)
+  if ((TOP || CAP || (OP == POLICY && a.out != nullptr)) && slice * static_cast<long>(sizeof(E)) > LONG_ROW)
     return launch_block<E, OP, TOP, CAP, HARD, 512>(a, parts, s, room, m, stream);
   return launch_block<E, OP, TOP, CAP, HARD, 256>(a, parts, s, room, m, stream);
 }
@@ -1233,7 +1277,8 @@ int run_rows(Op op, const RowArgs* r) {
 //   dz_j = (scale / tau) u'(z_j) [ -p_j (sum of the gradients of log p_t and of the alternatives + dH (log p_j + H)) + the gradients of j's own ]
 //
 // One pass, nothing between the tokens of a row: blocks of 256 threads take 1,024 pieces of 16 bytes, four a thread that are all asked for
-// before the first is used.  The tokens with gradients of their own are written again behind the others of their block.
+// before the first is used.  The tokens with gradients of their own are written again behind the others of their block.  Bound by memory:
+// 2048 x 128256 bf16 with a quarter of the rows left out 166 us (5.5 of 6.55 TB/s).
 constexpr int GRAD_NT = 256, GRAD_EACH = 4;
 template <typename E, bool CAP>
 __global__ void __launch_bounds__(GRAD_NT) grad_kernel(Row a, const float* lse, const float* dlogprob, const float* dentropy, const float* dtop, int blocks) {

@@ -239,3 +239,46 @@ def test_few_rows_count(live):
     out.fill_(3.0)
     ops.distill_loss_(z, t.clamp(min=0)[:, None], torch.zeros(T, 1, device="cuda"), targets=t, out=out)
     assert bool((out[: T - live] == 0).all()) and bool((out[T - live:].abs().sum(-1) > 0).all())
+
+
+def test_grpo_loss_takes_the_kernel():
+    """GRPOLoss: no mask but -100, the logits as they are; its values and gradient against the definition."""
+    from flextrain_b200.nn.loss import GRPOLoss, TokenSlice
+    from token_loss_oracle import near, near_grad, on_rows, policy
+    T, V = 12, 3001
+    z = wide(T, V, BF16, "cuda")[1].clone()
+    t = some_targets(T, V - 1, "cuda")
+    t[3] = -100
+    adv, ref = torch.linspace(-2, 2, T, device="cuda"), torch.linspace(-9, -7, T, device="cuda")
+    on = on_rows(T, V, t, None, device="cuda")
+    (loss, _, _), want, size = policy(z, t, on, 1.0, 0.0, adv, None, ref, 0.2, 0.2, 0.1, 0.0, 0.5)
+    logits = z.clone()
+    got = GRPOLoss(kl_beta=0.1)(z, TokenSlice(t, torch.zeros(T, device="cuda"), adv, ref), 0.5, 30.0)
+    # the penalty's e^d (d of up to 6 here: 400) multiplies the log probability's error
+    near(got, loss, V, factor=400.0)
+    near_grad(z, want, size, logits)
+
+
+def test_score_and_losses_through_the_engine():
+    """A bf16 model on the GPU: scores equal those of its own logits; distillation from itself is near nothing; a policy step runs."""
+    import flextrain_b200 as ft
+    from conftest import TINY_DIMS, build_tiny
+    from flextrain_b200.nn.loss import DistillationLoss, PolicyLoss
+    am = build_tiny(dims=TINY_DIMS, device="cuda", dtype=BF16)
+    g = torch.Generator().manual_seed(0)
+    seqs = []
+    for n in (100, 37, 64):
+        toks = torch.randint(0, 1024, (n,), generator=g)
+        tgt = torch.roll(toks, -1)
+        tgt[-1] = -100
+        seqs.append(ft.Sequence(toks, targets=tgt, seq_id=n))
+    scores = am.score(seqs, top_k=1024 if False else 128)
+    for s, x in zip(seqs, scores):
+        assert x.logprobs.shape == (len(s),) and x.top_ids.shape == (len(s), 128) and x.logprobs[-1] == 0
+        assert bool((x.logprobs[:-1] < 0).all()) and bool((x.entropy[:-1] <= 6.9315).all())
+        s.old_logprobs, s.teacher_ids, s.teacher_logprobs, s.advantages = x.logprobs, x.top_ids, x.top_logprobs, torch.ones(len(s))
+    # against itself: KL of equal distributions, terms of up to 13 that cancel (near(): 13 (40 + 8) 2^-24 = 4e-5 a position)
+    assert abs(am.evaluate(seqs, loss_fn=DistillationLoss(rest="bucket")).loss_sum) < 4e-5 * 198
+    st = am.fwd_bwd(seqs, loss_fn=PolicyLoss(kl_coef=0.1, entropy_coef=0.01))
+    am.step()
+    assert st.active_tokens == 198 and torch.isfinite(torch.tensor(st.loss_sum))

@@ -284,11 +284,12 @@ def check_policy(T, V, dtype, device, tau=1.0, cap=0.0, gap=0, shift=0, apart=Tr
     assert torch.equal(z, logits)
     out_buf, out = wide(T, V, dtype, device, gap + 3, shift + 1) if apart else (buf, z)
     got = ops.policy_loss_(z, t, a, grad_scale=0.125, out=out if apart else None, **kw)
-    assert all(torch.equal(x, y) for x, y in zip(got, alone))
-    # an advantage of up to 4 and a ratio of up to 4 multiply the log probability's error
-    near(got.loss, loss, V, cap / tau, factor=20.0)
-    near(got.logprobs, given, V, cap / tau)
-    near(got.entropy, ent, V, cap / tau, size=3.0)
+    # (the two may sum a row's terms in other groups: each is held to the definition)
+    for terms in (got, alone):
+        # an advantage of up to 4 and a ratio of up to 4 multiply the log probability's error
+        near(terms.loss, loss, V, cap / tau, factor=20.0)
+        near(terms.logprobs, given, V, cap / tau)
+        near(terms.entropy, ent, V, cap / tau, size=3.0)
     near_grad(out, want, size, logits, cap)
     untouched(out_buf, shift + (1 if apart else 0), V)
 
@@ -308,9 +309,9 @@ def check_distill(T, V, dtype, device, K=4, tau=1.0, cap=0.0, rest="drop", ce=0.
     assert torch.equal(z, logits)
     out_buf, out = wide(T, V, dtype, device, gap + 3, shift + 1) if apart else (buf, z)
     got = ops.distill_loss_(z, ids, teacher, grad_scale=0.125, out=out if apart else None, **kw)
-    assert torch.equal(got, alone)
     # sum q (log q - log p): terms of up to 12, times the temperature's square
-    near(got, loss, V, cap / tau, factor=max(1.0, tau * tau), size=12.0)
+    for value in (got, alone):
+        near(value, loss, V, cap / tau, factor=max(1.0, tau * tau), size=12.0)
     near_grad(out, want, size, logits, cap)
     untouched(out_buf, shift + (1 if apart else 0), V)
 
