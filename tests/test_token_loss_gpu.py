@@ -272,7 +272,7 @@ def test_score_and_losses_through_the_engine():
         tgt = torch.roll(toks, -1)
         tgt[-1] = -100
         seqs.append(ft.Sequence(toks, targets=tgt, seq_id=n))
-    scores = am.score(seqs, top_k=1024 if False else 128)
+    scores = am.score(seqs, top_k=128)
     for s, x in zip(seqs, scores):
         assert x.logprobs.shape == (len(s),) and x.top_ids.shape == (len(s), 128) and x.logprobs[-1] == 0
         assert bool((x.logprobs[:-1] < 0).all()) and bool((x.entropy[:-1] <= 6.9315).all())
