@@ -193,7 +193,7 @@ class DistillationLoss(_NativeLoss):
         self.options = dict(rest=rest, ce_weight=float(ce_weight), temperature=float(temperature), ignore_index=int(ignore_index))
 
     def check_sequences(self, seqs) -> None:
-        if not any(s.teacher_ids is not None for s in seqs):
+        if seqs and not any(s.teacher_ids is not None for s in seqs):      # (a rank without sequences takes part all the same)
             raise ValueError("DistillationLoss: no sequence carries teacher_ids and teacher_logprobs")
 
     def _given(self, logits, sl: TokenSlice, softcap: float):

@@ -392,7 +392,7 @@ def distill_loss(logits, ids, teacher, targets, on, bucket, ce_weight, temperatu
     q = t.exp()
     known = torch.zeros(logits.shape[0], V + 1, dtype=torch.bool, device=logits.device)
     known = known.scatter_(1, torch.where(inside, ids, V), True)[:, :V]
-    kl = torch.where(q > 0, q * (t - logp.gather(1, at)), 0.0).sum(-1)
+    kl = torch.where(q != 0, q * (t - logp.gather(1, at)), 0.0).sum(-1)
     share = q.sum(-1)
     if bucket:
         others = logp.masked_fill(known, float("-inf"))
