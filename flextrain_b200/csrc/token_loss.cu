@@ -698,8 +698,8 @@ __device__ __forceinline__ float logit_of(uint32_t order) {
 //
 // What bounds it (B200, 16-bit logits, device-timed, calls one behind the other): scores by memory, 151 us for 142 at 4096 x 151936 with a
 // quarter of the rows left out (6.2 of 6.55 TB/s); with the gradient by the second reading, whose rows the cache has lost in part (policy
-// gradients 430 us for 332: 6 TB/s with what is read twice), and with cross entropy at another temperature beside it by the exponentials,
-// four an element (distillation 471 us for 281).  Tried: rows in the shared memory of clusters of eight, each block a piece that stays for
+// gradients 411 us for 332; it goes through the row from its end, 423 from its beginning), and with cross entropy at another temperature beside it by the exponentials,
+// four an element (distillation 452 us for 281).  Tried: rows in the shared memory of clusters of eight, each block a piece that stays for
 // the gradient, with clusters that take over rows of others (policy gradients 427 us, but scores 206 and distillation 631: the blocks of
 // a row wait for the slowest of them at every row); pieces kept in shared memory up to 208 KB an SM (430 -> 507: what the first level of
 // cache loses was in use for loads on their way), up to 96 KB (425); three and five blocks an SM (173, 159 us of scores).
@@ -1166,9 +1166,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, in
       for (int i = 0; i < GU; ++i)
         if (i == 0 || v0 + i * NT < most_v) store(v0 + i * NT, grad(w[i]));
     };
-    int v0 = full + tid;
-    for (; v0 + (GU - 1) * NT < end_full; v0 += GU * NT) batch(v0, 0x7FFFFFFF);
+    // (from the row's end: what was read last is still in the cache)
+    const int whole_batches = max(0, (end_full - full - tid + NT - 1) / NT) / GU;
+    int v0 = full + tid + whole_batches * GU * NT;
     if (v0 < end_full) batch(v0, end_full);
+    for (v0 -= GU * NT; v0 >= full; v0 -= GU * NT) batch(v0, 0x7FFFFFFF);
     if (tid == 0 && full == 1 && nv > 0) store(0, grad(zv[0]));
     if (tid == NT - 1 && end_full < nv && end_full >= full) store(end_full, grad(zv[end_full]));
   };
