@@ -329,17 +329,17 @@ class ActiveModel:
         for s in {id(s): s for rseqs, _, _ in pending for s in rseqs}.values():
             s.scores = None
         for rseqs, meta, scores in pending:
-            if self.tp is not None:
-                scores = scores._make(None if t is None else self.tp.all_gather(t) for t in scores)
-            host = scores._make(None if t is None else t.to("cpu") for t in scores)
+            # (one field after the other: a gather over peer memory lies in a staging buffer that the next of its size writes over)
+            whole = (lambda t: t) if self.tp is None else self.tp.all_gather
+            host = scores._make(None if t is None else whole(t).to("cpu", copy=True) for t in scores)
             off = 0
             for i, start, n in meta.extra["pieces"]:
                 s = rseqs[i]
                 if s.scores is None:
                     s.scores = host._make(None if t is None else torch.zeros(len(s), *t.shape[1:], dtype=t.dtype) for t in host)
-                for whole, part in zip(s.scores, host):
-                    if whole is not None:
-                        whole[start:start + n] = part[off:off + n]
+                for mine, part in zip(s.scores, host):
+                    if mine is not None:
+                        mine[start:start + n] = part[off:off + n]
                 off += n
 
     def _fold_tied_head_grad(self) -> None:

@@ -1,0 +1,59 @@
+"""Operators on token probabilities on the CPU: scores behind a tensor-parallel gather, and what else a later look at them found."""
+import json
+import os
+import socket
+import subprocess
+import sys
+import types
+
+import torch
+
+from flextrain_b200.engine.active_model import ActiveModel
+from flextrain_b200.io.sequence import Sequence
+from flextrain_b200.ops import TokenLogprobs
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+class StagedGather:
+    """A tensor-parallel group of two equal halves whose results lie in one staging buffer for each size, as those over peer memory do:
+    the next gather of the same size writes over the last."""
+
+    def __init__(self):
+        self.stage = {}
+
+    def all_gather(self, t):
+        raw = torch.cat([t, t]).contiguous()
+        stage = self.stage.setdefault(raw.numel() * raw.element_size(), torch.empty(raw.numel() * raw.element_size(), dtype=torch.uint8))
+        stage.copy_(raw.view(-1).view(torch.uint8))
+        return stage.view(raw.dtype).view(raw.shape)
+
+
+def test_scores_gathered_through_one_staging_buffer():
+    """Every field of a score comes back as itself, also those of one size (with one alternative all four fp32 fields are)."""
+    n = 8
+    for K in (1, 3):
+        half = TokenLogprobs(*(torch.arange(n // 2, dtype=F32) + 10 * i for i in (1, 2, 3)), torch.arange(n // 2 * K).view(-1, K),
+                             torch.arange(n // 2 * K, dtype=F32).view(-1, K) + 40)
+        s = Sequence(torch.zeros(n, dtype=torch.int64))
+        meta = types.SimpleNamespace(extra={"pieces": [(0, 0, n)]})
+        ActiveModel._write_back_scores(types.SimpleNamespace(tp=StagedGather()), [([s], meta, half)])
+        for got, want in zip(s.scores, half):
+            assert torch.equal(got, torch.cat([want, want]))
+
+
+def test_scores_and_their_losses_under_tensor_parallelism(tmp_path):
+    """Two ranks, staged gathers: scores of ragged sequences, and losses of what sequences carry for each position, as unsharded.  Both
+    sides sum fp32 products of two layers in other orders; a swapped field, or a shard's values at another's positions, is off by units.
+    (Alternatives of nearly equal logits may change places: a few of them in a thousand.)"""
+    s = socket.socket()
+    s.bind(("127.0.0.1", 0))
+    port = s.getsockname()[1]
+    s.close()
+    out = str(tmp_path / "scores.json")
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=2", "--master-addr", "127.0.0.1", "--master-port", str(port),
+           os.path.join(os.path.dirname(os.path.abspath(__file__)), "tp_score_worker.py"), out]
+    r = subprocess.run(cmd, capture_output=True, text=True, timeout=900)
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-3000:]
+    res = json.load(open(out))
+    assert res["fields"] == 9 * (5 + 5 + 2) and res["worst"] < 1e-4 and res["ids"] <= res["ids_of"] // 200, res
