@@ -188,8 +188,6 @@ class ActiveModel:
                     ids.dim() != 2 or ids.shape != lps.shape or ids.is_floating_point() or not 1 <= ids.shape[1] <= MOST_TOP):
                 raise ValueError(f"sequence {s.seq_id}: teacher_ids {None if ids is None else (tuple(ids.shape), ids.dtype)} and teacher_logprobs "
                                  f"{None if lps is None else tuple(lps.shape)}; (tokens, K) of each, K of 1 to {MOST_TOP}")
-        if len({s.old_logprobs is None for s in seqs}) > 1:
-            raise ValueError("some sequences of the step carry old_logprobs and some do not")
 
     def _fwd_bwd(self, seqs, loss_scale_factor, total_tokens_per_step, loss_fn, forward_only, t0) -> StepStats:
         ws = self.ws

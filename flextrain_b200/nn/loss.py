@@ -172,6 +172,11 @@ class PolicyLoss(_NativeLoss):
         self.options = dict(clip_low=float(clip_low), clip_high=None if clip_high is None else float(clip_high), kl_beta=float(kl_coef),
                             entropy_coef=float(entropy_coef), temperature=float(temperature), ignore_index=int(ignore_index))
 
+    def check_sequences(self, seqs) -> None:
+        """What only some of a call's sequences carry would be zeros for the others."""
+        if len({s.old_logprobs is None for s in seqs}) > 1:
+            raise ValueError("PolicyLoss: some sequences of the step carry old_logprobs and some do not")
+
     def _given(self, sl: TokenSlice, softcap: float):
         ref = sl.ref_logprobs if sl.ref_logprobs is not None else sl.extra.get("ref_logprobs")
         return dict(old_logprobs=sl.extra.get("old_logprobs"), ref_logprobs=ref, softcap=softcap, loss_mask=sl.loss_mask, **self.options)

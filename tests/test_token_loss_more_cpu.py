@@ -6,13 +6,18 @@ import subprocess
 import sys
 import types
 
+import pytest
 import torch
 
+from conftest import build_tiny
 from flextrain_b200.engine.active_model import ActiveModel
 from flextrain_b200.io.sequence import Sequence
+from flextrain_b200.nn.loss import CrossEntropyLoss, GRPOLoss, PolicyLoss
 from flextrain_b200.ops import TokenLogprobs
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+DIMS = dict(vocab_size=256, n_layers=2, d_model=64, n_heads=4, n_kv_heads=2, head_dim=16, expert_dim=128, ffn_dim=128, num_routed_experts=0,
+            num_shared_experts=0, top_k=0, is_causal=True)
 
 
 class StagedGather:
@@ -57,3 +62,27 @@ def test_scores_and_their_losses_under_tensor_parallelism(tmp_path):
     assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-3000:]
     res = json.load(open(out))
     assert res["fields"] == 9 * (5 + 5 + 2) and res["worst"] < 1e-4 and res["ids"] <= res["ids_of"] // 200, res
+
+
+def _sequences(n=3, length=20):
+    g = torch.Generator().manual_seed(0)
+    out = []
+    for i in range(n):
+        t = torch.randint(0, 256, (length,), generator=g)
+        tgt = torch.roll(t, -1)
+        tgt[-1] = -100
+        out.append(Sequence(t, targets=tgt, seq_id=i))
+    return out
+
+
+def test_what_only_some_sequences_carry_is_refused_by_the_losses_that_read_it():
+    """Old log probabilities of some sequences only are refused by PolicyLoss, and by nothing that does not read them."""
+    am, seqs = build_tiny(dims=DIMS, max_seq_len=64, batch_tokens=96), _sequences()
+    for s, x in zip(seqs[:2], am.score(seqs)):
+        s.old_logprobs = x.logprobs
+    with pytest.raises(ValueError, match="old_logprobs"):
+        am.fwd_bwd(seqs, loss_fn=PolicyLoss())
+    assert am.fwd_bwd_serial == 0
+    assert am.score(seqs)[2].logprobs[0] < 0
+    assert am.evaluate(seqs).loss_sum > 0 and am.evaluate(seqs, loss_fn=GRPOLoss()).loss_sum > 0
+    am.fwd_bwd(seqs, loss_fn=CrossEntropyLoss())
