@@ -176,6 +176,8 @@ class PolicyLoss(_NativeLoss):
         """What only some of a call's sequences carry would be zeros for the others."""
         if len({s.old_logprobs is None for s in seqs}) > 1:
             raise ValueError("PolicyLoss: some sequences of the step carry old_logprobs and some do not")
+        if self.options["kl_beta"] != 0.0 and len({s.ref_logprobs is None for s in seqs}) > 1:
+            raise ValueError("PolicyLoss: some sequences of the step carry ref_logprobs and some do not")
 
     def _given(self, sl: TokenSlice, softcap: float):
         ref = sl.ref_logprobs if sl.ref_logprobs is not None else sl.extra.get("ref_logprobs")

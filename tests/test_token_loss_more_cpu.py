@@ -86,3 +86,16 @@ def test_what_only_some_sequences_carry_is_refused_by_the_losses_that_read_it():
     assert am.score(seqs)[2].logprobs[0] < 0
     assert am.evaluate(seqs).loss_sum > 0 and am.evaluate(seqs, loss_fn=GRPOLoss()).loss_sum > 0
     am.fwd_bwd(seqs, loss_fn=CrossEntropyLoss())
+
+
+def test_a_reference_of_some_sequences_only():
+    """With a penalty a mixture is refused: zeros in its place would be a penalty of e^(-logp); without one nothing reads it."""
+    am, seqs = build_tiny(dims=DIMS, max_seq_len=64, batch_tokens=96), _sequences()
+    for s in seqs:
+        s.advantages = torch.zeros(len(s))
+    seqs[0].ref_logprobs = am.score(seqs)[0].logprobs
+    for call in (am.evaluate, am.fwd_bwd):
+        with pytest.raises(ValueError, match="ref_logprobs"):
+            call(seqs, loss_fn=PolicyLoss(kl_coef=0.1))
+    assert am.evaluate(seqs, loss_fn=PolicyLoss()).loss_sum == 0
+    assert abs(am.evaluate(seqs[:1], loss_fn=PolicyLoss(kl_coef=0.1)).loss_sum) < 1e-6 and am.evaluate(seqs[1:], loss_fn=PolicyLoss(kl_coef=0.1)).loss_sum == 0
