@@ -151,12 +151,8 @@ class ActiveModel:
             return self._fwd_bwd(seqs, loss_scale_factor, total_tokens_per_step, loss_fn, forward_only, t0)
         finally:
             self.verbose = was_verbose
-            for mine, theirs in zip(seqs, given):              # per-token losses go back to the caller's own objects
-                if mine is not theirs and mine.per_token_loss is not None:
-                    try:
-                        theirs.per_token_loss = mine.per_token_loss
-                    except AttributeError:
-                        pass
+            for mine, theirs in zip(seqs, given):
+                self._hand_back(mine, theirs, "per_token_loss")
 
     def _check_sequences(self, seqs) -> None:
         """Host-side checks of what would otherwise be an out-of-range access on the device: a sequence longer than the
@@ -316,12 +312,24 @@ class ActiveModel:
         ``logprobs`` are what ``Sequence.old_logprobs`` and ``ref_logprobs`` hold, its ``top_ids`` and ``top_logprobs`` what a student's
         ``teacher_ids`` and ``teacher_logprobs`` do (at the same temperature).  Positions without a target or masked are zero.  The
         per-token losses written back are the negative log probabilities."""
-        given = list(seqs)
-        mine = [as_sequence(s) for s in given]
         if not 0 <= top_k <= min(MOST_TOP, int(self.embed.vocab_size)) or not 0.0 < temperature < float("inf"):
             raise ValueError(f"score: top_k {top_k} (0 to {min(MOST_TOP, int(self.embed.vocab_size))}), temperature {temperature} (above zero)")
+        given = list(seqs)
+        mine = [as_sequence(s) for s in given]
         self.fwd_bwd(mine, loss_scale_factor=1.0, loss_fn=TokenScorer(top_k, temperature), forward_only=True)
+        for s, theirs in zip(mine, given):
+            self._hand_back(s, theirs, "scores", "per_token_loss")
         return [s.scores for s in mine]
+
+    @staticmethod
+    def _hand_back(mine, theirs, *names) -> None:
+        """What the engine left in a sequence, for the caller's own object that it stands for."""
+        for name in names:
+            if mine is not theirs and getattr(mine, name) is not None:
+                try:
+                    setattr(theirs, name, getattr(mine, name))
+                except AttributeError:
+                    pass
 
     def _write_back_scores(self, pending) -> None:
         for s in {id(s): s for rseqs, _, _ in pending for s in rseqs}.values():

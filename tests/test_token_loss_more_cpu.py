@@ -99,3 +99,25 @@ def test_a_reference_of_some_sequences_only():
             call(seqs, loss_fn=PolicyLoss(kl_coef=0.1))
     assert am.evaluate(seqs, loss_fn=PolicyLoss()).loss_sum == 0
     assert abs(am.evaluate(seqs[:1], loss_fn=PolicyLoss(kl_coef=0.1)).loss_sum) < 1e-6 and am.evaluate(seqs[1:], loss_fn=PolicyLoss(kl_coef=0.1)).loss_sum == 0
+
+
+def test_scores_are_left_in_the_callers_own_objects():
+    """Sequences of one's own class: ``scores`` and ``per_token_loss`` arrive as with a Sequence; a class that refuses them is no error."""
+    am, seqs = build_tiny(dims=DIMS, max_seq_len=64, batch_tokens=96), _sequences()
+
+    class Bare:
+        def __init__(self, s):
+            self.tokens, self.targets = s.tokens, s.targets
+
+    class Closed:
+        __slots__ = ("tokens", "targets")
+
+        def __init__(self, s):
+            self.tokens, self.targets = s.tokens, s.targets
+
+    mine, closed = [Bare(s) for s in seqs[:2]], Closed(seqs[2])
+    got = am.score(mine + [closed], top_k=2)
+    for s, x, given in zip(seqs, am.score(seqs, top_k=2), got):
+        assert torch.equal(x.logprobs, given.logprobs) and torch.equal(x.top_ids, given.top_ids)
+    for s, x, given in zip(mine, got, seqs):
+        assert s.scores is x and torch.equal(s.per_token_loss, given.per_token_loss)
