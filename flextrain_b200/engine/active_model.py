@@ -250,6 +250,8 @@ class ActiveModel:
                                 pending_scores.append((rseqs, meta, loss_fn.take()))
                     if forward_only:
                         self.streams.synchronize_all()      # saved activations are dropped: let their copies finish
+                        self._write_back_scores(pending_scores)
+                        pending_scores = []
                     else:
                         with _nvtx("Backward"):
                             self._backward_pass(metas, plan, transitions, slots, ctx_base, stats, last_round)
@@ -269,7 +271,6 @@ class ActiveModel:
         stats.loss_sum = float(loss_acc)
         stats.active_tokens = int(act_acc)
         self._write_back_losses(pending_losses)
-        self._write_back_scores(pending_scores)
         if not forward_only:
             self._pending_tokens += stats.tokens
         stats.elapsed_s = time.perf_counter() - t0
@@ -332,6 +333,7 @@ class ActiveModel:
                     pass
 
     def _write_back_scores(self, pending) -> None:
+        """A round's scores into its sequences (1.5 KB a position at 128 alternatives, so no more of them stay on the device)."""
         for s in {id(s): s for rseqs, _, _ in pending for s in rseqs}.values():
             s.scores = None
         for rseqs, meta, scores in pending:

@@ -121,3 +121,16 @@ def test_scores_are_left_in_the_callers_own_objects():
         assert torch.equal(x.logprobs, given.logprobs) and torch.equal(x.top_ids, given.top_ids)
     for s, x, given in zip(mine, got, seqs):
         assert s.scores is x and torch.equal(s.per_token_loss, given.per_token_loss)
+
+
+def test_scores_leave_the_device_with_their_round(monkeypatch):
+    """What is held on the device is a round's scores at most, not a call's."""
+    am, seqs = build_tiny(dims=DIMS, max_seq_len=64, batch_tokens=48), _sequences(7)
+    held, write = [], ActiveModel._write_back_scores
+    monkeypatch.setattr(ActiveModel, "_write_back_scores", lambda self, pending: (held.append([len(r) for r, _, _ in pending]), write(self, pending)))
+    got = am.score(seqs, top_k=3)
+    held = [h for h in held if h]
+    assert len(held) > 2 and sum(h[0] for h in held) == 7
+    one_by_one = [am.score([s], top_k=3)[0] for s in seqs]
+    for x, y in zip(got, one_by_one):
+        torch.testing.assert_close(x.logprobs, y.logprobs, rtol=1e-5, atol=1e-5)
