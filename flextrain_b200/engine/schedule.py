@@ -151,8 +151,8 @@ def prepare_training_chunks(seqs: Seq[Sequence], max_chunk_size: int, device, *,
                 meta.extra["ref_logprobs"] = tail(ref, 0.0).to(dev, non_blocking=True)
         for name in ("old_logprobs", "ref_logprobs"):          # (the reference's also where there are no advantages)
             if name not in meta.extra and any(getattr(seqs[i], name) is not None for i, _, _ in plan.pieces):
-                v = torch.cat([(getattr(seqs[i], name)[st:st + n] if getattr(seqs[i], name) is not None else torch.zeros(n))
-                               for i, st, n in plan.pieces])
+                v = torch.cat([(torch.as_tensor(getattr(seqs[i], name)[st:st + n], dtype=torch.float32, device="cpu")
+                                if getattr(seqs[i], name) is not None else torch.zeros(n)) for i, st, n in plan.pieces])
                 meta.extra[name] = tail(v, 0.0).to(dev, non_blocking=True)
         K = max((seqs[i].teacher_ids.shape[1] for i, _, _ in plan.pieces if seqs[i].teacher_ids is not None), default=0)
         if K:

@@ -134,3 +134,18 @@ def test_scores_leave_the_device_with_their_round(monkeypatch):
     one_by_one = [am.score([s], top_k=3)[0] for s in seqs]
     for x, y in zip(got, one_by_one):
         torch.testing.assert_close(x.logprobs, y.logprobs, rtol=1e-5, atol=1e-5)
+
+
+def test_per_token_values_of_any_kind():
+    """Log probabilities as lists, arrays and doubles, also where the loss does not read them."""
+    am, seqs = build_tiny(dims=DIMS, max_seq_len=64, batch_tokens=96), _sequences()
+    plain = am.evaluate(seqs).loss_sum
+    values = [-torch.rand(len(s), dtype=torch.float64) - 5 for s in seqs]
+    want = None
+    for kind in (lambda v: v, lambda v: v.tolist(), lambda v: v.numpy(), lambda v: v.float()):
+        for s, v in zip(seqs, values):
+            s.ref_logprobs = s.old_logprobs = kind(v)
+        assert am.evaluate(seqs).loss_sum == plain
+        got = am.evaluate(seqs, loss_fn=PolicyLoss(kl_coef=0.1)).loss_sum
+        want = got if want is None else want
+        assert got == want
