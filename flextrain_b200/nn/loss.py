@@ -200,7 +200,10 @@ class DistillationLoss(_NativeLoss):
         self.options = dict(rest=rest, ce_weight=float(ce_weight), temperature=float(temperature), ignore_index=int(ignore_index))
 
     def check_sequences(self, seqs) -> None:
-        if seqs and not any(s.teacher_ids is not None for s in seqs):      # (a rank without sequences takes part all the same)
+        """Without a teacher's tokens anywhere there is nothing but cross entropy.  (A rank among others takes part all the same: the
+        teacher's sequences may be theirs, and they would wait for it.)"""
+        alone = not (torch.distributed.is_available() and torch.distributed.is_initialized() and torch.distributed.get_world_size() > 1)
+        if self.options["ce_weight"] == 0.0 and seqs and alone and not any(s.teacher_ids is not None for s in seqs):
             raise ValueError("DistillationLoss: no sequence carries teacher_ids and teacher_logprobs")
 
     def _given(self, logits, sl: TokenSlice, softcap: float):

@@ -12,7 +12,7 @@ import torch
 from conftest import build_tiny
 from flextrain_b200.engine.active_model import ActiveModel
 from flextrain_b200.io.sequence import Sequence
-from flextrain_b200.nn.loss import CrossEntropyLoss, GRPOLoss, PolicyLoss
+from flextrain_b200.nn.loss import CrossEntropyLoss, DistillationLoss, GRPOLoss, PolicyLoss
 from flextrain_b200.ops import TokenLogprobs
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -149,3 +149,16 @@ def test_per_token_values_of_any_kind():
         got = am.evaluate(seqs, loss_fn=PolicyLoss(kl_coef=0.1)).loss_sum
         want = got if want is None else want
         assert got == want
+
+
+def test_distillation_of_sequences_without_a_teacher(monkeypatch):
+    """With cross entropy in the mixture they have its part; without, a process by itself refuses, and a rank among others takes part
+    (others may hold the teacher's sequences, and would wait for it)."""
+    am, seqs = build_tiny(dims=DIMS, max_seq_len=64, batch_tokens=96), _sequences()
+    plain = am.evaluate(seqs).loss_sum
+    assert abs(am.evaluate(seqs, loss_fn=DistillationLoss(ce_weight=0.25)).loss_sum - 0.25 * plain) < 1e-4 * plain
+    with pytest.raises(ValueError, match="teacher_ids"):
+        am.evaluate(seqs, loss_fn=DistillationLoss())
+    monkeypatch.setattr(torch.distributed, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.distributed, "get_world_size", lambda *a: 2)
+    assert am.evaluate(seqs, loss_fn=DistillationLoss()).loss_sum == 0
