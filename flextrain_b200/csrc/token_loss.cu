@@ -268,11 +268,11 @@ __device__ __forceinline__ void total(const Row& a, int row, const Part* rec, fl
 #pragma unroll
     for (int r = 0; r < MOST_PARTS; ++r) {
         const Part& p = rec[r];
-      const bool none = p.m == -INFINITY, no_names = p.B == -INFINITY;
-      others += none ? 0.f : p.S * ex2((p.m - base) * a.c);
-      if (HARD) S1 += none ? 0.f : p.S1 * ex2((p.m - t.M) * LOG2E);
-      named += no_names ? 0.f : p.En * ex2((p.B - t.M) * a.c);
-      if (HARD) S1 += no_names ? 0.f : p.En1 * ex2((p.B - t.M) * LOG2E);
+      const bool none = p.m == -INFINITY, no_names = p.B == -INFINITY;        // (a sum of nothing may still be NaN: it is kept)
+      others += p.S * (none ? 0.f : ex2((p.m - base) * a.c));
+      if (HARD) S1 += p.S1 * (none ? 0.f : ex2((p.m - t.M) * LOG2E));
+      named += p.En * (no_names ? 0.f : ex2((p.B - t.M) * a.c));
+      if (HARD) S1 += p.En1 * (no_names ? 0.f : ex2((p.B - t.M) * LOG2E));
       kl += no_names || p.Q == 0.f ? 0.f : p.Q * (t.M - p.B) * a.inv_tau;
       kl += p.kl;
       Q += p.Q;
@@ -280,7 +280,7 @@ __device__ __forceinline__ void total(const Row& a, int row, const Part* rec, fl
     const float S = others * (rest == -INFINITY ? 0.f : ex2((base - t.M) * a.c)) + named;
     t.lS = S > 0.f ? log2f(S) : NAN;
     // q (log q - log p), where log p = (u - M) / tau - ln S and a part has (u - B) / tau
-    if (Q != 0.f) kl += Q * t.lS * LN2;
+    if (Q != 0.f || t.lS != t.lS) kl += Q * t.lS * LN2;        // (a row without a distribution is NaN without a teacher's tokens as well)
     t.base = base;
     t.k0 = (base - t.M) * a.c - t.lS;
     t.share = a.bucket ? Q + qr : (Q != 0.f ? 1.f : 0.f);
@@ -289,11 +289,11 @@ __device__ __forceinline__ void total(const Row& a, int row, const Part* rec, fl
       if (rest != -INFINITY && qr > 0.f) {
         const float l2 = (base - t.M) * a.c + log2f(others) - t.lS;       // log2 of the student's share of the others
         kl += qr * (logf(qr) - l2 * LN2);
-        if (l2 > -60.f) {
-          t.ka = t.share - qr / ex2(l2);
-        } else {                                              // (p itself is nothing beside the teacher's share there)
+        if (l2 <= -60.f) {                                    // (p itself is nothing beside the teacher's share there)
           t.k0 = -log2f(others);
           t.ka = -qr;
+        } else {                                              // (NaN too, which the gradients keep)
+          t.ka = t.share - qr / ex2(l2);
         }
       } else {                                                // nothing is left beside the named tokens
         t.share = t.ka = Q;

@@ -393,6 +393,7 @@ def distill_loss(logits, ids, teacher, targets, on, bucket, ce_weight, temperatu
     known = torch.zeros(logits.shape[0], V + 1, dtype=torch.bool, device=logits.device)
     known = known.scatter_(1, torch.where(inside, ids, V), True)[:, :V]
     kl = torch.where(q != 0, q * (t - logp.gather(1, at)), 0.0).sum(-1)
+    kl = torch.where(logp[:, 0].isnan(), logp[:, 0], kl)      # (a row without a distribution: NaN without a teacher's tokens as well)
     share = q.sum(-1)
     if bucket:
         others = logp.masked_fill(known, float("-inf"))

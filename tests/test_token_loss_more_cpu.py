@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from conftest import build_tiny
+from flextrain_b200 import ops
 from flextrain_b200.engine.active_model import ActiveModel
 from flextrain_b200.io.sequence import Sequence
 from flextrain_b200.nn.loss import CrossEntropyLoss, DistillationLoss, GRPOLoss, PolicyLoss
@@ -162,3 +163,34 @@ def test_distillation_of_sequences_without_a_teacher(monkeypatch):
     monkeypatch.setattr(torch.distributed, "is_initialized", lambda: True)
     monkeypatch.setattr(torch.distributed, "get_world_size", lambda *a: 2)
     assert am.evaluate(seqs, loss_fn=DistillationLoss()).loss_sum == 0
+
+
+def check_rows_of_nan(device):
+    """NaN wherever it lies in a row that counts reaches the loss and the whole gradient: a stretch as long as what one block of several
+    reads, all that is not the teacher's, a teacher's token of no weight, a row without a teacher's tokens; so do rows of -inf alone."""
+    V, K, nan, inf = 40000, 3, float("nan"), float("inf")
+    for dtype in (BF16, F16, F32):
+        z = torch.randn(8, V, generator=torch.Generator().manual_seed(8)).to(dtype).to(device)
+        ids = torch.tensor([1, 17, 39999], device=device).repeat(8, 1)
+        q = torch.tensor([-1.0, -2.0, -1.5], device=device).repeat(8, 1)
+        z[1, 10000:30000] = nan
+        z[2], z[2, [1, 17, 39999]] = nan, torch.randn(3).to(z)
+        z[3, 39999], q[3, 2] = nan, -inf
+        z[4, 20000:], ids[4] = nan, -1
+        z[5], ids[5] = -inf, -1
+        z[6, 5000:], z[6, :5000], ids[6] = nan, -inf, torch.tensor([2, 3, 4])
+        t = torch.full((8,), 7, device=device)
+        for rest in ("drop", "bucket"):
+            for ce in (0.0, 0.3):
+                for rows in (slice(0, 8), slice(3, 4)):
+                    out = torch.zeros_like(z[rows])
+                    kw = dict(targets=t[rows], rest=rest, ce_weight=ce)
+                    loss = ops.distill_loss_(z[rows], ids[rows], q[rows], out=out, **kw)
+                    clean = torch.tensor([r in (0, 7) for r in range(8)], device=device)[rows]
+                    for value in (loss, ops.distill_loss(z[rows], ids[rows], q[rows], **kw)):
+                        assert bool((value.isfinite() == clean).all()) and bool((value.isnan() == ~clean).all()), (dtype, rest, ce, value)
+                    assert bool((out.isfinite().all(-1) == clean).all()) and bool((out.isnan().all(-1) == ~clean).all()), (dtype, rest, ce)
+
+
+def test_rows_of_nan():
+    check_rows_of_nan("cpu")
