@@ -299,7 +299,9 @@ __device__ __forceinline__ void total(const Row& a, int row, const Part* rec, fl
         t.share = t.ka = Q;
       }
     }
-    float L = (1.f - a.ce) * a.tau * a.tau * kl;
+    const bool alone = HARD && a.ce >= 1.f;                   // cross entropy and nothing else: no share of an infinite divergence
+    if (alone) t.share = t.ka = 0.f;
+    float L = alone ? 0.f : (1.f - a.ce) * a.tau * a.tau * kl;
     if (HARD) {
       t.h0 = S1 > 0.f ? log2f(S1) : NAN;
       L -= a.ce * ((ut - t.M) * LOG2E - t.h0) * LN2;
@@ -322,7 +324,7 @@ __device__ __forceinline__ float grad_taken(const Totals& t, float bonus) {     
 }
 template <bool HARD>
 __device__ __forceinline__ float grad_named(const Row& a, const Totals& t, float u, float q, bool is_t) {
-  const float v = (1.f - a.ce) * a.tau * (ex2((u - t.M) * a.c - t.lS) * t.share - q);
+  const float v = HARD && a.ce >= 1.f ? 0.f : (1.f - a.ce) * a.tau * (ex2((u - t.M) * a.c - t.lS) * t.share - q);
   return HARD ? v + a.ce * (ex2((u - t.M) * LOG2E - t.h0) - (is_t ? 1.f : 0.f)) : v;
 }
 

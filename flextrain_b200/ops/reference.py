@@ -401,7 +401,7 @@ def distill_loss(logits, ids, teacher, targets, on, bucket, ce_weight, temperatu
         qr = torch.where(lr.isneginf(), 0.0, (1 - share).clamp(min=0))
         kl = kl + torch.where(qr > 0, qr * (qr.log() - lr), 0.0)
         share = share + qr
-    loss = (1 - ce_weight) * temperature * temperature * kl
+    loss = (1 - ce_weight) * temperature * temperature * kl if ce_weight < 1 else torch.zeros_like(kl)     # (no share of an infinite divergence)
     if ce_weight:
         hard = torch.log_softmax(u, -1)
         label = torch.where(on, targets, 0)[:, None]
@@ -412,7 +412,7 @@ def distill_loss(logits, ids, teacher, targets, on, bucket, ce_weight, temperatu
         if bucket:
             d = d - torch.where(known | (qr == 0)[:, None], 0.0, qr[:, None] * torch.exp(others - lr[:, None]))
         _added_at(d, ids, -q)
-        d = d * ((1 - ce_weight) * temperature)
+        d = d * ((1 - ce_weight) * temperature) if ce_weight < 1 else torch.zeros_like(d)
         if ce_weight:
             h = hard.exp()
             d = d + ce_weight * h.scatter_add_(1, label, torch.full_like(h[:, :1], -1.0))

@@ -275,7 +275,8 @@ def distill_loss_(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpr
 
     ``rest="drop"``: ``q`` is renormalised over the K tokens.  ``rest="bucket"``: ``q = exp(teacher_logprobs)``, and all other tokens
     are one further outcome, ``q_r = max(1 - sum(q), 0)`` (left out where no other token has a finite logit).  ``CE`` is the cross
-    entropy with ``targets`` at temperature 1.  Ids outside the vocabulary (padding: ``-1``) have no part; an id twice has both."""
+    entropy with ``targets`` at temperature 1; a ``ce_weight`` of one is the cross entropy alone, whatever KL is.  Ids outside the
+    vocabulary (padding: ``-1``) have no part; an id twice has both."""
     return _distill("distill_loss_", logits, teacher_ids, teacher_logprobs, targets, rest, ce_weight, temperature, softcap, grad_scale, loss_mask,
                     ignore_index, True, out)
 

@@ -15,6 +15,7 @@ from flextrain_b200.engine.active_model import ActiveModel
 from flextrain_b200.io.sequence import Sequence
 from flextrain_b200.nn.loss import CrossEntropyLoss, DistillationLoss, GRPOLoss, PolicyLoss
 from flextrain_b200.ops import TokenLogprobs
+from token_loss_oracle import near, near_grad
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 DIMS = dict(vocab_size=256, n_layers=2, d_model=64, n_heads=4, n_kv_heads=2, head_dim=16, expert_dim=128, ffn_dim=128, num_routed_experts=0,
@@ -194,3 +195,32 @@ def check_rows_of_nan(device):
 
 def test_rows_of_nan():
     check_rows_of_nan("cpu")
+
+
+def check_cross_entropy_alone(device):
+    """``ce_weight=1``: the cross entropy and its gradient, whatever the teacher says, also where the student has nothing at its token (a
+    divergence of infinity) and where its log probabilities are NaN."""
+    inf = float("inf")
+    for dtype in (BF16, F16, F32):
+        for V in (40, 20011):
+            z = torch.randn(4, V, generator=torch.Generator().manual_seed(6)).to(dtype).to(device)
+            z[0, 3] = z[2, 3] = -inf
+            t = torch.tensor([5, 3, 39, -100], device=device)
+            ids = torch.tensor([3, 5, -1], device=device).repeat(4, 1)
+            q = torch.log(torch.tensor([0.5, 0.2, 0.1], device=device)).repeat(4, 1)
+            q[2, 0] = float("nan")
+            x = z.double().requires_grad_()
+            want = torch.nn.functional.cross_entropy(x, t, reduction="none")
+            d, = torch.autograd.grad(want.sum(), x)
+            size = torch.softmax(z.double(), -1).scatter_add(1, t.clamp(min=0)[:, None], torch.ones(4, 1, dtype=torch.float64, device=device))
+            for rest in ("drop", "bucket"):
+                for tau in (1.0, 2.0):
+                    kw = dict(targets=t, rest=rest, ce_weight=1.0, temperature=tau)
+                    out = torch.empty_like(z)
+                    for loss in (ops.distill_loss(z, ids, q, **kw), ops.distill_loss_(z, ids, q, out=out, **kw)):
+                        near(loss, want.detach(), V)
+                    near_grad(out, d, size, z)
+
+
+def test_cross_entropy_alone():
+    check_cross_entropy_alone("cpu")

@@ -1,10 +1,14 @@
 """Operators on token probabilities on a GPU: what a later look at them found."""
 import pytest
 
-from test_token_loss_more_cpu import check_rows_of_nan
+from test_token_loss_more_cpu import check_cross_entropy_alone, check_rows_of_nan
 
 pytestmark = pytest.mark.gpu
 
 
 def test_rows_of_nan():
     check_rows_of_nan("cuda")
+
+
+def test_cross_entropy_alone():
+    check_cross_entropy_alone("cuda")
