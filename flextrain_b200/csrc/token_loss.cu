@@ -1116,13 +1116,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, in
   const float scale = OP == DISTILL ? a.scale : a.scale * a.inv_tau;
   const bool bonus = OP == POLICY && T.kb != 0.f;
   // One by one: entropy's gradient where a cap leaves -inf (elsewhere it is brought to a number that has no p log p, unless all of the row
-  // are such), and logits so large that their differences have to be formed first.
-  const bool careful = (bonus && (CAP || !(T.M > Vec<E>::LOW * 0.9f) || a.inv_tau < 0.05f)) ||
-                       (sizeof(E) == 2 && !(fabsf(T.base) * fmaxf(a.c, LOG2E) < 4096.f && fabsf(T.M) * LOG2E < 4096.f));
+  // are such).
+  const bool careful = bonus && (CAP || !(T.M > Vec<E>::LOW * 0.9f) || a.inv_tau < 0.05f);
   const f32x2 minus = pair(-T.base, -T.base), k0 = pair(T.k0, T.k0);
   const float fa = OP == POLICY ? T.ka * scale : (1.f - a.ce) * a.tau * T.ka * scale, fb = T.kb * LN2 * scale;
-  const float f0 = fmaf(-T.base, a.c, T.k0), f1 = fmaf(-T.M, LOG2E, -T.h0);
-  const f32x2 ka = pair(fa, fa), kb = pair(fb, fb), kc = pair(f0, f0), kh = pair(f1, f1);
+  const f32x2 ka = pair(fa, fa), kb = pair(fb, fb);
   const f32x2 minus_m = pair(-T.M, -T.M), h0 = pair(-T.h0, -T.h0), ce = pair(a.ce * scale, a.ce * scale);
   auto pass = [&](auto with_bonus, auto with_care) {
     constexpr bool BONUS = decltype(with_bonus)::value, CARE = decltype(with_care)::value;
@@ -1138,9 +1136,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, in
           split(x[i], b, c);
           r = pair(grad_rest<OP, HARD>(a, T, b) * scale, grad_rest<OP, HARD>(a, T, c) * scale);
         } else {
-          const f32x2 y = sizeof(E) == 2 ? fma2(x[i], cc, kc) : fma2(add2(x[i], minus), cc, k0);
+          const f32x2 y = fma2(add2(x[i], minus), cc, k0);    // (the difference first: a product of large logits has lost its last digits)
           r = mul2(exp2_2(y), BONUS ? fma2(kb, y, ka) : ka);
-          if (HARD) r = fma2(exp2_2(sizeof(E) == 2 ? fma2(x[i], l2, kh) : fma2(add2(x[i], minus_m), l2, h0)), ce, r);
+          if (HARD) r = fma2(exp2_2(fma2(add2(x[i], minus_m), l2, h0)), ce, r);
         }
         x[i] = CAP ? mul2(r, slope[i]) : r;
       }

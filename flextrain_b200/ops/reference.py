@@ -299,6 +299,13 @@ def _scaled(logits: torch.Tensor, temperature: float, softcap: float):
     return torch.where(z == float("-inf"), z, softcap * t), 1.0 - t * t
 
 
+def _differences(u, temperature):
+    """``(largest, (u - largest) / temperature)`` of each row: logits far from zero are subtracted before anything is rounded.  (NaN
+    where there is no largest finite one.)"""
+    most = u.amax(-1, keepdim=True)
+    return most, (u - most) / temperature
+
+
 def _where_on(on, *tensors):
     return tuple(torch.where(on if t.dim() == 1 else on[:, None], t, torch.zeros((), dtype=t.dtype, device=t.device)) for t in tensors)
 
@@ -315,10 +322,9 @@ def _added_at(d, ids, values):
 
 def token_logprobs(logits, targets, on, temperature, softcap, top_k):
     """``(logprobs or None, entropy, lse, top_ids or None, top_logprobs or None)`` of the rows that are ``on``."""
-    x = _scaled(logits, temperature, softcap)[0] / temperature
+    most, x = _differences(_scaled(logits, temperature, softcap)[0], temperature)
     logp = torch.log_softmax(x, -1)
-    lse = torch.logsumexp(x, -1)
-    lse = torch.where(lse.isinf(), torch.full_like(lse, float("nan")), lse)
+    lse = most[:, 0] / temperature + torch.logsumexp(x, -1)
     ent, lse = _where_on(on, _entropy(logp), lse)
     lp = ids = top = None
     if targets is not None:
@@ -352,7 +358,7 @@ def token_logprobs_bwd(logits, targets, on, lse, entropy, dlogprobs, dentropy, t
 def policy_loss(logits, targets, on, advantages, old, kept, clip_low, clip_high, kl_beta, entropy_coef, temperature, softcap, grad_scale, grad):
     """``((loss, logprobs, entropy), dlogits or None)``; see ``token_loss.policy_loss_``."""
     u, slope = _scaled(logits, temperature, softcap)
-    logp = torch.log_softmax(u / temperature, -1)
+    logp = torch.log_softmax(_differences(u, temperature)[1], -1)
     at = torch.where(on, targets, 0)[:, None]
     lp, ent = logp.gather(1, at)[:, 0], _entropy(logp)
     a = advantages if advantages is not None else torch.ones_like(lp)
@@ -381,7 +387,7 @@ def policy_loss(logits, targets, on, advantages, old, kept, clip_low, clip_high,
 def distill_loss(logits, ids, teacher, targets, on, bucket, ce_weight, temperature, softcap, grad_scale, grad):
     """``(loss, dlogits or None)``; see ``token_loss.distill_loss_``."""
     u, slope = _scaled(logits, temperature, softcap)
-    logp = torch.log_softmax(u / temperature, -1)
+    logp = torch.log_softmax(_differences(u, temperature)[1], -1)
     V = logits.shape[1]
     inside = (ids >= 0) & (ids < V)
     at = torch.where(inside, ids, 0)
