@@ -1239,8 +1239,10 @@ int launch_rows(const Row& a, cudaStream_t stream) {
   const long smem = TOP ? static_cast<long>(room) * parts * 8 : OP == DISTILL ? (slice / VE + 15) / 16 * 16 : 0;
   if (smem > MOST_SMEM) return -5;
   const int s = static_cast<int>(slice), m = static_cast<int>(smem);
-  if ((TOP || CAP || (OP == POLICY && a.out != nullptr)) && slice * static_cast<long>(sizeof(E)) > LONG_ROW)
-    return launch_block<E, OP, TOP, CAP, HARD, 512>(a, parts, s, room, m, stream);
+  if constexpr (TOP || CAP || OP == POLICY) {
+    if ((TOP || CAP || a.out != nullptr) && slice * static_cast<long>(sizeof(E)) > LONG_ROW)
+      return launch_block<E, OP, TOP, CAP, HARD, 512>(a, parts, s, room, m, stream);
+  }
   return launch_block<E, OP, TOP, CAP, HARD, 256>(a, parts, s, room, m, stream);
 }
 
