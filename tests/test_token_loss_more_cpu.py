@@ -226,26 +226,26 @@ def test_cross_entropy_alone():
     check_cross_entropy_alone("cpu")
 
 
-def check_common_offset(device, offset):
+def check_common_offset(device, offset, T=24):
     """Logits far from zero: a probability depends on their differences, so losses and gradients are held to what they are held to near
     zero (1e-5 of the gradient's terms and a rounding to its type)."""
-    T, V, K = 24, 2000, 5
+    V, K, scale = 2000, 5, 1024.0                             # (gradients of fp16 that are not among its smallest numbers)
     for dtype in (F16, BF16, F32):
         z = (wide(T, V, F32, device)[1] + offset).to(dtype)
         t = some_targets(T, V, device)
         on = on_rows(T, V, t, None, device=device)
         a = torch.linspace(-2, 2, T, device=device)
         for bonus in (0.0, 0.01):
-            (loss, lp, ent), want, size = policy(z, t, on, 1.0, 0.0, a, None, None, 0.2, 0.2, 0.0, bonus, 0.125)
-            got = ops.policy_loss_(z, t, a, entropy_coef=bonus, grad_scale=0.125, out=(out := torch.empty_like(z)))
+            (loss, lp, ent), want, size = policy(z, t, on, 1.0, 0.0, a, None, None, 0.2, 0.2, 0.0, bonus, scale)
+            got = ops.policy_loss_(z, t, a, entropy_coef=bonus, grad_scale=scale, out=(out := torch.empty_like(z)))
             near(got.loss, loss, V, factor=2.0)
             near(got.logprobs, lp, V)
             near(got.entropy, ent, V, size=3.0)
             near_grad(out, want, size, z)
         for rest, ce, tau in (("drop", 0.0, 1.0), ("bucket", 0.3, 2.0), ("drop", 0.3, 0.7)):
             ids, teacher = some_teacher(z, K, tau, 0.0)
-            loss, want, size = distill(z, ids, teacher, t, on, rest, ce, tau, 0.0, 0.125)
-            got = ops.distill_loss_(z, ids, teacher, targets=t, rest=rest, ce_weight=ce, temperature=tau, grad_scale=0.125, out=(out := torch.empty_like(z)))
+            loss, want, size = distill(z, ids, teacher, t, on, rest, ce, tau, 0.0, scale)
+            got = ops.distill_loss_(z, ids, teacher, targets=t, rest=rest, ce_weight=ce, temperature=tau, grad_scale=scale, out=(out := torch.empty_like(z)))
             near(got, loss, V, factor=max(1.0, tau * tau), size=12.0)
             near_grad(out, want, size, z)
 
