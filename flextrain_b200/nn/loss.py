@@ -12,6 +12,7 @@ from typing import Dict, Optional, Protocol
 import torch
 
 from .. import ops
+from ..ops.token_loss import MOST_TOKENS
 
 
 @dataclass
@@ -139,10 +140,14 @@ class GRPOLoss(_NativeLoss):
         self.kl_beta = float(kl_coef if kl_coef is not None else kl_beta)
 
     def __call__(self, logits, sl: TokenSlice, grad_scale: float, softcap: float = 0.0) -> torch.Tensor:
-        if logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float16, torch.float32):
-            # (as below: no mask but -100, and the logits as they are)
-            return ops.policy_loss_(logits, sl.targets, sl.advantages, ref_logprobs=sl.ref_logprobs, kl_beta=max(self.kl_beta, 0.0),
+        if logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float16, torch.float32) and logits.shape[1] <= MOST_TOKENS:
+            # (as below: no mask but -100, other negative targets are token 0, one advantage may stand for all, and the logits as they are)
+            t, rows = sl.targets.long(), logits if logits.stride(1) == 1 else logits.contiguous()
+            all_rows = lambda v: None if v is None else v.to(logits.device, torch.float32).expand(t.shape)                 # noqa: E731
+            loss = ops.policy_loss_(rows, torch.where(t == -100, t, t.clamp(min=0)), all_rows(sl.advantages),
+                                    ref_logprobs=all_rows(sl.ref_logprobs) if self.kl_beta > 0 else None, kl_beta=max(self.kl_beta, 0.0),
                                     grad_scale=grad_scale).loss
+            return loss if rows is logits else (logits.copy_(rows), loss)[1]
         z = logits.to(torch.float32)
         valid = (sl.targets != -100).to(torch.float32)
         tgt = sl.targets.clamp(min=0).long()
