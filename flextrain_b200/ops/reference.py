@@ -366,7 +366,7 @@ def policy_loss(logits, targets, on, advantages, old, kept, clip_low, clip_high,
         loss, g = -a * lp, -a
     else:
         r = torch.exp(lp - old)
-        free, held = r * a, r.clamp(1 - clip_low, 1 + clip_high) * a
+        free, held = torch.where((a == 0) & r.isinf(), a, r * a), r.clamp(1 - clip_low, 1 + clip_high) * a
         loss, g = -torch.minimum(free, held), torch.where(free <= held, -free, torch.where(free.isnan(), free, 0.0))
     if kept is not None and kl_beta:
         e = torch.expm1(kept - lp)

@@ -253,3 +253,19 @@ def check_common_offset(device, offset, T=24):
 @pytest.mark.parametrize("offset", [0.0, -300.0, 1000.0, 2500.0])
 def test_common_offset(offset):
     check_common_offset("cpu", offset)
+
+
+def check_infinite_ratio(device):
+    """A token that the old policy had no probability of: nothing times an advantage of zero is nothing, the clip holds a positive one."""
+    inf = float("inf")
+    z = torch.randn(4, 50, generator=torch.Generator().manual_seed(2)).to(device)
+    t, a = torch.tensor([1, 2, 3, 4], device=device), torch.tensor([0.0, -0.0, 2.0, -1.0], device=device)
+    old = torch.tensor([-1000.0, -inf, -1000.0, -1000.0], device=device)
+    out = torch.empty_like(z)
+    for loss in (ops.policy_loss(z, t, a, old_logprobs=old).loss, ops.policy_loss_(z, t, a, old_logprobs=old, out=out).loss):
+        assert loss[:2].tolist() == [0.0, 0.0] and abs(float(loss[2]) + 2.4) < 1e-6 and loss[3] == inf
+    assert bool((out[:3] == 0).all())
+
+
+def test_infinite_ratio():
+    check_infinite_ratio("cpu")

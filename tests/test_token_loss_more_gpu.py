@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from flextrain_b200.nn.loss import GRPOLoss, TokenSlice
-from test_token_loss_more_cpu import check_common_offset, check_cross_entropy_alone, check_rows_of_nan
+from test_token_loss_more_cpu import check_common_offset, check_cross_entropy_alone, check_infinite_ratio, check_rows_of_nan
 from token_loss_oracle import near, some_targets, wide
 
 pytestmark = pytest.mark.gpu
@@ -44,3 +44,7 @@ def test_grpo_loss_of_every_kind_that_it_took():
             # gradient is off by the same share of itself, 8e-5 of both sides, and 1e-5 by its probability
             near(got.cpu(), want.double(), V, factor=2 * 55.0)
             assert bool(((got_z.cpu() - want_z).abs() <= 1e-4 * (want_z.abs() + 1e-3)).all()), (kl, targets.dtype, list(more), columns)
+
+
+def test_infinite_ratio():
+    check_infinite_ratio("cuda")
