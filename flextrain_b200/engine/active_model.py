@@ -33,7 +33,7 @@ from ..core.save_level import (HardwareCost, SaveLevelPlan, TransmissionSchedule
 from ..core.working_set import WorkingSetConfig
 from ..io.sequence import Sequence, as_sequence
 from ..nn.loss import TokenScorer
-from ..ops.token_loss import MOST_TOP, TokenLogprobs
+from ..ops.token_loss import MOST_TOP, TEMPERATURES, TokenLogprobs
 from .buffers import BufferManager
 from .schedule import ChunkPolicy, prepare_training_chunks, split_sequences
 from .streams import EventBook, StreamBundle
@@ -313,8 +313,9 @@ class ActiveModel:
         ``logprobs`` are what ``Sequence.old_logprobs`` and ``ref_logprobs`` hold, its ``top_ids`` and ``top_logprobs`` what a student's
         ``teacher_ids`` and ``teacher_logprobs`` do (at the same temperature).  Positions without a target or masked are zero.  The
         per-token losses written back are the negative log probabilities."""
-        if not 0 <= top_k <= min(MOST_TOP, int(self.embed.vocab_size)) or not 0.0 < temperature < float("inf"):
-            raise ValueError(f"score: top_k {top_k} (0 to {min(MOST_TOP, int(self.embed.vocab_size))}), temperature {temperature} (above zero)")
+        most = min(MOST_TOP, int(self.embed.vocab_size))
+        if not 0 <= top_k <= most or not TEMPERATURES[0] <= temperature <= TEMPERATURES[1]:
+            raise ValueError(f"score: top_k {top_k} (0 to {most}), temperature {temperature} ({TEMPERATURES[0]:g} to {TEMPERATURES[1]:g})")
         given = list(seqs)
         mine = [as_sequence(s) for s in given]
         self.fwd_bwd(mine, loss_scale_factor=1.0, loss_fn=TokenScorer(top_k, temperature), forward_only=True)

@@ -25,6 +25,7 @@ F32 = torch.float32
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MOST_TOP = 128                 # alternatives of a row, tokens of a teacher
 MOST_TOKENS = 1600000          # of a vocabulary
+TEMPERATURES = (1e-37, 1e18)   # whose reciprocals and squares fp32 has
 
 
 class TokenLogprobs(NamedTuple):
@@ -58,8 +59,9 @@ def _of_rows(t, T: int, device, dtype, name: str, what: str, K: Optional[int] = 
 def _logits(logits, temperature, softcap, what: str):
     if logits.dim() != 2 or logits.dtype not in _TYPES:
         raise ValueError(f"{what}: logits {tuple(logits.shape)} {logits.dtype}, (T, V) in bf16, fp16 or fp32 are read")
-    if not 0.0 < temperature < float("inf") or not 0.0 <= softcap < float("inf"):
-        raise ValueError(f"{what}: temperature {temperature} (above zero), softcap {softcap} (zero: none)")
+    if not TEMPERATURES[0] <= temperature <= TEMPERATURES[1] or not (softcap == 0.0 or 1e-37 <= softcap <= 1e37):
+        raise ValueError(f"{what}: temperature {temperature}, {TEMPERATURES[0]:g} to {TEMPERATURES[1]:g} are read; softcap {softcap}, zero (none) or "
+                         "1e-37 to 1e37")
     T, V = logits.shape
     if V == 0 or V > MOST_TOKENS:
         raise ValueError(f"{what}: a vocabulary of {V} tokens, 1 to {MOST_TOKENS} are read")

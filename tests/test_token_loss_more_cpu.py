@@ -269,3 +269,27 @@ def check_infinite_ratio(device):
 
 def test_infinite_ratio():
     check_infinite_ratio("cpu")
+
+
+def check_extreme_scales(device):
+    """Temperatures and soft-caps whose reciprocals or squares fp32 does not have are refused; the ones beside them are not."""
+    z = torch.randn(3, 9, generator=torch.Generator().manual_seed(2)).to(device)
+    t = torch.tensor([1, 2, 3], device=device)
+    for kw in (dict(temperature=1e-40), dict(temperature=1e30), dict(softcap=1e-40), dict(softcap=1e39), dict(softcap=5e-324), dict(softcap=float("inf"))):
+        for call in (lambda kw: ops.token_logprobs(z, t, **kw), lambda kw: ops.policy_loss(z, t, **kw), lambda kw: ops.distill_loss(z, t[:, None], z[:, :1], **kw)):
+            with pytest.raises(ValueError):
+                call(kw)
+    flat = torch.full((3,), -torch.log(torch.tensor(9.0)).item(), device=device)
+    for kw in (dict(temperature=1e18), dict(softcap=1e-37)):
+        torch.testing.assert_close(ops.token_logprobs(z, t, **kw).logprobs, flat, rtol=1e-6, atol=0)
+    likeliest = ops.token_logprobs(z, z.argmax(-1), temperature=1e-6)
+    assert likeliest.logprobs.tolist() == [0.0] * 3 and likeliest.entropy.tolist() == [0.0] * 3
+    torch.testing.assert_close(ops.token_logprobs(z, t, softcap=1e30).logprobs, ops.token_logprobs(z, t).logprobs, rtol=1e-5, atol=1e-6)
+
+
+def test_extreme_scales():
+    check_extreme_scales("cpu")
+    am = build_tiny(dims=DIMS, max_seq_len=64, batch_tokens=96)
+    for tau in (1e-40, 1e30):
+        with pytest.raises(ValueError, match="score"):
+            am.score(_sequences(1), temperature=tau)

@@ -3,7 +3,8 @@ import pytest
 import torch
 
 from flextrain_b200.nn.loss import GRPOLoss, TokenSlice
-from test_token_loss_more_cpu import check_common_offset, check_cross_entropy_alone, check_infinite_ratio, check_rows_of_nan
+from test_token_loss_more_cpu import (check_common_offset, check_cross_entropy_alone, check_extreme_scales, check_infinite_ratio,
+                                      check_rows_of_nan)
 from token_loss_oracle import near, some_targets, wide
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +49,7 @@ def test_grpo_loss_of_every_kind_that_it_took():
 
 def test_infinite_ratio():
     check_infinite_ratio("cuda")
+
+
+def test_extreme_scales():
+    check_extreme_scales("cuda")
