@@ -13,7 +13,8 @@
 // Sums are in fp32, in base 2 relative to a row's largest logit m: e_j = 2^((u_j - m) log2(e) / tau), so that no difference of two
 // large numbers is rounded; the exponential is the hardware's (2^-22).  Rows that are left out (a target outside the vocabulary, a
 // mask of zero) are not read: their outputs and gradients are zero.  A row without a finite logit has no distribution and reads as
-// NaN, as does one with a NaN or +inf.  Compiled without fast math: logarithms and divisions of a row are the rounded ones.
+// NaN, as does one with a NaN or with +inf (which under a cap is a token at the cap).  Compiled without fast math: logarithms and divisions
+// of a row are the rounded ones.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -6,7 +6,8 @@ fp32, gradients have the logits' type and are by the logits as they were given.
 
 Rows that are left out have a target outside ``[0, V)`` (``ignore_index`` among them) or a ``loss_mask`` that is not above zero: they
 are not read, their scores, losses and gradients are zero, their alternatives ``-1`` with ``-inf``.  A logit of ``-inf`` is a token
-without probability, under a soft-cap too; a row of nothing else, or with a NaN or ``+inf``, reads as NaN.
+without probability, under a soft-cap too; a row of nothing else, or with a NaN, reads as NaN, and so does one with ``+inf``, but under
+a soft-cap that is a token at the cap.
 
 The calls whose names end in ``_`` write the gradient over the logits, or into ``out`` (the same shape and type, beside the logits or
 the logits themselves, not partly over them).  A call runs on the device of its tensors, on the stream that is current there; on a

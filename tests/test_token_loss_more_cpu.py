@@ -15,7 +15,7 @@ from flextrain_b200.engine.active_model import ActiveModel
 from flextrain_b200.io.sequence import Sequence
 from flextrain_b200.nn.loss import CrossEntropyLoss, DistillationLoss, GRPOLoss, PolicyLoss
 from flextrain_b200.ops import TokenLogprobs
-from token_loss_oracle import distill, near, near_grad, on_rows, policy, some_targets, some_teacher, wide
+from token_loss_oracle import distill, near, near_grad, on_rows, policy, scores, scores_grad, some_targets, some_teacher, wide
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 DIMS = dict(vocab_size=256, n_layers=2, d_model=64, n_heads=4, n_kv_heads=2, head_dim=16, expert_dim=128, ffn_dim=128, num_routed_experts=0,
@@ -293,3 +293,35 @@ def test_extreme_scales():
     for tau in (1e-40, 1e30):
         with pytest.raises(ValueError, match="score"):
             am.score(_sequences(1), temperature=tau)
+
+
+def check_infinity_under_a_cap(device):
+    """A logit of +inf is at the cap, with no slope: scores, losses and gradients as the definition has them."""
+    T, V, cap = 5, 2100, 15.0
+    for dtype in (BF16, F16, F32):
+        z = wide(T, V, dtype, device)[1].clone()
+        z[:, 7] = float("inf")
+        t = torch.tensor([7, 3, 2099, -100, 7], device=device)
+        on = on_rows(T, V, t, None, device=device)
+        _, _, lp, ent, lse, ids, top = scores(z, t, on, 1.0, cap, 4)
+        s = ops.token_logprobs(z, t, softcap=cap, top_k=4)
+        for got, want in zip((s.logprobs, s.entropy, s.lse), (lp, ent, lse)):
+            near(got[on], want.detach(), V, cap, size=3.0)
+        assert torch.equal(s.top_ids[on], ids)
+        near(s.top_logprobs[on], top.detach(), V, cap)
+        (loss, _, _), want, size = policy(z, t, on, 1.0, cap, None, None, None, 0.2, 0.2, 0.0, 0.01, 1.0)
+        near(ops.policy_loss_(z, t, entropy_coef=0.01, softcap=cap, out=(out := torch.empty_like(z))).loss, loss, V, cap)
+        near_grad(out, want, size, z, cap)
+        assert bool((out[:, 7].float().abs() < 1e-25).all())  # (4 e^-2y of a y that the kernel stops at; in fp32, fp16 has no 1e-25)
+        teacher_ids, q = some_teacher(z, 5, 1.0, cap)
+        loss, want, size = distill(z, teacher_ids, q, t, on, "bucket", 0.3, 1.0, cap, 1.0)
+        near(ops.distill_loss_(z, teacher_ids, q, targets=t, rest="bucket", ce_weight=0.3, softcap=cap, out=out), loss, V, cap, size=12.0)
+        near_grad(out, want, size, z, cap)
+        one = torch.ones(T, device=device)
+        want, size = scores_grad(z, t, on, 1.0, cap, one, one, None, None, 1.0)
+        ops.token_logprobs_bwd_(z, t, s, dlogprobs=one, dentropy=one, softcap=cap, out=out)
+        near_grad(out, want, size, z, cap)
+
+
+def test_infinity_under_a_cap():
+    check_infinity_under_a_cap("cpu")

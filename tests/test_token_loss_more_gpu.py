@@ -4,7 +4,7 @@ import torch
 
 from flextrain_b200.nn.loss import GRPOLoss, TokenSlice
 from test_token_loss_more_cpu import (check_common_offset, check_cross_entropy_alone, check_extreme_scales, check_infinite_ratio,
-                                      check_rows_of_nan)
+                                      check_infinity_under_a_cap, check_rows_of_nan)
 from token_loss_oracle import near, some_targets, wide
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +53,7 @@ def test_infinite_ratio():
 
 def test_extreme_scales():
     check_extreme_scales("cuda")
+
+
+def test_infinity_under_a_cap():
+    check_infinity_under_a_cap("cuda")
