@@ -241,7 +241,7 @@ __device__ __forceinline__ void total(const Row& a, int row, const Part* rec, fl
     // a token that has most of the row: the others' sum by itself, so that a small log p keeps its digits
     const bool most = has && ut >= rest && S > 0.f;
     const float ln_S = most ? log1pf(O) : t.lS * LN2;
-    t.lp = most ? -ln_S : (yt - t.lS) * LN2;
+    t.lp = most ? -ln_S : (ut - t.M) * a.inv_tau - ln_S;      // (not from yt: a mask's lowest value is beyond fp32 in base 2)
     t.H = ln_S - A / S * LN2;
     t.miss = O / S;
     t.base = t.M;
@@ -305,7 +305,7 @@ __device__ __forceinline__ void total(const Row& a, int row, const Part* rec, fl
     float L = alone ? 0.f : (1.f - a.ce) * a.tau * a.tau * kl;
     if (HARD) {
       t.h0 = S1 > 0.f ? log2f(S1) : NAN;
-      L -= a.ce * ((ut - t.M) * LOG2E - t.h0) * LN2;
+      L -= a.ce * ((ut - t.M) - t.h0 * LN2);
     }
     if (writes) a.loss[row] = L;
   }
@@ -1108,7 +1108,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, in
         const int token = static_cast<int>(~static_cast<uint32_t>(key));
         a.top_ids[(size_t)row * K + above] = token;
         a.top_logprob[(size_t)row * K + above] =
-            token == t ? T.lp : ((capped<CAP>(a, logit_of(static_cast<uint32_t>(key >> 32))) - T.M) * a.c - T.lS) * LN2;
+            token == t ? T.lp : (capped<CAP>(a, logit_of(static_cast<uint32_t>(key >> 32))) - T.M) * a.inv_tau - T.lS * LN2;
       }
     }
     return;

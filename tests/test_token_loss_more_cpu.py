@@ -325,3 +325,42 @@ def check_infinity_under_a_cap(device):
 
 def test_infinity_under_a_cap():
     check_infinity_under_a_cap("cpu")
+
+
+def check_given_token_under_a_mask(device):
+    """A given token, an alternative and a teacher's token whose logits are the type's lowest value: their log probabilities are that less
+    what the others sum to, finite numbers, so that the same policy's ratio is one and the cross entropy is finite."""
+    for dtype in (BF16, F32, F16):
+        for V in (6, 30000):
+            low = torch.finfo(dtype).min
+            z = torch.randn(3, V, generator=torch.Generator().manual_seed(11)).to(dtype).to(device)
+            z[:, 2] = low
+            if V == 6:
+                z[2, 1:5] = low
+            t = torch.tensor([2, 2, 1], device=device)
+            s = ops.token_logprobs(z, t, top_k=min(V, 6))
+            x = z.double()
+            want = torch.log_softmax(x, -1)
+            given = want.gather(1, t[:, None])[:, 0]
+            # (a rounding of the difference and one of the sum's logarithm, the first of the value's size)
+            at_most = lambda v: 2.0 ** -22 * (40 + 4 * (V / 256) ** 0.5) * (1 + v.abs())                                  # noqa: E731
+            assert bool(s.logprobs.isfinite().all()) and bool(((s.logprobs - given).abs() <= at_most(given)).all())
+            top = want.gather(1, s.top_ids)
+            assert bool(s.top_logprobs.isfinite().all()) and bool(((s.top_logprobs - top).abs() <= at_most(top)).all())
+            a = torch.tensor([1.0, -2.0, 0.5], device=device)
+            out = torch.empty_like(z)
+            for loss in (ops.policy_loss(z, t, a, old_logprobs=s.logprobs).loss, ops.policy_loss_(z, t, a, old_logprobs=s.logprobs, out=out).loss):
+                assert torch.equal(loss, -a)
+            # dL/dx = a (p - 1[t])
+            grad = a.double()[:, None] * (torch.softmax(x, -1) - torch.nn.functional.one_hot(t, V))
+            assert bool(((out - grad).abs() <= (torch.finfo(dtype).eps / 2 + 2e-5) * grad.abs() + torch.finfo(dtype).smallest_normal).all())
+            ids, q = torch.tensor([0, 1], device=device).repeat(3, 1), torch.log(torch.tensor([0.5, 0.25], device=device)).repeat(3, 1)
+            for rest in ("drop", "bucket"):
+                loss = ops.distill_loss_(z, ids, q, targets=t, rest=rest, ce_weight=0.5, out=out)
+                assert bool(loss.isfinite().all()) and bool(out.isfinite().all())
+                alone = ops.distill_loss(z, ids, q, targets=t, rest=rest, ce_weight=1.0)
+                assert bool(((alone + given).abs() <= at_most(given)).all())
+
+
+def test_given_token_under_a_mask():
+    check_given_token_under_a_mask("cpu")

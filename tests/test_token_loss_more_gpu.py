@@ -4,7 +4,7 @@ import torch
 
 from flextrain_b200.nn.loss import GRPOLoss, TokenSlice
 from test_token_loss_more_cpu import (check_common_offset, check_cross_entropy_alone, check_extreme_scales, check_infinite_ratio,
-                                      check_infinity_under_a_cap, check_rows_of_nan)
+                                      check_given_token_under_a_mask, check_infinity_under_a_cap, check_rows_of_nan)
 from token_loss_oracle import near, some_targets, wide
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +57,7 @@ def test_extreme_scales():
 
 def test_infinity_under_a_cap():
     check_infinity_under_a_cap("cuda")
+
+
+def test_given_token_under_a_mask():
+    check_given_token_under_a_mask("cuda")
