@@ -250,7 +250,7 @@ def check_common_offset(device, offset, T=24):
             near_grad(out, want, size, z)
 
 
-@pytest.mark.parametrize("offset", [0.0, -300.0, 1000.0, 2500.0])
+@pytest.mark.parametrize("offset", [0.0, 36.0, -300.0, 1000.0, 2500.0])
 def test_common_offset(offset):
     check_common_offset("cpu", offset)
 

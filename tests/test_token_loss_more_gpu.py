@@ -18,7 +18,7 @@ def test_cross_entropy_alone():
     check_cross_entropy_alone("cuda")
 
 
-@pytest.mark.parametrize("offset", [0.0, -300.0, 1000.0, 2500.0])
+@pytest.mark.parametrize("offset", [0.0, 36.0, -300.0, 1000.0, 2500.0])
 def test_common_offset(offset):
     check_common_offset("cuda", offset, T=600)                # (a row has a dozen gradients apart from each other, and fp16 shows one in a hundred)
 
