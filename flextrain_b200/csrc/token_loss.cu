@@ -100,7 +100,8 @@ template <>
 __device__ __forceinline__ float from_float<float>(float v) { return v; }
 
 // tanh y and 1 - tanh^2 y.  Near zero y (1 + s P(s)), s = y^2, P fitted to (tanh(y) / y - 1) / s on |y| <= 3/4 for the smallest largest
-// relative error (2e-9; with the roundings of fp32 it is some 2^-23.5); beyond it 1 - 2 / (1 + e^2y), whose slope is formed without 1 - t^2.
+// relative error (8e-9 with the coefficients in fp32, some 2^-23.5 with the steps' roundings); beyond it 1 - 2 / (1 + e^2y), whose slope is
+// formed without 1 - t^2.
 constexpr float TANH_NEAR = 0.75f;
 __device__ __forceinline__ float tanh_far(float y, float& slope) {
   const float r = __fdividef(2.f, 1.f + ex2(fminf(fabsf(y) * (2.f * LOG2E), 100.f)));
@@ -463,16 +464,23 @@ __device__ __forceinline__ void write_named(const Row& a, const Totals& t, const
 
 
 // ---------------------------------------------------------------------------------------------- clusters and pieces
-// Pieces of 16 bytes that a thread asks for at once: 8 for the totals (4096 x 151936 scores 151 us, 172 with 4), 4 under a soft-cap, whose
-// code is long (1001 x 256000: 345 us, 366 with 8), and for the gradient (4096 x 151936: 479 us, 490 with 8, 517 with 2).
+// (Times of this file: B200, us of a call back to back with others on two inputs beyond the second level of cache; 16-bit logits, a quarter
+// of the rows left out where there are 4,096 of them.  In turn with other work the longest ones take up to a seventh more.)
+// Pieces of 16 bytes that a thread asks for at once: 8 for the totals (4096 x 151936 scores 153, 173 with 4), 4 under a soft-cap, whose code
+// is long (1001 x 256000 policy gradient 321, 314 with 8), and for the gradient (4096 x 151936 417, 427 with 8, 455 with 2).
 constexpr int BATCH = 8, GRAD_BATCH = 4;
-// Bytes of a row from which a block has 512 threads and not 256, for some operators.  Alternatives: more threads give a closer bound (2048 x
-// 128256, 64 of them: 186 us, 244 with 256 threads).  Policy gradients, and soft-caps: half as many rows at a time, which the second level
-// of cache then still has when the gradient reads them again (4096 x 151936: 430 us, 480 with 256 threads; 1001 x 256000 343 and 348).
-// Scores and distillation: 256 threads, four blocks whose steps lie beside one another (scores 151 us, 187 with 512; held-out distillation
-// 2048 x 151936 113 and 158; with gradient 4096 x 128256 471 and 487).
+// Bytes of a row's slice from which a block has 512 threads and not 256, for some operators.  Alternatives: more threads give a closer bound.
+// Policy gradients, and soft-caps: half as many rows at a time, which the second level of cache then still has when the gradient reads them
+// again.  With 256 / 512 threads, 64 alternatives at 2048 x 32000 80 / 98, x 57600 (just above the border) 115 / 117, x 80000 157 / 150, 1024 x
+// 128256 123 / 98; policy gradients 60 / 67, 100 / 100, 142 / 133 and 121 / 107.  Under a cap the sides meet later: policy gradients at 1500 x
+// 57600 138 / 146, 1001 x 100000 154 / 155, x 256000 375 / 366; scores 64 / 71, 71 / 73, 166 / 165; alternatives 115 / 120, 134 / 118, 301 / 249.
+// Scores and distillation without a cap: 256 threads, four blocks whose steps lie beside one another (4096 x 151936 scores 153, 167 with 512;
+// held-out distillation 2048 x 151936 114 and 136; with gradient 4096 x 128256 450 and 477).
 constexpr int LONG_ROW = 114688;
-// Rows are cut over a cluster where there are fewer blocks than two for each SM (1 x 151936 with 20 alternatives: 18 us with the host's part).
+// Rows are cut over a cluster where there are fewer blocks than two for each SM.  In 1 / 2 / 4 parts: 148 x 50257 scores 10.1 / 8.7 / 10.4,
+// distillation 21 / 19 / 25; 295 x 50257 scores 11.8 / 11.3 / 15, 20 alternatives 19 / 19 / 30, policy gradient 18.4 / 17.4 / 24; 297 rows 12.6 /
+// 13.1 / 15, 20 / 24 / 31, 20.6 / 21.9 / 25.  Longer rows: 295 x 151936 scores 24 / 21 / 25, alternatives 32 / 39 / 45, distillation 64 / 59 / 70;
+// 400 rows 29 / 29 / 31, 50 / 54 / 54, 84 / 82 / 88.
 constexpr int FEW_BLOCKS = 2 * 148;
 __device__ __forceinline__ uint32_t in_cluster(const void* p, int rank) {          // the same place in another block's shared memory
   uint32_t r;
@@ -699,13 +707,17 @@ __device__ __forceinline__ float logit_of(uint32_t order) {
 // its own among them.  Where these are too many because the blocks' tokens differ, the bound is the highest of bounds by K threads of a
 // block; where thousands of logits are equal, the cluster halves the interval of (logit, index) of all tokens until exactly K are left.
 //
-// What bounds it (B200, 16-bit logits, device-timed, calls one behind the other): scores by memory, 151 us for 142 at 4096 x 151936 with a
-// quarter of the rows left out (6.2 of 6.55 TB/s); with the gradient by the second reading, whose rows the cache has lost in part (policy
-// gradients 411 us for 332; it goes through the row from its end, 423 from its beginning), and with cross entropy at another temperature beside it by the exponentials,
-// four an element (distillation 452 us for 281).  Tried: rows in the shared memory of clusters of eight, each block a piece that stays for
-// the gradient, with clusters that take over rows of others (policy gradients 427 us, but scores 206 and distillation 631: the blocks of
-// a row wait for the slowest of them at every row); pieces kept in shared memory up to 208 KB an SM (430 -> 507: what the first level of
-// cache loses was in use for loads on their way), up to 96 KB (425); three and five blocks an SM (173, 159 us of scores).
+// What bounds it: scores by memory, 153 us for 142 at 4096 x 151936 (6.1 of 6.55 TB/s); with the gradient by the second reading, whose rows
+// the cache has lost in part (policy gradients 412 for 332; the pass goes through the row from its end, 4 % more from its beginning), and
+// with cross entropy at another temperature beside it by the exponentials, four an element (distillation 4096 x 128256 450 for 281).  64
+// alternatives 2048 x 128256 184 for 80: rows by two blocks of 512 threads an SM, whose steps follow one another, and 44 to 76 bytes of
+// spilled registers.  64 registers a thread, so that four blocks of 256 or two of 512 fit: with registers
+// for three and one of them scores take 166, distillation 5 % and policy gradients a fifth more; for five and two 165, 1 % and 2 %.  The price
+// are spills in distillation with cross entropy (52 bytes) and under a soft-cap (up to 68).
+// Earlier builds: rows in the shared memory of clusters of eight, each block a piece that stays for the gradient, with clusters that take
+// over rows of others (policy gradients 427, but scores 206 and distillation 631: the blocks of a row wait for the slowest of them at every
+// row); pieces kept in shared memory, up to 208 KB an SM (a sixth slower: what the first level of cache loses was in use for loads on their
+// way), up to 96 KB (1 % faster).
 template <typename E, Op OP, bool TOP, bool CAP, bool HARD, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(Row a, int slice, int room) {
   constexpr int VE = Vec<E>::N, P = VE / 2, W = NT / 32, U = CAP ? BATCH / 2 : BATCH, GU = GRAD_BATCH;
@@ -1294,7 +1306,7 @@ int run_rows(Op op, const RowArgs* r) {
 //
 // One pass, nothing between the tokens of a row: blocks of 256 threads take 1,024 pieces of 16 bytes, four a thread that are all asked for
 // before the first is used.  The tokens with gradients of their own are written again behind the others of their block.  Bound by memory:
-// 2048 x 128256 bf16 with a quarter of the rows left out 166 us (5.5 of 6.55 TB/s).
+// 2048 x 128256 bf16 with a quarter of the rows left out 164 us (5.6 of 6.55 TB/s).
 constexpr int GRAD_NT = 256, GRAD_EACH = 4;
 template <typename E, bool CAP>
 __global__ void __launch_bounds__(GRAD_NT) grad_kernel(Row a, const float* lse, const float* dlogprob, const float* dentropy, const float* dtop, int blocks) {

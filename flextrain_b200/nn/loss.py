@@ -170,7 +170,8 @@ class GRPOLoss(_NativeLoss):
 class PolicyLoss(_NativeLoss):
     """Clipped policy gradient (``ops.policy_loss_``): the ratio to ``Sequence.old_logprobs`` (without them ``-A * logp``), per-token
     ``advantages``, a k3 KL penalty to ``ref_logprobs`` and an entropy bonus, under the head's soft-cap and at a temperature.  Rows
-    whose target is ``-100`` or whose ``loss_mask`` is not above zero contribute nothing."""
+    whose target is ``-100`` or whose ``loss_mask`` is not above zero contribute nothing.  All of a call's sequences carry
+    ``old_logprobs`` or none; with a penalty the same holds for ``ref_logprobs``."""
 
     def __init__(self, clip_low: float = 0.2, clip_high: Optional[float] = None, *, kl_coef: float = 0.0, entropy_coef: float = 0.0,
                  temperature: float = 1.0, ignore_index: int = -100):

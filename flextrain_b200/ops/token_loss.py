@@ -154,8 +154,8 @@ def token_logprobs_bwd_(logits: torch.Tensor, targets: Optional[torch.Tensor], s
     """``grad_scale`` times the logits' gradient from those of :func:`token_logprobs`'s outputs (any of them None: zero), written over
     the logits or into ``out``, which is returned.  ``scores`` is what the forward call returned for the same arguments: its ``lse``
     is read, its ``entropy`` with ``dentropy`` and its ``top_ids`` with ``dtop_logprobs`` (ids outside the vocabulary have no part,
-    an id twice has both).  Probabilities are taken from the fp32 ``lse``: a row whose largest logit is beyond some thousands, as one
-    that a mask's lowest value leaves nothing of, loses digits of them."""
+    an id twice has both).  Probabilities are taken from the fp32 ``lse``, whose rounding is some 2^-24 of it: at an lse of 1,000 they
+    are off by 6e-5, and a row that a mask's lowest value leaves nothing else of has lost them."""
     what = "token_logprobs_bwd_"
     T, V = _logits(logits, temperature, softcap, what)
     device = logits.device
