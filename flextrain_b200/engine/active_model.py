@@ -330,7 +330,7 @@ class ActiveModel:
             if mine is not theirs and getattr(mine, name) is not None:
                 try:
                     setattr(theirs, name, getattr(mine, name))
-                except AttributeError:
+                except (AttributeError, TypeError, ValueError):        # (a class that takes no such field)
                     pass
 
     def _write_back_scores(self, pending) -> None:

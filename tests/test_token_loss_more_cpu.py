@@ -117,8 +117,16 @@ def test_scores_are_left_in_the_callers_own_objects():
         def __init__(self, s):
             self.tokens, self.targets = s.tokens, s.targets
 
-    mine, closed = [Bare(s) for s in seqs[:2]], Closed(seqs[2])
-    got = am.score(mine + [closed], top_k=2)
+    class Strict(Closed):
+        __slots__ = ()
+
+        def __setattr__(self, name, value):
+            if name not in ("tokens", "targets"):
+                raise ValueError(f"no field {name}")
+            super().__setattr__(name, value)
+
+    mine, closed = [Bare(s) for s in seqs[:2]], [Closed(seqs[2]), Strict(seqs[2])]
+    got = am.score(mine + closed, top_k=2)
     for s, x, given in zip(seqs, am.score(seqs, top_k=2), got):
         assert torch.equal(x.logprobs, given.logprobs) and torch.equal(x.top_ids, given.top_ids)
     for s, x, given in zip(mine, got, seqs):
